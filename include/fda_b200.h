@@ -54,7 +54,8 @@ typedef enum fda_status {
     FDA_ERR_WORKSPACE = 8,        /* workspace missing or smaller than the part a call cannot do without */
     FDA_ERR_MISALIGNED = 9,       /* a tensor base address is not 16-byte aligned */
     FDA_ERR_CUDA = 10,            /* a CUDA runtime call or the kernel launch failed; see fda_last_cuda_error() */
-    FDA_ERR_TOO_LARGE_STATIC = 11 /* problem exceeds a compiled-in capacity */
+    FDA_ERR_TOO_LARGE_STATIC = 11, /* problem exceeds a compiled-in capacity */
+    FDA_ERR_BAD_ACTIVATION = 12   /* unknown activation */
 } fda_status_t;
 
 /* Human-readable name of a status code (static storage, never NULL). */
@@ -427,6 +428,53 @@ size_t fda_nms3d_scored_workspace_bytes(int num_boxes);
 int fda_nms3d_scored(const float *boxes, long long box_stride, long long coord_stride, const float *scores,
                      long long score_stride, int num_boxes, float iou_threshold, void *workspace, size_t workspace_bytes,
                      long long *keep, int *num_keep, void *stream);
+
+/*
+ * Linear layers with everything around the product in one pass, for one weight or one weight per group of rows:
+ *
+ *   pre = x W^T + bias,   y = act(pre) + residual
+ *   g = grad_output * act'(pre),   grad_x = g W,   grad_weight = g^T x,   grad_bias = sum of g's rows
+ *
+ *   x [batch][rows][in_features]   weight [groups][out_features][in_features]   bias [groups][out_features] or NULL
+ *   residual, y, grad_output [batch][rows][out_features]   residual or NULL; its gradient is grad_output
+ * all of `dtype`; sums in fp32, one rounding at the end.  Any sizes of at least one feature and any
+ * element-aligned addresses; rows * batch < 2^31.
+ *
+ * group_start_index NULL: one group of all rows (groups = 1).  Else int64 on the device, num_starts = groups or groups + 1
+ * entries: group e holds the rows group_start_index[e] <= m < group_start_index[e + 1] of every batch element (the last ends
+ * with the rows where there is no further entry).  An index below an earlier one counts as that one, indices outside
+ * 0 .. rows as the nearer end.  Rows of no group: y = residual or 0, grad_x = 0, nothing added to the other gradients.
+ * groups <= FDA_LINEAR_MAX_GROUPS.
+ *
+ * The backward computes pre again from x instead of reading it: that is in_features instead of 2 * out_features elements of
+ * traffic a row.  For 16-bit types g is rounded to `dtype` between the products.  grad_x, grad_weight and grad_bias may each be
+ * NULL.  Sums run in a fixed order: repeated calls give the same bits.
+ *
+ * The workspaces (256-byte aligned; sizes from the functions, 0 = none) hold intermediate results of the call only; two calls
+ * that may overlap need two.  A wait inside a kernel that ran out (2 s: never in a sound run) leaves the outputs undefined and
+ * counts in fda_linear_timeouts(), which synchronises with the device; the count is per device and never reset.
+ */
+typedef enum fda_activation {
+    FDA_ACT_NONE = 0,
+    FDA_ACT_RELU = 1,
+    FDA_ACT_GELU = 2,      /* v Phi(v) */
+    FDA_ACT_GELU_TANH = 3, /* v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) / 2 */
+    FDA_ACT_SILU = 4       /* v / (1 + e^-v) */
+} fda_activation_t;
+#define FDA_LINEAR_MAX_GROUPS 1024
+
+size_t fda_linear_forward_workspace_bytes(int batch, int rows, int groups, int in_features, int out_features, int dtype);
+int fda_linear_forward(const void *x, const void *weight, const void *bias, const void *residual,
+                       const int64_t *group_start_index, int num_starts, void *y, void *workspace, size_t workspace_bytes,
+                       int batch, int rows, int groups, int in_features, int out_features, int activation, int dtype,
+                       void *stream);
+size_t fda_linear_backward_workspace_bytes(int batch, int rows, int groups, int in_features, int out_features,
+                                           int activation, int dtype);
+int fda_linear_backward(const void *x, const void *weight, const void *bias, const void *grad_output,
+                        const int64_t *group_start_index, int num_starts, void *grad_x, void *grad_weight, void *grad_bias,
+                        void *workspace, size_t workspace_bytes, int batch, int rows, int groups, int in_features,
+                        int out_features, int activation, int dtype, void *stream);
+int fda_linear_timeouts(void);
 
 /*
  * Backward pass that needs no workspace from the caller and allocates nothing: same inputs,

@@ -6,6 +6,8 @@ CUDA kernels behind a C ABI (``include/fda_b200.h``, ``libfda_b200.so``), a thin
 """
 from ._extension import _C
 from .flash_deform_attn import FlashDeformAttnFunction, findspec, findspec_bwd
+from .linear import FeedForward, FusedLinearFunction, GroupedLinear, fused_linear, grouped_linear
 
-__all__ = ["FlashDeformAttnFunction", "findspec", "findspec_bwd", "_C"]
+__all__ = ["FlashDeformAttnFunction", "findspec", "findspec_bwd", "fused_linear", "grouped_linear", "FusedLinearFunction",
+           "GroupedLinear", "FeedForward", "_C"]
 # The layer around the operator lives in ops3d_b200.msda3d (MSDeformAttn3D); imported on demand.

@@ -23,6 +23,8 @@ EXPORTS = (
     "fda_dcnv4_backward_workspace_bytes", "fda_dcnv4_backward_scratch_bytes", "fda_dcnv4_output_size", "fda_roi_align3d_forward", "fda_roi_align3d_backward",
     "fda_nms3d", "fda_nms3d_workspace_bytes", "fda_nms3d_scored", "fda_nms3d_scored_workspace_bytes", "fda_reload_config", "fda_group_reduce_cast", "fda_head_slice_cast_push",
     "fda_backward_touched_rows", "fda_cast_grad_value_touched",
+    "fda_linear_forward_workspace_bytes", "fda_linear_forward", "fda_linear_backward_workspace_bytes", "fda_linear_backward",
+    "fda_linear_timeouts",
 )
 BWD_ZERO_IMAGE, BWD_RESUME, BWD_FINALIZE, BWD_BINNED_DONE, BWD_ZERO_TOUCHED = 1, 2, 4, 8, 16
 NOALLOC_MAX_ELEMENTS = 16 * 1024 * 1024
@@ -124,6 +126,11 @@ def load() -> ctypes.CDLL:
     lib.fda_peer_reduce_staged_cast.restype = i
     lib.fda_multimem_reduce_cast.argtypes = [vp, vp, i, i, sz, i, vp]
     lib.fda_multimem_reduce_cast.restype = i
+    lib.fda_linear_forward_workspace_bytes.argtypes, lib.fda_linear_forward_workspace_bytes.restype = [i] * 6, sz
+    lib.fda_linear_forward.argtypes, lib.fda_linear_forward.restype = [vp] * 5 + [i] + [vp] * 2 + [sz] + [i] * 7 + [vp], i
+    lib.fda_linear_backward_workspace_bytes.argtypes, lib.fda_linear_backward_workspace_bytes.restype = [i] * 7, sz
+    lib.fda_linear_backward.argtypes, lib.fda_linear_backward.restype = [vp] * 5 + [i] + [vp] * 4 + [sz] + [i] * 7 + [vp], i
+    lib.fda_linear_timeouts.argtypes, lib.fda_linear_timeouts.restype = [], i
     _lib = lib
     return lib
 

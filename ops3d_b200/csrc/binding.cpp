@@ -9,7 +9,8 @@
 // with the argument meaning and error behaviour of csrc/flash_deform_attn.h:7-52 and
 // csrc/cuda/flash_deform_attn_cuda.cu:20-179: RuntimeError for CPU / non-contiguous tensors and
 // for batch % min(batch, im2col_step) != 0, ValueError for an unsupported level or point count.
-// flash_deform_attn, dcnv4 and roi_align_3d are their differentiable forms (autograd_nodes.h), what the Python Functions call.
+// linear_forward / linear_backward are the linear layers with a fused epilogue (ops3d_b200/linear.py has the arguments).
+// flash_deform_attn, dcnv4, roi_align_3d and linear are the differentiable forms (autograd_nodes.h), what the Python Functions call.
 // This file only checks tensors, allocates outputs from torch's allocator, and forwards raw
 // pointers plus the current CUDA stream; all arithmetic lives behind the C ABI.
 #include <torch/extension.h>
@@ -19,6 +20,9 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
+#include <array>
+#include <cstdint>
+#include <optional>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -417,6 +421,170 @@ at::Tensor nms_3d(const at::Tensor &dets, const at::Tensor &scores, const float 
     return order.index_select(0, keep.narrow(0, 0, kept));
 }
 
+// Linear layers with bias, activation and residual in the product's epilogue; with group_start_index one weight per group.
+struct LinearArgs {
+    at::Tensor x, weight, bias, starts;  // contiguous; bias and starts may be undefined
+    int batch, rows, groups, in, out, num_starts, dtype;
+    std::vector<int64_t> out_size;
+    const void *bias_ptr() const { return bias.defined() ? bias.data_ptr() : nullptr; }
+    const int64_t *starts_ptr() const { return starts.defined() ? starts.data_ptr<int64_t>() : nullptr; }
+};
+
+using OptionalTensor = std::optional<at::Tensor>;
+at::Tensor or_undefined(const OptionalTensor &t) { return t.has_value() ? *t : at::Tensor(); }
+
+void check_linear_operand(const at::Tensor &t, const at::Tensor &x, const char *name) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (this operator has no CPU implementation)");
+    TORCH_CHECK(t.device() == x.device(), "x and ", name, " must be on the same device");
+    TORCH_CHECK(t.scalar_type() == x.scalar_type(), name, " must have the dtype of x, ", x.scalar_type(), ", got ", t.scalar_type());
+}
+
+LinearArgs check_linear(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &bias, const at::Tensor &starts) {
+    LinearArgs a;
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (this operator has no CPU implementation)");
+    a.dtype = dtype_code(x, "x");
+    check_linear_operand(weight, x, "weight");
+    const bool grouped = starts.defined();
+    const int64_t wd = weight.dim();
+    TORCH_CHECK(wd == (grouped ? 3 : 2), "weight must be ", grouped ? "[groups, out_features, in_features]" : "[out_features, in_features]");
+    const int64_t groups = grouped ? weight.size(0) : 1, out = weight.size(wd - 2), in = weight.size(wd - 1);
+    TORCH_CHECK(groups > 0 && out > 0 && in > 0, "weight must not be empty");
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) == in, "x must have ", in, " features like weight, got ", x.sizes());
+    if (bias.defined()) {
+        check_linear_operand(bias, x, "bias");
+        const bool fits = grouped ? bias.dim() == 2 && bias.size(0) == groups && bias.size(1) == out : bias.dim() == 1 && bias.size(0) == out;
+        TORCH_CHECK(fits, "bias must be ", grouped ? "[groups, out_features]" : "[out_features]", " like weight, got ", bias.sizes());
+    }
+    int64_t batch = 1, rows = x.numel() / in;
+    if (grouped) {
+        TORCH_CHECK(x.dim() == 2 || x.dim() == 3, "x must be [rows, in_features] or [batch, rows, in_features]");
+        TORCH_CHECK(starts.is_cuda() && starts.device() == x.device(), "x and group_start_index must be on the same device");
+        TORCH_CHECK(starts.scalar_type() == at::kLong && starts.dim() == 1, "group_start_index must be a one-dimensional int64 tensor");
+        TORCH_CHECK(starts.size(0) == groups || starts.size(0) == groups + 1,
+                    "group_start_index must have one entry per group, or one more for the end of the last; got ", starts.size(0), " for ",
+                    groups, " groups");
+        if (x.dim() == 3) { batch = x.size(0); rows = x.size(1); }
+        a.starts = starts.contiguous();
+    }
+    TORCH_CHECK(in <= INT32_MAX && out <= INT32_MAX && groups <= INT32_MAX && batch <= INT32_MAX && rows <= INT32_MAX,
+                "linear: too large dimension");
+    a.x = x.contiguous();
+    a.weight = weight.contiguous();
+    if (bias.defined()) a.bias = bias.contiguous();
+    a.batch = (int)batch; a.rows = (int)rows; a.groups = (int)groups; a.in = (int)in; a.out = (int)out;
+    a.num_starts = grouped ? (int)starts.size(0) : 0;
+    a.out_size = x.sizes().vec();
+    a.out_size.back() = out;
+    return a;
+}
+
+at::Tensor linear_workspace(const at::Tensor &like, size_t bytes) {
+    return bytes ? empty_on(like, {(int64_t)((bytes + 3) / 4)}, at::kFloat) : at::Tensor();
+}
+
+at::Tensor linear_forward_impl(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &bias, const at::Tensor &residual,
+                               const at::Tensor &starts, int activation) {
+    const LinearArgs a = check_linear(x, weight, bias, starts);
+    at::Tensor res;
+    if (residual.defined()) {
+        check_linear_operand(residual, x, "residual");
+        TORCH_CHECK(residual.sizes() == at::IntArrayRef(a.out_size), "residual must have the shape of the output, ",
+                    at::IntArrayRef(a.out_size), ", got ", residual.sizes());
+        res = residual.contiguous();
+    }
+    c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor y = empty_on(x, a.out_size, x.scalar_type());
+    const size_t bytes = fda_linear_forward_workspace_bytes(a.batch, a.rows, a.groups, a.in, a.out, a.dtype);
+    const at::Tensor ws = linear_workspace(x, bytes);
+    raise_status(fda_linear_forward(a.x.data_ptr(), a.weight.data_ptr(), a.bias_ptr(), res.defined() ? res.data_ptr() : nullptr,
+                                    a.starts_ptr(), a.num_starts, y.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr, bytes, a.batch,
+                                    a.rows, a.groups, a.in, a.out, activation, a.dtype, at::cuda::getCurrentCUDAStream().stream()),
+                 "linear_forward");
+    return y;
+}
+
+std::array<at::Tensor, 3> linear_backward_impl(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &bias,
+                                               const at::Tensor &starts, const at::Tensor &grad_output, int activation, bool need_x,
+                                               bool need_weight, bool need_bias) {
+    const LinearArgs a = check_linear(x, weight, bias, starts);
+    check_linear_operand(grad_output, x, "grad_output");
+    TORCH_CHECK(grad_output.sizes() == at::IntArrayRef(a.out_size), "grad_output must have the shape of the output, ",
+                at::IntArrayRef(a.out_size), ", got ", grad_output.sizes());
+    c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor grad = grad_output.contiguous();
+    std::array<at::Tensor, 3> out;
+    if (need_x) out[0] = empty_on(x, x.sizes(), x.scalar_type());
+    if (need_weight) out[1] = empty_on(x, weight.sizes(), x.scalar_type());
+    if (need_bias && bias.defined()) out[2] = empty_on(x, bias.sizes(), x.scalar_type());
+    const size_t bytes = fda_linear_backward_workspace_bytes(a.batch, a.rows, a.groups, a.in, a.out, activation, a.dtype);
+    const at::Tensor ws = linear_workspace(x, bytes);
+    const auto ptr = [](const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
+    raise_status(fda_linear_backward(a.x.data_ptr(), a.weight.data_ptr(), a.bias_ptr(), grad.data_ptr(), a.starts_ptr(), a.num_starts,
+                                     ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(ws), bytes, a.batch, a.rows, a.groups, a.in, a.out,
+                                     activation, a.dtype, at::cuda::getCurrentCUDAStream().stream()),
+                 "linear_backward");
+    return out;
+}
+
+at::Tensor linear_forward(const at::Tensor &x, const at::Tensor &weight, const OptionalTensor &bias, const OptionalTensor &residual,
+                          const OptionalTensor &group_start_index, int activation) {
+    return linear_forward_impl(x, weight, or_undefined(bias), or_undefined(residual), or_undefined(group_start_index), activation);
+}
+
+std::array<OptionalTensor, 3> linear_backward(const at::Tensor &x, const at::Tensor &weight, const OptionalTensor &bias,
+                                              const OptionalTensor &group_start_index, const at::Tensor &grad_output, int activation,
+                                              bool need_x, bool need_weight, bool need_bias) {
+    const auto grads = linear_backward_impl(x, weight, or_undefined(bias), or_undefined(group_start_index), grad_output, activation, need_x,
+                                            need_weight, need_bias);
+    std::array<OptionalTensor, 3> out;
+    for (int i = 0; i < 3; ++i)
+        if (grads[i].defined()) out[i] = grads[i];
+    return out;
+}
+
+// FusedLinearFunction.apply; the residual's gradient is the output's.
+struct FusedLinearBackward : public fda_nodes::SavedNode {
+    int activation;
+    std::string name() const override { return "FusedLinearFunctionBackward"; }
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        torch::autograd::variable_list results(4);
+        const bool recording = at::GradMode::is_enabled();
+        {
+            at::NoGradGuard no_grad;
+            const at::Tensor g = grad_output(grads);
+            const bool need_x = task_should_compute_output(0), need_weight = task_should_compute_output(1);
+            const bool need_bias = task_should_compute_output(2);
+            if (need_x || need_weight || need_bias) {
+                const auto r = linear_backward_impl(unpack(0), unpack(1), unpack(2), unpack(3), g, activation, need_x, need_weight, need_bias);
+                std::copy(r.begin(), r.end(), results.begin());
+            }
+            if (task_should_compute_output(3)) results[3] = g;
+        }
+        return fda_nodes::once_differentiable(std::move(results), recording);
+    }
+};
+
+at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const OptionalTensor &bias, const OptionalTensor &residual,
+                  const OptionalTensor &group_start_index, int activation) {
+    const at::Tensor b = or_undefined(bias), r = or_undefined(residual), starts = or_undefined(group_start_index);
+    at::Tensor y;
+    {
+        at::NoGradGuard no_grad;
+        y = linear_forward_impl(x, weight, b, r, starts, activation);
+    }
+    if (fda_nodes::needs_node({x, weight, b, r})) {
+        auto node = std::make_shared<FusedLinearBackward>();
+        node->activation = activation;
+        node->save(0, x);
+        node->save(1, weight);
+        node->save(2, b);
+        node->save(3, starts);
+        fda_nodes::connect(node, y, torch::autograd::collect_next_edges(x, weight, b, r));
+    }
+    return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -426,6 +594,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("flash_deform_attn", &flash_deform_attn, "differentiable Flash Deformable 3D Attention");
     m.def("dcnv4", &dcnv4, "differentiable DCNv4-3D");
     m.def("roi_align_3d", &roi_align_3d, "differentiable ROI-Align 3D");
+    m.def("linear", &linear, "differentiable linear layer with fused epilogue");
+    m.def("linear_forward", &linear_forward, "linear layer with fused epilogue, forward (sm_100a)");
+    m.def("linear_backward", &linear_backward, "linear layer with fused epilogue, backward (sm_100a)");
     m.def("nms_3d", &nms_3d, "non-maximum suppression for 3d boxes (sm_100a)");
     m.def("roi_align_3d_forward", &roi_align_3d_forward, "ROI-Align 3D forward (sm_100a)");
     m.def("roi_align_3d_backward", &roi_align_3d_backward, "ROI-Align 3D backward (sm_100a)");

@@ -552,6 +552,7 @@ const char *fda_status_string(int status) {
         case FDA_ERR_MISALIGNED: return "tensor base address not 16-byte aligned";
         case FDA_ERR_CUDA: return "CUDA runtime error";
         case FDA_ERR_TOO_LARGE_STATIC: return "problem exceeds a compiled-in capacity";
+        case FDA_ERR_BAD_ACTIVATION: return "unknown activation";
         default: return "unknown status";
     }
 }

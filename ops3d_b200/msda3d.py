@@ -13,6 +13,10 @@ after the two projections:
     out     = output_proj(FlashDeformAttnFunction(value, shapes, level_start_index, packed))
 
 ``reference_points`` are normalised ``(x, y, z)`` per level, ``[B, Q, L, 3]``.
+
+Two options take the fused linear operators (``ops3d_b200.linear``): ``level_value_proj=True`` gives each pyramid level a value
+projection of its own, one product over the ragged levels; ``residual`` in ``forward`` is added in the output projection's
+epilogue.
 """
 from __future__ import annotations
 
@@ -24,6 +28,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from .flash_deform_attn import FlashDeformAttnFunction
+from .linear import GroupedLinear, fused_linear, like
 
 
 class PackSamplingFunction(Function):
@@ -113,7 +118,7 @@ def project_and_pack(query, reference_points, w_offsets, b_offsets, w_logits, b_
 
 class MSDeformAttn3D(nn.Module):
     def __init__(self, d_model: int = 256, n_levels: int = 3, n_heads: int = 8, n_points: int = 4, im2col_step: int = 64,
-                 fused_projection: bool = True):
+                 fused_projection: bool = True, level_value_proj: bool = False):
         super().__init__()
         if d_model % n_heads:
             raise ValueError("d_model must be divisible by n_heads")
@@ -124,7 +129,8 @@ class MSDeformAttn3D(nn.Module):
         self.fused_projection = fused_projection  # packing inside the projection GEMM (CUDA); else projections + pack kernel
         self.sampling_offsets = nn.Linear(d_model, n_heads * n_levels * n_points * 3)
         self.attention_weights = nn.Linear(d_model, n_heads * n_levels * n_points)
-        self.value_proj = nn.Linear(d_model, d_model)
+        self.level_value_proj = level_value_proj  # a value projection per level: value_proj.weight [L, d_model, d_model]
+        self.value_proj = GroupedLinear(n_levels, d_model, d_model) if level_value_proj else nn.Linear(d_model, d_model)
         self.output_proj = nn.Linear(d_model, d_model)
         self._reset_parameters()
 
@@ -142,16 +148,17 @@ class MSDeformAttn3D(nn.Module):
             self.sampling_offsets.bias.copy_(grid.reshape(-1))
         nn.init.constant_(self.attention_weights.weight, 0.0)
         nn.init.constant_(self.attention_weights.bias, 0.0)
-        nn.init.xavier_uniform_(self.value_proj.weight)
-        nn.init.constant_(self.value_proj.bias, 0.0)
+        if not self.level_value_proj:  # GroupedLinear starts the same way, level by level
+            nn.init.xavier_uniform_(self.value_proj.weight)
+            nn.init.constant_(self.value_proj.bias, 0.0)
         nn.init.xavier_uniform_(self.output_proj.weight)
         nn.init.constant_(self.output_proj.bias, 0.0)
 
-    def forward(self, query, reference_points, input_flatten, spatial_shapes, level_start_index, input_padding_mask=None):
+    def forward(self, query, reference_points, input_flatten, spatial_shapes, level_start_index, input_padding_mask=None, residual=None):
         B, Q, _ = query.shape
         _, N, _ = input_flatten.shape
         G, L, K = self.n_heads, self.n_levels, self.n_points
-        value = self.value_proj(input_flatten)
+        value = self.value_proj(input_flatten, level_start_index) if self.level_value_proj else self.value_proj(input_flatten)
         if input_padding_mask is not None:
             value = value.masked_fill(input_padding_mask[..., None], 0.0)
         value = value.view(B, N, G, self.d_model // G).contiguous()
@@ -163,4 +170,6 @@ class MSDeformAttn3D(nn.Module):
             logits = self.attention_weights(query).view(B, Q, G, L, K)
             packed = PackSamplingFunction.apply(offsets, reference_points, logits, spatial_shapes)
         out = FlashDeformAttnFunction.apply(value, spatial_shapes, level_start_index, packed, self.im2col_step, K, True)
-        return self.output_proj(out)
+        if residual is None:
+            return self.output_proj(out)
+        return fused_linear(out, like(out, self.output_proj.weight), like(out, self.output_proj.bias), residual)
