@@ -437,8 +437,8 @@ int fda_nms3d_scored(const float *boxes, long long box_stride, long long coord_s
  *
  *   x [batch][rows][in_features]   weight [groups][out_features][in_features]   bias [groups][out_features] or NULL
  *   residual, y, grad_output [batch][rows][out_features]   residual or NULL; its gradient is grad_output
- * all of `dtype`; sums in fp32, one rounding at the end.  Any sizes of at least one feature and any
- * element-aligned addresses; rows * batch < 2^31.
+ * all of `dtype`; sums in fp32, one rounding at the end.  Any sizes of at least one feature; rows * batch < 2^31.
+ * 16-bit x, weight and grad_output start on 16-byte boundaries (FDA_ERR_MISALIGNED), the rest anywhere.
  *
  * group_start_index NULL: one group of all rows (groups = 1).  Else int64 on the device, num_starts = groups or groups + 1
  * entries: group e holds the rows group_start_index[e] <= m < group_start_index[e + 1] of every batch element (the last ends

@@ -439,6 +439,12 @@ void check_linear_operand(const at::Tensor &t, const at::Tensor &x, const char *
     TORCH_CHECK(t.scalar_type() == x.scalar_type(), name, " must have the dtype of x, ", x.scalar_type(), ", got ", t.scalar_type());
 }
 
+// Dense and on a 16-byte boundary, a copy where it is not.
+at::Tensor dense(const at::Tensor &t) {
+    const at::Tensor c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+}
+
 LinearArgs check_linear(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &bias, const at::Tensor &starts) {
     LinearArgs a;
     TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (this operator has no CPU implementation)");
@@ -468,8 +474,8 @@ LinearArgs check_linear(const at::Tensor &x, const at::Tensor &weight, const at:
     }
     TORCH_CHECK(in <= INT32_MAX && out <= INT32_MAX && groups <= INT32_MAX && batch <= INT32_MAX && rows <= INT32_MAX,
                 "linear: too large dimension");
-    a.x = x.contiguous();
-    a.weight = weight.contiguous();
+    a.x = dense(x);
+    a.weight = dense(weight);
     if (bias.defined()) a.bias = bias.contiguous();
     a.batch = (int)batch; a.rows = (int)rows; a.groups = (int)groups; a.in = (int)in; a.out = (int)out;
     a.num_starts = grouped ? (int)starts.size(0) : 0;
@@ -511,7 +517,7 @@ std::array<at::Tensor, 3> linear_backward_impl(const at::Tensor &x, const at::Te
     TORCH_CHECK(grad_output.sizes() == at::IntArrayRef(a.out_size), "grad_output must have the shape of the output, ",
                 at::IntArrayRef(a.out_size), ", got ", grad_output.sizes());
     c10::cuda::CUDAGuard guard(x.device());
-    const at::Tensor grad = grad_output.contiguous();
+    const at::Tensor grad = dense(grad_output);
     std::array<at::Tensor, 3> out;
     if (need_x) out[0] = empty_on(x, x.sizes(), x.scalar_type());
     if (need_weight) out[1] = empty_on(x, weight.sizes(), x.scalar_type());

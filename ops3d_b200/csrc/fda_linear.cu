@@ -1,5 +1,5 @@
 // Linear layers with bias, activation and residual in the product's epilogue, for one weight or one weight per ragged group of
-// rows: C ABI, and the kernels on the plain fp32 pipes, which take every type, size and alignment.
+// rows: C ABI, and the fp32 kernels.  16-bit products are in fda_linear_mma.cu.
 #include <algorithm>
 
 #include "fda_config.h"
@@ -8,10 +8,6 @@
 namespace {
 
 using namespace fda_linear;
-
-constexpr int kSms = 148;
-
-enum Mode { kForward, kPreGrad, kGradX };
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // Products on the fp32 pipes
@@ -230,21 +226,11 @@ __global__ void __launch_bounds__(kThreads) linear_weight_grad_sum_kernel(const 
 // ---------------------------------------------------------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------------------------------------------------------
-inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
-inline size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 inline size_t type_size(int dtype) { return dtype == FDA_DTYPE_F32 ? 4 : 2; }
 
-// Upper bounds that hold whatever the start indices are: every group adds at most one incomplete unit per batch element.
-inline long long most_units(int batch, int rows, int groups, int unit, bool rest) {
-    const long long sections = groups + (rest ? 2 : 0);
-    return (long long)batch * std::min<long long>(rows, rows / unit + sections);
-}
+}  // namespace
 
-// How the rows of the weight's gradient are cut (PieceTable).
-struct Cut {
-    int block, piece;
-    long long pieces, slots;  // at most
-};
+namespace fda_linear {
 
 Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int least_piece) {
     Cut c;
@@ -258,6 +244,10 @@ Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int le
     c.slots = blocks <= c.piece ? 0 : std::min(c.pieces, 2 * (blocks / c.piece) + 1);
     return c;
 }
+
+}  // namespace fda_linear
+
+namespace {
 
 struct Shape {
     int batch, rows, groups, in_features, out_features, dtype;
@@ -286,11 +276,6 @@ int launched() {
 constexpr int kTileSize = 64;
 constexpr int kPlainBlock = 64, kPlainLeastPiece = 4;
 
-Cut plain_cut(const Shape &s) {
-    return cut_rows(s.batch, s.rows, s.groups, ceil_div(s.out_features, kTileSize) * ceil_div(s.in_features, kTileSize), kPlainBlock,
-                    kPlainLeastPiece);
-}
-
 template <typename T, int kMode, int kAct>
 int run_rows_plain(const RowProduct<T> &p, cudaStream_t st) {
     const long long tiles = most_units(p.g.batch, p.g.rows, p.g.groups, kTileSize, kMode != kPreGrad) * ceil_div(p.cols, kTileSize);
@@ -309,92 +294,193 @@ int run_rows(const RowProduct<T> &p, int activation, cudaStream_t st) {
     }
 }
 
-template <typename T>
-int forward(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *residual, void *y,
-            int activation, cudaStream_t st) {
-    RowProduct<T> p;
-    p.a = static_cast<const T *>(x);
-    p.w = static_cast<const T *>(weight);
-    p.bias = static_cast<const T *>(bias);
-    p.extra = static_cast<const T *>(residual);
-    p.out = static_cast<T *>(y);
-    p.depth = p.in_features = s.in_features;
-    p.cols = s.out_features;
-    p.g = g;
-    return run_rows<T, kForward>(p, activation, st);
+// 16-bit operands whose rows do not start on 16-byte boundaries are copied to rows that do.
+__global__ void __launch_bounds__(kThreads) linear_pad_kernel(const unsigned short *__restrict__ src, unsigned short *__restrict__ dst,
+                                                              unsigned long long elements, int line, int pitch) {
+    const unsigned long long step = (unsigned long long)gridDim.x * kThreads;
+    for (unsigned long long i = (unsigned long long)blockIdx.x * kThreads + threadIdx.x; i < elements; i += step)
+        dst[i / (unsigned)line * (unsigned)pitch + i % (unsigned)line] = src[i];
 }
 
-// Workspace of the backward: g (with an activation), then the slots.
-struct BackwardLayout {
-    size_t g = 0, slots = 0, bias_slots = 0, total = 0;
+inline int padded(int line) { return (line + 7) & ~7; }
+
+// src itself where its rows are aligned, else a padded copy in `place`; launches the copy.
+int aligned_rows(const void *&src, char *place, size_t rows, int line, cudaStream_t st) {
+    if (line % 8 == 0) return FDA_OK;
+    const unsigned long long elements = (unsigned long long)rows * line;
+    const unsigned blocks = (unsigned)std::min<unsigned long long>((elements + kThreads - 1) / kThreads, 16 * kSms);
+    linear_pad_kernel<<<blocks, kThreads, 0, st>>>(static_cast<const unsigned short *>(src), reinterpret_cast<unsigned short *>(place),
+                                                   elements, line, padded(line));
+    src = place;
+    return launched();
+}
+
+// What the workspaces hold, one behind the other.
+struct Layout {
+    size_t x = 0, w = 0, g = 0, slots = 0, bias_slots = 0, total = 0;
+    size_t take(size_t bytes) {
+        const size_t at = total;
+        total += round256(bytes);
+        return at;
+    }
 };
 
-BackwardLayout backward_layout(const Shape &s, int activation) {
-    BackwardLayout l;
-    size_t at = 0;
-    if (activation != FDA_ACT_NONE) at += round256((size_t)s.batch * s.rows * s.out_features * type_size(s.dtype));
-    const Cut c = plain_cut(s);
-    l.slots = at;
-    at += round256((size_t)c.slots * s.out_features * s.in_features * sizeof(float));
-    l.bias_slots = at;
-    at += round256((size_t)c.slots * s.out_features * sizeof(float));
-    l.total = at;
+size_t total_rows(const Shape &s) { return (size_t)s.batch * s.rows; }
+
+void add_padded_operands(Layout &l, const Shape &s) {
+    if (s.dtype == FDA_DTYPE_F32 || s.in_features % 8 == 0) return;
+    l.x = l.take(total_rows(s) * padded(s.in_features) * 2);
+    l.w = l.take((size_t)s.groups * s.out_features * padded(s.in_features) * 2);
+}
+
+Cut weight_cut(const Shape &s) {
+    if (s.dtype != FDA_DTYPE_F32) return mma_cut(s.batch, s.rows, s.groups, s.in_features, s.out_features);
+    return cut_rows(s.batch, s.rows, s.groups, ceil_div(s.out_features, kTileSize) * ceil_div(s.in_features, kTileSize), kPlainBlock,
+                    kPlainLeastPiece);
+}
+
+Layout forward_layout(const Shape &s) {
+    Layout l;
+    add_padded_operands(l, s);
     return l;
 }
 
+// g: the pre-activation's gradient, or a padded copy of grad_output.
+Layout backward_layout(const Shape &s, int activation) {
+    Layout l;
+    add_padded_operands(l, s);
+    const bool narrow = s.dtype != FDA_DTYPE_F32;
+    if (activation != FDA_ACT_NONE || (narrow && s.out_features % 8))
+        l.g = l.take(total_rows(s) * (narrow ? padded(s.out_features) : s.out_features) * type_size(s.dtype));
+    const Cut c = weight_cut(s);
+    l.slots = l.take((size_t)c.slots * s.out_features * s.in_features * sizeof(float));
+    l.bias_slots = l.take((size_t)c.slots * s.out_features * sizeof(float));
+    return l;
+}
+
+int forward_f32(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *residual, void *y,
+                int activation, cudaStream_t st) {
+    RowProduct<float> p;
+    p.a = static_cast<const float *>(x);
+    p.w = static_cast<const float *>(weight);
+    p.bias = static_cast<const float *>(bias);
+    p.extra = static_cast<const float *>(residual);
+    p.out = static_cast<float *>(y);
+    p.depth = p.in_features = s.in_features;
+    p.cols = s.out_features;
+    p.g = g;
+    return run_rows<float, kForward>(p, activation, st);
+}
+
+int forward_narrow(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *residual, void *y,
+                   char *ws, int activation, cudaStream_t st) {
+    const Layout l = forward_layout(s);
+    if (const int rc = aligned_rows(x, ws + l.x, total_rows(s), s.in_features, st)) return rc;
+    if (const int rc = aligned_rows(weight, ws + l.w, (size_t)s.groups * s.out_features, s.in_features, st)) return rc;
+    const long long in = padded(s.in_features);
+    const MmaRows p{x, weight, bias, residual, y, in, in, s.out_features, s.out_features, s.in_features, s.out_features, s.dtype, activation, g};
+    return mma_rows(kForward, p, st);
+}
+
+struct Gradients {
+    void *x, *weight, *bias;
+};
+
 template <typename T>
-int backward(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *grad_output, void *grad_x,
-             void *grad_weight, void *grad_bias, char *ws, int activation, cudaStream_t st) {
-    const BackwardLayout l = backward_layout(s, activation);
-    const T *grad = static_cast<const T *>(grad_output);
-    RowProduct<T> p;
-    p.w = static_cast<const T *>(weight);
-    p.bias = static_cast<const T *>(bias);
+int sum_slots(const WeightGrad<T> &q, const Shape &s, const Cut &c, cudaStream_t st) {
+    if (c.slots == 0) return FDA_OK;
+    const size_t elements = ((size_t)s.in_features + 1) * s.out_features;
+    const dim3 grid((unsigned)std::min<size_t>((elements + kThreads - 1) / kThreads, 4 * kSms), (unsigned)std::min(s.groups, 256));
+    linear_weight_grad_sum_kernel<T><<<grid, kThreads, 0, st>>>(q);
+    return launched();
+}
+
+template <typename T>
+WeightGrad<T> weight_grad_args(const Shape &s, const Groups &g, const Cut &c, const void *grad, const void *x, const Gradients &out,
+                               char *ws, const Layout &l) {
+    WeightGrad<T> q;
+    q.grad = static_cast<const T *>(grad);
+    q.x = static_cast<const T *>(x);
+    q.grad_weight = static_cast<T *>(out.weight);
+    q.grad_bias = static_cast<T *>(out.bias);
+    q.slots = reinterpret_cast<float *>(ws + l.slots);
+    q.bias_slots = reinterpret_cast<float *>(ws + l.bias_slots);
+    q.in_features = s.in_features;
+    q.out_features = s.out_features;
+    q.block = c.block;
+    q.piece = c.piece;
+    q.g = g;
+    return q;
+}
+
+int backward_f32(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *grad_output,
+                 const Gradients &out, char *ws, int activation, cudaStream_t st) {
+    const Layout l = backward_layout(s, activation);
+    RowProduct<float> p;
+    p.w = static_cast<const float *>(weight);
+    p.bias = static_cast<const float *>(bias);
     p.in_features = s.in_features;
     p.g = g;
+    const float *grad = static_cast<const float *>(grad_output);
     if (activation != FDA_ACT_NONE) {
-        p.a = static_cast<const T *>(x);
+        p.a = static_cast<const float *>(x);
         p.extra = grad;
-        p.out = reinterpret_cast<T *>(ws + l.g);
+        p.out = reinterpret_cast<float *>(ws + l.g);
         p.depth = s.in_features;
         p.cols = s.out_features;
-        if (const int rc = run_rows<T, kPreGrad>(p, activation, st)) return rc;
+        if (const int rc = run_rows<float, kPreGrad>(p, activation, st)) return rc;
         grad = p.out;
     }
-    if (grad_x) {
+    if (out.x) {
         p.a = grad;
         p.bias = p.extra = nullptr;
-        p.out = static_cast<T *>(grad_x);
+        p.out = static_cast<float *>(out.x);
         p.depth = s.out_features;
         p.cols = s.in_features;
-        if (const int rc = run_rows<T, kGradX>(p, FDA_ACT_NONE, st)) return rc;
+        if (const int rc = run_rows<float, kGradX>(p, FDA_ACT_NONE, st)) return rc;
     }
-    if (grad_weight || grad_bias) {
-        const Cut c = plain_cut(s);
-        WeightGrad<T> q;
-        q.grad = grad;
-        q.x = static_cast<const T *>(x);
-        q.grad_weight = static_cast<T *>(grad_weight);
-        q.grad_bias = static_cast<T *>(grad_bias);
-        q.slots = reinterpret_cast<float *>(ws + l.slots);
-        q.bias_slots = reinterpret_cast<float *>(ws + l.bias_slots);
-        q.in_features = s.in_features;
-        q.out_features = s.out_features;
-        q.block = c.block;
-        q.piece = c.piece;
-        q.g = g;
-        const long long items = c.pieces * ceil_div(s.out_features, kTileSize) * ceil_div(s.in_features, kTileSize);
-        linear_weight_grad_kernel<T, kTileSize, kTileSize><<<(unsigned)std::min<long long>(items, 8 * kSms), kThreads, 0, st>>>(q);
-        if (const int rc = launched()) return rc;
-        if (c.slots > 0) {
-            const size_t elements = ((size_t)s.in_features + 1) * s.out_features;
-            const dim3 grid((unsigned)std::min<size_t>((elements + kThreads - 1) / kThreads, 4 * kSms), (unsigned)std::min(s.groups, 256));
-            linear_weight_grad_sum_kernel<T><<<grid, kThreads, 0, st>>>(q);
-            if (const int rc = launched()) return rc;
-        }
-    }
-    return FDA_OK;
+    if (!out.weight && !out.bias) return FDA_OK;
+    const Cut c = weight_cut(s);
+    const WeightGrad<float> q = weight_grad_args<float>(s, g, c, grad, x, out, ws, l);
+    const long long items = c.pieces * ceil_div(s.out_features, kTileSize) * ceil_div(s.in_features, kTileSize);
+    linear_weight_grad_kernel<float, kTileSize, kTileSize><<<(unsigned)std::min<long long>(items, 8 * kSms), kThreads, 0, st>>>(q);
+    if (const int rc = launched()) return rc;
+    return sum_slots(q, s, c, st);
 }
+
+int backward_narrow(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *grad_output,
+                    const Gradients &out, char *ws, int activation, cudaStream_t st) {
+    const Layout l = backward_layout(s, activation);
+    const bool weights = out.weight || out.bias;
+    const long long in = padded(s.in_features), outs = padded(s.out_features);
+    if (activation != FDA_ACT_NONE || weights)
+        if (const int rc = aligned_rows(x, ws + l.x, total_rows(s), s.in_features, st)) return rc;
+    if (activation != FDA_ACT_NONE || out.x)
+        if (const int rc = aligned_rows(weight, ws + l.w, (size_t)s.groups * s.out_features, s.in_features, st)) return rc;
+    const void *grad = grad_output;
+    if (activation != FDA_ACT_NONE) {
+        const MmaRows p{x, weight, bias, grad_output, ws + l.g, in, in, s.out_features, outs, s.in_features, s.out_features, s.dtype,
+                        activation, g};
+        if (const int rc = mma_rows(kPreGrad, p, st)) return rc;
+        grad = ws + l.g;
+    } else if (const int rc = aligned_rows(grad, ws + l.g, total_rows(s), s.out_features, st)) {
+        return rc;
+    }
+    if (out.x) {
+        const MmaRows p{grad, weight, nullptr, nullptr, out.x, outs, in, 0, s.in_features, s.in_features, s.out_features, s.dtype,
+                        FDA_ACT_NONE, g};
+        if (const int rc = mma_rows(kGradX, p, st)) return rc;
+    }
+    if (!weights) return FDA_OK;
+    const Cut c = weight_cut(s);
+    const MmaWeightGrad q{grad, x, outs, in, out.weight, out.bias, reinterpret_cast<float *>(ws + l.slots),
+                          reinterpret_cast<float *>(ws + l.bias_slots), s.in_features, s.out_features, s.dtype, c, g};
+    if (const int rc = mma_weight_grad(q, st)) return rc;
+    if (s.dtype == FDA_DTYPE_F16) return sum_slots(weight_grad_args<__half>(s, g, c, nullptr, nullptr, out, ws, l), s, c, st);
+    return sum_slots(weight_grad_args<__nv_bfloat16>(s, g, c, nullptr, nullptr, out, ws, l), s, c, st);
+}
+
+bool misaligned16(const void *p) { return (uintptr_t)p % 16 != 0; }
 
 }  // namespace
 
@@ -402,8 +488,7 @@ extern "C" {
 
 size_t fda_linear_forward_workspace_bytes(int batch, int rows, int groups, int in_features, int out_features, int dtype) {
     const Shape s{batch, rows, groups, in_features, out_features, dtype};
-    if (check_shape(s) != FDA_OK) return 0;
-    return 0;
+    return check_shape(s) == FDA_OK ? forward_layout(s).total : 0;
 }
 
 int fda_linear_forward(const void *x, const void *weight, const void *bias, const void *residual, const int64_t *group_start_index,
@@ -415,17 +500,19 @@ int fda_linear_forward(const void *x, const void *weight, const void *bias, cons
     if (const int rc = check_groups(s, group_start_index, num_starts)) return rc;
     if (batch == 0 || rows == 0) return FDA_OK;
     if (!x || !weight || !y) return FDA_ERR_NULL_POINTER;
+    const size_t need = forward_layout(s).total;
+    if (need > 0 && (!workspace || workspace_bytes < need)) return FDA_ERR_WORKSPACE;
+    if ((uintptr_t)workspace % 256) return FDA_ERR_MISALIGNED;
     const Groups g{group_start_index, num_starts, groups, batch, rows};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == FDA_DTYPE_F32) return forward<float>(s, g, x, weight, bias, residual, y, activation, st);
-    if (dtype == FDA_DTYPE_F16) return forward<__half>(s, g, x, weight, bias, residual, y, activation, st);
-    return forward<__nv_bfloat16>(s, g, x, weight, bias, residual, y, activation, st);
+    if (dtype == FDA_DTYPE_F32) return forward_f32(s, g, x, weight, bias, residual, y, activation, st);
+    if (misaligned16(x) || misaligned16(weight)) return FDA_ERR_MISALIGNED;
+    return forward_narrow(s, g, x, weight, bias, residual, y, static_cast<char *>(workspace), activation, st);
 }
 
 size_t fda_linear_backward_workspace_bytes(int batch, int rows, int groups, int in_features, int out_features, int activation, int dtype) {
     const Shape s{batch, rows, groups, in_features, out_features, dtype};
-    if (check_shape(s) != FDA_OK) return 0;
-    return backward_layout(s, activation).total;
+    return check_shape(s) == FDA_OK ? backward_layout(s, activation).total : 0;
 }
 
 int fda_linear_backward(const void *x, const void *weight, const void *bias, const void *grad_output, const int64_t *group_start_index,
@@ -449,14 +536,13 @@ int fda_linear_backward(const void *x, const void *weight, const void *bias, con
     if (need > 0 && (!workspace || workspace_bytes < need)) return FDA_ERR_WORKSPACE;
     if ((uintptr_t)workspace % 256) return FDA_ERR_MISALIGNED;
     const Groups g{group_start_index, num_starts, groups, batch, rows};
+    const Gradients out{grad_x, grad_weight, grad_bias};
     char *ws = static_cast<char *>(workspace);
-    if (dtype == FDA_DTYPE_F32)
-        return backward<float>(s, g, x, weight, bias, grad_output, grad_x, grad_weight, grad_bias, ws, activation, st);
-    if (dtype == FDA_DTYPE_F16)
-        return backward<__half>(s, g, x, weight, bias, grad_output, grad_x, grad_weight, grad_bias, ws, activation, st);
-    return backward<__nv_bfloat16>(s, g, x, weight, bias, grad_output, grad_x, grad_weight, grad_bias, ws, activation, st);
+    if (dtype == FDA_DTYPE_F32) return backward_f32(s, g, x, weight, bias, grad_output, out, ws, activation, st);
+    if (misaligned16(x) || misaligned16(weight) || misaligned16(grad_output)) return FDA_ERR_MISALIGNED;
+    return backward_narrow(s, g, x, weight, bias, grad_output, out, ws, activation, st);
 }
 
-int fda_linear_timeouts(void) { return 0; }
+int fda_linear_timeouts(void) { return mma_timeouts(); }
 
 }  // extern "C"

@@ -221,4 +221,56 @@ __device__ __forceinline__ void block_rows(const Groups &g, const int *start, in
     count = min(block, start[e + 1] - first);
 }
 
+// ---- host -------------------------------------------------------------------------------------------------------------------
+inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+inline size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+constexpr int kSms = 148;
+
+// Upper bound of a row table's units, whatever the start indices are: every section adds at most one incomplete unit per batch
+// element.
+inline long long most_units(int batch, int rows, int groups, int unit, bool rest) {
+    const long long sections = groups + (rest ? 2 : 0);
+    return (long long)batch * (rows < rows / unit + sections ? rows : rows / unit + sections);
+}
+
+// How the rows of the weight's gradient are cut (PieceTable).
+struct Cut {
+    int block, piece;
+    long long pieces, slots;  // at most
+};
+
+// What a product over row units does with its sums (run_rows, mma_rows).
+enum Mode {
+    kForward,  // out = act(a W^T + bias) + extra
+    kPreGrad,  // out = extra * act'(a W^T + bias)
+    kGradX     // out = a W
+};
+
+// 16-bit products on the tensor cores (fda_linear_mma.cu).  Rows of a and of w start on 16-byte boundaries: their pitches (in
+// elements) are multiples of 8.
+struct MmaRows {
+    const void *a, *w, *bias, *extra;
+    void *out;
+    long long a_pitch, w_pitch, extra_pitch, out_pitch;
+    int in_features, out_features, dtype, activation;
+    Groups g;
+};
+int mma_rows(int mode, const MmaRows &p, cudaStream_t st);
+
+struct MmaWeightGrad {
+    const void *grad, *x;
+    long long grad_pitch, x_pitch;
+    void *grad_weight, *grad_bias;  // either may be nullptr
+    float *slots, *bias_slots;
+    int in_features, out_features, dtype;
+    Cut cut;
+    Groups g;
+};
+// At most two pieces per SM over `tiles` tiles of the weight, none shorter than `least_piece` blocks.
+Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int least_piece);
+Cut mma_cut(int batch, int rows, int groups, int in_features, int out_features);
+int mma_weight_grad(const MmaWeightGrad &p, cudaStream_t st);  // without the sum over slots
+int mma_timeouts();
+
 }  // namespace fda_linear

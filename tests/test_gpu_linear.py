@@ -356,6 +356,30 @@ def test_repeats_are_equal_and_streams_are_kept():
             assert torch.equal(g, first[n]), n
 
 
+def test_calls_from_a_thread_that_has_not_used_the_device():
+    import threading
+
+    x, w, b, r, dy = make((200,), 64, 72, torch.bfloat16, seed=16)
+    want, grads = check(x, w, b, r, dy, "none")
+    got = []
+
+    def call():
+        from ops3d_b200 import _C
+
+        try:
+            got.append(_C.linear_forward(x, w, b, r, None, 0))
+            got.extend(_C.linear_backward(x, w, b, None, dy, 0, True, True, True))
+        except RuntimeError as e:
+            got.append(e)
+
+    thread = threading.Thread(target=call)
+    thread.start()
+    thread.join()
+    assert len(got) == 4 and not isinstance(got[-1], RuntimeError), got[-1]
+    for a, e in zip(got, (want, grads["x"], grads["weight"], grads["bias"])):
+        assert torch.equal(a, e)
+
+
 def test_captured_training_pass_follows_its_inputs():
     """One graph of forward and backward; inputs and group boundaries change between replays.  No eager graph of the same leaves may
     live meanwhile: torch ties a leaf's accumulation node to the stream of its first use, and a capture that meets the default
