@@ -1,5 +1,5 @@
 // Linear layers with bias, activation and residual in the product's epilogue, for one weight or one weight per ragged group of
-// rows: C ABI, and the fp32 kernels.  16-bit products are in fda_linear_mma.cu.
+// rows: C ABI, and the fp32 kernels.  16-bit products are in fda_linear_mma_kernels.cuh.
 #include <algorithm>
 
 #include "fda_config.h"
@@ -200,25 +200,64 @@ __global__ void __launch_bounds__(kThreads) linear_weight_grad_kernel(const Weig
     }
 }
 
-// Adds the slots of the groups that were computed in pieces, in the order of their rows.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) linear_weight_grad_sum_kernel(const WeightGrad<T> p) {
+// Adds the slots of the groups that were computed in pieces, in order.  A block takes 1024 elements of a group's slots, or with
+// kSplit 128, whose slots its eight warps share and whose eight sums are added in order: for many slots, where a thread's
+// chain of loads would be the time (148 slots of 256 x 256: 28 us in one chain, 11 in eight; 40 slots of 16 groups 27 us against 84).
+constexpr int kSumWarps = 8, kLaneElements = 4;
+
+template <typename T, bool kSplit>
+__global__ void __launch_bounds__(32 * kSumWarps) linear_weight_grad_sum_kernel(const WeightGrad<T> p) {
     __shared__ PieceTable table;
+    __shared__ float partial[kSplit ? kSumWarps : 1][32 * kLaneElements];
     build_piece_table(p.g, p.block, p.piece, table);
     __syncthreads();
-    const size_t size = (size_t)p.out_features * p.in_features;
-    for (int e = blockIdx.y; e < p.g.groups; e += gridDim.y) {
+    const size_t size = (size_t)p.out_features * p.in_features, both = size + p.out_features;
+    constexpr int kEach = 32 * kLaneElements * (kSplit ? 1 : kSumWarps);
+    const long long blocks = (long long)((both + kEach - 1) / kEach);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    for (long long item = blockIdx.x; item < blocks * p.g.groups; item += gridDim.x) {
+        const int e = (int)(item / blocks);
         const int first = table.slot_begin[e], count = table.slot_begin[e + 1] - first;
         if (count == 0) continue;
-        for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < size + p.out_features; i += (size_t)gridDim.x * kThreads) {
+        const size_t base = (size_t)(item % blocks) * kEach + (kSplit ? 0 : warp * 32 * kLaneElements) + lane;
+        float sum[kLaneElements] = {};
+        // weights: element i of slot s at slots[s * size + i]; biases behind them, in slots of their own
+        const float *src[kLaneElements];
+        size_t step[kLaneElements];
+#pragma unroll
+        for (int j = 0; j < kLaneElements; ++j) {
+            const size_t i = base + 32 * j;
             const bool weight = i < size;
-            if (!(weight ? p.grad_weight : p.grad_bias)) continue;
-            const float *src = weight ? p.slots + first * size + i : p.bias_slots + (size_t)first * p.out_features + (i - size);
-            const size_t step = weight ? size : (size_t)p.out_features;
-            float sum = 0.f;
-            for (int s = 0; s < count; ++s) sum += src[s * step];
-            if (weight) p.grad_weight[e * size + i] = from_f32<T>(sum);
-            else p.grad_bias[(size_t)e * p.out_features + (i - size)] = from_f32<T>(sum);
+            step[j] = weight ? size : (size_t)p.out_features;
+            src[j] = weight ? p.slots + first * size + i : p.bias_slots + (size_t)first * p.out_features + (i - size);
+            if (i >= both || !(weight ? p.grad_weight : p.grad_bias)) src[j] = nullptr;
+        }
+#pragma unroll 4
+        for (int s = kSplit ? warp : 0; s < count; s += kSplit ? kSumWarps : 1)
+#pragma unroll
+            for (int j = 0; j < kLaneElements; ++j)
+                if (src[j]) sum[j] += src[j][s * step[j]];
+        const auto put = [&](size_t i, float total) {
+            if (i < size) {
+                if (p.grad_weight) p.grad_weight[e * size + i] = from_f32<T>(total);
+            } else if (i < both && p.grad_bias) {
+                p.grad_bias[(size_t)e * p.out_features + (i - size)] = from_f32<T>(total);
+            }
+        };
+        if constexpr (!kSplit) {
+#pragma unroll
+            for (int j = 0; j < kLaneElements; ++j) put(base + 32 * j, sum[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kLaneElements; ++j) partial[warp][32 * j + lane] = sum[j];
+            __syncthreads();
+            if (warp < kLaneElements) {
+                float total = 0.f;
+#pragma unroll
+                for (int w = 0; w < kSumWarps; ++w) total += partial[w][32 * warp + lane];
+                put(base + 32 * warp, total);
+            }
+            __syncthreads();
         }
     }
 }
@@ -236,9 +275,11 @@ Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int le
     Cut c;
     c.block = block;
     const long long blocks = std::max<long long>(1, most_units(batch, rows, groups, block, false));
-    // pieces enough for two per SM, but none so short that writing its sums costs more than making them
-    const long long wanted = std::max<long long>(1, ceil_div(2 * kSms, tiles));
-    c.piece = (int)std::max<long long>(least_piece, ceil_div(blocks, wanted));
+    // As many pieces as the SMs take at once: one more would be a round of its own.  Every further group can add a piece that is
+    // not full; where there are too many groups for that, pieces half as long, so that the last round is short.
+    const long long wanted = std::max<long long>(1, kSms / tiles);
+    const long long full = wanted >= 2 * groups ? wanted - (groups - 1) : 2 * wanted;
+    c.piece = (int)std::max<long long>(least_piece, ceil_div(blocks, full));
     c.pieces = ceil_div(blocks, c.piece) + groups;
     // a group of n > 1 pieces has more than (n - 1) * piece blocks, so at least n / 2 * piece
     c.slots = blocks <= c.piece ? 0 : std::min(c.pieces, 2 * (blocks / c.piece) + 1);
@@ -325,6 +366,13 @@ struct Layout {
     }
 };
 
+int mma_rows(int mode, const MmaRows &p, cudaStream_t st) {
+    return p.dtype == FDA_DTYPE_F16 ? mma_rows_f16(mode, p, st) : mma_rows_bf16(mode, p, st);
+}
+int mma_weight_grad(const MmaWeightGrad &p, cudaStream_t st) {
+    return p.dtype == FDA_DTYPE_F16 ? mma_weight_grad_f16(p, st) : mma_weight_grad_bf16(p, st);
+}
+
 size_t total_rows(const Shape &s) { return (size_t)s.batch * s.rows; }
 
 void add_padded_operands(Layout &l, const Shape &s) {
@@ -334,7 +382,10 @@ void add_padded_operands(Layout &l, const Shape &s) {
 }
 
 Cut weight_cut(const Shape &s) {
-    if (s.dtype != FDA_DTYPE_F32) return mma_cut(s.batch, s.rows, s.groups, s.in_features, s.out_features);
+    if (s.dtype != FDA_DTYPE_F32) {
+        const long long tiles = ceil_div(s.out_features, kMmaTileRows) * ceil_div(s.in_features, mma_weight_tile(s.in_features));
+        return cut_rows(s.batch, s.rows, s.groups, tiles, kMmaSlice, 8);
+    }
     return cut_rows(s.batch, s.rows, s.groups, ceil_div(s.out_features, kTileSize) * ceil_div(s.in_features, kTileSize), kPlainBlock,
                     kPlainLeastPiece);
 }
@@ -389,9 +440,11 @@ struct Gradients {
 template <typename T>
 int sum_slots(const WeightGrad<T> &q, const Shape &s, const Cut &c, cudaStream_t st) {
     if (c.slots == 0) return FDA_OK;
-    const size_t elements = ((size_t)s.in_features + 1) * s.out_features;
-    const dim3 grid((unsigned)std::min<size_t>((elements + kThreads - 1) / kThreads, 4 * kSms), (unsigned)std::min(s.groups, 256));
-    linear_weight_grad_sum_kernel<T><<<grid, kThreads, 0, st>>>(q);
+    const bool split = c.pieces > 16ll * s.groups;
+    const long long items = ceil_div(((long long)s.in_features + 1) * s.out_features, 32 * kLaneElements * (split ? 1 : kSumWarps)) * s.groups;
+    const unsigned blocks = (unsigned)std::min<long long>(items, 4 * kSms);
+    if (split) linear_weight_grad_sum_kernel<T, true><<<blocks, 32 * kSumWarps, 0, st>>>(q);
+    else linear_weight_grad_sum_kernel<T, false><<<blocks, 32 * kSumWarps, 0, st>>>(q);
     return launched();
 }
 
@@ -543,6 +596,9 @@ int fda_linear_backward(const void *x, const void *weight, const void *bias, con
     return backward_narrow(s, g, x, weight, bias, grad_output, out, ws, activation, st);
 }
 
-int fda_linear_timeouts(void) { return mma_timeouts(); }
+int fda_linear_timeouts(void) {
+    const int a = mma_timeouts_f16(), b = mma_timeouts_bf16();
+    return a < 0 || b < 0 ? -1 : a + b;
+}
 
 }  // extern "C"

@@ -247,7 +247,7 @@ enum Mode {
     kGradX     // out = a W
 };
 
-// 16-bit products on the tensor cores (fda_linear_mma.cu).  Rows of a and of w start on 16-byte boundaries: their pitches (in
+// 16-bit products on the tensor cores (fda_linear_mma_kernels.cuh).  Rows of a and of w start on 16-byte boundaries: their pitches (in
 // elements) are multiples of 8.
 struct MmaRows {
     const void *a, *w, *bias, *extra;
@@ -256,7 +256,8 @@ struct MmaRows {
     int in_features, out_features, dtype, activation;
     Groups g;
 };
-int mma_rows(int mode, const MmaRows &p, cudaStream_t st);
+int mma_rows_f16(int mode, const MmaRows &p, cudaStream_t st);
+int mma_rows_bf16(int mode, const MmaRows &p, cudaStream_t st);
 
 struct MmaWeightGrad {
     const void *grad, *x;
@@ -267,10 +268,13 @@ struct MmaWeightGrad {
     Cut cut;
     Groups g;
 };
-// At most two pieces per SM over `tiles` tiles of the weight, none shorter than `least_piece` blocks.
+// About a piece per SM over `tiles` tiles of the weight, none shorter than `least_piece` blocks.
 Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int least_piece);
-Cut mma_cut(int batch, int rows, int groups, int in_features, int out_features);
-int mma_weight_grad(const MmaWeightGrad &p, cudaStream_t st);  // without the sum over slots
-int mma_timeouts();
+constexpr int kMmaTileRows = 128, kMmaSlice = 64;  // accumulator rows; contraction indices of a slice (and rows of a PieceTable's block)
+inline int mma_weight_tile(int in_features) { return in_features > 128 ? 256 : in_features > 64 ? 128 : 64; }
+int mma_weight_grad_f16(const MmaWeightGrad &p, cudaStream_t st);  // without the sum over slots
+int mma_weight_grad_bf16(const MmaWeightGrad &p, cudaStream_t st);
+int mma_timeouts_f16();  // -1 where the device cannot be asked
+int mma_timeouts_bf16();
 
 }  // namespace fda_linear

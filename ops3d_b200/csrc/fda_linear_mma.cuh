@@ -78,6 +78,10 @@ __device__ __forceinline__ void tma_3d(const CUtensorMap *map, void *dst, Barrie
                  "l"(map), "r"(smem_address(bar)), "r"(x), "r"(y), "r"(z)
                  : "memory");
 }
+// A box of a matrix into L2.
+__device__ __forceinline__ void prefetch_2d(const CUtensorMap *map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 // ---- tcgen05 ----------------------------------------------------------------------------------------------------------------
@@ -100,7 +104,14 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
 __device__ __forceinline__ void mma_commit(Barrier *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_address(bar)) : "memory");
 }
-// 32 lanes x 32 columns of fp32: register j of a lane is column j of its row.
+// 32 lanes x 16 or 32 columns of fp32: register j of a lane is column j of its row.
+__device__ __forceinline__ void tmem_load(uint32_t address, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(address));
+}
 __device__ __forceinline__ void tmem_load(uint32_t address, uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
@@ -134,8 +145,125 @@ __host__ __device__ constexpr uint32_t instruction(int m, int n, bool a_mn_major
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// ---- activations beside 16-bit outputs --------------------------------------------------------------------------------------------
+// A tile of 128 x 256 has 256 elements a lane of an SM, and its bytes pass in about 5500 cycles: more than some 20 instructions
+// an element and the epilogue, not memory, sets the pace (erff, expf and a division took 5.7 us a tile forward and 9.4 backward).
+// So: one exp2 and one reciprocal of the special-function unit each, the rest on pairs of elements where the instruction set has
+// the pair's form.  Errors stay below 1e-6 of 1 + |v|, a two-thousandth of the rounding to bf16 that follows.
+struct Pair {
+    unsigned long long bits;
+    __device__ __forceinline__ Pair() {}
+    __device__ __forceinline__ Pair(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(lo), "f"(hi)); }
+    __device__ __forceinline__ explicit Pair(float both) : Pair(both, both) {}
+    __device__ __forceinline__ void split(float &lo, float &hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(bits)); }
+};
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+    return r;
+}
+__device__ __forceinline__ Pair exp2_2(Pair v) {
+    float lo, hi;
+    v.split(lo, hi);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(lo));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(hi));
+    return Pair(lo, hi);
+}
+__device__ __forceinline__ Pair reciprocal_2(Pair v) {
+    float lo, hi;
+    v.split(lo, hi);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(lo));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(hi));
+    return Pair(lo, hi);
+}
+__device__ __forceinline__ float max_keeping_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The normal density at a >= 0 and the tail above a: density times a polynomial in 1 / (1 + p a), Abramowitz and Stegun 26.2.17, off by
+// at most 7.5e-8.
+__device__ __forceinline__ Pair normal_tail(Pair a, Pair &density) {
+    const Pair t = reciprocal_2(fma2(a, Pair(0.2316419f), Pair(1.f)));
+    density = exp2_2(fma2(a * a, Pair(-0.72134752f), Pair(-1.32574806f)));  // e^(-a^2 / 2) / sqrt(2 pi)
+    Pair q = fma2(t, Pair(1.330274429f), Pair(-1.821255978f));
+    q = fma2(t, q, Pair(1.781477937f));
+    q = fma2(t, q, Pair(-0.356563782f));
+    q = fma2(t, q, Pair(0.319381530f));
+    return density * (t * q);
+}
+// (1 + tanh(u)) / 2 = 1 / (1 + e^(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
+__device__ __forceinline__ Pair tanh_gate(Pair v) {
+    return reciprocal_2(exp2_2(v * fma2(v * v, Pair(-0.102943240f), Pair(-2.302208198f))) + Pair(1.f));
+}
+__device__ __forceinline__ Pair sigmoid_2(Pair v) { return reciprocal_2(exp2_2(v * Pair(-1.44269504f)) + Pair(1.f)); }
+
+template <int kAct>
+__device__ __forceinline__ Pair activate_2(Pair v) {
+    if (kAct == FDA_ACT_GELU) {
+        // v Phi(v) = max(v, 0) - |v| tail(|v|).  From 30 on the tail is 0 (and must not meet an infinite |v|).
+        float lo, hi, tail_lo, tail_hi;
+        v.split(lo, hi);
+        const float a_lo = fminf(fabsf(lo), 30.f), a_hi = fminf(fabsf(hi), 30.f);
+        Pair density;
+        normal_tail(Pair(a_lo, a_hi), density).split(tail_lo, tail_hi);
+        return Pair(fmaf(-a_lo, tail_lo, max_keeping_nan(lo, 0.f)), fmaf(-a_hi, tail_hi, max_keeping_nan(hi, 0.f)));
+    }
+    if (kAct == FDA_ACT_GELU_TANH) return v * tanh_gate(v);
+    if (kAct == FDA_ACT_SILU) return v * sigmoid_2(v);
+    if (kAct == FDA_ACT_RELU) {
+        float lo, hi;
+        v.split(lo, hi);
+        return Pair(max_keeping_nan(lo, 0.f), max_keeping_nan(hi, 0.f));
+    }
+    return v;
+}
+template <int kAct>
+__device__ __forceinline__ Pair activate_backward_2(Pair v, Pair dy) {
+    float lo, hi;
+    v.split(lo, hi);
+    if (kAct == FDA_ACT_GELU) {
+        Pair density;
+        float h_lo, h_hi;
+        fma2(normal_tail(Pair(fabsf(lo), fabsf(hi)), density), Pair(-1.f), Pair(0.5f)).split(h_lo, h_hi);
+        const Pair cdf = Pair(copysignf(h_lo, lo), copysignf(h_hi, hi)) + Pair(0.5f);
+        return dy * fma2(v, density, cdf);
+    }
+    if (kAct == FDA_ACT_GELU_TANH) {
+        // beyond 12 the gate is 0 or 1 to the last bit, and the slope's polynomial would overflow for very large v
+        const Pair s = tanh_gate(v), c(fminf(fmaxf(lo, -12.f), 12.f), fminf(fmaxf(hi, -12.f), 12.f));
+        return dy * fma2(c * (s * fma2(s, Pair(-1.f), Pair(1.f))), fma2(c * c, Pair(0.214064437f), Pair(1.595769122f)), s);
+    }
+    if (kAct == FDA_ACT_SILU) {
+        const Pair s = sigmoid_2(v);
+        return dy * (s * fma2(v, fma2(s, Pair(-1.f), Pair(1.f)), Pair(1.f)));
+    }
+    if (kAct == FDA_ACT_RELU) {
+        float dlo, dhi;
+        dy.split(dlo, dhi);
+        return Pair(activate_backward<kAct>(lo, dlo), activate_backward<kAct>(hi, dhi));
+    }
+    return dy;
+}
+
 // ---- 16-bit rows in registers -------------------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <typename T> __device__ __forceinline__ uint32_t pack2(Pair v) {
+    float lo, hi;
+    v.split(lo, hi);
+    return pack2<T>(lo, hi);
+}
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -144,59 +272,99 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
-template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
-template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+template <typename T> __device__ __forceinline__ Pair unpack2(uint32_t v);
+template <> __device__ __forceinline__ Pair unpack2<__half>(uint32_t v) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v));
+    return Pair(f.x, f.y);
+}
+template <> __device__ __forceinline__ Pair unpack2<__nv_bfloat16>(uint32_t v) {
+    return Pair(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
-__device__ __forceinline__ void load_32_bytes(const void *p, uint32_t *v) {
-    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                 : "l"(p));
-}
-__device__ __forceinline__ void store_32_bytes(void *p, const uint32_t *v) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
-                 "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
+// A warp's 32 rows x 32 elements of a 16-bit matrix, between global memory and registers (lane = row, two elements a register).
+// The transfer to or from global memory is coalesced, four lanes a row of 64 bytes where the rows' addresses are multiples of 16
+// bytes (kVector), else one lane an element; rows change hands in shared memory, 16 of them at a time.  (Each lane writing its
+// own row in sectors: 122 instead of 113 us for 598016 x 256 x 256.)  `count` of the columns and the first `rows` rows exist; p
+// is the first row's address.
+using Stage = uint4[16 * 4];
+
+// Unit u (16 bytes) of row r: eight lanes with rows of their own and four lanes of a row both meet every bank once.
+__device__ __forceinline__ int stage_unit(int r, int u) { return r * 4 + (u ^ ((r >> 1) & 3)); }
+__device__ __forceinline__ unsigned short *stage_element(Stage &stage, int r, int c) {
+    return reinterpret_cast<unsigned short *>(&stage[stage_unit(r, c / 8)]) + c % 8;
 }
 
-// 32 elements of a 16-bit row, of which `count` exist; `vector` is what the row's address is a multiple of (32, 16 or less, in bytes).
+// What a lane holds of the rows between its loads and the exchange: rows lane / 4 + 8 i, unit lane % 4.
+struct Fetched {
+    uint4 part[4];
+};
 template <typename T>
-__device__ __forceinline__ void load_row(const T *p, int count, int vector, uint32_t (&v)[16]) {
+__device__ __forceinline__ void fetch_rows(const T *p, long long pitch, int rows, int count, Fetched &f) {
+    const int lane = threadIdx.x % 32, unit = lane % 4;
+    const T *mine = p + (lane / 4) * pitch + 8 * unit;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = 0;
-    if (vector == 32 && count == 32) {
-        load_32_bytes(p, v);
-        load_32_bytes(p + 16, v + 8);
-    } else if (vector >= 16) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (8 * j < count) {
-                const uint4 q = *reinterpret_cast<const uint4 *>(p + 8 * j);
-                v[4 * j] = q.x; v[4 * j + 1] = q.y; v[4 * j + 2] = q.z; v[4 * j + 3] = q.w;
-            }
-    } else {
-        const unsigned short *s = reinterpret_cast<const unsigned short *>(p);
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < count) v[j / 2] |= (uint32_t)s[j] << (16 * (j & 1));
+    for (int i = 0; i < 4; ++i) {
+        f.part[i] = make_uint4(0, 0, 0, 0);
+        if (lane / 4 + 8 * i < rows && 8 * unit < count) f.part[i] = __ldg(reinterpret_cast<const uint4 *>(mine + 8 * i * pitch));
     }
 }
+__device__ __forceinline__ void own_row_from(Stage &stage, int half, uint32_t (&v)[16]) {
+    const int lane = threadIdx.x % 32;
+    if (lane / 16 == half)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint4 q = stage[stage_unit(lane % 16, u)];
+            v[4 * u] = q.x; v[4 * u + 1] = q.y; v[4 * u + 2] = q.z; v[4 * u + 3] = q.w;
+        }
+}
+__device__ __forceinline__ void rows_of_fetched(const Fetched &f, Stage &stage, uint32_t (&v)[16]) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        __syncwarp();
+        stage[stage_unit(lane / 4, lane % 4)] = f.part[2 * half];
+        stage[stage_unit(lane / 4 + 8, lane % 4)] = f.part[2 * half + 1];
+        __syncwarp();
+        own_row_from(stage, half, v);
+    }
+}
+// Rows that no vector access reaches.
 template <typename T>
-__device__ __forceinline__ void store_row(T *p, int count, int vector, const uint32_t (&v)[16]) {
-    if (vector == 32 && count == 32) {
-        store_32_bytes(p, v);
-        store_32_bytes(p + 16, v + 8);
-    } else if (vector >= 16) {
+__device__ __forceinline__ void load_elements(const T *p, long long pitch, int rows, int count, Stage &stage, uint32_t (&v)[16]) {
+    const int lane = threadIdx.x % 32;
+    const unsigned short *s = reinterpret_cast<const unsigned short *>(p);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (8 * j < count) *reinterpret_cast<uint4 *>(p + 8 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-    } else {
-        unsigned short *s = reinterpret_cast<unsigned short *>(p);
+    for (int half = 0; half < 2; ++half) {
+        __syncwarp();
+#pragma unroll 4
+        for (int r = 0; r < 16; ++r) *stage_element(stage, r, lane) = (16 * half + r < rows && lane < count) ? s[(16 * half + r) * pitch + lane] : 0;
+        __syncwarp();
+        own_row_from(stage, half, v);
+    }
+}
+template <bool kVector, typename T>
+__device__ __forceinline__ void store_rows(T *p, long long pitch, int rows, int count, Stage &stage, const uint32_t (&v)[16]) {
+    const int lane = threadIdx.x % 32;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < count) s[j] = (unsigned short)(v[j / 2] >> (16 * (j & 1)));
+    for (int half = 0; half < 2; ++half) {
+        __syncwarp();
+        if (lane / 16 == half)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                stage[stage_unit(lane % 16, u)] = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+        __syncwarp();
+        if (kVector) {
+            T *mine = p + (16 * half + lane / 4) * pitch + 8 * (lane % 4);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (16 * half + lane / 4 + 8 * i < rows && 8 * (lane % 4) < count)
+                    *reinterpret_cast<uint4 *>(mine + 8 * i * pitch) = stage[stage_unit(lane / 4 + 8 * i, lane % 4)];
+        } else {
+            unsigned short *s = reinterpret_cast<unsigned short *>(p);
+#pragma unroll 4
+            for (int r = 0; r < 16; ++r)
+                if (16 * half + r < rows && lane < count) s[(16 * half + r) * pitch + lane] = *stage_element(stage, r, lane);
+        }
     }
 }
 

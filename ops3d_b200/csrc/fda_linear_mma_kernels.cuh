@@ -1,9 +1,13 @@
 // The linear operators' products on the tensor cores, for 16-bit types: tcgen05.mma over operands that the copy engine brings into
 // swizzled shared memory, accumulators in tensor memory, everything after the product from there.
 //
-// One block per SM walks the output tiles.  Warp 0 keeps a ring of operand slices filled, warp 1 issues the products, warps 2-9
+// One block per SM walks the output tiles.  Warp 0 keeps a ring of operand slices filled, warp 1 issues the products, warps 4 and up
 // take finished sums out of tensor memory: accumulators are doubled, so that a tile's epilogue runs beside the next tile's
 // products.  Every wait is bounded: a role that waited in vain leaves, the others follow, and the block counts the event.
+//
+// Included by one translation unit per type.
+#pragma once
+
 #include <algorithm>
 
 #include "fda_config.h"
@@ -13,11 +17,9 @@ namespace fda_linear {
 
 namespace {
 
-constexpr int kTileRows = 128;                     // rows of an accumulator: one per lane of tensor memory
-constexpr int kSliceK = 64;                        // contraction indices per slice: one swizzled line
+constexpr int kTileRows = kMmaTileRows;            // rows of an accumulator: one per lane of tensor memory
+constexpr int kSliceK = kMmaSlice;                 // contraction indices per slice: one swizzled line
 constexpr int kBytesA = kTileRows * kSliceK * 2;
-constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpilogueWarps);
 constexpr int kRingBytes = 192 * 1024;
 
 template <int BN>
@@ -25,7 +27,12 @@ struct Shape {
     static constexpr int kBytesB = BN * kSliceK * 2;
     static constexpr int kBytes = kBytesA + kBytesB;
     static constexpr int kStages = kRingBytes / kBytes;  // 4, 6, 8
+    // Warps 0 and 1 work on operands, 2 and 3 idle (an epilogue warp's number modulo 4 decides which lanes of tensor memory it can
+    // read), then four for each part of the columns.
+    static constexpr int kPart = BN == 256 ? 64 : 32, kParts = BN / kPart;
+    static constexpr int kEpilogueWarps = 4 * kParts, kThreads = 32 * (4 + kEpilogueWarps);
 };
+constexpr int kFirstEpilogueWarp = 4;
 
 // Common to both kernels: the ring, the accumulators' barriers, tensor memory.
 template <int kStages>
@@ -36,7 +43,7 @@ struct Pipeline {
 };
 
 template <int kStages>
-__device__ __forceinline__ void pipeline_begin(Pipeline<kStages> &p, int columns) {
+__device__ __forceinline__ void pipeline_begin(Pipeline<kStages> &p, int columns, int epilogue_warps) {
     if (threadIdx.x == 32) {
         for (int i = 0; i < kStages; ++i) {
             p.full[i].init(1);
@@ -44,7 +51,7 @@ __device__ __forceinline__ void pipeline_begin(Pipeline<kStages> &p, int columns
         }
         for (int i = 0; i < 2; ++i) {
             p.sums_full[i].init(1);
-            p.sums_empty[i].init(kEpilogueWarps);
+            p.sums_empty[i].init(epilogue_warps);
         }
         p.drained.init(1);
         p.failed = 0;
@@ -90,48 +97,58 @@ struct RowsArgs {
     T *out;
     long long extra_pitch, out_pitch;
     int depth, cols;
-    int bias_vector, extra_vector, out_vector;  // bytes that the rows' addresses are multiples of: 32, 16 or less
-    int activation;
     Groups g;
 };
 
+constexpr int kForwardPlain = 3;  // kForward without a residual
+
+// 16 columns of a lane's row: `row` comes as the extra elements and leaves as the results.  `bias` is in shared memory, the same
+// address for the whole warp.
 template <typename T, int kMode, int kAct>
-__device__ __forceinline__ void finish_chunk(uint32_t (&v)[32], const uint32_t (&bias)[16], const uint32_t (&extra)[16], uint32_t (&out)[16]) {
+__device__ __forceinline__ void finish_columns(const uint32_t (&v)[16], const float *bias, uint32_t *row) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const float2 b = unpack2<T>(bias[j]), e = unpack2<T>(extra[j]);
-        float lo = __uint_as_float(v[2 * j]) + b.x, hi = __uint_as_float(v[2 * j + 1]) + b.y;
-        if (kMode == kForward) {
-            lo = activate<kAct>(lo) + e.x;
-            hi = activate<kAct>(hi) + e.y;
-        } else if (kMode == kPreGrad) {
-            lo = activate_backward<kAct>(lo, e.x);
-            hi = activate_backward<kAct>(hi, e.y);
+    for (int j = 0; j < 8; ++j) {
+        Pair r(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+        if (kMode != kGradX) {
+            const float2 b = *reinterpret_cast<const float2 *>(bias + 2 * j);
+            r = r + Pair(b.x, b.y);
+            if (kMode == kPreGrad) {
+                r = activate_backward_2<kAct>(r, unpack2<T>(row[j]));
+            } else {
+                r = activate_2<kAct>(r);
+                if (kMode == kForward) r = r + unpack2<T>(row[j]);
+            }
         }
-        out[j] = pack2<T>(lo, hi);
+        row[j] = pack2<T>(r);
     }
 }
 
-template <typename T, int kMode, int BN>
-__global__ void __launch_bounds__(kThreads, 1)
-    linear_rows_mma_kernel(const RowsArgs<T> p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w) {
+// kVector: the rows of out and of extra start on 16-byte boundaries.
+template <typename T, int kMode, int kAct, int BN, bool kVector>
+__global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
+    linear_rows_mma_kernel(const RowsArgs<T> p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                           const __grid_constant__ CUtensorMap map_extra) {
     constexpr int kStages = Shape<BN>::kStages, kColumns = 2 * BN;
     constexpr bool kWeightMn = kMode == kGradX;  // the weight's lines run along the output columns
+    constexpr bool kExtra = kMode == kForward || kMode == kPreGrad;
     extern __shared__ char dynamic[];
     __shared__ RowTable table;
     __shared__ Pipeline<kStages> pipe;
+    __shared__ __align__(16) float bias_of[Shape<BN>::kEpilogueWarps][Shape<BN>::kPart];
+    __shared__ __align__(16) Stage stages[Shape<BN>::kEpilogueWarps];
     char *const ring = reinterpret_cast<char *>(((uintptr_t)dynamic + kAtom - 1) & ~(uintptr_t)(kAtom - 1));
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
         prefetch_map(&map_a);
         prefetch_map(&map_w);
     }
-    pipeline_begin(pipe, kColumns);
+    pipeline_begin(pipe, kColumns, Shape<BN>::kEpilogueWarps);
     build_row_table(p.g, kTileRows, kMode != kPreGrad, table);
     __syncthreads();
     fence_after_sync();
-    const int column_tiles = (p.cols + BN - 1) / BN, slices = (p.depth + kSliceK - 1) / kSliceK;
-    const long long tiles = (long long)table.unit_begin[p.g.groups + 2] * p.g.batch * column_tiles;
+    const unsigned column_tiles = (p.cols + BN - 1) / BN;
+    const int slices = (p.depth + kSliceK - 1) / kSliceK;
+    const unsigned tiles = (unsigned)table.unit_begin[p.g.groups + 2] * p.g.batch * column_tiles;  // the host has checked that they fit
     volatile int *const failed = &pipe.failed;
     Ring<kStages> ring_at;
     bool any = false;
@@ -139,10 +156,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
         if (lane == 0) {
             bool sound = true;
-            for (long long tile = blockIdx.x; tile < tiles && sound; tile += gridDim.x) {
-                const RowUnit u = row_unit(p.g, table, kTileRows, (unsigned)(tile / column_tiles));
+            for (unsigned tile = blockIdx.x; tile < tiles && sound; tile += gridDim.x) {
+                const RowUnit u = row_unit(p.g, table, kTileRows, tile / column_tiles);
                 if (u.group < 0) continue;
-                const int col0 = (int)(tile % column_tiles) * BN;
+                const int col0 = (int)(tile % column_tiles * BN);
+                if (kExtra && kVector)  // on their way to L2 while the tile's products run: the epilogue's loads then wait for L2 only
+#pragma unroll
+                    for (int i = 0; i < BN / 64; ++i) prefetch_2d(&map_extra, col0 + 64 * i, (int)u.row);
                 for (int s = 0; s < slices; ++s) {
                     sound = pipe.empty[ring_at.stage].wait(ring_at.round ^ 1, failed);
                     if (!sound) break;
@@ -167,8 +187,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr uint32_t kInstruction = instruction<T>(kTileRows, BN, false, kWeightMn);
             Ring<2> sums;
             bool sound = true;
-            for (long long tile = blockIdx.x; tile < tiles && sound; tile += gridDim.x) {
-                const RowUnit u = row_unit(p.g, table, kTileRows, (unsigned)(tile / column_tiles));
+            for (unsigned tile = blockIdx.x; tile < tiles && sound; tile += gridDim.x) {
+                const RowUnit u = row_unit(p.g, table, kTileRows, tile / column_tiles);
                 if (u.group < 0) continue;
                 sound = pipe.sums_empty[sums.stage].wait(sums.round ^ 1, failed);
                 if (!sound) break;
@@ -194,63 +214,82 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncwarp();
-    } else {
-        // Each warp owns the 32 lanes of tensor memory that its number allows it, and half of the columns.
-        constexpr int kChunks = BN / 64;  // of 32 columns
-        const int quarter = warp % 4, half = (warp - 2) / 4;
+    } else if (warp >= kFirstEpilogueWarp) {
+        // Each warp owns the 32 lanes of tensor memory that its number allows it, and a part of the columns.  What it needs from
+        // global memory it asks for before it waits for the sums: loads chunk by chunk, each waited for, cost a tile of
+        // 128 x 256 two of its five microseconds.
+        constexpr int kPart = Shape<BN>::kPart, kChunks = kPart / 32;
+        const int quarter = warp % 4, part = (warp - kFirstEpilogueWarp) / 4;
+        float *const bias = bias_of[warp - kFirstEpilogueWarp];
+        Stage &stage = stages[warp - kFirstEpilogueWarp];
+        for (int i = lane; i < kPart; i += 32) bias[i] = 0.f;
+        int bias_group = -1, bias_col = -1;
         Ring<2> sums;
-        for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-            const RowUnit u = row_unit(p.g, table, kTileRows, (unsigned)(tile / column_tiles));
-            const int col0 = (int)(tile % column_tiles) * BN + half * (BN / 2);
-            const int r = quarter * 32 + lane;
-            const bool mine = r < u.count;
-            const T *extra_row = p.extra ? p.extra + (size_t)(u.row + r) * p.extra_pitch + col0 : nullptr;
-            T *out_row = p.out + (size_t)(u.row + r) * p.out_pitch + col0;
-            if (u.group >= 0) {
-                if (!__all_sync(0xffffffffu, pipe.sums_full[sums.stage].wait(sums.round, failed))) break;
-                fence_after_sync();
-            }
-            const uint32_t address = pipe.tmem + sums.stage * BN + half * (BN / 2) + ((uint32_t)(quarter * 32) << 16);
+        for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+            const RowUnit u = row_unit(p.g, table, kTileRows, tile / column_tiles);
+            const int col0 = (int)(tile % column_tiles * BN) + part * kPart;
+            const int rows = u.count - quarter * 32;  // of this warp; none or fewer where not positive
+            const long long first = u.row + quarter * 32;
+            T *out_rows = p.out + first * p.out_pitch + col0;
+            const T *extra_rows = kExtra ? p.extra + first * p.extra_pitch + col0 : nullptr;
+            Fetched fetched;  // the next chunk's extra rows
+            const auto fetch = [&](int c) {
+                if (kExtra && kVector && c < kChunks)
+                    fetch_rows(extra_rows + 32 * c, p.extra_pitch, rows, p.cols - col0 - 32 * c, fetched);
+            };
+            const auto extra_of = [&](int c, int count, uint32_t(&v)[16]) {  // chunk c of the extra rows, lane by row; asks for the next
+                if (kExtra && kVector) {
+                    rows_of_fetched(fetched, stage, v);
+                    fetch(c + 1);
+                } else if (kExtra) {
+                    load_elements(extra_rows + 32 * c, p.extra_pitch, rows, count, stage, v);
+                }
+            };
+            fetch(0);
+            if (kMode != kGradX) {
+                if (p.bias && u.group >= 0 && (u.group != bias_group || col0 != bias_col)) {
+                    __syncwarp();
 #pragma unroll
+                    for (int i = 0; i < kPart / 32; ++i)
+                        if (col0 + 32 * i + lane < p.cols) bias[32 * i + lane] = to_f32<T>(p.bias[(size_t)u.group * p.cols + col0 + 32 * i + lane]);
+                    bias_group = u.group;
+                    bias_col = col0;
+                    __syncwarp();
+                }
+            }
+            if (u.group < 0) {  // no product: the residual, or zeros
+#pragma unroll 1
+                for (int c = 0; c < kChunks; ++c)
+                    if (col0 + 32 * c < p.cols) {
+                        uint32_t row[16] = {};
+                        extra_of(c, p.cols - col0 - 32 * c, row);
+                        store_rows<kVector>(out_rows + 32 * c, p.out_pitch, rows, p.cols - col0 - 32 * c, stage, row);
+                    }
+                continue;
+            }
+            if (!__all_sync(0xffffffffu, pipe.sums_full[sums.stage].wait(sums.round, failed))) break;
+            fence_after_sync();
+            const uint32_t address = pipe.tmem + sums.stage * BN + part * kPart + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
             for (int c = 0; c < kChunks; ++c) {
-                const int count = min(32, p.cols - col0 - 32 * c);
+                const int count = p.cols - col0 - 32 * c;
                 if (count <= 0) break;
-                uint32_t v[32], extra[16], bias[16], out[16];
-                __syncwarp();
-                if (u.group >= 0) {
-                    tmem_load(address + 32 * c, v);
-                } else {
+                uint32_t row[16];
+                extra_of(c, count, row);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0;
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t v[16];
+                    __syncwarp();
+                    tmem_load(address + 32 * c + 16 * h, v);
+                    tmem_load_wait();
+                    finish_columns<T, kMode, kAct>(v, bias + 32 * c + 16 * h, row + 8 * h);
                 }
-                if (kMode != kGradX && extra_row && mine) {
-                    load_row(extra_row + 32 * c, count, p.extra_vector, extra);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) extra[j] = 0;
-                }
-                if (kMode != kGradX && p.bias && u.group >= 0) {
-                    load_row(p.bias + (size_t)u.group * p.cols + col0 + 32 * c, count, p.bias_vector, bias);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) bias[j] = 0;
-                }
-                tmem_load_wait();
-                switch (kMode == kGradX || u.group < 0 ? FDA_ACT_NONE : p.activation) {
-                    case FDA_ACT_NONE: finish_chunk<T, kMode, FDA_ACT_NONE>(v, bias, extra, out); break;
-                    case FDA_ACT_RELU: finish_chunk<T, kMode, FDA_ACT_RELU>(v, bias, extra, out); break;
-                    case FDA_ACT_GELU: finish_chunk<T, kMode, FDA_ACT_GELU>(v, bias, extra, out); break;
-                    case FDA_ACT_GELU_TANH: finish_chunk<T, kMode, FDA_ACT_GELU_TANH>(v, bias, extra, out); break;
-                    default: finish_chunk<T, kMode, FDA_ACT_SILU>(v, bias, extra, out); break;
-                }
-                if (mine) store_row(out_row + 32 * c, count, p.out_vector, out);
+                store_rows<kVector>(out_rows + 32 * c, p.out_pitch, rows, count, stage, row);
             }
-            if (u.group >= 0) {
-                fence_before_sync();
-                __syncwarp();
-                if (lane == 0) pipe.sums_empty[sums.stage].arrive();
-                sums.next();
-            }
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) pipe.sums_empty[sums.stage].arrive();
+            sums.next();
         }
     }
     pipeline_end(pipe, kColumns, ring_at, any);
@@ -270,27 +309,27 @@ struct WeightGradArgs {
     float *slots, *bias_slots;
     int in_features, out_features;
     int piece;
-    bool weight_vector;  // rows of grad_weight and of the slots start on 16-byte boundaries
     Groups g;
 };
 
-template <typename T, int BN>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int BN, bool kVector>
+__global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
     linear_weight_grad_mma_kernel(const WeightGradArgs<T> p, const __grid_constant__ CUtensorMap map_g,
                                   const __grid_constant__ CUtensorMap map_x) {
     constexpr int kStages = Shape<BN>::kStages, kColumns = 512;
     extern __shared__ char dynamic[];
     __shared__ PieceTable table;
     __shared__ Pipeline<kStages> pipe;
+    __shared__ __align__(16) Stage stages[Shape<BN>::kEpilogueWarps];
     char *const ring = reinterpret_cast<char *>(((uintptr_t)dynamic + kAtom - 1) & ~(uintptr_t)(kAtom - 1));
     char *const ones = ring + kStages * Shape<BN>::kBytes;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
         prefetch_map(&map_g);
         prefetch_map(&map_x);
     }
-    pipeline_begin(pipe, kColumns);
-    for (int i = threadIdx.x; i < kOnesBytes / 4; i += kThreads) reinterpret_cast<uint32_t *>(ones)[i] = pack2<T>(1.f, 1.f);
+    pipeline_begin(pipe, kColumns, Shape<BN>::kEpilogueWarps);
+    for (int i = threadIdx.x; i < kOnesBytes / 4; i += Shape<BN>::kThreads) reinterpret_cast<uint32_t *>(ones)[i] = pack2<T>(1.f, 1.f);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     build_piece_table(p.g, kSliceK, p.piece, table);
     __syncthreads();
@@ -391,9 +430,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             round ^= 1;
         }
         __syncwarp();
-    } else {
-        constexpr int kChunks = BN / 64;
-        const int quarter = warp % 4, half = (warp - 2) / 4;
+    } else if (warp >= kFirstEpilogueWarp) {
+        constexpr int kPart = Shape<BN>::kPart, kChunks = kPart / 32;
+        const int quarter = warp % 4, part = (warp - kFirstEpilogueWarp) / 4;
+        Stage &stage = stages[warp - kFirstEpilogueWarp];
         unsigned round = 0;
         for (long long i = blockIdx.x; i < items; i += gridDim.x) {
             const Item it = item_at(i);
@@ -408,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t address = pipe.tmem + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
             for (int c = 0; c < kChunks; ++c) {
-                const int in0 = it.in0 + half * (BN / 2) + 32 * c;
+                const int in0 = it.in0 + part * kPart + 32 * c;
                 const int count = min(32, p.in_features - in0);
                 if (count <= 0 || !p.grad_weight) break;
                 uint32_t v[32];
@@ -417,17 +457,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = 0;
                 } else {
-                    tmem_load(address + half * (BN / 2) + 32 * c, v);
+                    tmem_load(address + part * kPart + 32 * c, v);
                     tmem_load_wait();
                 }
                 const size_t at = (slot * p.out_features + out) * p.in_features + in0;
-                if (out >= p.out_features) {
-                } else if (whole) {
+                if (whole) {
                     uint32_t packed[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) packed[j] = pack2<T>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-                    store_row(p.grad_weight + at, count, p.weight_vector ? 16 : 2, packed);
-                } else if (p.weight_vector) {
+                    store_rows<kVector>(p.grad_weight + at - (size_t)lane * p.in_features, p.in_features, p.out_features - (out - lane), count,
+                                        stage, packed);
+                } else if (out >= p.out_features) {
+                } else if (kVector) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if (4 * j < count)
@@ -439,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             __syncwarp();
-            if (half == 0 && it.in0 == 0 && p.grad_bias) {
+            if (part == 0 && it.in0 == 0 && p.grad_bias) {
                 uint32_t sum = 0;
                 if (!none) {
                     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(sum) : "r"(address + BN));
@@ -498,10 +539,7 @@ int make_map(CUtensorMap &map, int dtype, const void *base, long long line, long
     return FDA_ERR_CUDA;
 }
 
-int vector_bytes(const void *base, long long pitch_elements) {
-    const uintptr_t bits = (uintptr_t)base | (uintptr_t)(pitch_elements * 2);
-    return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 2;
-}
+bool whole_vectors(const void *base, long long pitch) { return ((uintptr_t)base | (uintptr_t)(pitch * 2)) % 16 == 0; }
 
 int status(cudaError_t e) {
     if (e == cudaSuccess) return FDA_OK;
@@ -516,22 +554,28 @@ int allow_shared(Kernel kernel, int bytes) {
     return status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
 }
 
-template <typename T, int kMode, int BN>
+template <typename T, int kMode, int kAct, int BN, bool kVector>
 int launch_rows(const RowsArgs<T> &a, const MmaRows &p, long long units, cudaStream_t st) {
     constexpr int kSmem = Shape<BN>::kStages * Shape<BN>::kBytes + kAtom;
-    const auto kernel = linear_rows_mma_kernel<T, kMode, BN>;
+    const auto kernel = linear_rows_mma_kernel<T, kMode, kAct, BN, kVector>;
     if (const int rc = allow_shared(kernel, kSmem)) return rc;
-    CUtensorMap map_a, map_w;
+    CUtensorMap map_a, map_w, map_extra;
     const long long rows = (long long)p.g.batch * p.g.rows;
     if (const int rc = make_map(map_a, p.dtype, p.a, a.depth, rows, p.a_pitch, kTileRows, 0)) return rc;
     if (const int rc = make_map(map_w, p.dtype, p.w, p.in_features, p.out_features, p.w_pitch, kMode == kGradX ? kSliceK : BN, p.g.groups))
         return rc;
+    if (a.extra && kVector) {
+        if (const int rc = make_map(map_extra, p.dtype, p.extra, a.cols, rows, p.extra_pitch, kTileRows, 0)) return rc;
+    } else {
+        map_extra = map_a;
+    }
     const long long tiles = units * ceil_div(a.cols, BN);
-    kernel<<<(unsigned)std::min<long long>(tiles, kSms), kThreads, kSmem, st>>>(a, map_a, map_w);
+    if (tiles >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
+    kernel<<<(unsigned)std::min<long long>(tiles, kSms), Shape<BN>::kThreads, kSmem, st>>>(a, map_a, map_w, map_extra);
     return status(cudaGetLastError());
 }
 
-template <typename T, int kMode>
+template <typename T, int kMode, int kAct>
 int rows_of(const MmaRows &p, cudaStream_t st) {
     RowsArgs<T> a;
     a.bias = static_cast<const T *>(p.bias);
@@ -541,28 +585,37 @@ int rows_of(const MmaRows &p, cudaStream_t st) {
     a.out_pitch = p.out_pitch;
     a.depth = kMode == kGradX ? p.out_features : p.in_features;
     a.cols = kMode == kGradX ? p.in_features : p.out_features;
-    a.bias_vector = vector_bytes(p.bias, a.cols);
-    a.extra_vector = vector_bytes(p.extra, p.extra_pitch);
-    a.out_vector = vector_bytes(p.out, p.out_pitch);
-    a.activation = p.activation;
     a.g = p.g;
     // the widest tile that still gives every SM one
     const long long units = most_units(p.g.batch, p.g.rows, p.g.groups, kTileRows, kMode != kPreGrad && p.g.starts);
-    if (a.cols > 128 && units * ceil_div(a.cols, 256) >= kSms) return launch_rows<T, kMode, 256>(a, p, units, st);
-    if (a.cols > 64 && units * ceil_div(a.cols, 128) >= kSms) return launch_rows<T, kMode, 128>(a, p, units, st);
-    return launch_rows<T, kMode, 64>(a, p, units, st);
+    if (!whole_vectors(p.out, p.out_pitch) || (p.extra && !whole_vectors(p.extra, p.extra_pitch))) {
+        if (a.cols > 64 && units * ceil_div(a.cols, 128) >= kSms) return launch_rows<T, kMode, kAct, 128, false>(a, p, units, st);
+        return launch_rows<T, kMode, kAct, 64, false>(a, p, units, st);
+    }
+    if (a.cols > 128 && units * ceil_div(a.cols, 256) >= kSms) return launch_rows<T, kMode, kAct, 256, true>(a, p, units, st);
+    if (a.cols > 64 && units * ceil_div(a.cols, 128) >= kSms) return launch_rows<T, kMode, kAct, 128, true>(a, p, units, st);
+    return launch_rows<T, kMode, kAct, 64, true>(a, p, units, st);
+}
+
+template <typename T, int kMode>
+int rows_of(const MmaRows &p, cudaStream_t st) {
+    switch (p.activation) {
+        case FDA_ACT_NONE: return rows_of<T, kMode, FDA_ACT_NONE>(p, st);
+        case FDA_ACT_RELU: return rows_of<T, kMode, FDA_ACT_RELU>(p, st);
+        case FDA_ACT_GELU: return rows_of<T, kMode, FDA_ACT_GELU>(p, st);
+        case FDA_ACT_GELU_TANH: return rows_of<T, kMode, FDA_ACT_GELU_TANH>(p, st);
+        default: return rows_of<T, kMode, FDA_ACT_SILU>(p, st);
+    }
 }
 
 template <typename T>
 int rows_of(int mode, const MmaRows &p, cudaStream_t st) {
-    if (mode == kForward) return rows_of<T, kForward>(p, st);
+    if (mode == kForward) return p.extra ? rows_of<T, kForward>(p, st) : rows_of<T, kForwardPlain>(p, st);
     if (mode == kPreGrad) return rows_of<T, kPreGrad>(p, st);
-    return rows_of<T, kGradX>(p, st);
+    return rows_of<T, kGradX, FDA_ACT_NONE>(p, st);
 }
 
-int weight_tile(int in_features) { return in_features > 128 ? 256 : in_features > 64 ? 128 : 64; }
-
-template <typename T, int BN>
+template <typename T, int BN, bool kVector>
 int launch_weight_grad(const MmaWeightGrad &p, cudaStream_t st) {
     WeightGradArgs<T> a;
     a.grad_weight = static_cast<T *>(p.grad_weight);
@@ -572,47 +625,38 @@ int launch_weight_grad(const MmaWeightGrad &p, cudaStream_t st) {
     a.in_features = p.in_features;
     a.out_features = p.out_features;
     a.piece = p.cut.piece;
-    a.weight_vector = vector_bytes(p.grad_weight, p.in_features) >= 16;
     a.g = p.g;
     constexpr int kSmem = Shape<BN>::kStages * Shape<BN>::kBytes + kOnesBytes + kAtom;
-    const auto kernel = linear_weight_grad_mma_kernel<T, BN>;
+    const auto kernel = linear_weight_grad_mma_kernel<T, BN, kVector>;
     if (const int rc = allow_shared(kernel, kSmem)) return rc;
     CUtensorMap map_g, map_x;
     const long long rows = (long long)p.g.batch * p.g.rows;
     if (const int rc = make_map(map_g, p.dtype, p.grad, p.out_features, rows, p.grad_pitch, kSliceK, 0)) return rc;
     if (const int rc = make_map(map_x, p.dtype, p.x, p.in_features, rows, p.x_pitch, kSliceK, 0)) return rc;
     const long long items = p.cut.pieces * ceil_div(p.out_features, kTileRows) * ceil_div(p.in_features, BN);
-    kernel<<<(unsigned)std::min<long long>(items, kSms), kThreads, kSmem, st>>>(a, map_g, map_x);
+    kernel<<<(unsigned)std::min<long long>(items, kSms), Shape<BN>::kThreads, kSmem, st>>>(a, map_g, map_x);
     return status(cudaGetLastError());
+}
+
+template <typename T, bool kVector>
+int weight_grad_of(const MmaWeightGrad &p, cudaStream_t st) {
+    switch (mma_weight_tile(p.in_features)) {
+        case 256: return launch_weight_grad<T, 256, kVector>(p, st);
+        case 128: return launch_weight_grad<T, 128, kVector>(p, st);
+        default: return launch_weight_grad<T, 64, kVector>(p, st);
+    }
 }
 
 template <typename T>
 int weight_grad_of(const MmaWeightGrad &p, cudaStream_t st) {
-    switch (weight_tile(p.in_features)) {
-        case 256: return launch_weight_grad<T, 256>(p, st);
-        case 128: return launch_weight_grad<T, 128>(p, st);
-        default: return launch_weight_grad<T, 64>(p, st);
-    }
+    return whole_vectors(p.grad_weight, p.in_features) ? weight_grad_of<T, true>(p, st) : weight_grad_of<T, false>(p, st);
+}
+
+int timeouts() {
+    unsigned int n = 0;
+    return cudaMemcpyFromSymbol(&n, g_timeouts, sizeof(n)) == cudaSuccess ? (int)n : -1;
 }
 
 }  // namespace
-
-int mma_rows(int mode, const MmaRows &p, cudaStream_t st) {
-    return p.dtype == FDA_DTYPE_F16 ? rows_of<__half>(mode, p, st) : rows_of<__nv_bfloat16>(mode, p, st);
-}
-
-Cut mma_cut(int batch, int rows, int groups, int in_features, int out_features) {
-    return cut_rows(batch, rows, groups, ceil_div(out_features, kTileRows) * ceil_div(in_features, weight_tile(in_features)), kSliceK, 8);
-}
-
-int mma_weight_grad(const MmaWeightGrad &p, cudaStream_t st) {
-    return p.dtype == FDA_DTYPE_F16 ? weight_grad_of<__half>(p, st) : weight_grad_of<__nv_bfloat16>(p, st);
-}
-
-int mma_timeouts() {
-    unsigned int n = 0;
-    if (cudaMemcpyFromSymbol(&n, g_timeouts, sizeof(n)) != cudaSuccess) return -1;
-    return (int)n;
-}
 
 }  // namespace fda_linear
