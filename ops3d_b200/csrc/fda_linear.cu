@@ -12,73 +12,69 @@ using namespace fda_linear;
 // ---------------------------------------------------------------------------------------------------------------------------
 // Products on the fp32 pipes
 // ---------------------------------------------------------------------------------------------------------------------------
-// A block computes a BM x BN tile; its 256 threads own TM x TN sums each (rows ty + 16 i, columns tx + 16 j: neighbouring
-// threads read neighbouring words of a k-slice from shared memory and write neighbouring outputs).  Operands pass through
-// shared memory in slices of 16 along k, the next slice travelling in registers meanwhile.
-constexpr int kThreads = 256, kSlice = 16;
+// A block computes a 64 x 64 tile; its 256 threads own 4 x 4 sums each.  Operands pass through shared memory in slices of 16 along k,
+// copied element by element (any size, any alignment; what does not exist arrives as zero) and three slices ahead: with one
+// slice ahead, in registers, 3001 x 99 x 131 took 24 us, most of it waiting for memory slice by slice.
+constexpr int kThreads = 256, kSlice = 16, kTile = 64, kOwn = 4, kAhead = 4, kPitch = kTile + 4;
 
-// A(i, k) = a[i * ai + k * ak], of which i < rows, k < depth exist; the stride that is 1 decides how threads cover a slice.
-template <typename T, int kTile, bool kContiguousK>
-struct SliceLoader {
-    static constexpr int kEach = kTile * kSlice / kThreads;
-    float reg[kEach];
-    __device__ __forceinline__ static int index(int j) {  // along the tile
-        return kContiguousK ? (int)threadIdx.x / kSlice + j * (kThreads / kSlice) : ((int)threadIdx.x + j * kThreads) % kTile;
-    }
-    __device__ __forceinline__ static int depth(int j) {
-        return kContiguousK ? (int)threadIdx.x % kSlice : ((int)threadIdx.x + j * kThreads) / kTile;
-    }
-    __device__ __forceinline__ void load(const T *a, long long ai, long long ak, int rows, int k0, int k_end) {
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const int i = index(j), k = k0 + depth(j);
-            reg[j] = (i < rows && k < k_end) ? to_f32<T>(a[i * ai + k * ak]) : 0.f;
-        }
-    }
-    __device__ __forceinline__ void store(float (*s)[kTile + 1]) const {
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) s[depth(j)][index(j)] = reg[j];
-    }
-};
-
-template <int BM, int BN>
 struct Slices {
-    float a[kSlice][BM + 1];
-    float b[kSlice][BN + 1];
+    float a[kAhead][kSlice][kPitch];
+    float b[kAhead][kSlice][kPitch];
 };
 
-// acc += A B over k in [0, depth); A is BM x depth, B depth x BN.
-template <typename T, int BM, int BN, bool kAK, bool kBK>
-__device__ __forceinline__ void tile_product(float (&acc)[BM / 16][BN / 16], Slices<BM, BN> &s, const T *a, long long ai, long long ak,
-                                             int rows, const T *b, long long bj, long long bk, int cols, int depth) {
-    constexpr int TM = BM / 16, TN = BN / 16;
+__device__ __forceinline__ void copy_element(float *dst, const float *src, bool exists) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(exists ? 4 : 0)
+                 : "memory");
+}
+
+// Slice k0 .. k0 + 15 of A(i, k) = a[i * ai + k * ak], of which i < rows, k < depth exist; the stride that is 1 decides how
+// threads cover it.
+template <bool kContiguousK>
+__device__ __forceinline__ void copy_slice(float (*dst)[kPitch], const float *a, long long ai, long long ak, int rows, int k0, int depth) {
+#pragma unroll
+    for (int j = 0; j < kTile * kSlice / kThreads; ++j) {
+        const int i = kContiguousK ? (int)threadIdx.x / kSlice + j * (kThreads / kSlice) : (int)threadIdx.x % kTile;
+        const int k = kContiguousK ? (int)threadIdx.x % kSlice : (int)threadIdx.x / kTile + j * (kThreads / kTile);
+        const bool exists = i < rows && k0 + k < depth;
+        copy_element(&dst[k][i], exists ? a + i * ai + (k0 + k) * ak : a, exists);
+    }
+}
+
+// acc += A B over k in [0, depth); A is 64 x depth, B depth x 64.  A thread owns rows 4 ty .., columns 4 tx ..; with kSumA
+// also sums = its rows of A added over k.  Every thread of the block takes part; the slices are free again at the end.
+template <bool kAK, bool kBK, bool kSumA>
+__device__ __forceinline__ void tile_product(float (&acc)[kOwn][kOwn], float (&sums)[kOwn], Slices &s, const float *a, long long ai, long long ak,
+                                             int rows, const float *b, long long bj, long long bk, int cols, int depth) {
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    SliceLoader<T, BM, kAK> la;
-    SliceLoader<T, BN, kBK> lb;
-    la.load(a, ai, ak, rows, 0, depth);
-    lb.load(b, bj, bk, cols, 0, depth);
-    for (int k0 = 0; k0 < depth; k0 += kSlice) {
-        __syncthreads();
-        la.store(s.a);
-        lb.store(s.b);
-        __syncthreads();
-        if (k0 + kSlice < depth) {
-            la.load(a, ai, ak, rows, k0 + kSlice, depth);
-            lb.load(b, bj, bk, cols, k0 + kSlice, depth);
+    const int slices = (depth + kSlice - 1) / kSlice;
+    const auto copy = [&](int i) {
+        if (i < slices) {
+            copy_slice<kAK>(s.a[i % kAhead], a, ai, ak, rows, i * kSlice, depth);
+            copy_slice<kBK>(s.b[i % kAhead], b, bj, bk, cols, i * kSlice, depth);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead - 1; ++i) copy(i);
+    for (int i = 0; i < slices; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
+        __syncthreads();  // slice i has arrived for every thread, and every thread is done with the one that is overwritten next
+        copy(i + kAhead - 1);
+        const float(*sa)[kPitch] = s.a[i % kAhead], (*sb)[kPitch] = s.b[i % kAhead];
 #pragma unroll
         for (int k = 0; k < kSlice; ++k) {
-            float ra[TM], rb[TN];
+            const float4 qa = *reinterpret_cast<const float4 *>(&sa[k][kOwn * ty]), qb = *reinterpret_cast<const float4 *>(&sb[k][kOwn * tx]);
+            const float ra[kOwn] = {qa.x, qa.y, qa.z, qa.w}, rb[kOwn] = {qb.x, qb.y, qb.z, qb.w};
 #pragma unroll
-            for (int i = 0; i < TM; ++i) ra[i] = s.a[k][ty + 16 * i];
+            for (int r = 0; r < kOwn; ++r) {
+                if (kSumA) sums[r] += ra[r];
 #pragma unroll
-            for (int j = 0; j < TN; ++j) rb[j] = s.b[k][tx + 16 * j];
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = fmaf(ra[i], rb[j], acc[i][j]);
+                for (int c = 0; c < kOwn; ++c) acc[r][c] = fmaf(ra[r], rb[c], acc[r][c]);
+            }
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
 }
 
 template <typename T>
@@ -90,52 +86,139 @@ struct RowProduct {
     T *out;
     int depth, cols;  // contraction; columns of the result
     int in_features;  // row length of w
+    int out_pitch;
     Groups g;
 };
 
 // kForward:  out = act(a W^T + bias) + extra    kPreGrad:  out = extra * act'(a W^T + bias)    kGradX:  out = a W
-template <typename T, int kMode, int kAct, int BM, int BN>
-__global__ void __launch_bounds__(kThreads) linear_rows_kernel(const RowProduct<T> p) {
+template <int kMode, int kAct>
+__global__ void __launch_bounds__(kThreads) linear_rows_kernel(const RowProduct<float> p) {
     __shared__ RowTable table;
-    __shared__ Slices<BM, BN> slices;
-    build_row_table(p.g, BM, kMode != kPreGrad, table);
+    __shared__ __align__(16) Slices slices;
+    build_row_table(p.g, kTile, kMode != kPreGrad, table);
     __syncthreads();
-    const int column_tiles = (p.cols + BN - 1) / BN;
+    const int column_tiles = (p.cols + kTile - 1) / kTile;
     const long long tiles = (long long)table.unit_begin[p.g.groups + 2] * p.g.batch * column_tiles;
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const RowUnit u = row_unit(p.g, table, BM, (unsigned)(tile / column_tiles));
-        const int col0 = (int)(tile % column_tiles) * BN, cols = min(BN, p.cols - col0);
-        float acc[BM / 16][BN / 16] = {};
+        const RowUnit u = row_unit(p.g, table, kTile, (unsigned)(tile / column_tiles));
+        const int col0 = (int)(tile % column_tiles) * kTile, cols = min(kTile, p.cols - col0);
+        float acc[kOwn][kOwn] = {}, none[kOwn];
         if (u.group >= 0) {
-            const T *w = p.w + (size_t)u.group * ((kMode == kGradX ? (size_t)p.depth : (size_t)p.cols) * p.in_features);
-            const T *a = p.a + (size_t)u.row * p.depth;
+            const float *w = p.w + (size_t)u.group * ((kMode == kGradX ? (size_t)p.depth : (size_t)p.cols) * p.in_features);
+            const float *a = p.a + (size_t)u.row * p.depth;
             if (kMode == kGradX)
-                tile_product<T, BM, BN, true, false>(acc, slices, a, p.depth, 1, u.count, w + col0, 1, p.in_features, cols, p.depth);
+                tile_product<true, false, false>(acc, none, slices, a, p.depth, 1, u.count, w + col0, 1, p.in_features, cols, p.depth);
             else
-                tile_product<T, BM, BN, true, true>(acc, slices, a, p.depth, 1, u.count, w + (size_t)col0 * p.in_features, p.in_features, 1,
-                                                    cols, p.depth);
+                tile_product<true, true, false>(acc, none, slices, a, p.depth, 1, u.count, w + (size_t)col0 * p.in_features, p.in_features, 1,
+                                                cols, p.depth);
         }
+        float bias[kOwn] = {};
+        if (kMode != kGradX && p.bias && u.group >= 0)
 #pragma unroll
-        for (int j = 0; j < BN / 16; ++j) {
-            const int c = tx + 16 * j;
-            if (c >= cols) continue;
-            const float bias = (kMode != kGradX && p.bias && u.group >= 0) ? to_f32<T>(p.bias[(size_t)u.group * p.cols + col0 + c]) : 0.f;
+            for (int c = 0; c < kOwn; ++c)
+                if (kOwn * tx + c < cols) bias[c] = p.bias[(size_t)u.group * p.cols + col0 + kOwn * tx + c];
 #pragma unroll
-            for (int i = 0; i < BM / 16; ++i) {
-                const int r = ty + 16 * i;
-                if (r >= u.count) continue;
-                const size_t at = (size_t)(u.row + r) * p.cols + col0 + c;
-                float v = acc[i][j] + bias;
-                if (kMode == kForward) {
-                    if (u.group >= 0) v = activate<kAct>(v);
-                    if (p.extra) v += to_f32<T>(p.extra[at]);
-                } else if (kMode == kPreGrad) {
-                    v = activate_backward<kAct>(v, to_f32<T>(p.extra[at]));
-                }
-                p.out[at] = from_f32<T>(v);
+        for (int i = 0; i < kOwn; ++i) {
+            const int r = kOwn * ty + i;
+            if (r >= u.count) continue;
+            float extra[kOwn] = {};
+            if (kMode != kGradX && p.extra)
+#pragma unroll
+                for (int c = 0; c < kOwn; ++c)
+                    if (kOwn * tx + c < cols) extra[c] = p.extra[(size_t)(u.row + r) * p.cols + col0 + kOwn * tx + c];
+            float *out = p.out + (size_t)(u.row + r) * p.out_pitch + col0 + kOwn * tx;
+#pragma unroll
+            for (int c = 0; c < kOwn; ++c) {
+                if (kOwn * tx + c >= cols) continue;
+                float v = acc[i][c] + bias[c];
+                if (kMode == kForward) v = (u.group >= 0 ? activate<kAct>(v) : v) + extra[c];
+                else if (kMode == kPreGrad) v = activate_backward<kAct>(v, extra[c]);
+                out[c] = v;
             }
         }
+    }
+}
+
+// Few rows (one token, or a few per group): bound by latency and by reading the weight, which no tile of 128 rows helps.  A warp takes
+// two outputs and up to eight rows, its lanes along the contraction, 16 bytes a load; lane 8 o + r finishes row r of output o.
+// One token, 256 -> 1024: 5.3 us in the tile kernel, 2.9 here.
+constexpr int kFewRows = 8, kFewOutputs = 2, kFewThreads = 128;
+
+// 16 bytes of a row from element k on, or as many elements as exist.
+template <typename T, bool kVector>
+__device__ __forceinline__ void load_some(const T *row, int k, int depth, float (&v)[16 / sizeof(T)]) {
+    constexpr int kCount = 16 / sizeof(T);
+    if (kVector) {
+        alignas(16) T raw[kCount];
+        *reinterpret_cast<uint4 *>(raw) = __ldg(reinterpret_cast<const uint4 *>(row + k));
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) v[j] = to_f32<T>(raw[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) v[j] = k + j < depth ? to_f32<T>(row[k + j]) : 0.f;
+    }
+}
+
+// kForward and kPreGrad.
+template <typename T, int kMode, bool kVector>
+__global__ void __launch_bounds__(kFewThreads) linear_few_rows_kernel(const RowProduct<T> p, const int activation) {
+    constexpr int kCount = 16 / sizeof(T);
+    __shared__ RowTable table;
+    build_row_table(p.g, kFewRows, kMode != kPreGrad, table);
+    __syncthreads();
+    const int lane = threadIdx.x % 32;
+    const unsigned steps = (unsigned)((p.cols + kFewOutputs - 1) / kFewOutputs);
+    const long long items = (long long)table.unit_begin[p.g.groups + 2] * p.g.batch * steps;
+    const long long warps = (long long)gridDim.x * (kFewThreads / 32);
+    for (long long item = (long long)blockIdx.x * (kFewThreads / 32) + threadIdx.x / 32; item < items; item += warps) {
+        const RowUnit u = row_unit(p.g, table, kFewRows, (unsigned)(item / steps));
+        const int col0 = (int)(item % steps) * kFewOutputs;
+        float acc[kFewOutputs][kFewRows] = {};
+        if (u.group >= 0) {
+            const T *a = p.a + (size_t)u.row * p.depth;
+            const T *w = p.w + ((size_t)u.group * p.cols + col0) * p.depth;
+            const bool second = col0 + 1 < p.cols;
+#pragma unroll 2
+            for (int k = lane * kCount; k < p.depth; k += 32 * kCount) {
+                float w0[kCount], w1[kCount];
+                load_some<T, kVector>(w, k, p.depth, w0);
+                load_some<T, kVector>(second ? w + p.depth : w, k, p.depth, w1);
+#pragma unroll
+                for (int r = 0; r < kFewRows; ++r)
+                    if (r < u.count) {
+                        float x[kCount];
+                        load_some<T, kVector>(a + (size_t)r * p.depth, k, p.depth, x);
+#pragma unroll
+                        for (int j = 0; j < kCount; ++j) {
+                            acc[0][r] = fmaf(x[j], w0[j], acc[0][r]);
+                            acc[1][r] = fmaf(x[j], w1[j], acc[1][r]);
+                        }
+                    }
+            }
+        }
+        float v = 0.f;
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r)
+            if (r < u.count)
+#pragma unroll
+                for (int o = 0; o < kFewOutputs; ++o) {
+                    float sum = acc[o][r];
+#pragma unroll
+                    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                    if (lane == o * kFewRows + r) v = sum;
+                }
+        const int r = lane % kFewRows, c = col0 + lane / kFewRows;
+        if (lane >= kFewOutputs * kFewRows || r >= u.count || c >= p.cols) continue;
+        const size_t at = (size_t)(u.row + r) * p.cols + c;
+        if (p.bias && u.group >= 0) v += to_f32<T>(p.bias[(size_t)u.group * p.cols + c]);
+        if (kMode == kForward) {
+            if (u.group >= 0) v = activate_any(activation, v);
+            if (p.extra) v += to_f32<T>(p.extra[at]);
+        } else {
+            v = activate_backward_any(activation, v, to_f32<T>(p.extra[at]));
+        }
+        p.out[(size_t)(u.row + r) * p.out_pitch + c] = from_f32<T>(v);
     }
 }
 
@@ -150,52 +233,46 @@ struct WeightGrad {
     Groups g;
 };
 
-// grad_weight tile BM (outputs) x BN (inputs) over one piece of a group's rows.
-template <typename T, int BM, int BN>
-__global__ void __launch_bounds__(kThreads) linear_weight_grad_kernel(const WeightGrad<T> p) {
+// A 64 x 64 tile of grad_weight (outputs x inputs) over one piece of a group's rows.
+__global__ void __launch_bounds__(kThreads) linear_weight_grad_kernel(const WeightGrad<float> p) {
     __shared__ PieceTable table;
-    __shared__ Slices<BM, BN> slices;
+    __shared__ __align__(16) Slices slices;
     build_piece_table(p.g, p.block, p.piece, table);
     __syncthreads();
-    const int out_tiles = (p.out_features + BM - 1) / BM, in_tiles = (p.in_features + BN - 1) / BN;
+    const int out_tiles = (p.out_features + kTile - 1) / kTile, in_tiles = (p.in_features + kTile - 1) / kTile;
     const int per_piece = out_tiles * in_tiles;
     const long long items = (long long)table.piece_begin[p.g.groups] * per_piece;
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     for (long long item = blockIdx.x; item < items; item += gridDim.x) {
         const int piece = (int)(item / per_piece), t = (int)(item % per_piece);
         const int e = find_section(table.piece_begin, p.g.groups, piece), s = piece - table.piece_begin[e];
-        const int out0 = (t / in_tiles) * BM, in0 = (t % in_tiles) * BN;
-        const int outs = min(BM, p.out_features - out0), ins = min(BN, p.in_features - in0);
+        const int out0 = (t / in_tiles) * kTile, in0 = (t % in_tiles) * kTile;
+        const int outs = min(kTile, p.out_features - out0), ins = min(kTile, p.in_features - in0);
         const int blocks = group_blocks(p.g, table.start, e, p.block);
-        float acc[BM / 16][BN / 16] = {};
-        float bias = 0.f;
+        const bool with_bias = in0 == 0 && p.grad_bias;
+        float acc[kOwn][kOwn] = {}, bias[kOwn] = {};
         for (int j = s * p.piece; j < min(blocks, (s + 1) * p.piece); ++j) {
             long long row;
             int count;
             block_rows(p.g, table.start, e, p.block, j, row, count);
-            const T *grad = p.grad + (size_t)row * p.out_features + out0;
-            tile_product<T, BM, BN, false, false>(acc, slices, grad, 1, p.out_features, outs,
-                                                  p.x + (size_t)row * p.in_features + in0, 1, p.in_features, ins, count);
-            if (in0 == 0 && p.grad_bias && (int)threadIdx.x < outs)
-                for (int r = 0; r < count; ++r) bias += to_f32<T>(grad[(size_t)r * p.out_features + threadIdx.x]);
+            const float *grad = p.grad + (size_t)row * p.out_features + out0, *x = p.x + (size_t)row * p.in_features + in0;
+            if (with_bias)
+                tile_product<false, false, true>(acc, bias, slices, grad, 1, p.out_features, outs, x, 1, p.in_features, ins, count);
+            else
+                tile_product<false, false, false>(acc, bias, slices, grad, 1, p.out_features, outs, x, 1, p.in_features, ins, count);
         }
         const bool whole = table.slot_begin[e + 1] == table.slot_begin[e];
-        const size_t slot = (size_t)table.slot_begin[e] + s;
-        if (p.grad_weight)
+        const size_t slot = whole ? (size_t)e : (size_t)table.slot_begin[e] + s;
+        float *const weight = whole ? p.grad_weight : p.slots, *const biases = whole ? p.grad_bias : p.bias_slots;
 #pragma unroll
-            for (int i = 0; i < BM / 16; ++i)
+        for (int i = 0; i < kOwn; ++i) {
+            const int r = kOwn * ty + i;
+            if (r >= outs) continue;
+            if (p.grad_weight)
 #pragma unroll
-                for (int j = 0; j < BN / 16; ++j) {
-                    const int r = ty + 16 * i, c = tx + 16 * j;
-                    if (r >= outs || c >= ins) continue;
-                    const size_t at = (size_t)(out0 + r) * p.in_features + in0 + c, size = (size_t)p.out_features * p.in_features;
-                    if (whole) p.grad_weight[e * size + at] = from_f32<T>(acc[i][j]);
-                    else p.slots[slot * size + at] = acc[i][j];
-                }
-        if (in0 == 0 && p.grad_bias && (int)threadIdx.x < outs) {
-            const size_t at = out0 + threadIdx.x;
-            if (whole) p.grad_bias[(size_t)e * p.out_features + at] = from_f32<T>(bias);
-            else p.bias_slots[slot * p.out_features + at] = bias;
+                for (int c = 0; c < kOwn; ++c)
+                    if (kOwn * tx + c < ins) weight[(slot * p.out_features + out0 + r) * p.in_features + in0 + kOwn * tx + c] = acc[i][c];
+            if (with_bias && tx == 0) biases[slot * p.out_features + out0 + r] = bias[i];
         }
     }
 }
@@ -267,28 +344,24 @@ __global__ void __launch_bounds__(32 * kSumWarps) linear_weight_grad_sum_kernel(
 // ---------------------------------------------------------------------------------------------------------------------------
 inline size_t type_size(int dtype) { return dtype == FDA_DTYPE_F32 ? 4 : 2; }
 
-}  // namespace
-
-namespace fda_linear {
-
+// As many pieces as the SMs take at once over `tiles` tiles of the weight, none shorter than `least_piece` blocks.
 Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int least_piece) {
     Cut c;
     c.block = block;
     const long long blocks = std::max<long long>(1, most_units(batch, rows, groups, block, false));
-    // As many pieces as the SMs take at once: one more would be a round of its own.  Every further group can add a piece that is
-    // not full; where there are too many groups for that, pieces half as long, so that the last round is short.
+    // One piece more than the SMs take would be a round of its own.  Every further group can add a piece that is not full; where
+    // there are too many groups for that, pieces half as long, so that the last round is short.
     const long long wanted = std::max<long long>(1, kSms / tiles);
     const long long full = wanted >= 2 * groups ? wanted - (groups - 1) : 2 * wanted;
     c.piece = (int)std::max<long long>(least_piece, ceil_div(blocks, full));
+    if (blocks <= 2 * least_piece) c.piece = (int)blocks;  // the second launch would cost more than it spreads
     c.pieces = ceil_div(blocks, c.piece) + groups;
     // a group of n > 1 pieces has more than (n - 1) * piece blocks, so at least n / 2 * piece
     c.slots = blocks <= c.piece ? 0 : std::min(c.pieces, 2 * (blocks / c.piece) + 1);
     return c;
 }
 
-}  // namespace fda_linear
 
-namespace {
 
 struct Shape {
     int batch, rows, groups, in_features, out_features, dtype;
@@ -314,45 +387,69 @@ int launched() {
     return FDA_ERR_CUDA;
 }
 
-constexpr int kTileSize = 64;
-constexpr int kPlainBlock = 64, kPlainLeastPiece = 4;
+constexpr int kPlainBlock = 256, kPlainLeastPiece = 1;
 
-template <typename T, int kMode, int kAct>
-int run_rows_plain(const RowProduct<T> &p, cudaStream_t st) {
-    const long long tiles = most_units(p.g.batch, p.g.rows, p.g.groups, kTileSize, kMode != kPreGrad) * ceil_div(p.cols, kTileSize);
-    linear_rows_kernel<T, kMode, kAct, kTileSize, kTileSize><<<(unsigned)std::min<long long>(tiles, 8 * kSms), kThreads, 0, st>>>(p);
+template <int kMode, int kAct>
+int run_rows(const RowProduct<float> &p, cudaStream_t st) {
+    const long long tiles = most_units(p.g.batch, p.g.rows, p.g.groups, kTile, kMode != kPreGrad) * ceil_div(p.cols, kTile);
+    linear_rows_kernel<kMode, kAct><<<(unsigned)std::min<long long>(tiles, 8 * kSms), kThreads, 0, st>>>(p);
     return launched();
 }
 
-template <typename T, int kMode>
-int run_rows(const RowProduct<T> &p, int activation, cudaStream_t st) {
-    switch (kMode == kGradX ? FDA_ACT_NONE : activation) {
-        case FDA_ACT_NONE: return run_rows_plain<T, kMode, FDA_ACT_NONE>(p, st);
-        case FDA_ACT_RELU: return run_rows_plain<T, kMode, FDA_ACT_RELU>(p, st);
-        case FDA_ACT_GELU: return run_rows_plain<T, kMode, FDA_ACT_GELU>(p, st);
-        case FDA_ACT_GELU_TANH: return run_rows_plain<T, kMode, FDA_ACT_GELU_TANH>(p, st);
-        default: return run_rows_plain<T, kMode, FDA_ACT_SILU>(p, st);
+template <int kMode>
+int run_rows(const RowProduct<float> &p, int activation, cudaStream_t st) {
+    switch (activation) {
+        case FDA_ACT_NONE: return run_rows<kMode, FDA_ACT_NONE>(p, st);
+        case FDA_ACT_RELU: return run_rows<kMode, FDA_ACT_RELU>(p, st);
+        case FDA_ACT_GELU: return run_rows<kMode, FDA_ACT_GELU>(p, st);
+        case FDA_ACT_GELU_TANH: return run_rows<kMode, FDA_ACT_GELU_TANH>(p, st);
+        default: return run_rows<kMode, FDA_ACT_SILU>(p, st);
     }
 }
 
-// 16-bit operands whose rows do not start on 16-byte boundaries are copied to rows that do.
-__global__ void __launch_bounds__(kThreads) linear_pad_kernel(const unsigned short *__restrict__ src, unsigned short *__restrict__ dst,
-                                                              unsigned long long elements, int line, int pitch) {
-    const unsigned long long step = (unsigned long long)gridDim.x * kThreads;
-    for (unsigned long long i = (unsigned long long)blockIdx.x * kThreads + threadIdx.x; i < elements; i += step)
-        dst[i / (unsigned)line * (unsigned)pitch + i % (unsigned)line] = src[i];
+// 16-bit operands whose rows do not start on 16-byte boundaries are copied to rows that do, up to three of them in one launch.  A
+// thread writes 16 bytes; what lies behind a row's elements is never read as anything.
+struct Padding {
+    const unsigned short *src[3];
+    uint4 *dst[3];
+    unsigned long long units[3];
+    int line[3], count;
+};
+
+__global__ void __launch_bounds__(kThreads) linear_pad_kernel(const Padding p) {
+    const unsigned long long step = (unsigned long long)gridDim.x * kThreads, first = (unsigned long long)blockIdx.x * kThreads + threadIdx.x;
+    for (int i = 0; i < p.count; ++i) {
+        const int line = p.line[i];
+        const unsigned units = (unsigned)(line + 7) / 8;
+        for (unsigned long long u = first; u < p.units[i]; u += step) {
+            const unsigned long long row = u / units;
+            const int c = (int)(u - row * units) * 8;
+            const unsigned short *s = p.src[i] + row * line + c;
+            unsigned v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j] = (c + 2 * j < line ? (unsigned)s[2 * j] : 0u) | (c + 2 * j + 1 < line ? (unsigned)s[2 * j + 1] << 16 : 0u);
+            p.dst[i][u] = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+    }
 }
 
 inline int padded(int line) { return (line + 7) & ~7; }
 
-// src itself where its rows are aligned, else a padded copy in `place`; launches the copy.
-int aligned_rows(const void *&src, char *place, size_t rows, int line, cudaStream_t st) {
-    if (line % 8 == 0) return FDA_OK;
-    const unsigned long long elements = (unsigned long long)rows * line;
-    const unsigned blocks = (unsigned)std::min<unsigned long long>((elements + kThreads - 1) / kThreads, 16 * kSms);
-    linear_pad_kernel<<<blocks, kThreads, 0, st>>>(static_cast<const unsigned short *>(src), reinterpret_cast<unsigned short *>(place),
-                                                   elements, line, padded(line));
+// Where rows of `line` elements are aligned src stays itself, else it becomes `place`, and the copy is noted.
+void align_rows(Padding &p, const void *&src, char *place, size_t rows, int line) {
+    if (line % 8 == 0) return;
+    p.src[p.count] = static_cast<const unsigned short *>(src);
+    p.dst[p.count] = reinterpret_cast<uint4 *>(place);
+    p.units[p.count] = rows * (padded(line) / 8);
+    p.line[p.count++] = line;
     src = place;
+}
+
+int pad(const Padding &p, cudaStream_t st) {
+    if (p.count == 0) return FDA_OK;
+    const unsigned long long most = *std::max_element(p.units, p.units + p.count);
+    linear_pad_kernel<<<(unsigned)std::min<unsigned long long>((most + kThreads - 1) / kThreads, 16 * kSms), kThreads, 0, st>>>(p);
     return launched();
 }
 
@@ -381,18 +478,28 @@ void add_padded_operands(Layout &l, const Shape &s) {
     l.w = l.take((size_t)s.groups * s.out_features * padded(s.in_features) * 2);
 }
 
+// Inputs of an accumulator of the 16-bit weight gradient: the widest that leaves every SM a piece of 8 blocks.
+int mma_weight_tile(const Shape &s) {
+    const long long blocks = most_units(s.batch, s.rows, s.groups, kMmaSlice, false), rows = ceil_div(s.out_features, kMmaTileRows);
+    for (int tile = 256; tile > 64; tile /= 2)
+        if (s.in_features > tile / 2 && rows * ceil_div(s.in_features, tile) * ceil_div(blocks, 8) >= kSms) return tile;
+    return 64;
+}
+
 Cut weight_cut(const Shape &s) {
     if (s.dtype != FDA_DTYPE_F32) {
-        const long long tiles = ceil_div(s.out_features, kMmaTileRows) * ceil_div(s.in_features, mma_weight_tile(s.in_features));
+        const long long tiles = ceil_div(s.out_features, kMmaTileRows) * ceil_div(s.in_features, mma_weight_tile(s));
         return cut_rows(s.batch, s.rows, s.groups, tiles, kMmaSlice, 8);
     }
-    return cut_rows(s.batch, s.rows, s.groups, ceil_div(s.out_features, kTileSize) * ceil_div(s.in_features, kTileSize), kPlainBlock,
+    return cut_rows(s.batch, s.rows, s.groups, ceil_div(s.out_features, kTile) * ceil_div(s.in_features, kTile), kPlainBlock,
                     kPlainLeastPiece);
 }
 
+bool few_rows(const Shape &s);
+
 Layout forward_layout(const Shape &s) {
     Layout l;
-    add_padded_operands(l, s);
+    if (!few_rows(s)) add_padded_operands(l, s);
     return l;
 }
 
@@ -409,25 +516,57 @@ Layout backward_layout(const Shape &s, int activation) {
     return l;
 }
 
-int forward_f32(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *residual, void *y,
-                int activation, cudaStream_t st) {
-    RowProduct<float> p;
-    p.a = static_cast<const float *>(x);
-    p.w = static_cast<const float *>(weight);
-    p.bias = static_cast<const float *>(bias);
-    p.extra = static_cast<const float *>(residual);
-    p.out = static_cast<float *>(y);
-    p.depth = p.in_features = s.in_features;
-    p.cols = s.out_features;
-    p.g = g;
-    return run_rows<float, kForward>(p, activation, st);
+// Few rows in all (with groups: few enough that most groups have hardly any).
+bool few_rows(const Shape &s) { return total_rows(s) <= (s.groups > 1 ? 64 : 8); }
+
+template <typename T, int kMode>
+int run_few_rows(const RowProduct<T> &p, int activation, cudaStream_t st) {
+    const long long steps = ceil_div(p.cols, kFewOutputs);
+    const long long warps = most_units(p.g.batch, p.g.rows, p.g.groups, kFewRows, kMode != kPreGrad && p.g.starts) * steps;
+    const unsigned blocks = (unsigned)std::min<long long>(ceil_div(warps, kFewThreads / 32), 16 * kSms);
+    const bool vector = p.depth % (16 / sizeof(T)) == 0 && ((uintptr_t)p.a | (uintptr_t)p.w) % 16 == 0;
+    if (vector) linear_few_rows_kernel<T, kMode, true><<<blocks, kFewThreads, 0, st>>>(p, activation);
+    else linear_few_rows_kernel<T, kMode, false><<<blocks, kFewThreads, 0, st>>>(p, activation);
+    return launched();
 }
 
-int forward_narrow(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *residual, void *y,
-                   char *ws, int activation, cudaStream_t st) {
+// out = act(x W^T + bias) + extra, or extra * act'(x W^T + bias)
+template <typename T>
+RowProduct<T> row_product(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *extra, void *out,
+                          int out_pitch) {
+    RowProduct<T> p;
+    p.a = static_cast<const T *>(x);
+    p.w = static_cast<const T *>(weight);
+    p.bias = static_cast<const T *>(bias);
+    p.extra = static_cast<const T *>(extra);
+    p.out = static_cast<T *>(out);
+    p.depth = p.in_features = s.in_features;
+    p.cols = s.out_features;
+    p.out_pitch = out_pitch;
+    p.g = g;
+    return p;
+}
+
+template <int kMode>
+int run_few_rows(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *extra, void *out,
+                 int out_pitch, int activation, cudaStream_t st) {
+    if (s.dtype == FDA_DTYPE_F32)
+        return run_few_rows<float, kMode>(row_product<float>(s, g, x, weight, bias, extra, out, out_pitch), activation, st);
+    if (s.dtype == FDA_DTYPE_F16)
+        return run_few_rows<__half, kMode>(row_product<__half>(s, g, x, weight, bias, extra, out, out_pitch), activation, st);
+    return run_few_rows<__nv_bfloat16, kMode>(row_product<__nv_bfloat16>(s, g, x, weight, bias, extra, out, out_pitch), activation, st);
+}
+
+int forward(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *residual, void *y, char *ws,
+            int activation, cudaStream_t st) {
+    if (few_rows(s)) return run_few_rows<kForward>(s, g, x, weight, bias, residual, y, s.out_features, activation, st);
+    if (s.dtype == FDA_DTYPE_F32)
+        return run_rows<kForward>(row_product<float>(s, g, x, weight, bias, residual, y, s.out_features), activation, st);
     const Layout l = forward_layout(s);
-    if (const int rc = aligned_rows(x, ws + l.x, total_rows(s), s.in_features, st)) return rc;
-    if (const int rc = aligned_rows(weight, ws + l.w, (size_t)s.groups * s.out_features, s.in_features, st)) return rc;
+    Padding pads{};
+    align_rows(pads, x, ws + l.x, total_rows(s), s.in_features);
+    align_rows(pads, weight, ws + l.w, (size_t)s.groups * s.out_features, s.in_features);
+    if (const int rc = pad(pads, st)) return rc;
     const long long in = padded(s.in_features);
     const MmaRows p{x, weight, bias, residual, y, in, in, s.out_features, s.out_features, s.in_features, s.out_features, s.dtype, activation, g};
     return mma_rows(kForward, p, st);
@@ -469,34 +608,25 @@ WeightGrad<T> weight_grad_args(const Shape &s, const Groups &g, const Cut &c, co
 int backward_f32(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *grad_output,
                  const Gradients &out, char *ws, int activation, cudaStream_t st) {
     const Layout l = backward_layout(s, activation);
-    RowProduct<float> p;
-    p.w = static_cast<const float *>(weight);
-    p.bias = static_cast<const float *>(bias);
-    p.in_features = s.in_features;
-    p.g = g;
-    const float *grad = static_cast<const float *>(grad_output);
+    const void *grad = grad_output;
     if (activation != FDA_ACT_NONE) {
-        p.a = static_cast<const float *>(x);
-        p.extra = grad;
-        p.out = reinterpret_cast<float *>(ws + l.g);
-        p.depth = s.in_features;
-        p.cols = s.out_features;
-        if (const int rc = run_rows<float, kPreGrad>(p, activation, st)) return rc;
-        grad = p.out;
+        grad = ws + l.g;
+        const int rc = few_rows(s) ? run_few_rows<kPreGrad>(s, g, x, weight, bias, grad_output, ws + l.g, s.out_features, activation, st)
+                                   : run_rows<kPreGrad>(row_product<float>(s, g, x, weight, bias, grad_output, ws + l.g, s.out_features),
+                                                               activation, st);
+        if (rc) return rc;
     }
     if (out.x) {
-        p.a = grad;
-        p.bias = p.extra = nullptr;
-        p.out = static_cast<float *>(out.x);
+        RowProduct<float> p = row_product<float>(s, g, grad, weight, nullptr, nullptr, out.x, s.in_features);
         p.depth = s.out_features;
         p.cols = s.in_features;
-        if (const int rc = run_rows<float, kGradX>(p, FDA_ACT_NONE, st)) return rc;
+        if (const int rc = run_rows<kGradX, FDA_ACT_NONE>(p, st)) return rc;
     }
     if (!out.weight && !out.bias) return FDA_OK;
     const Cut c = weight_cut(s);
     const WeightGrad<float> q = weight_grad_args<float>(s, g, c, grad, x, out, ws, l);
-    const long long items = c.pieces * ceil_div(s.out_features, kTileSize) * ceil_div(s.in_features, kTileSize);
-    linear_weight_grad_kernel<float, kTileSize, kTileSize><<<(unsigned)std::min<long long>(items, 8 * kSms), kThreads, 0, st>>>(q);
+    const long long items = c.pieces * ceil_div(s.out_features, kTile) * ceil_div(s.in_features, kTile);
+    linear_weight_grad_kernel<<<(unsigned)std::min<long long>(items, 8 * kSms), kThreads, 0, st>>>(q);
     if (const int rc = launched()) return rc;
     return sum_slots(q, s, c, st);
 }
@@ -504,20 +634,20 @@ int backward_f32(const Shape &s, const Groups &g, const void *x, const void *wei
 int backward_narrow(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *grad_output,
                     const Gradients &out, char *ws, int activation, cudaStream_t st) {
     const Layout l = backward_layout(s, activation);
-    const bool weights = out.weight || out.bias;
+    const bool weights = out.weight || out.bias, few = few_rows(s);
     const long long in = padded(s.in_features), outs = padded(s.out_features);
-    if (activation != FDA_ACT_NONE || weights)
-        if (const int rc = aligned_rows(x, ws + l.x, total_rows(s), s.in_features, st)) return rc;
-    if (activation != FDA_ACT_NONE || out.x)
-        if (const int rc = aligned_rows(weight, ws + l.w, (size_t)s.groups * s.out_features, s.in_features, st)) return rc;
-    const void *grad = grad_output;
+    const void *dense_x = x, *dense_weight = weight, *grad = activation != FDA_ACT_NONE ? ws + l.g : grad_output;
+    Padding pads{};
+    if ((activation != FDA_ACT_NONE && !few) || weights) align_rows(pads, x, ws + l.x, total_rows(s), s.in_features);
+    if ((activation != FDA_ACT_NONE && !few) || out.x) align_rows(pads, weight, ws + l.w, (size_t)s.groups * s.out_features, s.in_features);
+    if (activation == FDA_ACT_NONE) align_rows(pads, grad, ws + l.g, total_rows(s), s.out_features);
+    if (const int rc = pad(pads, st)) return rc;
     if (activation != FDA_ACT_NONE) {
         const MmaRows p{x, weight, bias, grad_output, ws + l.g, in, in, s.out_features, outs, s.in_features, s.out_features, s.dtype,
                         activation, g};
-        if (const int rc = mma_rows(kPreGrad, p, st)) return rc;
-        grad = ws + l.g;
-    } else if (const int rc = aligned_rows(grad, ws + l.g, total_rows(s), s.out_features, st)) {
-        return rc;
+        const int rc = few ? run_few_rows<kPreGrad>(s, g, dense_x, dense_weight, bias, grad_output, ws + l.g, (int)outs, activation, st)
+                           : mma_rows(kPreGrad, p, st);
+        if (rc) return rc;
     }
     if (out.x) {
         const MmaRows p{grad, weight, nullptr, nullptr, out.x, outs, in, 0, s.in_features, s.in_features, s.out_features, s.dtype,
@@ -527,7 +657,7 @@ int backward_narrow(const Shape &s, const Groups &g, const void *x, const void *
     if (!weights) return FDA_OK;
     const Cut c = weight_cut(s);
     const MmaWeightGrad q{grad, x, outs, in, out.weight, out.bias, reinterpret_cast<float *>(ws + l.slots),
-                          reinterpret_cast<float *>(ws + l.bias_slots), s.in_features, s.out_features, s.dtype, c, g};
+                          reinterpret_cast<float *>(ws + l.bias_slots), s.in_features, s.out_features, s.dtype, mma_weight_tile(s), c, g};
     if (const int rc = mma_weight_grad(q, st)) return rc;
     if (s.dtype == FDA_DTYPE_F16) return sum_slots(weight_grad_args<__half>(s, g, c, nullptr, nullptr, out, ws, l), s, c, st);
     return sum_slots(weight_grad_args<__nv_bfloat16>(s, g, c, nullptr, nullptr, out, ws, l), s, c, st);
@@ -558,9 +688,8 @@ int fda_linear_forward(const void *x, const void *weight, const void *bias, cons
     if ((uintptr_t)workspace % 256) return FDA_ERR_MISALIGNED;
     const Groups g{group_start_index, num_starts, groups, batch, rows};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == FDA_DTYPE_F32) return forward_f32(s, g, x, weight, bias, residual, y, activation, st);
-    if (misaligned16(x) || misaligned16(weight)) return FDA_ERR_MISALIGNED;
-    return forward_narrow(s, g, x, weight, bias, residual, y, static_cast<char *>(workspace), activation, st);
+    if (dtype != FDA_DTYPE_F32 && (misaligned16(x) || misaligned16(weight))) return FDA_ERR_MISALIGNED;
+    return forward(s, g, x, weight, bias, residual, y, static_cast<char *>(workspace), activation, st);
 }
 
 size_t fda_linear_backward_workspace_bytes(int batch, int rows, int groups, int in_features, int out_features, int activation, int dtype) {

@@ -63,6 +63,26 @@ __device__ __forceinline__ float activate_backward(float v, float dy) {
     return dy;
 }
 
+// The same with the activation as an argument, where few elements pass.
+__device__ __forceinline__ float activate_any(int act, float v) {
+    switch (act) {
+        case FDA_ACT_RELU: return activate<FDA_ACT_RELU>(v);
+        case FDA_ACT_GELU: return activate<FDA_ACT_GELU>(v);
+        case FDA_ACT_GELU_TANH: return activate<FDA_ACT_GELU_TANH>(v);
+        case FDA_ACT_SILU: return activate<FDA_ACT_SILU>(v);
+        default: return v;
+    }
+}
+__device__ __forceinline__ float activate_backward_any(int act, float v, float dy) {
+    switch (act) {
+        case FDA_ACT_RELU: return activate_backward<FDA_ACT_RELU>(v, dy);
+        case FDA_ACT_GELU: return activate_backward<FDA_ACT_GELU>(v, dy);
+        case FDA_ACT_GELU_TANH: return activate_backward<FDA_ACT_GELU_TANH>(v, dy);
+        case FDA_ACT_SILU: return activate_backward<FDA_ACT_SILU>(v, dy);
+        default: return dy;
+    }
+}
+
 struct Groups {
     const int64_t *starts;  // nullptr: one group of all rows
     int num_starts;         // groups or groups + 1
@@ -265,13 +285,11 @@ struct MmaWeightGrad {
     void *grad_weight, *grad_bias;  // either may be nullptr
     float *slots, *bias_slots;
     int in_features, out_features, dtype;
+    int tile;  // inputs of an accumulator: 64, 128 or 256
     Cut cut;
     Groups g;
 };
-// About a piece per SM over `tiles` tiles of the weight, none shorter than `least_piece` blocks.
-Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int least_piece);
 constexpr int kMmaTileRows = 128, kMmaSlice = 64;  // accumulator rows; contraction indices of a slice (and rows of a PieceTable's block)
-inline int mma_weight_tile(int in_features) { return in_features > 128 ? 256 : in_features > 64 ? 128 : 64; }
 int mma_weight_grad_f16(const MmaWeightGrad &p, cudaStream_t st);  // without the sum over slots
 int mma_weight_grad_bf16(const MmaWeightGrad &p, cudaStream_t st);
 int mma_timeouts_f16();  // -1 where the device cannot be asked

@@ -640,7 +640,7 @@ int launch_weight_grad(const MmaWeightGrad &p, cudaStream_t st) {
 
 template <typename T, bool kVector>
 int weight_grad_of(const MmaWeightGrad &p, cudaStream_t st) {
-    switch (mma_weight_tile(p.in_features)) {
+    switch (p.tile) {
         case 256: return launch_weight_grad<T, 256, kVector>(p, st);
         case 128: return launch_weight_grad<T, 128, kVector>(p, st);
         default: return launch_weight_grad<T, 64, kVector>(p, st);
