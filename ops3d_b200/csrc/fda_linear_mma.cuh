@@ -56,13 +56,13 @@ struct Barrier {
     }
 };
 
-// A place in a ring of kStages, with the parity of its current round.
-template <int kStages>
+// A place in a ring, with the parity of its current round.
 struct Ring {
-    int stage = 0;
+    int stages, stage = 0;
     unsigned round = 0;
+    __device__ __forceinline__ explicit Ring(int stages) : stages(stages) {}
     __device__ __forceinline__ void next() {
-        if (++stage == kStages) { stage = 0; round ^= 1; }
+        if (++stage == stages) { stage = 0; round ^= 1; }
     }
 };
 
@@ -299,13 +299,13 @@ struct Fetched {
     uint4 part[4];
 };
 template <typename T>
-__device__ __forceinline__ void fetch_rows(const T *p, long long pitch, int rows, int count, Fetched &f) {
+__device__ __forceinline__ void fetch_rows(const T *p, unsigned pitch, int rows, int count, Fetched &f) {
     const int lane = threadIdx.x % 32, unit = lane % 4;
-    const T *mine = p + (lane / 4) * pitch + 8 * unit;
+    const T *mine = p + ((size_t)((lane / 4) * pitch) + 8 * unit);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         f.part[i] = make_uint4(0, 0, 0, 0);
-        if (lane / 4 + 8 * i < rows && 8 * unit < count) f.part[i] = __ldg(reinterpret_cast<const uint4 *>(mine + 8 * i * pitch));
+        if (lane / 4 + 8 * i < rows && 8 * unit < count) f.part[i] = __ldg(reinterpret_cast<const uint4 *>(mine + (size_t)(8 * i * pitch)));
     }
 }
 __device__ __forceinline__ void own_row_from(Stage &stage, int half, uint32_t (&v)[16]) {
@@ -330,20 +330,20 @@ __device__ __forceinline__ void rows_of_fetched(const Fetched &f, Stage &stage, 
 }
 // Rows that no vector access reaches.
 template <typename T>
-__device__ __forceinline__ void load_elements(const T *p, long long pitch, int rows, int count, Stage &stage, uint32_t (&v)[16]) {
+__device__ __forceinline__ void load_elements(const T *p, unsigned pitch, int rows, int count, Stage &stage, uint32_t (&v)[16]) {
     const int lane = threadIdx.x % 32;
     const unsigned short *s = reinterpret_cast<const unsigned short *>(p);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         __syncwarp();
 #pragma unroll 4
-        for (int r = 0; r < 16; ++r) *stage_element(stage, r, lane) = (16 * half + r < rows && lane < count) ? s[(16 * half + r) * pitch + lane] : 0;
+        for (int r = 0; r < 16; ++r) *stage_element(stage, r, lane) = (16 * half + r < rows && lane < count) ? s[(size_t)((16 * half + r) * pitch) + lane] : 0;
         __syncwarp();
         own_row_from(stage, half, v);
     }
 }
 template <bool kVector, typename T>
-__device__ __forceinline__ void store_rows(T *p, long long pitch, int rows, int count, Stage &stage, const uint32_t (&v)[16]) {
+__device__ __forceinline__ void store_rows(T *p, unsigned pitch, int rows, int count, Stage &stage, const uint32_t (&v)[16]) {
     const int lane = threadIdx.x % 32;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -354,16 +354,16 @@ __device__ __forceinline__ void store_rows(T *p, long long pitch, int rows, int 
                 stage[stage_unit(lane % 16, u)] = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
         __syncwarp();
         if (kVector) {
-            T *mine = p + (16 * half + lane / 4) * pitch + 8 * (lane % 4);
+            T *mine = p + ((size_t)((16 * half + lane / 4) * pitch) + 8 * (lane % 4));
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 if (16 * half + lane / 4 + 8 * i < rows && 8 * (lane % 4) < count)
-                    *reinterpret_cast<uint4 *>(mine + 8 * i * pitch) = stage[stage_unit(lane / 4 + 8 * i, lane % 4)];
+                    *reinterpret_cast<uint4 *>(mine + (size_t)(8 * i * pitch)) = stage[stage_unit(lane / 4 + 8 * i, lane % 4)];
         } else {
             unsigned short *s = reinterpret_cast<unsigned short *>(p);
 #pragma unroll 4
             for (int r = 0; r < 16; ++r)
-                if (16 * half + r < rows && lane < count) s[(16 * half + r) * pitch + lane] = *stage_element(stage, r, lane);
+                if (16 * half + r < rows && lane < count) s[(size_t)((16 * half + r) * pitch) + lane] = *stage_element(stage, r, lane);
         }
     }
 }

@@ -37,7 +37,7 @@ constexpr int kFirstEpilogueWarp = 4;
 // Common to both kernels: the ring, the accumulators' barriers, tensor memory.
 template <int kStages>
 struct Pipeline {
-    Barrier full[kStages], empty[kStages], sums_full[2], sums_empty[2], drained;
+    Barrier full[kStages], empty[kStages], sums_full[2], sums_empty[2], weight_empty, drained;
     uint32_t tmem;
     volatile int failed;
 };
@@ -53,6 +53,7 @@ __device__ __forceinline__ void pipeline_begin(Pipeline<kStages> &p, int columns
             p.sums_full[i].init(1);
             p.sums_empty[i].init(epilogue_warps);
         }
+        p.weight_empty.init(1);
         p.drained.init(1);
         p.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -65,7 +66,7 @@ __device__ __forceinline__ void pipeline_begin(Pipeline<kStages> &p, int columns
 // After every role has left.  In a sound run nothing is in flight any more (the epilogue has waited for every product, and so
 // for every copy); after a wait that ran out, copies and products still running are waited for, again with a limit.
 template <int kStages>
-__device__ __forceinline__ void pipeline_end(Pipeline<kStages> &p, int columns, const Ring<kStages> &issued, bool any) {
+__device__ __forceinline__ void pipeline_end(Pipeline<kStages> &p, int columns, const Ring &issued, bool any) {
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
@@ -73,7 +74,7 @@ __device__ __forceinline__ void pipeline_end(Pipeline<kStages> &p, int columns, 
         atomicAdd(&g_timeouts, 1u);
         volatile int again = 0;
         if (any)
-            for (int i = 0; i < kStages; ++i) {
+            for (int i = 0; i < issued.stages; ++i) {
                 // the ring's next place is `issued`: a place before it was last filled in the current round, the others in the one before
                 const unsigned parity = i < issued.stage ? issued.round : issued.round ^ 1;
                 p.full[i].wait(parity, &again);
@@ -95,10 +96,17 @@ template <typename T>
 struct RowsArgs {
     const T *bias, *extra;
     T *out;
-    long long extra_pitch, out_pitch;
+    unsigned extra_pitch, out_pitch;  // 32 of them fit 32 bits (the host has checked)
     int depth, cols;
+    bool resident;
     Groups g;
 };
+
+// A resident weight: where all slices of a column tile fit (kResidentBytes), a block keeps them and only rows stream through the
+// ring.  Blocks walk the tiles column by column, a contiguous range each, so the weight changes with the group or not at all.
+// Per 128 x 256 tile of 256 inputs 64 KB instead of 192 pass from L2, whose 9 TB/s had been the bound (149504 x 256 x 1024: 107 us).
+constexpr int kResidentStages = 4;
+constexpr int kResidentBytes = kRingBytes - kResidentStages * kBytesA;
 
 constexpr int kForwardPlain = 3;  // kForward without a residual
 
@@ -146,35 +154,52 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
     build_row_table(p.g, kTileRows, kMode != kPreGrad, table);
     __syncthreads();
     fence_after_sync();
-    const unsigned column_tiles = (p.cols + BN - 1) / BN;
+    const unsigned units = (unsigned)table.unit_begin[p.g.groups + 2] * p.g.batch;
+    const unsigned tiles = units * ((p.cols + BN - 1) / BN);  // the host has checked that they fit
+    const unsigned tile_begin = (unsigned)((unsigned long long)blockIdx.x * tiles / gridDim.x);
+    const unsigned tile_end = (unsigned)((unsigned long long)(blockIdx.x + 1) * tiles / gridDim.x);
     const int slices = (p.depth + kSliceK - 1) / kSliceK;
-    const unsigned tiles = (unsigned)table.unit_begin[p.g.groups + 2] * p.g.batch * column_tiles;  // the host has checked that they fit
+    char *const weight = p.resident ? ring + kResidentStages * kBytesA : ring + kBytesA;  // of the first slice or the first stage
+    const int stage_bytes = p.resident ? kBytesA : Shape<BN>::kBytes, weight_step = p.resident ? Shape<BN>::kBytesB : 0;
     volatile int *const failed = &pipe.failed;
-    Ring<kStages> ring_at;
+    Ring ring_at(p.resident ? kResidentStages : kStages);
     bool any = false;
 
     if (warp == 0) {
         if (lane == 0) {
             bool sound = true;
-            for (unsigned tile = blockIdx.x; tile < tiles && sound; tile += gridDim.x) {
-                const RowUnit u = row_unit(p.g, table, kTileRows, tile / column_tiles);
+            int weight_group = -1, weight_col = -1;
+            unsigned changes = 0;
+            for (unsigned tile = tile_begin; tile < tile_end && sound; ++tile) {
+                const RowUnit u = row_unit(p.g, table, kTileRows, tile % units);
                 if (u.group < 0) continue;
-                const int col0 = (int)(tile % column_tiles * BN);
+                const int col0 = (int)(tile / units * BN);
                 if (kExtra && kVector)  // on their way to L2 while the tile's products run: the epilogue's loads then wait for L2 only
 #pragma unroll
                     for (int i = 0; i < BN / 64; ++i) prefetch_2d(&map_extra, col0 + 64 * i, (int)u.row);
+                const bool fresh = !p.resident || u.group != weight_group || col0 != weight_col;
+                if (p.resident && fresh) {  // the products with the weight before have to be through
+                    if (changes++) sound = pipe.weight_empty.wait(changes & 1, failed);
+                    if (!sound) break;
+                    weight_group = u.group;
+                    weight_col = col0;
+                }
                 for (int s = 0; s < slices; ++s) {
                     sound = pipe.empty[ring_at.stage].wait(ring_at.round ^ 1, failed);
                     if (!sound) break;
-                    char *a = ring + ring_at.stage * Shape<BN>::kBytes, *b = a + kBytesA;
+                    char *a = ring + ring_at.stage * stage_bytes;
                     Barrier *bar = &pipe.full[ring_at.stage];
-                    bar->arrive_expect(Shape<BN>::kBytes);
+                    bar->arrive_expect(kBytesA + (fresh ? Shape<BN>::kBytesB : 0));
                     tma_2d(&map_a, a, bar, s * kSliceK, (int)u.row);
-                    if (kWeightMn) {
+                    if (fresh) {
+                        char *b = weight + (p.resident ? s * weight_step : ring_at.stage * stage_bytes);
+                        if (kWeightMn) {
 #pragma unroll
-                        for (int i = 0; i < BN / 64; ++i) tma_3d(&map_w, b + i * (64 * kSliceK * 2), bar, col0 + 64 * i, s * kSliceK, u.group);
-                    } else {
-                        tma_3d(&map_w, b, bar, s * kSliceK, col0, u.group);
+                            for (int i = 0; i < BN / 64; ++i)
+                                tma_3d(&map_w, b + i * (64 * kSliceK * 2), bar, col0 + 64 * i, s * kSliceK, u.group);
+                        } else {
+                            tma_3d(&map_w, b, bar, s * kSliceK, col0, u.group);
+                        }
                     }
                     ring_at.next();
                     any = true;
@@ -185,11 +210,18 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t kInstruction = instruction<T>(kTileRows, BN, false, kWeightMn);
-            Ring<2> sums;
+            Ring sums(2);
             bool sound = true;
-            for (unsigned tile = blockIdx.x; tile < tiles && sound; tile += gridDim.x) {
-                const RowUnit u = row_unit(p.g, table, kTileRows, tile / column_tiles);
+            int weight_group = -1, weight_col = -1;
+            for (unsigned tile = tile_begin; tile < tile_end && sound; ++tile) {
+                const RowUnit u = row_unit(p.g, table, kTileRows, tile % units);
                 if (u.group < 0) continue;
+                const int col0 = (int)(tile / units * BN);
+                if (p.resident && (u.group != weight_group || col0 != weight_col)) {
+                    if (weight_group >= 0) mma_commit(&pipe.weight_empty);
+                    weight_group = u.group;
+                    weight_col = col0;
+                }
                 sound = pipe.sums_empty[sums.stage].wait(sums.round ^ 1, failed);
                 if (!sound) break;
                 fence_after_sync();
@@ -198,7 +230,8 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                     sound = pipe.full[ring_at.stage].wait(ring_at.round, failed);
                     if (!sound) break;
                     fence_after_sync();
-                    const char *a = ring + ring_at.stage * Shape<BN>::kBytes, *b = a + kBytesA;
+                    const char *a = ring + ring_at.stage * stage_bytes;
+                    const char *b = weight + (p.resident ? s * weight_step : ring_at.stage * stage_bytes);
 #pragma unroll
                     for (int k = 0; k < kSliceK / 16; ++k) {
                         const uint64_t da = operand(a + 32 * k, 16, kAtom);
@@ -224,28 +257,47 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         Stage &stage = stages[warp - kFirstEpilogueWarp];
         for (int i = lane; i < kPart; i += 32) bias[i] = 0.f;
         int bias_group = -1, bias_col = -1;
-        Ring<2> sums;
-        for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-            const RowUnit u = row_unit(p.g, table, kTileRows, tile / column_tiles);
-            const int col0 = (int)(tile % column_tiles * BN) + part * kPart;
-            const int rows = u.count - quarter * 32;  // of this warp; none or fewer where not positive
-            const long long first = u.row + quarter * 32;
-            T *out_rows = p.out + first * p.out_pitch + col0;
-            const T *extra_rows = kExtra ? p.extra + first * p.extra_pitch + col0 : nullptr;
-            Fetched fetched;  // the next chunk's extra rows
-            const auto fetch = [&](int c) {
-                if (kExtra && kVector && c < kChunks)
-                    fetch_rows(extra_rows + 32 * c, p.extra_pitch, rows, p.cols - col0 - 32 * c, fetched);
-            };
-            const auto extra_of = [&](int c, int count, uint32_t(&v)[16]) {  // chunk c of the extra rows, lane by row; asks for the next
+        Ring sums(2);
+        struct Place {
+            long long first;  // row of the warp's part of a tile
+            int rows, col0, group;
+        };
+        const auto place = [&](unsigned tile) {
+            const RowUnit u = row_unit(p.g, table, kTileRows, tile % units);
+            Place at;
+            at.first = u.row + quarter * 32;
+            at.rows = u.count - quarter * 32;  // none or fewer where not positive
+            at.col0 = (int)(tile / units * BN) + part * kPart;
+            at.group = u.group;
+            return at;
+        };
+        Fetched fetched;  // the extra rows of the chunk to come
+        const auto fetch = [&](const Place &at, int c) {
+            if (kExtra && kVector)
+                fetch_rows(p.extra + (size_t)at.first * p.extra_pitch + at.col0 + 32 * c, p.extra_pitch, at.rows, p.cols - at.col0 - 32 * c, fetched);
+        };
+        Place next;
+        if (tile_begin < tile_end) {
+            next = place(tile_begin);
+            fetch(next, 0);
+        }
+        for (unsigned tile = tile_begin; tile < tile_end; ++tile) {
+            const Place u = next;
+            if (tile + 1 < tile_end) next = place(tile + 1);
+            const int rows = u.rows, col0 = u.col0;
+            T *const out_rows = p.out + (size_t)u.first * p.out_pitch + col0;
+            const auto extra_of = [&](int c, int count, uint32_t(&v)[16]) {  // chunk c of the extra rows, lane by row; asks for the one after
                 if (kExtra && kVector) {
                     rows_of_fetched(fetched, stage, v);
-                    fetch(c + 1);
+                    if (c + 1 < kChunks && count > 32) fetch(u, c + 1);
+                    else if (tile + 1 < tile_end) fetch(next, 0);
                 } else if (kExtra) {
-                    load_elements(extra_rows + 32 * c, p.extra_pitch, rows, count, stage, v);
+                    load_elements(p.extra + (size_t)u.first * p.extra_pitch + col0 + 32 * c, p.extra_pitch, rows, count, stage, v);
                 }
             };
-            fetch(0);
+            if (col0 >= p.cols) {  // no column of this part: nothing is fetched or stored, but the tile counts
+                if (tile + 1 < tile_end) fetch(next, 0);
+            }
             if (kMode != kGradX) {
                 if (p.bias && u.group >= 0 && (u.group != bias_group || col0 != bias_col)) {
                     __syncwarp();
@@ -338,7 +390,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
     const int per_piece = out_tiles * in_tiles;
     const long long items = (long long)table.piece_begin[p.g.groups] * per_piece;
     volatile int *const failed = &pipe.failed;
-    Ring<kStages> ring_at;
+    Ring ring_at(kStages);
     bool any = false;
 
     struct Item {
@@ -555,7 +607,7 @@ int allow_shared(Kernel kernel, int bytes) {
 }
 
 template <typename T, int kMode, int kAct, int BN, bool kVector>
-int launch_rows(const RowsArgs<T> &a, const MmaRows &p, long long units, cudaStream_t st) {
+int launch_rows(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t st) {
     constexpr int kSmem = Shape<BN>::kStages * Shape<BN>::kBytes + kAtom;
     const auto kernel = linear_rows_mma_kernel<T, kMode, kAct, BN, kVector>;
     if (const int rc = allow_shared(kernel, kSmem)) return rc;
@@ -569,6 +621,7 @@ int launch_rows(const RowsArgs<T> &a, const MmaRows &p, long long units, cudaStr
     } else {
         map_extra = map_a;
     }
+    a.resident = ceil_div(a.depth, kSliceK) * Shape<BN>::kBytesB <= kResidentBytes;
     const long long tiles = units * ceil_div(a.cols, BN);
     if (tiles >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
     kernel<<<(unsigned)std::min<long long>(tiles, kSms), Shape<BN>::kThreads, kSmem, st>>>(a, map_a, map_w, map_extra);
@@ -581,8 +634,9 @@ int rows_of(const MmaRows &p, cudaStream_t st) {
     a.bias = static_cast<const T *>(p.bias);
     a.extra = static_cast<const T *>(p.extra);
     a.out = static_cast<T *>(p.out);
-    a.extra_pitch = p.extra_pitch;
-    a.out_pitch = p.out_pitch;
+    a.extra_pitch = (unsigned)p.extra_pitch;
+    a.out_pitch = (unsigned)p.out_pitch;
+    if (p.extra_pitch >= (1 << 26) || p.out_pitch >= (1 << 26)) return FDA_ERR_BAD_SHAPE;
     a.depth = kMode == kGradX ? p.out_features : p.in_features;
     a.cols = kMode == kGradX ? p.in_features : p.out_features;
     a.g = p.g;
