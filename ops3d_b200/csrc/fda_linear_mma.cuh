@@ -56,6 +56,26 @@ struct Barrier {
     }
 };
 
+// The address in another block of the cluster that corresponds to one of this block's.
+__device__ __forceinline__ uint32_t cluster_address(const void *p, unsigned rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_address(p)), "r"(rank));
+    return r;
+}
+// Relaxed: what it announces are reads of tensor memory, which tcgen05.wait::ld has ended and tcgen05.fence orders.  A release across the
+// cluster would wait for the caller's global stores besides (per tile of 256 x 256: 9 us instead of 6).
+__device__ __forceinline__ void arrive_at(uint32_t cluster_barrier) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_barrier) : "memory");
+}
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // A place in a ring, with the parity of its current round.
 struct Ring {
     int stages, stage = 0;
@@ -77,6 +97,20 @@ __device__ __forceinline__ void tma_3d(const CUtensorMap *map, void *dst, Barrie
                      smem_address(dst)),
                  "l"(map), "r"(smem_address(bar)), "r"(x), "r"(y), "r"(z)
                  : "memory");
+}
+// The same for a pair of blocks: the copy goes to this block's memory and signals a barrier of either.
+__device__ __forceinline__ void tma_2d_pair(const CUtensorMap *map, void *dst, uint32_t bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+                     smem_address(dst)),
+                 "l"(map), "r"(bar), "r"(x), "r"(y)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_3d_pair(const CUtensorMap *map, void *dst, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            smem_address(dst)),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
 }
 // A box of a matrix into L2.
 __device__ __forceinline__ void prefetch_2d(const CUtensorMap *map, int x, int y) {
@@ -103,6 +137,26 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
 // Arrives on the barrier when every tcgen05 operation issued so far by this thread has ended.
 __device__ __forceinline__ void mma_commit(Barrier *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_address(bar)) : "memory");
+}
+// The same for a pair of blocks (cta_group::2): both allocate and free, the first issues the products, a commit arrives in both.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t *slot, int columns) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(slot)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free_pair(uint32_t address, int columns) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
+}
+__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b),
+        "r"(instruction), "r"((unsigned)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit_pair(Barrier *bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                     smem_address(bar)),
+                 "h"((unsigned short)3)
+                 : "memory");
 }
 // 32 lanes x 16 or 32 columns of fp32: register j of a lane is column j of its row.
 __device__ __forceinline__ void tmem_load(uint32_t address, uint32_t (&v)[16]) {

@@ -103,7 +103,9 @@ struct RowsArgs {
 };
 
 // A resident weight: where all slices of a column tile fit (kResidentBytes), a block keeps them and only rows stream through the
-// ring.  Blocks walk the tiles column by column, a contiguous range each, so the weight changes with the group or not at all.
+// ring.  The grid is a multiple of the column tiles, so a block's column stays and its weight changes with the group or not at all;
+// at any time the blocks work on neighbouring rows (a contiguous range of rows each was slower: 172 instead of 15x us for
+// 149504 x 256 x 1024 with a residual).
 // Per 128 x 256 tile of 256 inputs 64 KB instead of 192 pass from L2, whose 9 TB/s had been the bound (149504 x 256 x 1024: 107 us).
 constexpr int kResidentStages = 4;
 constexpr int kResidentBytes = kRingBytes - kResidentStages * kBytesA;
@@ -154,10 +156,8 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
     build_row_table(p.g, kTileRows, kMode != kPreGrad, table);
     __syncthreads();
     fence_after_sync();
-    const unsigned units = (unsigned)table.unit_begin[p.g.groups + 2] * p.g.batch;
-    const unsigned tiles = units * ((p.cols + BN - 1) / BN);  // the host has checked that they fit
-    const unsigned tile_begin = (unsigned)((unsigned long long)blockIdx.x * tiles / gridDim.x);
-    const unsigned tile_end = (unsigned)((unsigned long long)(blockIdx.x + 1) * tiles / gridDim.x);
+    const unsigned columns = (p.cols + BN - 1) / BN;
+    const unsigned tiles = (unsigned)table.unit_begin[p.g.groups + 2] * p.g.batch * columns;  // the host has checked that they fit
     const int slices = (p.depth + kSliceK - 1) / kSliceK;
     char *const weight = p.resident ? ring + kResidentStages * kBytesA : ring + kBytesA;  // of the first slice or the first stage
     const int stage_bytes = p.resident ? kBytesA : Shape<BN>::kBytes, weight_step = p.resident ? Shape<BN>::kBytesB : 0;
@@ -170,10 +170,10 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
             bool sound = true;
             int weight_group = -1, weight_col = -1;
             unsigned changes = 0;
-            for (unsigned tile = tile_begin; tile < tile_end && sound; ++tile) {
-                const RowUnit u = row_unit(p.g, table, kTileRows, tile % units);
+            for (unsigned tile = blockIdx.x; tile < tiles && sound; tile += gridDim.x) {
+                const RowUnit u = row_unit(p.g, table, kTileRows, tile / columns);
                 if (u.group < 0) continue;
-                const int col0 = (int)(tile / units * BN);
+                const int col0 = (int)(tile % columns * BN);
                 if (kExtra && kVector)  // on their way to L2 while the tile's products run: the epilogue's loads then wait for L2 only
 #pragma unroll
                     for (int i = 0; i < BN / 64; ++i) prefetch_2d(&map_extra, col0 + 64 * i, (int)u.row);
@@ -213,10 +213,10 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
             Ring sums(2);
             bool sound = true;
             int weight_group = -1, weight_col = -1;
-            for (unsigned tile = tile_begin; tile < tile_end && sound; ++tile) {
-                const RowUnit u = row_unit(p.g, table, kTileRows, tile % units);
+            for (unsigned tile = blockIdx.x; tile < tiles && sound; tile += gridDim.x) {
+                const RowUnit u = row_unit(p.g, table, kTileRows, tile / columns);
                 if (u.group < 0) continue;
-                const int col0 = (int)(tile / units * BN);
+                const int col0 = (int)(tile % columns * BN);
                 if (p.resident && (u.group != weight_group || col0 != weight_col)) {
                     if (weight_group >= 0) mma_commit(&pipe.weight_empty);
                     weight_group = u.group;
@@ -263,11 +263,11 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
             int rows, col0, group;
         };
         const auto place = [&](unsigned tile) {
-            const RowUnit u = row_unit(p.g, table, kTileRows, tile % units);
+            const RowUnit u = row_unit(p.g, table, kTileRows, tile / columns);
             Place at;
             at.first = u.row + quarter * 32;
             at.rows = u.count - quarter * 32;  // none or fewer where not positive
-            at.col0 = (int)(tile / units * BN) + part * kPart;
+            at.col0 = (int)(tile % columns * BN) + part * kPart;
             at.group = u.group;
             return at;
         };
@@ -277,26 +277,26 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                 fetch_rows(p.extra + (size_t)at.first * p.extra_pitch + at.col0 + 32 * c, p.extra_pitch, at.rows, p.cols - at.col0 - 32 * c, fetched);
         };
         Place next;
-        if (tile_begin < tile_end) {
-            next = place(tile_begin);
+        if (blockIdx.x < tiles) {
+            next = place(blockIdx.x);
             fetch(next, 0);
         }
-        for (unsigned tile = tile_begin; tile < tile_end; ++tile) {
+        for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
             const Place u = next;
-            if (tile + 1 < tile_end) next = place(tile + 1);
+            if (tile + gridDim.x < tiles) next = place(tile + gridDim.x);
             const int rows = u.rows, col0 = u.col0;
             T *const out_rows = p.out + (size_t)u.first * p.out_pitch + col0;
             const auto extra_of = [&](int c, int count, uint32_t(&v)[16]) {  // chunk c of the extra rows, lane by row; asks for the one after
                 if (kExtra && kVector) {
                     rows_of_fetched(fetched, stage, v);
                     if (c + 1 < kChunks && count > 32) fetch(u, c + 1);
-                    else if (tile + 1 < tile_end) fetch(next, 0);
+                    else if (tile + gridDim.x < tiles) fetch(next, 0);
                 } else if (kExtra) {
                     load_elements(p.extra + (size_t)u.first * p.extra_pitch + col0 + 32 * c, p.extra_pitch, rows, count, stage, v);
                 }
             };
             if (col0 >= p.cols) {  // no column of this part: nothing is fetched or stored, but the tile counts
-                if (tile + 1 < tile_end) fetch(next, 0);
+                if (tile + gridDim.x < tiles) fetch(next, 0);
             }
             if (kMode != kGradX) {
                 if (p.bias && u.group >= 0 && (u.group != bias_group || col0 != bias_col)) {
@@ -345,6 +345,288 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         }
     }
     pipeline_end(pipe, kColumns, ring_at, any);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// Products over rows by pairs of blocks
+// ---------------------------------------------------------------------------------------------------------------------------
+// Two blocks of a cluster make one tile of 256 x 256 (cta_group::2): each brings its own 128 rows and its half of the weight's 256
+// columns and keeps 128 rows of sums, so per block half the weight passes from L2 and lies in shared memory.  Where there are
+// extra rows, what that leaves holds a buffer of 32 rows x 64 columns for each of the 16 epilogue warps, which the copy engine
+// fills a tile ahead; otherwise it makes the ring longer.
+//
+// The first block issues all products; the barriers that these wait for are its own, and the second block's copies and epilogue
+// warps signal them across the cluster.
+constexpr int kPairRows = 256, kPairColumns = 256, kPairEpilogueWarps = 16;
+constexpr int kPairThreads = 32 * (kFirstEpilogueWarp + kPairEpilogueWarps);
+constexpr int kPairBytesB = kPairColumns / 2 * kSliceK * 2;  // a block's half of a weight slice
+constexpr int kPairMaxStages = 8, kPairLeastStages = 4;
+constexpr int kPairOperands = 192 * 1024, kBufferBytes = 32 * 64 * 2;
+__host__ __device__ constexpr int pair_ring(bool extra) { return kPairOperands - (extra ? kPairEpilogueWarps * kBufferBytes : 0); }
+constexpr int kPairSmem = kPairOperands + kAtom;
+
+struct PairPipeline {
+    Barrier full[kPairMaxStages], empty[kPairMaxStages], sums_full[2], sums_empty[2], weight_empty, drained;
+    Barrier extra_full[kPairEpilogueWarps], extra_empty[kPairEpilogueWarps];
+    uint32_t tmem;
+    volatile int failed;
+};
+
+// Unit u (16 bytes) of row r in a buffer, as the copy engine's 128-byte swizzle has it.
+__device__ __forceinline__ const uint4 *buffer_unit(const char *buffer, int r, int u) {
+    return reinterpret_cast<const uint4 *>(buffer + r * 128 + ((u ^ (r & 7)) * 16));
+}
+
+template <typename T, int kMode, int kAct>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    linear_rows_pair_kernel(const RowsArgs<T> p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                            const __grid_constant__ CUtensorMap map_extra) {
+    constexpr bool kWeightMn = kMode == kGradX;
+    constexpr bool kExtra = kMode == kForward || kMode == kPreGrad;
+    constexpr int kColumns = 512;
+    extern __shared__ char dynamic[];
+    __shared__ RowTable table;
+    __shared__ PairPipeline pipe;
+    __shared__ __align__(16) float bias_of[kPairEpilogueWarps][64];
+    __shared__ __align__(16) Stage stages_of[kPairEpilogueWarps];
+    char *const ring = reinterpret_cast<char *>(((uintptr_t)dynamic + kAtom - 1) & ~(uintptr_t)(kAtom - 1));
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    const unsigned rank = cluster_rank();
+    if (threadIdx.x == 32) {
+        for (int i = 0; i < kPairMaxStages; ++i) {
+            pipe.full[i].init(1);
+            pipe.empty[i].init(1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            pipe.sums_full[i].init(1);
+            pipe.sums_empty[i].init(2 * kPairEpilogueWarps);
+        }
+        pipe.weight_empty.init(1);
+        pipe.drained.init(1);
+        for (int i = 0; i < kPairEpilogueWarps; ++i) {
+            pipe.extra_full[i].init(1);
+            pipe.extra_empty[i].init(32);
+        }
+        pipe.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    if (warp == 0) tmem_alloc_pair(&pipe.tmem, kColumns);
+    build_row_table(p.g, kPairRows, kMode != kPreGrad, table);
+    fence_before_sync();
+    __syncthreads();
+    cluster_sync();
+    fence_after_sync();
+    const unsigned columns = (p.cols + kPairColumns - 1) / kPairColumns, pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+    const unsigned tiles = (unsigned)table.unit_begin[p.g.groups + 2] * p.g.batch * columns;
+    const int slices = (p.depth + kSliceK - 1) / kSliceK;
+    // as many stages as fit beside the weight, if that stays
+    const int stage_bytes = p.resident ? kBytesA : kBytesA + kPairBytesB, weight_step = p.resident ? kPairBytesB : 0;
+    const int stages = min(kPairMaxStages, (pair_ring(kExtra) - slices * weight_step) / stage_bytes);
+    char *const weight = p.resident ? ring + stages * kBytesA : ring + kBytesA;  // of the first slice or the first stage
+    volatile int *const failed = &pipe.failed;
+    Ring ring_at(stages);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            bool sound = true;
+            int weight_group = -1, weight_col = -1;
+            unsigned changes = 0;
+            for (unsigned tile = pair; tile < tiles && sound; tile += pairs) {
+                const RowUnit u = row_unit(p.g, table, kPairRows, tile / columns);
+                if (u.group < 0) continue;
+                const int tile_col = (int)(tile % columns * kPairColumns), col0 = tile_col + (int)rank * (kPairColumns / 2);
+                const int row0 = (int)u.row + (int)rank * kTileRows;
+                if (kExtra)  // on their way to L2 while the tile's products run
+#pragma unroll
+                    for (int i = 0; i < 4 * (kPairColumns / 64); ++i) prefetch_2d(&map_extra, tile_col + 64 * (i / 4), row0 + 32 * (i % 4));
+                const bool fresh = !p.resident || u.group != weight_group || col0 != weight_col;
+                if (p.resident && fresh) {  // the products with the weight before have to be through
+                    if (changes++) sound = pipe.weight_empty.wait(changes & 1, failed);
+                    if (!sound) break;
+                    weight_group = u.group;
+                    weight_col = col0;
+                }
+                for (int s = 0; s < slices; ++s) {
+                    sound = pipe.empty[ring_at.stage].wait(ring_at.round ^ 1, failed);
+                    if (!sound) break;
+                    char *a = ring + ring_at.stage * stage_bytes;
+                    // the first block's barrier counts the bytes of both
+                    const uint32_t bar = cluster_address(&pipe.full[ring_at.stage], 0);
+                    if (rank == 0) pipe.full[ring_at.stage].arrive_expect(2 * (kBytesA + (fresh ? kPairBytesB : 0)));
+                    tma_2d_pair(&map_a, a, bar, s * kSliceK, row0);
+                    if (fresh) {
+                        char *b = weight + (p.resident ? s * weight_step : ring_at.stage * stage_bytes);
+                        if (kWeightMn) {
+#pragma unroll
+                            for (int i = 0; i < kPairColumns / 128; ++i)
+                                tma_3d_pair(&map_w, b + i * (64 * kSliceK * 2), bar, col0 + 64 * i, s * kSliceK, u.group);
+                        } else {
+                            tma_3d_pair(&map_w, b, bar, s * kSliceK, col0, u.group);
+                        }
+                    }
+                    ring_at.next();
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t kInstruction = instruction<T>(kPairRows, kPairColumns, false, kWeightMn);
+            Ring sums(2);
+            bool sound = true;
+            int weight_group = -1, weight_col = -1;
+            for (unsigned tile = pair; tile < tiles && sound; tile += pairs) {
+                const RowUnit u = row_unit(p.g, table, kPairRows, tile / columns);
+                if (u.group < 0) continue;
+                const int tile_col = (int)(tile % columns * kPairColumns);
+                if (p.resident && (u.group != weight_group || tile_col != weight_col)) {
+                    if (weight_group >= 0) mma_commit_pair(&pipe.weight_empty);
+                    weight_group = u.group;
+                    weight_col = tile_col;
+                }
+                sound = pipe.sums_empty[sums.stage].wait(sums.round ^ 1, failed);
+                if (!sound) break;
+                fence_after_sync();
+                const uint32_t d = pipe.tmem + sums.stage * kPairColumns;
+                for (int s = 0; s < slices; ++s) {
+                    sound = pipe.full[ring_at.stage].wait(ring_at.round, failed);
+                    if (!sound) break;
+                    fence_after_sync();
+                    const char *a = ring + ring_at.stage * stage_bytes;
+                    const char *b = weight + (p.resident ? s * weight_step : ring_at.stage * stage_bytes);
+#pragma unroll
+                    for (int k = 0; k < kSliceK / 16; ++k) {
+                        const uint64_t da = operand(a + 32 * k, 16, kAtom);
+                        const uint64_t db = kWeightMn ? operand(b + 2 * kAtom * k, 64 * kSliceK * 2, kAtom) : operand(b + 32 * k, 16, kAtom);
+                        mma_f16_pair(d, da, db, kInstruction, s > 0 || k > 0);
+                    }
+                    mma_commit_pair(&pipe.empty[ring_at.stage]);
+                    ring_at.next();
+                }
+                if (!sound) break;
+                mma_commit_pair(&pipe.sums_full[sums.stage]);
+                sums.next();
+            }
+        }
+        __syncwarp();
+    } else if (warp >= kFirstEpilogueWarp) {
+        const int mine = warp - kFirstEpilogueWarp, quarter = warp % 4, part = mine / 4;
+        char *const buffer = ring + pair_ring(true) + mine * kBufferBytes;
+        float *const bias = bias_of[mine];
+        Stage &stage = stages_of[mine];
+        for (int i = lane; i < 64; i += 32) bias[i] = 0.f;
+        int bias_group = -1, bias_col = -1;
+        const uint32_t sums_empty[2] = {cluster_address(&pipe.sums_empty[0], 0), cluster_address(&pipe.sums_empty[1], 0)};
+        Ring sums(2);
+        struct Place {
+            long long first;  // row of the warp's part of a tile
+            int rows, col0, group;
+        };
+        const auto place = [&](unsigned tile) {
+            const RowUnit u = row_unit(p.g, table, kPairRows, tile / columns);
+            const int above = (int)rank * kTileRows + quarter * 32;
+            Place at;
+            at.first = u.row + above;
+            at.rows = u.count - above;  // none where not positive
+            at.col0 = (int)(tile % columns * kPairColumns) + part * 64;
+            at.group = u.group;
+            return at;
+        };
+        const auto works = [&](const Place &at) { return at.rows > 0 && at.col0 < p.cols; };
+        // A place's extra rows into the buffer.  Lanes arrive at extra_empty behind the stores of what they made of the rows before: an
+        // arrival right behind the reads themselves let the copy overtake some of them.
+        unsigned asked = 0, loads = 0;
+        const auto request = [&](const Place &at) {
+            if (!kExtra || !works(at)) return;
+            ++asked;
+            if (lane == 0 && pipe.extra_empty[mine].wait(asked & 1, failed)) {
+                pipe.extra_full[mine].arrive_expect(kBufferBytes);
+                tma_2d(&map_extra, buffer, &pipe.extra_full[mine], at.col0, (int)at.first);
+            }
+        };
+        Place next;
+        if (pair < tiles) {
+            next = place(pair);
+            request(next);
+        }
+        for (unsigned tile = pair; tile < tiles; tile += pairs) {
+            const Place u = next;
+            const bool more = tile + pairs < tiles;
+            if (more) next = place(tile + pairs);
+            if (kMode != kGradX && p.bias && u.group >= 0 && (u.group != bias_group || u.col0 != bias_col)) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (u.col0 + 32 * i + lane < p.cols) bias[32 * i + lane] = to_f32<T>(p.bias[(size_t)u.group * p.cols + u.col0 + 32 * i + lane]);
+                bias_group = u.group;
+                bias_col = u.col0;
+                __syncwarp();
+            }
+            if (u.group >= 0) {
+                if (!__all_sync(0xffffffffu, pipe.sums_full[sums.stage].wait(sums.round, failed))) break;
+                fence_after_sync();
+            }
+            if (works(u)) {
+                if (kExtra && !__all_sync(0xffffffffu, pipe.extra_full[mine].wait(loads++ & 1, failed))) break;
+                const uint32_t address = pipe.tmem + sums.stage * kPairColumns + part * 64 + ((uint32_t)(quarter * 32) << 16);
+                T *const out = p.out + (size_t)u.first * p.out_pitch + u.col0;
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t row[16] = {};
+                    if (kExtra) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint4 q = *buffer_unit(buffer, lane, 4 * c + j);
+                            row[4 * j] = q.x; row[4 * j + 1] = q.y; row[4 * j + 2] = q.z; row[4 * j + 3] = q.w;
+                        }
+                    }
+                    if (u.group >= 0)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t v[16];
+                            __syncwarp();
+                            tmem_load(address + 32 * c + 16 * h, v);
+                            tmem_load_wait();
+                            finish_columns<T, kMode, kAct>(v, bias + 32 * c + 16 * h, row + 8 * h);
+                        }
+                    store_rows<true>(out + 32 * c, p.out_pitch, u.rows, p.cols - u.col0 - 32 * c, stage, row);
+                }
+                if (kExtra) pipe.extra_empty[mine].arrive();
+            }
+            if (more) request(next);
+            if (u.group >= 0) {
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) arrive_at(sums_empty[sums.stage]);
+                sums.next();
+            }
+        }
+        if (kExtra && asked != loads && lane == 0) {  // only after a wait that ran out
+            volatile int again = 0;
+            pipe.extra_full[mine].wait((asked - 1) & 1, &again);
+        }
+        __syncwarp();
+    }
+
+    // As in pipeline_end; nothing of the other block may be touched once it has left.
+    fence_before_sync();
+    __syncthreads();
+    if (threadIdx.x == 32 && rank == 0 && pipe.failed) {
+        volatile int again = 0;
+        mma_commit_pair(&pipe.drained);
+        pipe.drained.wait(0, &again);
+    }
+    if (threadIdx.x == 0 && pipe.failed) {
+        atomicAdd(&g_timeouts, 1u);
+        volatile int again = 0;
+        if (rank == 0)
+            for (int i = 0; i < stages; ++i) pipe.full[i].wait(i < ring_at.stage ? ring_at.round : ring_at.round ^ 1, &again);
+    }
+    __syncthreads();
+    cluster_sync();
+    fence_after_sync();
+    if (warp == 0) tmem_free_pair(pipe.tmem, kColumns);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
@@ -606,6 +888,12 @@ int allow_shared(Kernel kernel, int bytes) {
     return status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
 }
 
+// Blocks (or pairs) for `tiles`: a multiple of the column tiles where the weight is resident and that leaves few SMs idle.
+unsigned row_grid(long long tiles, long long columns, unsigned most, bool resident) {
+    if (tiles <= most) return (unsigned)tiles;
+    return resident && columns <= most / 8 ? most - most % (unsigned)columns : most;
+}
+
 template <typename T, int kMode, int kAct, int BN, bool kVector>
 int launch_rows(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t st) {
     constexpr int kSmem = Shape<BN>::kStages * Shape<BN>::kBytes + kAtom;
@@ -624,7 +912,27 @@ int launch_rows(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t s
     a.resident = ceil_div(a.depth, kSliceK) * Shape<BN>::kBytesB <= kResidentBytes;
     const long long tiles = units * ceil_div(a.cols, BN);
     if (tiles >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
-    kernel<<<(unsigned)std::min<long long>(tiles, kSms), Shape<BN>::kThreads, kSmem, st>>>(a, map_a, map_w, map_extra);
+    kernel<<<row_grid(tiles, ceil_div(a.cols, BN), kSms, a.resident), Shape<BN>::kThreads, kSmem, st>>>(a, map_a, map_w, map_extra);
+    return status(cudaGetLastError());
+}
+
+template <typename T, int kMode, int kAct>
+int launch_pair(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t st) {
+    const auto kernel = linear_rows_pair_kernel<T, kMode, kAct>;
+    if (const int rc = allow_shared(kernel, kPairSmem)) return rc;
+    CUtensorMap map_a, map_w, map_extra;
+    const long long rows = (long long)p.g.batch * p.g.rows;
+    if (const int rc = make_map(map_a, p.dtype, p.a, a.depth, rows, p.a_pitch, kTileRows, 0)) return rc;
+    if (const int rc = make_map(map_w, p.dtype, p.w, p.in_features, p.out_features, p.w_pitch, kMode == kGradX ? kSliceK : kPairColumns / 2,
+                                p.g.groups))
+        return rc;
+    map_extra = map_a;
+    if (a.extra)
+        if (const int rc = make_map(map_extra, p.dtype, p.extra, a.cols, rows, p.extra_pitch, 32, 0)) return rc;
+    a.resident = pair_ring(kMode == kForward || kMode == kPreGrad) - ceil_div(a.depth, kSliceK) * kPairBytesB >= kPairLeastStages * kBytesA;
+    const long long tiles = units * ceil_div(a.cols, kPairColumns);
+    if (tiles >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
+    kernel<<<2 * row_grid(tiles, ceil_div(a.cols, kPairColumns), kSms / 2, a.resident), kPairThreads, kPairSmem, st>>>(a, map_a, map_w, map_extra);
     return status(cudaGetLastError());
 }
 
@@ -646,6 +954,10 @@ int rows_of(const MmaRows &p, cudaStream_t st) {
         if (a.cols > 64 && units * ceil_div(a.cols, 128) >= kSms) return launch_rows<T, kMode, kAct, 128, false>(a, p, units, st);
         return launch_rows<T, kMode, kAct, 64, false>(a, p, units, st);
     }
+    const bool ragged = p.g.starts != nullptr;
+    const long long pair_units = most_units(p.g.batch, p.g.rows, p.g.groups, kPairRows, kMode != kPreGrad && ragged);
+    if (a.cols > 128 && pair_units * ceil_div(a.cols, kPairColumns) >= kSms / 2 && (!ragged || p.g.rows / p.g.groups >= 2 * kPairRows))
+        return launch_pair<T, kMode, kAct>(a, p, pair_units, st);
     if (a.cols > 128 && units * ceil_div(a.cols, 256) >= kSms) return launch_rows<T, kMode, kAct, 256, true>(a, p, units, st);
     if (a.cols > 64 && units * ceil_div(a.cols, 128) >= kSms) return launch_rows<T, kMode, kAct, 128, true>(a, p, units, st);
     return launch_rows<T, kMode, kAct, 64, true>(a, p, units, st);

@@ -216,6 +216,24 @@ def test_many_groups_and_long_groups(dtype):
     check(*make((2, 20000), 64, 32, dtype, 3), "none", torch.tensor([0, 15000, 19990], device=DEV))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act", ACTS)
+def test_enough_tiles_for_every_sm(act, dtype):
+    """Tall inputs, where blocks work in pairs on 256 rows: the last rows incomplete, contractions that stay in shared memory and that
+    do not, widths that end inside a tile."""
+    for (M, K, N), residual in (((19003, 200, 264), True), ((9607, 328, 520), False), ((19203, 256, 256), act == "none")):
+        check(*make((M,), K, N, dtype, residual=residual, seed=M, exact=act == "relu"), act)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_tall_groups(act, dtype):
+    """The same with groups that end inside the pairs' tiles, rows of no group before, between batch elements and behind."""
+    starts = torch.tensor([100, 5003, 5003, 9000, 9391], device=DEV)
+    check(*make((2, 10240), 136, 200, dtype, 4, seed=3), act, starts)
+    check(*make((2, 10240), 264, 136, dtype, 5, seed=4, residual=False), act, starts)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_of_other_groups_and_of_none_stay_out(dtype):
     """NaN and infinities in rows of no group, in another group's rows and weights: nothing of them reaches the group's results."""
