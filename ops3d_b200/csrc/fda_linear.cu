@@ -344,14 +344,14 @@ __global__ void __launch_bounds__(32 * kSumWarps) linear_weight_grad_sum_kernel(
 // ---------------------------------------------------------------------------------------------------------------------------
 inline size_t type_size(int dtype) { return dtype == FDA_DTYPE_F32 ? 4 : 2; }
 
-// As many pieces as the SMs take at once over `tiles` tiles of the weight, none shorter than `least_piece` blocks.
-Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int least_piece) {
+// As many pieces as `workers` take at once over `tiles` tiles of the weight, none shorter than `least_piece` blocks.
+Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int least_piece, int workers) {
     Cut c;
     c.block = block;
     const long long blocks = std::max<long long>(1, most_units(batch, rows, groups, block, false));
     // One piece more than the SMs take would be a round of its own.  Every further group can add a piece that is not full; where
     // there are too many groups for that, pieces half as long, so that the last round is short.
-    const long long wanted = std::max<long long>(1, kSms / tiles);
+    const long long wanted = std::max<long long>(1, workers / tiles);
     const long long full = wanted >= 2 * groups ? wanted - (groups - 1) : 2 * wanted;
     c.piece = (int)std::max<long long>(least_piece, ceil_div(blocks, full));
     if (blocks <= 2 * least_piece) c.piece = (int)blocks;  // the second launch would cost more than it spreads
@@ -478,21 +478,32 @@ void add_padded_operands(Layout &l, const Shape &s) {
     l.w = l.take((size_t)s.groups * s.out_features * padded(s.in_features) * 2);
 }
 
-// Inputs of an accumulator of the 16-bit weight gradient: the widest that leaves every SM a piece of 8 blocks.
-int mma_weight_tile(const Shape &s) {
-    const long long blocks = most_units(s.batch, s.rows, s.groups, kMmaSlice, false), rows = ceil_div(s.out_features, kMmaTileRows);
+// The 16-bit weight gradient's accumulators: 256 x 256 by pairs of blocks where that leaves every pair a piece of 16 blocks, else 128
+// outputs and as many inputs as leave every SM a piece of 8.
+struct WeightTile {
+    int outputs, inputs;
+    bool pair;
+};
+
+WeightTile mma_weight_tile(const Shape &s) {
+    const long long blocks = most_units(s.batch, s.rows, s.groups, kMmaSlice, false);
+    if (s.out_features > 128 && s.in_features > 128 &&
+        ceil_div(s.out_features, 256) * ceil_div(s.in_features, 256) * ceil_div(blocks, 16) >= kSms / 2)
+        return {256, 256, true};
     for (int tile = 256; tile > 64; tile /= 2)
-        if (s.in_features > tile / 2 && rows * ceil_div(s.in_features, tile) * ceil_div(blocks, 8) >= kSms) return tile;
-    return 64;
+        if (s.in_features > tile / 2 && ceil_div(s.out_features, kMmaTileRows) * ceil_div(s.in_features, tile) * ceil_div(blocks, 8) >= kSms)
+            return {kMmaTileRows, tile, false};
+    return {kMmaTileRows, 64, false};
 }
 
 Cut weight_cut(const Shape &s) {
     if (s.dtype != FDA_DTYPE_F32) {
-        const long long tiles = ceil_div(s.out_features, kMmaTileRows) * ceil_div(s.in_features, mma_weight_tile(s));
-        return cut_rows(s.batch, s.rows, s.groups, tiles, kMmaSlice, 8);
+        const WeightTile t = mma_weight_tile(s);
+        return cut_rows(s.batch, s.rows, s.groups, ceil_div(s.out_features, t.outputs) * ceil_div(s.in_features, t.inputs), kMmaSlice, 8,
+                        t.pair ? kSms / 2 : kSms);
     }
     return cut_rows(s.batch, s.rows, s.groups, ceil_div(s.out_features, kTile) * ceil_div(s.in_features, kTile), kPlainBlock,
-                    kPlainLeastPiece);
+                    kPlainLeastPiece, kSms);
 }
 
 bool few_rows(const Shape &s);
@@ -579,7 +590,8 @@ struct Gradients {
 template <typename T>
 int sum_slots(const WeightGrad<T> &q, const Shape &s, const Cut &c, cudaStream_t st) {
     if (c.slots == 0) return FDA_OK;
-    const bool split = c.pieces > 16ll * s.groups;
+    const long long unsplit = ceil_div(((long long)s.in_features + 1) * s.out_features, 32 * kLaneElements * kSumWarps) * s.groups;
+    const bool split = c.pieces > 16ll * s.groups && unsplit < kSms;
     const long long items = ceil_div(((long long)s.in_features + 1) * s.out_features, 32 * kLaneElements * (split ? 1 : kSumWarps)) * s.groups;
     const unsigned blocks = (unsigned)std::min<long long>(items, 4 * kSms);
     if (split) linear_weight_grad_sum_kernel<T, true><<<blocks, 32 * kSumWarps, 0, st>>>(q);
@@ -657,7 +669,7 @@ int backward_narrow(const Shape &s, const Groups &g, const void *x, const void *
     if (!weights) return FDA_OK;
     const Cut c = weight_cut(s);
     const MmaWeightGrad q{grad, x, outs, in, out.weight, out.bias, reinterpret_cast<float *>(ws + l.slots),
-                          reinterpret_cast<float *>(ws + l.bias_slots), s.in_features, s.out_features, s.dtype, mma_weight_tile(s), c, g};
+                          reinterpret_cast<float *>(ws + l.bias_slots), s.in_features, s.out_features, s.dtype, mma_weight_tile(s).inputs, mma_weight_tile(s).pair, c, g};
     if (const int rc = mma_weight_grad(q, st)) return rc;
     if (s.dtype == FDA_DTYPE_F16) return sum_slots(weight_grad_args<__half>(s, g, c, nullptr, nullptr, out, ws, l), s, c, st);
     return sum_slots(weight_grad_args<__nv_bfloat16>(s, g, c, nullptr, nullptr, out, ws, l), s, c, st);

@@ -286,6 +286,7 @@ struct MmaWeightGrad {
     float *slots, *bias_slots;
     int in_features, out_features, dtype;
     int tile;  // inputs of an accumulator: 64, 128 or 256
+    bool pair; // two blocks to 256 outputs x 256 inputs
     Cut cut;
     Groups g;
 };

@@ -67,6 +67,9 @@ __device__ __forceinline__ uint32_t cluster_address(const void *p, unsigned rank
 __device__ __forceinline__ void arrive_at(uint32_t cluster_barrier) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_barrier) : "memory");
 }
+__device__ __forceinline__ void release_at(uint32_t cluster_barrier) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_barrier) : "memory");
+}
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
     asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));

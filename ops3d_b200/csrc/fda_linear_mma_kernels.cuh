@@ -38,11 +38,12 @@ constexpr int kFirstEpilogueWarp = 4;
 template <int kStages>
 struct Pipeline {
     Barrier full[kStages], empty[kStages], sums_full[2], sums_empty[2], weight_empty, drained;
+    Barrier mask_go, masked;  // of pairs
     uint32_t tmem;
     volatile int failed;
 };
 
-template <int kStages>
+template <bool kPair, int kStages>
 __device__ __forceinline__ void pipeline_begin(Pipeline<kStages> &p, int columns, int epilogue_warps) {
     if (threadIdx.x == 32) {
         for (int i = 0; i < kStages; ++i) {
@@ -51,21 +52,26 @@ __device__ __forceinline__ void pipeline_begin(Pipeline<kStages> &p, int columns
         }
         for (int i = 0; i < 2; ++i) {
             p.sums_full[i].init(1);
-            p.sums_empty[i].init(epilogue_warps);
+            p.sums_empty[i].init(epilogue_warps * (kPair ? 2 : 1));
         }
+        p.mask_go.init(1);
+        p.masked.init(1);
         p.weight_empty.init(1);
         p.drained.init(1);
         p.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    if (threadIdx.x < 32) tmem_alloc(&p.tmem, columns);
+    if (threadIdx.x < 32) {
+        if (kPair) tmem_alloc_pair(&p.tmem, columns);
+        else tmem_alloc(&p.tmem, columns);
+    }
     fence_before_sync();
 }
 
 // After every role has left.  In a sound run nothing is in flight any more (the epilogue has waited for every product, and so
 // for every copy); after a wait that ran out, copies and products still running are waited for, again with a limit.
-template <int kStages>
+template <bool kPair, int kStages>
 __device__ __forceinline__ void pipeline_end(Pipeline<kStages> &p, int columns, const Ring &issued, bool any) {
     fence_before_sync();
     __syncthreads();
@@ -82,11 +88,16 @@ __device__ __forceinline__ void pipeline_end(Pipeline<kStages> &p, int columns, 
     }
     if (threadIdx.x == 32 && p.failed) {
         volatile int again = 0;
-        mma_commit(&p.drained);
+        if (!kPair) mma_commit(&p.drained);
+        else if (cluster_rank() == 0) mma_commit_pair(&p.drained);
         p.drained.wait(0, &again);
     }
     __syncthreads();
-    if (threadIdx.x < 32) tmem_free(p.tmem, columns);
+    if (kPair) cluster_sync();  // nothing of the other block may be touched once it has left
+    if (threadIdx.x < 32) {
+        if (kPair) tmem_free_pair(p.tmem, columns);
+        else tmem_free(p.tmem, columns);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
@@ -152,7 +163,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         prefetch_map(&map_a);
         prefetch_map(&map_w);
     }
-    pipeline_begin(pipe, kColumns, Shape<BN>::kEpilogueWarps);
+    pipeline_begin<false>(pipe, kColumns, Shape<BN>::kEpilogueWarps);
     build_row_table(p.g, kTileRows, kMode != kPreGrad, table);
     __syncthreads();
     fence_after_sync();
@@ -344,7 +355,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
             sums.next();
         }
     }
-    pipeline_end(pipe, kColumns, ring_at, any);
+    pipeline_end<false>(pipe, kColumns, ring_at, any);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
@@ -634,8 +645,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 // ---------------------------------------------------------------------------------------------------------------------------
 // An accumulator holds 128 outputs x BN inputs of g^T x over a piece of a group's rows; both operands have their lines across
 // the contraction.  The bias's gradient is one more narrow product of the same g with ones.
+//
+// kPair: two blocks make 256 outputs x 256 inputs, each with its own 128 outputs and half of the inputs, so that 32 instead of 48 KB
+// pass from L2 for 64 rows (73728 rows, 256 -> 1024: 54 -> 4x us).
 constexpr int kOnesColumns = 16;
 constexpr int kOnesBytes = kOnesColumns * kSliceK * 2;
+
+template <int BN, bool kPair>
+struct WeightShape {
+    static constexpr int kOutputs = kPair ? 2 * kTileRows : kTileRows, kColumnsB = kPair ? BN / 2 : BN;
+    static constexpr int kBytes = kBytesA + kColumnsB * kSliceK * 2, kStages = kRingBytes / kBytes;
+};
 
 template <typename T>
 struct WeightGradArgs {
@@ -646,29 +666,32 @@ struct WeightGradArgs {
     Groups g;
 };
 
-template <typename T, int BN, bool kVector>
+template <typename T, int BN, bool kVector, bool kPair>
 __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
     linear_weight_grad_mma_kernel(const WeightGradArgs<T> p, const __grid_constant__ CUtensorMap map_g,
                                   const __grid_constant__ CUtensorMap map_x) {
-    constexpr int kStages = Shape<BN>::kStages, kColumns = 512;
+    using W = WeightShape<BN, kPair>;
+    constexpr int kStages = W::kStages, kColumns = 512;
     extern __shared__ char dynamic[];
     __shared__ PieceTable table;
     __shared__ Pipeline<kStages> pipe;
     __shared__ __align__(16) Stage stages[Shape<BN>::kEpilogueWarps];
     char *const ring = reinterpret_cast<char *>(((uintptr_t)dynamic + kAtom - 1) & ~(uintptr_t)(kAtom - 1));
-    char *const ones = ring + kStages * Shape<BN>::kBytes;
+    char *const ones = ring + kStages * W::kBytes;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
         prefetch_map(&map_g);
         prefetch_map(&map_x);
     }
-    pipeline_begin(pipe, kColumns, Shape<BN>::kEpilogueWarps);
+    pipeline_begin<kPair>(pipe, kColumns, Shape<BN>::kEpilogueWarps);
     for (int i = threadIdx.x; i < kOnesBytes / 4; i += Shape<BN>::kThreads) reinterpret_cast<uint32_t *>(ones)[i] = pack2<T>(1.f, 1.f);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     build_piece_table(p.g, kSliceK, p.piece, table);
     __syncthreads();
+    if (kPair) cluster_sync();
     fence_after_sync();
-    const int out_tiles = (p.out_features + kTileRows - 1) / kTileRows, in_tiles = (p.in_features + BN - 1) / BN;
+    const unsigned rank = kPair ? cluster_rank() : 0, worker = kPair ? blockIdx.x / 2 : blockIdx.x, workers = kPair ? gridDim.x / 2 : gridDim.x;
+    const int out_tiles = (p.out_features + W::kOutputs - 1) / W::kOutputs, in_tiles = (p.in_features + BN - 1) / BN;
     const int per_piece = out_tiles * in_tiles;
     const long long items = (long long)table.piece_begin[p.g.groups] * per_piece;
     volatile int *const failed = &pipe.failed;
@@ -683,7 +706,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         const int piece = (int)(i / per_piece), t = (int)(i % per_piece);
         it.group = find_section(table.piece_begin, p.g.groups, piece);
         it.piece = piece - table.piece_begin[it.group];
-        it.out0 = (t / in_tiles) * kTileRows;
+        it.out0 = (t / in_tiles) * W::kOutputs + (int)rank * kTileRows;  // this block's
         it.in0 = (t % in_tiles) * BN;
         it.first = it.piece * p.piece;
         it.last = min(group_blocks(p.g, table.start, it.group, kSliceK), it.first + p.piece);
@@ -693,7 +716,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
     if (warp == 0) {
         if (lane == 0) {
             bool sound = true;
-            for (long long i = blockIdx.x; i < items && sound; i += gridDim.x) {
+            for (long long i = worker; i < items && sound; i += workers) {
                 const Item it = item_at(i);
                 for (int j = it.first; j < it.last; ++j) {
                     long long row;
@@ -701,13 +724,24 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                     block_rows(p.g, table.start, it.group, kSliceK, j, row, count);
                     sound = pipe.empty[ring_at.stage].wait(ring_at.round ^ 1, failed);
                     if (!sound) break;
-                    char *a = ring + ring_at.stage * Shape<BN>::kBytes, *b = a + kBytesA;
+                    char *a = ring + ring_at.stage * W::kBytes, *b = a + kBytesA;
                     Barrier *bar = &pipe.full[ring_at.stage];
-                    bar->arrive_expect(Shape<BN>::kBytes);
+                    if (rank == 0) bar->arrive_expect(W::kBytes * (kPair ? 2 : 1));
+                    const int in0 = it.in0 + (int)rank * W::kColumnsB;
+                    if (kPair) {  // the first block's barrier counts the bytes of both
+                        const uint32_t first = cluster_address(bar, 0);
 #pragma unroll
-                    for (int k = 0; k < kTileRows / 64; ++k) tma_2d(&map_g, a + k * (64 * kSliceK * 2), bar, it.out0 + 64 * k, (int)row);
+                        for (int k = 0; k < kTileRows / 64; ++k)
+                            tma_2d_pair(&map_g, a + k * (64 * kSliceK * 2), first, it.out0 + 64 * k, (int)row);
 #pragma unroll
-                    for (int k = 0; k < BN / 64; ++k) tma_2d(&map_x, b + k * (64 * kSliceK * 2), bar, it.in0 + 64 * k, (int)row);
+                        for (int k = 0; k < W::kColumnsB / 64; ++k)
+                            tma_2d_pair(&map_x, b + k * (64 * kSliceK * 2), first, in0 + 64 * k, (int)row);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < kTileRows / 64; ++k) tma_2d(&map_g, a + k * (64 * kSliceK * 2), bar, it.out0 + 64 * k, (int)row);
+#pragma unroll
+                        for (int k = 0; k < W::kColumnsB / 64; ++k) tma_2d(&map_x, b + k * (64 * kSliceK * 2), bar, in0 + 64 * k, (int)row);
+                    }
                     ring_at.next();
                     any = true;
                 }
@@ -715,51 +749,83 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         }
         __syncwarp();
     } else if (warp == 1) {
-        constexpr uint32_t kInstruction = instruction<T>(kTileRows, BN, true, true);
-        constexpr uint32_t kOnesInstruction = instruction<T>(kTileRows, kOnesColumns, true, false);
-        unsigned round = 0;
+        constexpr uint32_t kInstruction = instruction<T>(W::kOutputs, BN, true, true);
+        constexpr uint32_t kOnesInstruction = instruction<T>(W::kOutputs, kOnesColumns, true, false);
+        // Lines of the next group's rows (or of nothing) go out of both operands, for 0 times NaN is NaN.  A line of 128 bytes is one
+        // row of a block of 64 columns, wherever the swizzle has its parts.
+        const auto clear_lines = [&](char *a, int count) {
+            constexpr int kBlocks = kTileRows / 64 + W::kColumnsB / 64;
+            const int lines = kSliceK - count;
+            for (int l = lane; l < kBlocks * lines * 8; l += 32) {
+                const int block = l / (lines * 8), rest = l - block * lines * 8;
+                reinterpret_cast<uint4 *>(a + block * (64 * kSliceK * 2) + count * 128)[rest] = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
+        unsigned round = 0, masks = 0;
         bool sound = true;
-        for (long long i = blockIdx.x; i < items && sound; i += gridDim.x) {
+        for (long long i = worker; i < items && sound; i += workers) {
             const Item it = item_at(i);
             if (it.first >= it.last) continue;
             const bool bias = it.in0 == 0 && p.grad_bias;
-            sound = __all_sync(0xffffffffu, pipe.sums_empty[0].wait(round ^ 1, failed));
-            if (!sound) break;
-            fence_after_sync();
+            if (rank == 0) {
+                sound = __all_sync(0xffffffffu, pipe.sums_empty[0].wait(round ^ 1, failed));
+                if (!sound) break;
+                fence_after_sync();
+            }
             for (int j = it.first; j < it.last; ++j) {
                 long long row;
                 int count;
                 block_rows(p.g, table.start, it.group, kSliceK, j, row, count);
+                char *a = ring + ring_at.stage * W::kBytes, *b = a + kBytesA;
+                if (rank != 0) {  // the second block clears its lines when the first has seen the copies of both
+                    if (count < kSliceK) {
+                        sound = __all_sync(0xffffffffu, pipe.mask_go.wait(masks++ & 1, failed));
+                        if (!sound) break;
+                        clear_lines(a, count);
+                        if (lane == 0) release_at(cluster_address(&pipe.masked, 0));
+                    }
+                    ring_at.next();
+                    continue;
+                }
                 sound = __all_sync(0xffffffffu, pipe.full[ring_at.stage].wait(ring_at.round, failed));
                 if (!sound) break;
-                char *a = ring + ring_at.stage * Shape<BN>::kBytes, *b = a + kBytesA;
                 if (count < kSliceK) {
-                    // lines of the next group's rows (or of nothing): out of both operands, for 0 times NaN is NaN.  A line of 128
-                    // bytes is one row of a block of 64 columns, wherever the swizzle has its parts.
-                    constexpr int kBlocks = kTileRows / 64 + BN / 64;
-                    const int lines = kSliceK - count;
-                    for (int l = lane; l < kBlocks * lines * 8; l += 32) {
-                        const int block = l / (lines * 8), rest = l - block * lines * 8;
-                        reinterpret_cast<uint4 *>(a + block * (64 * kSliceK * 2) + count * 128)[rest] = make_uint4(0, 0, 0, 0);
+                    if (kPair && lane == 0) release_at(cluster_address(&pipe.mask_go, 1));
+                    clear_lines(a, count);
+                    if (kPair) {
+                        sound = __all_sync(0xffffffffu, pipe.masked.wait(masks++ & 1, failed));
+                        if (!sound) break;
+                        asm volatile("fence.acq_rel.cluster;" ::: "memory");
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
                 }
                 fence_after_sync();
                 if (lane == 0) {
 #pragma unroll
                     for (int k = 0; k < kSliceK / 16; ++k) {
                         const uint64_t da = operand(a + 2 * kAtom * k, 64 * kSliceK * 2, kAtom);
-                        mma_f16(pipe.tmem, da, operand(b + 2 * kAtom * k, 64 * kSliceK * 2, kAtom), kInstruction, j > it.first || k > 0);
-                        if (bias) mma_f16(pipe.tmem + BN, da, operand(ones + 32 * k, 16, kAtom), kOnesInstruction, j > it.first || k > 0);
+                        const uint64_t db = operand(b + 2 * kAtom * k, 64 * kSliceK * 2, kAtom), d1 = operand(ones + 32 * k, 16, kAtom);
+                        const bool more = j > it.first || k > 0;
+                        if (kPair) {
+                            mma_f16_pair(pipe.tmem, da, db, kInstruction, more);
+                            if (bias) mma_f16_pair(pipe.tmem + BN, da, d1, kOnesInstruction, more);
+                        } else {
+                            mma_f16(pipe.tmem, da, db, kInstruction, more);
+                            if (bias) mma_f16(pipe.tmem + BN, da, d1, kOnesInstruction, more);
+                        }
                     }
-                    mma_commit(&pipe.empty[ring_at.stage]);
+                    if (kPair) mma_commit_pair(&pipe.empty[ring_at.stage]);
+                    else mma_commit(&pipe.empty[ring_at.stage]);
                 }
                 __syncwarp();
                 ring_at.next();
             }
             if (!sound) break;
-            if (lane == 0) mma_commit(&pipe.sums_full[0]);
+            if (lane == 0 && rank == 0) {
+                if (kPair) mma_commit_pair(&pipe.sums_full[0]);
+                else mma_commit(&pipe.sums_full[0]);
+            }
             __syncwarp();
             round ^= 1;
         }
@@ -769,7 +835,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         const int quarter = warp % 4, part = (warp - kFirstEpilogueWarp) / 4;
         Stage &stage = stages[warp - kFirstEpilogueWarp];
         unsigned round = 0;
-        for (long long i = blockIdx.x; i < items; i += gridDim.x) {
+        for (long long i = worker; i < items; i += workers) {
             const Item it = item_at(i);
             const bool none = it.first >= it.last;
             const bool whole = table.slot_begin[it.group + 1] == table.slot_begin[it.group];
@@ -829,12 +895,15 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
             if (!none) {
                 fence_before_sync();
                 __syncwarp();
-                if (lane == 0) pipe.sums_empty[0].arrive();
+                if (lane == 0) {
+                    if (kPair) arrive_at(cluster_address(&pipe.sums_empty[0], 0));
+                    else pipe.sums_empty[0].arrive();
+                }
                 round ^= 1;
             }
         }
     }
-    pipeline_end(pipe, kColumns, ring_at, any);
+    pipeline_end<kPair>(pipe, kColumns, ring_at, any && rank == 0);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
@@ -954,9 +1023,13 @@ int rows_of(const MmaRows &p, cudaStream_t st) {
         if (a.cols > 64 && units * ceil_div(a.cols, 128) >= kSms) return launch_rows<T, kMode, kAct, 128, false>(a, p, units, st);
         return launch_rows<T, kMode, kAct, 64, false>(a, p, units, st);
     }
-    const bool ragged = p.g.starts != nullptr;
+    // Pairs where they pay: extra rows (73728 x 256 x 1024 with a residual 74 us against 94 by single blocks) or a contraction too long
+    // for a resident weight (149504 x 1024 x 256: 78 against 86); else single blocks, whose epilogues wait for no other (598016 x
+    // 256 x 256: 105 against 117).  Groups shorter than two of the pairs' units would leave too much of these empty.
+    const bool ragged = p.g.starts != nullptr, extra = kMode == kForward || kMode == kPreGrad;
+    const bool pays = extra || ceil_div(a.depth, kSliceK) * Shape<256>::kBytesB > kResidentBytes;
     const long long pair_units = most_units(p.g.batch, p.g.rows, p.g.groups, kPairRows, kMode != kPreGrad && ragged);
-    if (a.cols > 128 && pair_units * ceil_div(a.cols, kPairColumns) >= kSms / 2 && (!ragged || p.g.rows / p.g.groups >= 2 * kPairRows))
+    if (pays && a.cols > 128 && pair_units * ceil_div(a.cols, kPairColumns) >= kSms / 2 && (!ragged || p.g.rows / p.g.groups >= 2 * kPairRows))
         return launch_pair<T, kMode, kAct>(a, p, pair_units, st);
     if (a.cols > 128 && units * ceil_div(a.cols, 256) >= kSms) return launch_rows<T, kMode, kAct, 256, true>(a, p, units, st);
     if (a.cols > 64 && units * ceil_div(a.cols, 128) >= kSms) return launch_rows<T, kMode, kAct, 128, true>(a, p, units, st);
@@ -981,7 +1054,7 @@ int rows_of(int mode, const MmaRows &p, cudaStream_t st) {
     return rows_of<T, kGradX, FDA_ACT_NONE>(p, st);
 }
 
-template <typename T, int BN, bool kVector>
+template <typename T, int BN, bool kVector, bool kPair = false>
 int launch_weight_grad(const MmaWeightGrad &p, cudaStream_t st) {
     WeightGradArgs<T> a;
     a.grad_weight = static_cast<T *>(p.grad_weight);
@@ -992,20 +1065,32 @@ int launch_weight_grad(const MmaWeightGrad &p, cudaStream_t st) {
     a.out_features = p.out_features;
     a.piece = p.cut.piece;
     a.g = p.g;
-    constexpr int kSmem = Shape<BN>::kStages * Shape<BN>::kBytes + kOnesBytes + kAtom;
-    const auto kernel = linear_weight_grad_mma_kernel<T, BN, kVector>;
+    using W = WeightShape<BN, kPair>;
+    constexpr int kSmem = W::kStages * W::kBytes + kOnesBytes + kAtom;
+    const auto kernel = linear_weight_grad_mma_kernel<T, BN, kVector, kPair>;
     if (const int rc = allow_shared(kernel, kSmem)) return rc;
     CUtensorMap map_g, map_x;
     const long long rows = (long long)p.g.batch * p.g.rows;
     if (const int rc = make_map(map_g, p.dtype, p.grad, p.out_features, rows, p.grad_pitch, kSliceK, 0)) return rc;
     if (const int rc = make_map(map_x, p.dtype, p.x, p.in_features, rows, p.x_pitch, kSliceK, 0)) return rc;
-    const long long items = p.cut.pieces * ceil_div(p.out_features, kTileRows) * ceil_div(p.in_features, BN);
-    kernel<<<(unsigned)std::min<long long>(items, kSms), Shape<BN>::kThreads, kSmem, st>>>(a, map_g, map_x);
-    return status(cudaGetLastError());
+    const long long items = p.cut.pieces * ceil_div(p.out_features, W::kOutputs) * ceil_div(p.in_features, BN);
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = kPair ? 2 : 1;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cudaLaunchConfig_t launch{};
+    launch.gridDim = dim3((unsigned)std::min<long long>(items, kPair ? kSms / 2 : kSms) * (kPair ? 2 : 1));
+    launch.blockDim = dim3(Shape<BN>::kThreads);
+    launch.dynamicSmemBytes = kSmem;
+    launch.stream = st;
+    launch.attrs = &cluster;
+    launch.numAttrs = 1;
+    return status(cudaLaunchKernelEx(&launch, kernel, a, map_g, map_x));
 }
 
 template <typename T, bool kVector>
 int weight_grad_of(const MmaWeightGrad &p, cudaStream_t st) {
+    if (p.pair) return launch_weight_grad<T, 256, kVector, true>(p, st);
     switch (p.tile) {
         case 256: return launch_weight_grad<T, 256, kVector>(p, st);
         case 128: return launch_weight_grad<T, 128, kVector>(p, st);

@@ -234,6 +234,21 @@ def test_tall_groups(act, dtype):
     check(*make((2, 10240), 264, 136, dtype, 5, seed=4, residual=False), act, starts)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_weight_gradients_over_many_rows(dtype):
+    """Rows enough that pairs of blocks share the weight's gradient: one group, ragged ones, and NaN in the rows behind each group's end."""
+    check(*make((40003,), 264, 520, dtype, seed=5), "none")
+    starts = torch.tensor([70, 15000, 15001, 15001, 20300], device=DEV)   # five entries: the last group ends before the rows do
+    x, w, b, r, dy = make((2, 20480), 264, 264, dtype, 4, seed=6)
+    _, grads = check(x, w, b, r, dy, "none", starts)
+    for lo, hi in ((0, 70), (20300, 20480)):
+        x[:, lo:hi], dy[:, lo:hi] = float("nan"), float("inf")
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    gx, gw, gb = torch.autograd.grad(grouped_linear(leaves[0], leaves[1], starts, leaves[2]), leaves, dy)
+    assert torch.equal(gw, grads["weight"]) and torch.equal(gb, grads["bias"])
+    assert torch.equal(gx[:, 70:20300], grads["x"][:, 70:20300]) and not gx[:, :70].any() and not gx[:, 20300:].any()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_of_other_groups_and_of_none_stay_out(dtype):
     """NaN and infinities in rows of no group, in another group's rows and weights: nothing of them reaches the group's results."""
