@@ -12,11 +12,8 @@ static __device__ unsigned int g_timeouts;
 
 __device__ __forceinline__ uint32_t smem_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-__device__ __forceinline__ unsigned long long time_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
+// Limit of a wait: about two seconds of the SM's clock.
+constexpr long long kWaitCycles = 4000000000ll;
 
 struct Barrier {
     unsigned long long word;
@@ -40,19 +37,19 @@ struct Barrier {
     }
     // False when the phase did not end within two seconds or another wait of the block ran out before: the caller leaves.
     __device__ __noinline__ bool wait_slowly(unsigned parity, volatile int *failed) {
-        const unsigned long long begin = time_ns();
+        const long long begin = clock64();
         for (;;) {
             for (int i = 0; i < 64; ++i)
                 if (passed(parity)) return true;
             if (*failed) return false;
-            if (time_ns() - begin > 2000000000ull) {
+            if (clock64() - begin > kWaitCycles) {
                 *failed = 1;
                 return false;
             }
         }
     }
     __device__ __forceinline__ bool wait(unsigned parity, volatile int *failed) {
-        return passed(parity) || passed(parity) || wait_slowly(parity, failed);
+        return passed(parity) || passed(parity) || passed(parity) || passed(parity) || wait_slowly(parity, failed);
     }
 };
 
@@ -131,11 +128,28 @@ __device__ __forceinline__ void tmem_free(uint32_t address, int columns) {
 }
 __device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate) {
-    asm volatile(
-        "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b),
-        "r"(instruction), "r"((unsigned)accumulate)
-        : "memory");
+// One lane of a converged warp.  The issuing loops keep the whole warp together around it: their operands then stay in uniform
+// registers, where a loop of one lane moves each of them there for every product.
+__device__ __forceinline__ bool elected() {
+    unsigned is;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(is));
+    return is;
+}
+// A descriptor's upper half is the same for all slices of an operand, its lower half holds the address.
+template <bool kPair>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint32_t a, uint32_t a_high, uint32_t b, uint32_t b_high, uint32_t instruction, bool accumulate) {
+    if (kPair)
+        asm volatile(
+            "{ .reg .pred p; .reg .b64 a, b; mov.b64 a, {%1, %2}; mov.b64 b, {%3, %4}; setp.ne.u32 p, %6, 0; "
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %5, p; }" ::"r"(d), "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(instruction),
+            "r"((unsigned)accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{ .reg .pred p; .reg .b64 a, b; mov.b64 a, {%1, %2}; mov.b64 b, {%3, %4}; setp.ne.u32 p, %6, 0; "
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p; }" ::"r"(d), "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(instruction),
+            "r"((unsigned)accumulate)
+            : "memory");
 }
 // Arrives on the barrier when every tcgen05 operation issued so far by this thread has ended.
 __device__ __forceinline__ void mma_commit(Barrier *bar) {
@@ -149,18 +163,16 @@ __device__ __forceinline__ void tmem_alloc_pair(uint32_t *slot, int columns) {
 __device__ __forceinline__ void tmem_free_pair(uint32_t address, int columns) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
 }
-__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate) {
-    asm volatile(
-        "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b),
-        "r"(instruction), "r"((unsigned)accumulate)
-        : "memory");
-}
+template <bool kPair>
+__device__ __forceinline__ void commit(Barrier *bar);
 __device__ __forceinline__ void mma_commit_pair(Barrier *bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
                      smem_address(bar)),
                  "h"((unsigned short)3)
                  : "memory");
 }
+template <> __device__ __forceinline__ void commit<false>(Barrier *bar) { mma_commit(bar); }
+template <> __device__ __forceinline__ void commit<true>(Barrier *bar) { mma_commit_pair(bar); }
 // 32 lanes x 16 or 32 columns of fp32: register j of a lane is column j of its row.
 __device__ __forceinline__ void tmem_load(uint32_t address, uint32_t (&v)[16]) {
     asm volatile(
@@ -185,10 +197,10 @@ __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::l
 // bytes.  Contraction along a line ("K-major"): `stride` bytes between atoms of 8 rows; a step of 16 elements is 32 bytes further.
 // Rows along a line ("MN-major"): an atom is 64 rows x 8 contraction indices, `stride` bytes between atoms along the
 // contraction, `leading` bytes between blocks of 64 rows; a step of 16 is two atoms further.
-__device__ __forceinline__ uint64_t operand(const void *p, uint32_t leading, uint32_t stride) {
-    return (uint64_t)((smem_address(p) & 0x3ffff) >> 4) | ((uint64_t)((leading & 0x3ffff) >> 4) << 16) |
-           ((uint64_t)((stride & 0x3ffff) >> 4) << 32) | (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ uint32_t operand_low(const void *p, uint32_t leading) {
+    return ((smem_address(p) & 0x3ffff) >> 4) | ((leading & 0x3ffff) >> 4) << 16;
 }
+__host__ __device__ constexpr uint32_t operand_high(uint32_t stride) { return ((stride & 0x3ffff) >> 4) | 1u << 14 | 2u << 29; }
 constexpr uint32_t kAtom = 1024;       // bytes of a swizzle atom
 constexpr uint32_t kLineElements = 64; // 16-bit elements of a line
 

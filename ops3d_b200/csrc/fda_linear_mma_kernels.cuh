@@ -219,41 +219,42 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
+        {
             constexpr uint32_t kInstruction = instruction<T>(kTileRows, BN, false, kWeightMn);
+            constexpr uint32_t kHigh = operand_high(kAtom), kStepB = kWeightMn ? 2 * kAtom / 16 : 2;  // of 16 contraction indices
+            const uint32_t a0 = operand_low(ring, 16), b0 = operand_low(weight, kWeightMn ? 64 * kSliceK * 2 : 16);
             Ring sums(2);
             bool sound = true;
             int weight_group = -1, weight_col = -1;
             for (unsigned tile = blockIdx.x; tile < tiles && sound; tile += gridDim.x) {
                 const RowUnit u = row_unit(p.g, table, kTileRows, tile / columns);
                 if (u.group < 0) continue;
-                const int col0 = (int)(tile % columns * BN);
-                if (p.resident && (u.group != weight_group || col0 != weight_col)) {
-                    if (weight_group >= 0) mma_commit(&pipe.weight_empty);
+                const int tile_col = (int)(tile % columns * BN);
+                if (p.resident && (u.group != weight_group || tile_col != weight_col)) {
+                    if (weight_group >= 0 && elected()) commit<false>(&pipe.weight_empty);
                     weight_group = u.group;
-                    weight_col = col0;
+                    weight_col = tile_col;
                 }
-                sound = pipe.sums_empty[sums.stage].wait(sums.round ^ 1, failed);
+                sound = __all_sync(0xffffffffu, pipe.sums_empty[sums.stage].wait(sums.round ^ 1, failed));
                 if (!sound) break;
                 fence_after_sync();
                 const uint32_t d = pipe.tmem + sums.stage * BN;
                 for (int s = 0; s < slices; ++s) {
-                    sound = pipe.full[ring_at.stage].wait(ring_at.round, failed);
+                    sound = __all_sync(0xffffffffu, pipe.full[ring_at.stage].wait(ring_at.round, failed));
                     if (!sound) break;
                     fence_after_sync();
-                    const char *a = ring + ring_at.stage * stage_bytes;
-                    const char *b = weight + (p.resident ? s * weight_step : ring_at.stage * stage_bytes);
+                    const uint32_t at = ring_at.stage * (stage_bytes / 16);
+                    const uint32_t a = a0 + at, b = b0 + (p.resident ? s * (weight_step / 16) : at);
+                    if (elected()) {
 #pragma unroll
-                    for (int k = 0; k < kSliceK / 16; ++k) {
-                        const uint64_t da = operand(a + 32 * k, 16, kAtom);
-                        const uint64_t db = kWeightMn ? operand(b + 2 * kAtom * k, 64 * kSliceK * 2, kAtom) : operand(b + 32 * k, 16, kAtom);
-                        mma_f16(d, da, db, kInstruction, s > 0 || k > 0);
+                        for (int k = 0; k < kSliceK / 16; ++k)
+                            mma_f16<false>(d, a + 2 * k, kHigh, b + kStepB * k, kHigh, kInstruction, s > 0 || k > 0);
+                        commit<false>(&pipe.empty[ring_at.stage]);
                     }
-                    mma_commit(&pipe.empty[ring_at.stage]);
                     ring_at.next();
                 }
                 if (!sound) break;
-                mma_commit(&pipe.sums_full[sums.stage]);
+                if (elected()) commit<false>(&pipe.sums_full[sums.stage]);
                 sums.next();
             }
         }
@@ -482,8 +483,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             constexpr uint32_t kInstruction = instruction<T>(kPairRows, kPairColumns, false, kWeightMn);
+            constexpr uint32_t kHigh = operand_high(kAtom), kStepB = kWeightMn ? 2 * kAtom / 16 : 2;  // of 16 contraction indices
+            const uint32_t a0 = operand_low(ring, 16), b0 = operand_low(weight, kWeightMn ? 64 * kSliceK * 2 : 16);
             Ring sums(2);
             bool sound = true;
             int weight_group = -1, weight_col = -1;
@@ -492,31 +495,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 if (u.group < 0) continue;
                 const int tile_col = (int)(tile % columns * kPairColumns);
                 if (p.resident && (u.group != weight_group || tile_col != weight_col)) {
-                    if (weight_group >= 0) mma_commit_pair(&pipe.weight_empty);
+                    if (weight_group >= 0 && elected()) commit<true>(&pipe.weight_empty);
                     weight_group = u.group;
                     weight_col = tile_col;
                 }
-                sound = pipe.sums_empty[sums.stage].wait(sums.round ^ 1, failed);
+                sound = __all_sync(0xffffffffu, pipe.sums_empty[sums.stage].wait(sums.round ^ 1, failed));
                 if (!sound) break;
                 fence_after_sync();
                 const uint32_t d = pipe.tmem + sums.stage * kPairColumns;
                 for (int s = 0; s < slices; ++s) {
-                    sound = pipe.full[ring_at.stage].wait(ring_at.round, failed);
+                    sound = __all_sync(0xffffffffu, pipe.full[ring_at.stage].wait(ring_at.round, failed));
                     if (!sound) break;
                     fence_after_sync();
-                    const char *a = ring + ring_at.stage * stage_bytes;
-                    const char *b = weight + (p.resident ? s * weight_step : ring_at.stage * stage_bytes);
+                    const uint32_t at = ring_at.stage * (stage_bytes / 16);
+                    const uint32_t a = a0 + at, b = b0 + (p.resident ? s * (weight_step / 16) : at);
+                    if (elected()) {
 #pragma unroll
-                    for (int k = 0; k < kSliceK / 16; ++k) {
-                        const uint64_t da = operand(a + 32 * k, 16, kAtom);
-                        const uint64_t db = kWeightMn ? operand(b + 2 * kAtom * k, 64 * kSliceK * 2, kAtom) : operand(b + 32 * k, 16, kAtom);
-                        mma_f16_pair(d, da, db, kInstruction, s > 0 || k > 0);
+                        for (int k = 0; k < kSliceK / 16; ++k)
+                            mma_f16<true>(d, a + 2 * k, kHigh, b + kStepB * k, kHigh, kInstruction, s > 0 || k > 0);
+                        commit<true>(&pipe.empty[ring_at.stage]);
                     }
-                    mma_commit_pair(&pipe.empty[ring_at.stage]);
                     ring_at.next();
                 }
                 if (!sound) break;
-                mma_commit_pair(&pipe.sums_full[sums.stage]);
+                if (elected()) commit<true>(&pipe.sums_full[sums.stage]);
                 sums.next();
             }
         }
@@ -699,7 +701,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
     bool any = false;
 
     struct Item {
-        int group, piece, out0, in0, first, last;  // blocks first .. last - 1 of the group
+        int group, piece, out0, in0, first, last, step;  // blocks first, first + step, ... of the group, below last
     };
     const auto item_at = [&](long long i) {
         Item it;
@@ -708,9 +710,43 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         it.piece = piece - table.piece_begin[it.group];
         it.out0 = (t / in_tiles) * W::kOutputs + (int)rank * kTileRows;  // this block's
         it.in0 = (t % in_tiles) * BN;
-        it.first = it.piece * p.piece;
-        it.last = min(group_blocks(p.g, table.start, it.group, kSliceK), it.first + p.piece);
+        // the pieces of a group take its blocks in turn, so that at any time they read neighbouring rows
+        it.first = it.piece;
+        it.step = table.piece_begin[it.group + 1] - table.piece_begin[it.group];
+        it.last = group_blocks(p.g, table.start, it.group, kSliceK);
         return it;
+    };
+
+    // An item's blocks one after the other, without a division for each: 0.75 us a block of 256 x 256 x 64 with one, twice what the
+    // products take.
+    struct Walk {
+        int row, count;  // of the current block: its first row over all batch elements, its rows
+        int left;        // blocks to come, this one among them
+        int index, per, length, rows, step, base;
+        __device__ __forceinline__ void place() {
+            row = base + index * kSliceK;
+            count = min(kSliceK, length - index * kSliceK);
+        }
+        __device__ __forceinline__ void next() {
+            for (index += step; index >= per; index -= per) base += rows;
+            place();
+            --left;
+        }
+    };
+    const auto walk = [&](const Item &it) {
+        Walk w;
+        const int start = table.start[it.group];
+        w.length = table.start[it.group + 1] - start;
+        w.per = (int)(((long long)w.length + kSliceK - 1) / kSliceK);
+        w.left = it.first < it.last ? (it.last - it.first + it.step - 1) / it.step : 0;
+        w.rows = p.g.rows;
+        w.step = it.step;
+        if (w.left > 0) {
+            w.index = it.first % w.per;
+            w.base = start + it.first / w.per * p.g.rows;
+            w.place();
+        }
+        return w;
     };
 
     if (warp == 0) {
@@ -718,10 +754,8 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
             bool sound = true;
             for (long long i = worker; i < items && sound; i += workers) {
                 const Item it = item_at(i);
-                for (int j = it.first; j < it.last; ++j) {
-                    long long row;
-                    int count;
-                    block_rows(p.g, table.start, it.group, kSliceK, j, row, count);
+                for (Walk at = walk(it); at.left > 0; at.next()) {
+                    const int row = at.row;
                     sound = pipe.empty[ring_at.stage].wait(ring_at.round ^ 1, failed);
                     if (!sound) break;
                     char *a = ring + ring_at.stage * W::kBytes, *b = a + kBytesA;
@@ -732,15 +766,15 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                         const uint32_t first = cluster_address(bar, 0);
 #pragma unroll
                         for (int k = 0; k < kTileRows / 64; ++k)
-                            tma_2d_pair(&map_g, a + k * (64 * kSliceK * 2), first, it.out0 + 64 * k, (int)row);
+                            tma_2d_pair(&map_g, a + k * (64 * kSliceK * 2), first, it.out0 + 64 * k, row);
 #pragma unroll
                         for (int k = 0; k < W::kColumnsB / 64; ++k)
-                            tma_2d_pair(&map_x, b + k * (64 * kSliceK * 2), first, in0 + 64 * k, (int)row);
+                            tma_2d_pair(&map_x, b + k * (64 * kSliceK * 2), first, in0 + 64 * k, row);
                     } else {
 #pragma unroll
-                        for (int k = 0; k < kTileRows / 64; ++k) tma_2d(&map_g, a + k * (64 * kSliceK * 2), bar, it.out0 + 64 * k, (int)row);
+                        for (int k = 0; k < kTileRows / 64; ++k) tma_2d(&map_g, a + k * (64 * kSliceK * 2), bar, it.out0 + 64 * k, row);
 #pragma unroll
-                        for (int k = 0; k < W::kColumnsB / 64; ++k) tma_2d(&map_x, b + k * (64 * kSliceK * 2), bar, in0 + 64 * k, (int)row);
+                        for (int k = 0; k < W::kColumnsB / 64; ++k) tma_2d(&map_x, b + k * (64 * kSliceK * 2), bar, in0 + 64 * k, row);
                     }
                     ring_at.next();
                     any = true;
@@ -763,6 +797,9 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
+        constexpr uint32_t kHigh = operand_high(kAtom);
+        const uint32_t a0 = operand_low(ring, 64 * kSliceK * 2), b0 = operand_low(ring + kBytesA, 64 * kSliceK * 2), ones0 = operand_low(ones, 16);
+        const uint32_t pipe_tmem = pipe.tmem;
         unsigned round = 0, masks = 0;
         bool sound = true;
         for (long long i = worker; i < items && sound; i += workers) {
@@ -774,11 +811,10 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                 if (!sound) break;
                 fence_after_sync();
             }
-            for (int j = it.first; j < it.last; ++j) {
-                long long row;
-                int count;
-                block_rows(p.g, table.start, it.group, kSliceK, j, row, count);
-                char *a = ring + ring_at.stage * W::kBytes, *b = a + kBytesA;
+            bool more = false;
+            for (Walk at = walk(it); at.left > 0; at.next()) {
+                const int count = at.count;
+                char *a = ring + ring_at.stage * W::kBytes;
                 if (rank != 0) {  // the second block clears its lines when the first has seen the copies of both
                     if (count < kSliceK) {
                         sound = __all_sync(0xffffffffu, pipe.mask_go.wait(masks++ & 1, failed));
@@ -801,31 +837,23 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                     }
                 }
                 fence_after_sync();
-                if (lane == 0) {
+                if (elected()) {
+                    const uint32_t at = ring_at.stage * (W::kBytes / 16);
 #pragma unroll
                     for (int k = 0; k < kSliceK / 16; ++k) {
-                        const uint64_t da = operand(a + 2 * kAtom * k, 64 * kSliceK * 2, kAtom);
-                        const uint64_t db = operand(b + 2 * kAtom * k, 64 * kSliceK * 2, kAtom), d1 = operand(ones + 32 * k, 16, kAtom);
-                        const bool more = j > it.first || k > 0;
-                        if (kPair) {
-                            mma_f16_pair(pipe.tmem, da, db, kInstruction, more);
-                            if (bias) mma_f16_pair(pipe.tmem + BN, da, d1, kOnesInstruction, more);
-                        } else {
-                            mma_f16(pipe.tmem, da, db, kInstruction, more);
-                            if (bias) mma_f16(pipe.tmem + BN, da, d1, kOnesInstruction, more);
-                        }
+                        const bool sum = more || k > 0;
+                        const uint32_t ak = a0 + at + 2 * kAtom / 16 * k;
+                        mma_f16<kPair>(pipe_tmem, ak, kHigh, b0 + at + 2 * kAtom / 16 * k, kHigh, kInstruction, sum);
+                        if (bias) mma_f16<kPair>(pipe_tmem + BN, ak, kHigh, ones0 + 2 * k, kHigh, kOnesInstruction, sum);
                     }
-                    if (kPair) mma_commit_pair(&pipe.empty[ring_at.stage]);
-                    else mma_commit(&pipe.empty[ring_at.stage]);
+                    commit<kPair>(&pipe.empty[ring_at.stage]);
                 }
+                more = true;
                 __syncwarp();
                 ring_at.next();
             }
             if (!sound) break;
-            if (lane == 0 && rank == 0) {
-                if (kPair) mma_commit_pair(&pipe.sums_full[0]);
-                else mma_commit(&pipe.sums_full[0]);
-            }
+            if (rank == 0 && elected()) commit<kPair>(&pipe.sums_full[0]);
             __syncwarp();
             round ^= 1;
         }
