@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(kThreads) linear_weight_grad_kernel(const Weig
 
 // Adds the slots of the groups that were computed in pieces, in order.  A block takes 1024 elements of a group's slots, or with
 // kSplit 128, whose slots its eight warps share and whose eight sums are added in order: for many slots, where a thread's
-// chain of loads would be the time (148 slots of 256 x 256: 28 us in one chain, 11 in eight; 40 slots of 16 groups 27 us against 84).
+// chain of loads would be the time (74 slots of 256 x 256 for each of 3 groups: 28 us in one chain, 13 in eight; 18 slots of 1024 x
+// 256 8 us against 15).
 constexpr int kSumWarps = 8, kLaneElements = 4;
 
 template <typename T, bool kSplit>
@@ -349,11 +350,12 @@ Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int le
     Cut c;
     c.block = block;
     const long long blocks = std::max<long long>(1, most_units(batch, rows, groups, block, false));
-    // One piece more than the SMs take would be a round of its own.  Every further group can add a piece that is not full; where
-    // there are too many groups for that, pieces half as long, so that the last round is short.
+    // One piece more than the SMs take would be a round of its own, and every further group can add one that is not full.  Where there
+    // are many groups for the SMs, only those twice the mean are cut: each piece has its start and its sums to write and add
+    // (16 uneven groups, 256 -> 1024: pieces of 8 blocks 42 + 14 us, of 34 2x + y).
     const long long wanted = std::max<long long>(1, workers / tiles);
-    const long long full = wanted >= 2 * groups ? wanted - (groups - 1) : 2 * wanted;
-    c.piece = (int)std::max<long long>(least_piece, ceil_div(blocks, full));
+    const long long length = wanted >= 2 * groups ? ceil_div(blocks, wanted - (groups - 1)) : 2 * ceil_div(blocks, groups);
+    c.piece = (int)std::max<long long>(least_piece, length);
     if (blocks <= 2 * least_piece) c.piece = (int)blocks;  // the second launch would cost more than it spreads
     c.pieces = ceil_div(blocks, c.piece) + groups;
     // a group of n > 1 pieces has more than (n - 1) * piece blocks, so at least n / 2 * piece
@@ -418,11 +420,13 @@ struct Padding {
 
 __global__ void __launch_bounds__(kThreads) linear_pad_kernel(const Padding p) {
     const unsigned long long step = (unsigned long long)gridDim.x * kThreads, first = (unsigned long long)blockIdx.x * kThreads + threadIdx.x;
-    for (int i = 0; i < p.count; ++i) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        if (i >= p.count) break;
         const int line = p.line[i];
         const unsigned units = (unsigned)(line + 7) / 8;
         for (unsigned long long u = first; u < p.units[i]; u += step) {
-            const unsigned long long row = u / units;
+            const unsigned long long row = u >> 32 ? u / units : (unsigned)u / units;
             const int c = (int)(u - row * units) * 8;
             const unsigned short *s = p.src[i] + row * line + c;
             unsigned v[4];
@@ -590,8 +594,7 @@ struct Gradients {
 template <typename T>
 int sum_slots(const WeightGrad<T> &q, const Shape &s, const Cut &c, cudaStream_t st) {
     if (c.slots == 0) return FDA_OK;
-    const long long unsplit = ceil_div(((long long)s.in_features + 1) * s.out_features, 32 * kLaneElements * kSumWarps) * s.groups;
-    const bool split = c.pieces > 16ll * s.groups && unsplit < kSms;
+    const bool split = c.pieces > 32 + s.groups && c.pieces > 8ll * s.groups;
     const long long items = ceil_div(((long long)s.in_features + 1) * s.out_features, 32 * kLaneElements * (split ? 1 : kSumWarps)) * s.groups;
     const unsigned blocks = (unsigned)std::min<long long>(items, 4 * kSms);
     if (split) linear_weight_grad_sum_kernel<T, true><<<blocks, 32 * kSumWarps, 0, st>>>(q);

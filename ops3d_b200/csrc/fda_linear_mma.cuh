@@ -397,16 +397,19 @@ __device__ __forceinline__ void rows_of_fetched(const Fetched &f, Stage &stage, 
         own_row_from(stage, half, v);
     }
 }
-// Rows that no vector access reaches.
+// Rows that no vector access reaches, an element a lane.  All loads are on their way before the first is used.
 template <typename T>
 __device__ __forceinline__ void load_elements(const T *p, unsigned pitch, int rows, int count, Stage &stage, uint32_t (&v)[16]) {
     const int lane = threadIdx.x % 32;
     const unsigned short *s = reinterpret_cast<const unsigned short *>(p);
+    unsigned short e[32];
+#pragma unroll
+    for (int r = 0; r < 32; ++r) e[r] = (r < rows && lane < count) ? s[(size_t)(r * pitch) + lane] : 0;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         __syncwarp();
-#pragma unroll 4
-        for (int r = 0; r < 16; ++r) *stage_element(stage, r, lane) = (16 * half + r < rows && lane < count) ? s[(size_t)((16 * half + r) * pitch) + lane] : 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) *stage_element(stage, r, lane) = e[16 * half + r];
         __syncwarp();
         own_row_from(stage, half, v);
     }

@@ -303,10 +303,13 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                     rows_of_fetched(fetched, stage, v);
                     if (c + 1 < kChunks && count > 32) fetch(u, c + 1);
                     else if (tile + gridDim.x < tiles) fetch(next, 0);
-                } else if (kExtra) {
-                    load_elements(p.extra + (size_t)u.first * p.extra_pitch + col0 + 32 * c, p.extra_pitch, rows, count, stage, v);
                 }
             };
+            // (tiles of which no vector access reaches the rows have one chunk a warp)
+            uint32_t elements[16] = {};
+            static_assert(kVector || kChunks == 1, "");
+            if (kExtra && !kVector)
+                load_elements(p.extra + (size_t)u.first * p.extra_pitch + col0, p.extra_pitch, rows, p.cols - col0, stage, elements);
             if (col0 >= p.cols) {  // no column of this part: nothing is fetched or stored, but the tile counts
                 if (tile + gridDim.x < tiles) fetch(next, 0);
             }
@@ -326,8 +329,8 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                 for (int c = 0; c < kChunks; ++c)
                     if (col0 + 32 * c < p.cols) {
                         uint32_t row[16] = {};
-                        extra_of(c, p.cols - col0 - 32 * c, row);
-                        store_rows<kVector>(out_rows + 32 * c, p.out_pitch, rows, p.cols - col0 - 32 * c, stage, row);
+                        if (kVector) extra_of(c, p.cols - col0 - 32 * c, row);
+                        store_rows<kVector>(out_rows + 32 * c, p.out_pitch, rows, p.cols - col0 - 32 * c, stage, kVector ? row : elements);
                     }
                 continue;
             }
@@ -339,7 +342,12 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                 const int count = p.cols - col0 - 32 * c;
                 if (count <= 0) break;
                 uint32_t row[16];
-                extra_of(c, count, row);
+                if (kVector) {
+                    extra_of(c, count, row);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) row[j] = elements[j];
+                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t v[16];
@@ -985,6 +993,10 @@ int allow_shared(Kernel kernel, int bytes) {
     return status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
 }
 
+// Whether a block (or pair) of `most` meets the same group several times in a row; otherwise slices of the weight stream with the rows,
+// which waits for no tile to end.
+bool weight_stays(long long tiles, int groups, int most) { return groups == 1 || tiles >= 2ll * groups * most; }
+
 // Blocks (or pairs) for `tiles`: a multiple of the column tiles where the weight is resident and that leaves few SMs idle.
 unsigned row_grid(long long tiles, long long columns, unsigned most, bool resident) {
     if (tiles <= most) return (unsigned)tiles;
@@ -1006,8 +1018,8 @@ int launch_rows(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t s
     } else {
         map_extra = map_a;
     }
-    a.resident = ceil_div(a.depth, kSliceK) * Shape<BN>::kBytesB <= kResidentBytes;
     const long long tiles = units * ceil_div(a.cols, BN);
+    a.resident = ceil_div(a.depth, kSliceK) * Shape<BN>::kBytesB <= kResidentBytes && weight_stays(tiles, p.g.groups, kSms);
     if (tiles >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
     kernel<<<row_grid(tiles, ceil_div(a.cols, BN), kSms, a.resident), Shape<BN>::kThreads, kSmem, st>>>(a, map_a, map_w, map_extra);
     return status(cudaGetLastError());
@@ -1026,8 +1038,9 @@ int launch_pair(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t s
     map_extra = map_a;
     if (a.extra)
         if (const int rc = make_map(map_extra, p.dtype, p.extra, a.cols, rows, p.extra_pitch, 32, 0)) return rc;
-    a.resident = pair_ring(kMode == kForward || kMode == kPreGrad) - ceil_div(a.depth, kSliceK) * kPairBytesB >= kPairLeastStages * kBytesA;
     const long long tiles = units * ceil_div(a.cols, kPairColumns);
+    a.resident = pair_ring(kMode == kForward || kMode == kPreGrad) - ceil_div(a.depth, kSliceK) * kPairBytesB >= kPairLeastStages * kBytesA &&
+                 weight_stays(tiles, p.g.groups, kSms / 2);
     if (tiles >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
     kernel<<<2 * row_grid(tiles, ceil_div(a.cols, kPairColumns), kSms / 2, a.resident), kPairThreads, kPairSmem, st>>>(a, map_a, map_w, map_extra);
     return status(cudaGetLastError());
