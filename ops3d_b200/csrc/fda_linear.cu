@@ -95,6 +95,7 @@ template <int kMode, int kAct>
 __global__ void __launch_bounds__(kThreads) linear_rows_kernel(const RowProduct<float> p) {
     __shared__ RowTable table;
     __shared__ __align__(16) Slices slices;
+    wait_for_previous_kernel();
     build_row_table(p.g, kTile, kMode != kPreGrad, table);
     __syncthreads();
     const int column_tiles = (p.cols + kTile - 1) / kTile;
@@ -165,6 +166,7 @@ template <typename T, int kMode, bool kVector>
 __global__ void __launch_bounds__(kFewThreads) linear_few_rows_kernel(const RowProduct<T> p, const int activation) {
     constexpr int kCount = 16 / sizeof(T);
     __shared__ RowTable table;
+    wait_for_previous_kernel();
     build_row_table(p.g, kFewRows, kMode != kPreGrad, table);
     __syncthreads();
     const int lane = threadIdx.x % 32;
@@ -237,6 +239,7 @@ struct WeightGrad {
 __global__ void __launch_bounds__(kThreads) linear_weight_grad_kernel(const WeightGrad<float> p) {
     __shared__ PieceTable table;
     __shared__ __align__(16) Slices slices;
+    wait_for_previous_kernel();
     build_piece_table(p.g, p.block, p.piece, table);
     __syncthreads();
     const int out_tiles = (p.out_features + kTile - 1) / kTile, in_tiles = (p.in_features + kTile - 1) / kTile;
@@ -287,6 +290,7 @@ template <typename T, bool kSplit>
 __global__ void __launch_bounds__(32 * kSumWarps) linear_weight_grad_sum_kernel(const WeightGrad<T> p) {
     __shared__ PieceTable table;
     __shared__ float partial[kSplit ? kSumWarps : 1][32 * kLaneElements];
+    wait_for_previous_kernel();
     build_piece_table(p.g, p.block, p.piece, table);
     __syncthreads();
     const size_t size = (size_t)p.out_features * p.in_features, both = size + p.out_features;
@@ -382,8 +386,7 @@ int check_groups(const Shape &s, const int64_t *starts, int num_starts) {
     return (num_starts == s.groups || num_starts == s.groups + 1) ? FDA_OK : FDA_ERR_BAD_SHAPE;
 }
 
-int launched() {
-    const cudaError_t e = cudaGetLastError();
+int launched(cudaError_t e) {
     if (e == cudaSuccess) return FDA_OK;
     fda::record_cuda_error((int)e);
     return FDA_ERR_CUDA;
@@ -394,8 +397,7 @@ constexpr int kPlainBlock = 256, kPlainLeastPiece = 1;
 template <int kMode, int kAct>
 int run_rows(const RowProduct<float> &p, cudaStream_t st) {
     const long long tiles = most_units(p.g.batch, p.g.rows, p.g.groups, kTile, kMode != kPreGrad) * ceil_div(p.cols, kTile);
-    linear_rows_kernel<kMode, kAct><<<(unsigned)std::min<long long>(tiles, 8 * kSms), kThreads, 0, st>>>(p);
-    return launched();
+    return launched(launch_early(linear_rows_kernel<kMode, kAct>, (unsigned)std::min<long long>(tiles, 8 * kSms), kThreads, 0, st, 1, p));
 }
 
 template <int kMode>
@@ -419,6 +421,7 @@ struct Padding {
 };
 
 __global__ void __launch_bounds__(kThreads) linear_pad_kernel(const Padding p) {
+    wait_for_previous_kernel();
     const unsigned long long step = (unsigned long long)gridDim.x * kThreads, first = (unsigned long long)blockIdx.x * kThreads + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
@@ -453,8 +456,8 @@ void align_rows(Padding &p, const void *&src, char *place, size_t rows, int line
 int pad(const Padding &p, cudaStream_t st) {
     if (p.count == 0) return FDA_OK;
     const unsigned long long most = *std::max_element(p.units, p.units + p.count);
-    linear_pad_kernel<<<(unsigned)std::min<unsigned long long>((most + kThreads - 1) / kThreads, 16 * kSms), kThreads, 0, st>>>(p);
-    return launched();
+    const unsigned blocks = (unsigned)std::min<unsigned long long>((most + kThreads - 1) / kThreads, 16 * kSms);
+    return launched(launch_early(linear_pad_kernel, blocks, kThreads, 0, st, 1, p));
 }
 
 // What the workspaces hold, one behind the other.
@@ -540,9 +543,8 @@ int run_few_rows(const RowProduct<T> &p, int activation, cudaStream_t st) {
     const long long warps = most_units(p.g.batch, p.g.rows, p.g.groups, kFewRows, kMode != kPreGrad && p.g.starts) * steps;
     const unsigned blocks = (unsigned)std::min<long long>(ceil_div(warps, kFewThreads / 32), 16 * kSms);
     const bool vector = p.depth % (16 / sizeof(T)) == 0 && ((uintptr_t)p.a | (uintptr_t)p.w) % 16 == 0;
-    if (vector) linear_few_rows_kernel<T, kMode, true><<<blocks, kFewThreads, 0, st>>>(p, activation);
-    else linear_few_rows_kernel<T, kMode, false><<<blocks, kFewThreads, 0, st>>>(p, activation);
-    return launched();
+    return launched(launch_early(vector ? linear_few_rows_kernel<T, kMode, true> : linear_few_rows_kernel<T, kMode, false>, blocks, kFewThreads, 0,
+                                 st, 1, p, activation));
 }
 
 // out = act(x W^T + bias) + extra, or extra * act'(x W^T + bias)
@@ -597,9 +599,8 @@ int sum_slots(const WeightGrad<T> &q, const Shape &s, const Cut &c, cudaStream_t
     const bool split = c.pieces > 32 + s.groups && c.pieces > 8ll * s.groups;
     const long long items = ceil_div(((long long)s.in_features + 1) * s.out_features, 32 * kLaneElements * (split ? 1 : kSumWarps)) * s.groups;
     const unsigned blocks = (unsigned)std::min<long long>(items, 4 * kSms);
-    if (split) linear_weight_grad_sum_kernel<T, true><<<blocks, 32 * kSumWarps, 0, st>>>(q);
-    else linear_weight_grad_sum_kernel<T, false><<<blocks, 32 * kSumWarps, 0, st>>>(q);
-    return launched();
+    return launched(launch_early(split ? linear_weight_grad_sum_kernel<T, true> : linear_weight_grad_sum_kernel<T, false>, blocks,
+                                 32 * kSumWarps, 0, st, 1, q));
 }
 
 template <typename T>
@@ -641,8 +642,8 @@ int backward_f32(const Shape &s, const Groups &g, const void *x, const void *wei
     const Cut c = weight_cut(s);
     const WeightGrad<float> q = weight_grad_args<float>(s, g, c, grad, x, out, ws, l);
     const long long items = c.pieces * ceil_div(s.out_features, kTile) * ceil_div(s.in_features, kTile);
-    linear_weight_grad_kernel<<<(unsigned)std::min<long long>(items, 8 * kSms), kThreads, 0, st>>>(q);
-    if (const int rc = launched()) return rc;
+    if (const int rc = launched(launch_early(linear_weight_grad_kernel, (unsigned)std::min<long long>(items, 8 * kSms), kThreads, 0, st, 1, q)))
+        return rc;
     return sum_slots(q, s, c, st);
 }
 

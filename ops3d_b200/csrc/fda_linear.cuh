@@ -21,6 +21,13 @@ namespace fda_linear {
 
 constexpr int kMaxGroups = FDA_LINEAR_MAX_GROUPS;
 
+// A kernel may be set up while the one before it in the stream still runs: everything in front of this call touches no memory
+// but its own block's, and nothing behind it comes before the earlier kernel has ended and its results are visible.
+__device__ __forceinline__ void wait_for_previous_kernel() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
@@ -246,6 +253,26 @@ inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 inline size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 constexpr int kSms = 148;
+
+// Launch of a kernel that calls wait_for_previous_kernel, by clusters of `cluster` blocks.
+template <typename... Parameters, typename... Arguments>
+cudaError_t launch_early(void (*kernel)(Parameters...), unsigned grid, unsigned threads, int shared, cudaStream_t st, int cluster,
+                         const Arguments &...arguments) {
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t launch{};
+    launch.gridDim = dim3(grid);
+    launch.blockDim = dim3(threads);
+    launch.dynamicSmemBytes = shared;
+    launch.stream = st;
+    launch.attrs = attributes;
+    launch.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&launch, kernel, Parameters(arguments)...);
+}
 
 // Upper bound of a row table's units, whatever the start indices are: every section adds at most one incomplete unit per batch
 // element.

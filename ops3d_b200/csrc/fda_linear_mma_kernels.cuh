@@ -164,6 +164,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         prefetch_map(&map_w);
     }
     pipeline_begin<false>(pipe, kColumns, Shape<BN>::kEpilogueWarps);
+    wait_for_previous_kernel();
     build_row_table(p.g, kTileRows, kMode != kPreGrad, table);
     __syncthreads();
     fence_after_sync();
@@ -398,7 +399,7 @@ __device__ __forceinline__ const uint4 *buffer_unit(const char *buffer, int r, i
 }
 
 template <typename T, int kMode, int kAct>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
     linear_rows_pair_kernel(const RowsArgs<T> p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                             const __grid_constant__ CUtensorMap map_extra) {
     constexpr bool kWeightMn = kMode == kGradX;
@@ -432,6 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
     __syncwarp();
     if (warp == 0) tmem_alloc_pair(&pipe.tmem, kColumns);
+    wait_for_previous_kernel();
     build_row_table(p.g, kPairRows, kMode != kPreGrad, table);
     fence_before_sync();
     __syncthreads();
@@ -696,6 +698,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
     pipeline_begin<kPair>(pipe, kColumns, Shape<BN>::kEpilogueWarps);
     for (int i = threadIdx.x; i < kOnesBytes / 4; i += Shape<BN>::kThreads) reinterpret_cast<uint32_t *>(ones)[i] = pack2<T>(1.f, 1.f);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    wait_for_previous_kernel();
     build_piece_table(p.g, kSliceK, p.piece, table);
     __syncthreads();
     if (kPair) cluster_sync();
@@ -1021,8 +1024,8 @@ int launch_rows(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t s
     const long long tiles = units * ceil_div(a.cols, BN);
     a.resident = ceil_div(a.depth, kSliceK) * Shape<BN>::kBytesB <= kResidentBytes && weight_stays(tiles, p.g.groups, kSms);
     if (tiles >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
-    kernel<<<row_grid(tiles, ceil_div(a.cols, BN), kSms, a.resident), Shape<BN>::kThreads, kSmem, st>>>(a, map_a, map_w, map_extra);
-    return status(cudaGetLastError());
+    return status(launch_early(kernel, row_grid(tiles, ceil_div(a.cols, BN), kSms, a.resident), Shape<BN>::kThreads, kSmem, st, 1, a, map_a,
+                               map_w, map_extra));
 }
 
 template <typename T, int kMode, int kAct>
@@ -1042,8 +1045,8 @@ int launch_pair(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t s
     a.resident = pair_ring(kMode == kForward || kMode == kPreGrad) - ceil_div(a.depth, kSliceK) * kPairBytesB >= kPairLeastStages * kBytesA &&
                  weight_stays(tiles, p.g.groups, kSms / 2);
     if (tiles >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
-    kernel<<<2 * row_grid(tiles, ceil_div(a.cols, kPairColumns), kSms / 2, a.resident), kPairThreads, kPairSmem, st>>>(a, map_a, map_w, map_extra);
-    return status(cudaGetLastError());
+    return status(launch_early(kernel, 2 * row_grid(tiles, ceil_div(a.cols, kPairColumns), kSms / 2, a.resident), kPairThreads, kPairSmem, st,
+                               2, a, map_a, map_w, map_extra));
 }
 
 template <typename T, int kMode, int kAct>
@@ -1115,18 +1118,8 @@ int launch_weight_grad(const MmaWeightGrad &p, cudaStream_t st) {
     if (const int rc = make_map(map_g, p.dtype, p.grad, p.out_features, rows, p.grad_pitch, kSliceK, 0)) return rc;
     if (const int rc = make_map(map_x, p.dtype, p.x, p.in_features, rows, p.x_pitch, kSliceK, 0)) return rc;
     const long long items = p.cut.pieces * ceil_div(p.out_features, W::kOutputs) * ceil_div(p.in_features, BN);
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = kPair ? 2 : 1;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    cudaLaunchConfig_t launch{};
-    launch.gridDim = dim3((unsigned)std::min<long long>(items, kPair ? kSms / 2 : kSms) * (kPair ? 2 : 1));
-    launch.blockDim = dim3(Shape<BN>::kThreads);
-    launch.dynamicSmemBytes = kSmem;
-    launch.stream = st;
-    launch.attrs = &cluster;
-    launch.numAttrs = 1;
-    return status(cudaLaunchKernelEx(&launch, kernel, a, map_g, map_x));
+    const unsigned workers = (unsigned)std::min<long long>(items, kPair ? kSms / 2 : kSms);
+    return status(launch_early(kernel, kPair ? 2 * workers : workers, Shape<BN>::kThreads, kSmem, st, kPair ? 2 : 1, a, map_g, map_x));
 }
 
 template <typename T, bool kVector>
