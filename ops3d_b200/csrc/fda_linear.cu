@@ -375,7 +375,7 @@ Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int le
     const long long blocks = std::max<long long>(1, most_units(batch, rows, groups, block, false));
     // One piece more than the SMs take would be a round of its own, and every further group can add one that is not full.  Where there
     // are many groups for the SMs, only those twice the mean are cut: each piece has its start and its sums to write and add
-    // (16 uneven groups, 256 -> 1024: pieces of 8 blocks 42 + 14 us, of 34 2x + y).
+    // (16 uneven groups, 256 -> 1024: pieces of 8 blocks 42 + 14 us, of 34 28 + 7).
     const long long wanted = std::max<long long>(1, workers / tiles);
     const long long length = wanted >= 2 * groups ? ceil_div(blocks, wanted - (groups - 1)) : 2 * ceil_div(blocks, groups);
     c.piece = (int)std::max<long long>(least_piece, length);

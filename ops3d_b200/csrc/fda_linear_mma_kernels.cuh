@@ -115,7 +115,7 @@ struct RowsArgs {
 
 // A resident weight: where all slices of a column tile fit (kResidentBytes), a block keeps them and only rows stream through the
 // ring.  The grid is a multiple of the column tiles, so a block's column stays and its weight changes with the group or not at all;
-// at any time the blocks work on neighbouring rows (a contiguous range of rows each was slower: 172 instead of 15x us for
+// at any time the blocks work on neighbouring rows (a contiguous range of rows each was slower: 172 instead of 131 us for
 // 149504 x 256 x 1024 with a residual).
 // Per 128 x 256 tile of 256 inputs 64 KB instead of 192 pass from L2, whose 9 TB/s had been the bound (149504 x 256 x 1024: 107 us).
 constexpr int kResidentStages = 4;
@@ -220,44 +220,42 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         }
         __syncwarp();
     } else if (warp == 1) {
-        {
-            constexpr uint32_t kInstruction = instruction<T>(kTileRows, BN, false, kWeightMn);
-            constexpr uint32_t kHigh = operand_high(kAtom), kStepB = kWeightMn ? 2 * kAtom / 16 : 2;  // of 16 contraction indices
-            const uint32_t a0 = operand_low(ring, 16), b0 = operand_low(weight, kWeightMn ? 64 * kSliceK * 2 : 16);
-            Ring sums(2);
-            bool sound = true;
-            int weight_group = -1, weight_col = -1;
-            for (unsigned tile = blockIdx.x; tile < tiles && sound; tile += gridDim.x) {
-                const RowUnit u = row_unit(p.g, table, kTileRows, tile / columns);
-                if (u.group < 0) continue;
-                const int tile_col = (int)(tile % columns * BN);
-                if (p.resident && (u.group != weight_group || tile_col != weight_col)) {
-                    if (weight_group >= 0 && elected()) commit<false>(&pipe.weight_empty);
-                    weight_group = u.group;
-                    weight_col = tile_col;
-                }
-                sound = __all_sync(0xffffffffu, pipe.sums_empty[sums.stage].wait(sums.round ^ 1, failed));
+        constexpr uint32_t kInstruction = instruction<T>(kTileRows, BN, false, kWeightMn);
+        constexpr uint32_t kHigh = operand_high(kAtom), kStepB = kWeightMn ? 2 * kAtom / 16 : 2;  // of 16 contraction indices
+        const uint32_t a0 = operand_low(ring, 16), b0 = operand_low(weight, kWeightMn ? 64 * kSliceK * 2 : 16);
+        Ring sums(2);
+        bool sound = true;
+        int weight_group = -1, weight_col = -1;
+        for (unsigned tile = blockIdx.x; tile < tiles && sound; tile += gridDim.x) {
+            const RowUnit u = row_unit(p.g, table, kTileRows, tile / columns);
+            if (u.group < 0) continue;
+            const int tile_col = (int)(tile % columns * BN);
+            if (p.resident && (u.group != weight_group || tile_col != weight_col)) {
+                if (weight_group >= 0 && elected()) commit<false>(&pipe.weight_empty);
+                weight_group = u.group;
+                weight_col = tile_col;
+            }
+            sound = __all_sync(0xffffffffu, pipe.sums_empty[sums.stage].wait(sums.round ^ 1, failed));
+            if (!sound) break;
+            fence_after_sync();
+            const uint32_t d = pipe.tmem + sums.stage * BN;
+            for (int s = 0; s < slices; ++s) {
+                sound = __all_sync(0xffffffffu, pipe.full[ring_at.stage].wait(ring_at.round, failed));
                 if (!sound) break;
                 fence_after_sync();
-                const uint32_t d = pipe.tmem + sums.stage * BN;
-                for (int s = 0; s < slices; ++s) {
-                    sound = __all_sync(0xffffffffu, pipe.full[ring_at.stage].wait(ring_at.round, failed));
-                    if (!sound) break;
-                    fence_after_sync();
-                    const uint32_t at = ring_at.stage * (stage_bytes / 16);
-                    const uint32_t a = a0 + at, b = b0 + (p.resident ? s * (weight_step / 16) : at);
-                    if (elected()) {
+                const uint32_t at = ring_at.stage * (stage_bytes / 16);
+                const uint32_t a = a0 + at, b = b0 + (p.resident ? s * (weight_step / 16) : at);
+                if (elected()) {
 #pragma unroll
-                        for (int k = 0; k < kSliceK / 16; ++k)
-                            mma_f16<false>(d, a + 2 * k, kHigh, b + kStepB * k, kHigh, kInstruction, s > 0 || k > 0);
-                        commit<false>(&pipe.empty[ring_at.stage]);
-                    }
-                    ring_at.next();
+                    for (int k = 0; k < kSliceK / 16; ++k)
+                        mma_f16<false>(d, a + 2 * k, kHigh, b + kStepB * k, kHigh, kInstruction, s > 0 || k > 0);
+                    commit<false>(&pipe.empty[ring_at.stage]);
                 }
-                if (!sound) break;
-                if (elected()) commit<false>(&pipe.sums_full[sums.stage]);
-                sums.next();
+                ring_at.next();
             }
+            if (!sound) break;
+            if (elected()) commit<false>(&pipe.sums_full[sums.stage]);
+            sums.next();
         }
         __syncwarp();
     } else if (warp >= kFirstEpilogueWarp) {
@@ -659,7 +657,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // the contraction.  The bias's gradient is one more narrow product of the same g with ones.
 //
 // kPair: two blocks make 256 outputs x 256 inputs, each with its own 128 outputs and half of the inputs, so that 32 instead of 48 KB
-// pass from L2 for 64 rows (73728 rows, 256 -> 1024: 54 -> 4x us).
+// pass from L2 for 64 rows (73728 rows, 256 -> 1024: 51 -> 45 us).
 constexpr int kOnesColumns = 16;
 constexpr int kOnesBytes = kOnesColumns * kSliceK * 2;
 
@@ -728,8 +726,8 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         return it;
     };
 
-    // An item's blocks one after the other, without a division for each: 0.75 us a block of 256 x 256 x 64 with one, twice what the
-    // products take.
+    // An item's blocks one after the other, without a division for each (with one the 512 blocks of 4736 x 8192 x 1024 took 166 us, 154
+    // without).
     struct Walk {
         int row, count;  // of the current block: its first row over all batch elements, its rows
         int left;        // blocks to come, this one among them
@@ -739,9 +737,9 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
             count = min(kSliceK, length - index * kSliceK);
         }
         __device__ __forceinline__ void next() {
+            if (--left <= 0) return;
             for (index += step; index >= per; index -= per) base += rows;
             place();
-            --left;
         }
     };
     const auto walk = [&](const Item &it) {
@@ -996,14 +994,16 @@ int allow_shared(Kernel kernel, int bytes) {
     return status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
 }
 
-// Whether a block (or pair) of `most` meets the same group several times in a row; otherwise slices of the weight stream with the rows,
-// which waits for no tile to end.
-bool weight_stays(long long tiles, int groups, int most) { return groups == 1 || tiles >= 2ll * groups * most; }
+// Whether a block (or pair) of `most` meets the same group and column tile several times in a row; otherwise slices of the weight
+// stream with the rows, which waits for no tile to end.
+bool weight_stays(long long tiles, long long columns, int groups, int most) {
+    return columns <= most / 8 && (groups == 1 || tiles >= 2ll * groups * most);
+}
 
-// Blocks (or pairs) for `tiles`: a multiple of the column tiles where the weight is resident and that leaves few SMs idle.
+// Blocks (or pairs) for `tiles`: a multiple of the column tiles where the weight is resident.
 unsigned row_grid(long long tiles, long long columns, unsigned most, bool resident) {
     if (tiles <= most) return (unsigned)tiles;
-    return resident && columns <= most / 8 ? most - most % (unsigned)columns : most;
+    return resident ? most - most % (unsigned)columns : most;
 }
 
 template <typename T, int kMode, int kAct, int BN, bool kVector>
@@ -1022,7 +1022,7 @@ int launch_rows(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t s
         map_extra = map_a;
     }
     const long long tiles = units * ceil_div(a.cols, BN);
-    a.resident = ceil_div(a.depth, kSliceK) * Shape<BN>::kBytesB <= kResidentBytes && weight_stays(tiles, p.g.groups, kSms);
+    a.resident = ceil_div(a.depth, kSliceK) * Shape<BN>::kBytesB <= kResidentBytes && weight_stays(tiles, ceil_div(a.cols, BN), p.g.groups, kSms);
     if (tiles >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
     return status(launch_early(kernel, row_grid(tiles, ceil_div(a.cols, BN), kSms, a.resident), Shape<BN>::kThreads, kSmem, st, 1, a, map_a,
                                map_w, map_extra));
@@ -1043,7 +1043,7 @@ int launch_pair(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t s
         if (const int rc = make_map(map_extra, p.dtype, p.extra, a.cols, rows, p.extra_pitch, 32, 0)) return rc;
     const long long tiles = units * ceil_div(a.cols, kPairColumns);
     a.resident = pair_ring(kMode == kForward || kMode == kPreGrad) - ceil_div(a.depth, kSliceK) * kPairBytesB >= kPairLeastStages * kBytesA &&
-                 weight_stays(tiles, p.g.groups, kSms / 2);
+                 weight_stays(tiles, ceil_div(a.cols, kPairColumns), p.g.groups, kSms / 2);
     if (tiles >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
     return status(launch_early(kernel, 2 * row_grid(tiles, ceil_div(a.cols, kPairColumns), kSms / 2, a.resident), kPairThreads, kPairSmem, st,
                                2, a, map_a, map_w, map_extra));

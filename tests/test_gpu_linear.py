@@ -235,6 +235,22 @@ def test_tall_groups(act, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("K,N,residual", [(64, 72, False), (64, 136, True), (200, 33, True), (72, 1200, False)])
+def test_groups_of_many_tiles(K, N, residual, dtype):
+    """Few groups with so many tiles each that blocks keep a group's weight: it changes inside a block's tiles, and with the batch
+    element back again; aligned and odd widths, several column tiles."""
+    starts = torch.tensor([300, 20011, 20100, 59000], device=DEV)
+    check(*make((2, 60000), K, N, dtype, 3, seed=7, residual=residual), "silu" if residual else "none", starts)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_wide_outputs(dtype):
+    """More column tiles than a block's weight could stay for."""
+    check(*make((700,), 40, 6000, dtype, seed=8), "none")
+    check(*make((2500,), 136, 5128, dtype, seed=9), "silu")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_weight_gradients_over_many_rows(dtype):
     """Rows enough that pairs of blocks share the weight's gradient: one group, ragged ones, and NaN in the rows behind each group's end."""
     check(*make((40003,), 264, 520, dtype, seed=5), "none")
