@@ -180,7 +180,7 @@ __device__ __forceinline__ void load_some(const T *row, int k, int depth, float 
     }
 }
 
-// kForward and kPreGrad.
+// kForward and kPreGrad, whose results the backward of few rows keeps in fp32.
 template <typename T, int kMode, bool kVector>
 __global__ void __launch_bounds__(kFewThreads) linear_few_rows_kernel(const RowProduct<T> p, const int activation) {
     constexpr int kCount = 16 / sizeof(T);
@@ -236,10 +236,142 @@ __global__ void __launch_bounds__(kFewThreads) linear_few_rows_kernel(const RowP
         if (kMode == kForward) {
             if (u.group >= 0) v = activate_any(activation, v);
             if (p.extra) v += to_f32<T>(p.extra[at]);
+            p.out[at] = from_f32<T>(v);
         } else {
-            v = activate_backward_any(activation, v, to_f32<T>(p.extra[at]));
+            reinterpret_cast<float *>(p.out)[at] = activate_backward_any(activation, v, to_f32<T>(p.extra[at]));
         }
-        p.out[(size_t)(u.row + r) * p.out_pitch + c] = from_f32<T>(v);
+    }
+}
+
+// The backward of few rows (64 in all), without a rounding between its products: g in fp32, or the output's gradient itself.
+template <typename T, typename G>
+struct FewGrad {
+    const G *grad;  // [rows][out]
+    const T *x, *w;
+    T *grad_x, *grad_weight, *grad_bias;
+    int in_features, out_features;
+    Groups g;
+};
+
+// grad_x: 64 inputs of up to eight rows a block, two a lane; its warps share out the outputs and add their sums in order.
+constexpr int kFewWarps = 8, kFewInputs = 64;
+
+template <typename T, typename G>
+__global__ void __launch_bounds__(32 * kFewWarps) linear_few_grad_x_kernel(const FewGrad<T, G> p) {
+    __shared__ RowTable table;
+    __shared__ float partial[kFewWarps][kFewRows][kFewInputs];
+    wait_for_previous_kernel();
+    build_row_table(p.g, kFewRows, true, table);
+    __syncthreads();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const unsigned steps = (unsigned)((p.in_features + kFewInputs - 1) / kFewInputs);
+    const long long items = (long long)table.unit_begin[p.g.groups + 2] * p.g.batch * steps;
+    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+        const RowUnit u = row_unit(p.g, table, kFewRows, (unsigned)(item / steps));
+        const int in0 = (int)(item % steps) * kFewInputs;
+        const bool first = in0 + lane < p.in_features, second = in0 + 32 + lane < p.in_features;
+        float acc[2][kFewRows] = {};
+        if (u.group >= 0) {
+            const T *w = p.w + (size_t)u.group * p.out_features * p.in_features + in0 + lane;
+            const G *grad = p.grad + (size_t)u.row * p.out_features;
+#pragma unroll 4
+            for (int n = warp; n < p.out_features; n += kFewWarps) {
+                const T *line = w + (size_t)n * p.in_features;
+                const float w0 = first ? to_f32<T>(line[0]) : 0.f, w1 = second ? to_f32<T>(line[32]) : 0.f;
+#pragma unroll
+                for (int r = 0; r < kFewRows; ++r)
+                    if (r < u.count) {
+                        const float v = to_f32<G>(grad[(size_t)r * p.out_features + n]);
+                        acc[0][r] = fmaf(v, w0, acc[0][r]);
+                        acc[1][r] = fmaf(v, w1, acc[1][r]);
+                    }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r) {
+            partial[warp][r][lane] = acc[0][r];
+            partial[warp][r][32 + lane] = acc[1][r];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < u.count * kFewInputs; i += 32 * kFewWarps) {
+            const int r = i / kFewInputs, c = i % kFewInputs;
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < kFewWarps; ++k) sum += partial[k][r][c];
+            if (in0 + c < p.in_features) p.grad_x[(size_t)(u.row + r) * p.in_features + in0 + c] = from_f32<T>(sum);
+        }
+        __syncthreads();
+    }
+}
+
+// grad_weight and grad_bias: a warp an output and 256 inputs of it, eight a lane; the group's rows one after the other.
+template <typename T, typename G>
+__global__ void __launch_bounds__(kThreads) linear_few_weight_grad_kernel(const FewGrad<T, G> p) {
+    constexpr int kEach = 8, kLine = 32 * kEach;
+    __shared__ int start[kMaxGroups + 2];
+    wait_for_previous_kernel();
+    if (threadIdx.x < 32) scan_starts(p.g, start);
+    __syncthreads();
+    const int lane = threadIdx.x % 32, lines = (p.in_features + kLine - 1) / kLine;
+    const long long items = (long long)p.g.groups * p.out_features * lines;
+    const long long warps = (long long)gridDim.x * (kThreads / 32);
+    for (long long item = (long long)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; item < items; item += warps) {
+        const int line = (int)(item % lines);
+        const long long output = item / lines;  // counted over the groups
+        const int e = (int)(output / p.out_features), n = (int)(output - (long long)e * p.out_features);
+        float acc[kEach] = {}, bias = 0.f;
+        for (int b = 0; b < p.g.batch; ++b)
+            for (int m = start[e]; m < start[e + 1]; ++m) {
+                const size_t row = (size_t)b * p.g.rows + m;
+                const float v = to_f32<G>(p.grad[row * p.out_features + n]);
+                const T *x = p.x + row * p.in_features + line * kLine + lane;
+                bias += v;
+#pragma unroll
+                for (int j = 0; j < kEach; ++j)
+                    if (line * kLine + 32 * j + lane < p.in_features) acc[j] = fmaf(v, to_f32<T>(x[32 * j]), acc[j]);
+            }
+        if (p.grad_weight)
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                const int k = line * kLine + 32 * j + lane;
+                if (k < p.in_features) p.grad_weight[(size_t)output * p.in_features + k] = from_f32<T>(acc[j]);
+            }
+        if (p.grad_bias && line == 0 && lane == 0) p.grad_bias[output] = from_f32<T>(bias);
+    }
+}
+
+// The bias's gradient from the sums over 32 rows that the pre-activation's gradient left behind (MmaRows::sums): a block takes 32 outputs
+// of a group, its warps every 16th of the sums, and adds the warps' in order.
+constexpr int kBiasWarps = 16;
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kBiasWarps) linear_bias_sum_kernel(const Groups g, const float *__restrict__ sums, int unit, int cols,
+                                                                          T *__restrict__ grad_bias) {
+    __shared__ RowTable table;
+    __shared__ float partial[kBiasWarps][32];
+    wait_for_previous_kernel();
+    build_row_table(g, unit, false, table);
+    __syncthreads();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, steps = (cols + 31) / 32, subs = unit / kSumRows;
+    for (int item = blockIdx.x; item < g.groups * steps; item += gridDim.x) {
+        const int e = item / steps, c = item % steps * 32 + lane;
+        const int each = (table.start[e + 1] - table.start[e] + kSumRows - 1) / kSumRows;  // sums of one batch element
+        float sum = 0.f;
+        if (c < cols)
+            for (int b = 0; b < g.batch; ++b) {
+                const size_t first = ((size_t)b * table.unit_begin[g.groups + 2] + table.unit_begin[e + 1]) * subs;
+#pragma unroll 8
+                for (int k = warp; k < each; k += kBiasWarps) sum += sums[(first + k) * cols + c];
+            }
+        partial[warp][lane] = sum;
+        __syncthreads();
+        if (warp == 0 && c < cols) {
+            float total = 0.f;
+#pragma unroll
+            for (int w = 0; w < kBiasWarps; ++w) total += partial[w][lane];
+            grad_bias[(size_t)e * cols + c] = from_f32<T>(total);
+        }
+        __syncthreads();
     }
 }
 
@@ -481,7 +613,7 @@ int pad(const Padding &p, cudaStream_t st) {
 
 // What the workspaces hold, one behind the other.
 struct Layout {
-    size_t x = 0, w = 0, g = 0, slots = 0, bias_slots = 0, total = 0;
+    size_t x = 0, w = 0, g = 0, slots = 0, bias_slots = 0, sums = 0, total = 0;
     size_t take(size_t bytes) {
         const size_t at = total;
         total += round256(bytes);
@@ -540,13 +672,20 @@ Layout forward_layout(const Shape &s) {
     return l;
 }
 
+bool few_rows_backward(const Shape &s) { return total_rows(s) <= 64; }
+
 // g: the pre-activation's gradient, or a padded copy of grad_output.
 Layout backward_layout(const Shape &s, int activation) {
     Layout l;
+    if (few_rows_backward(s)) {
+        if (activation != FDA_ACT_NONE) l.g = l.take(total_rows(s) * s.out_features * sizeof(float));
+        return l;
+    }
     add_padded_operands(l, s);
     const bool narrow = s.dtype != FDA_DTYPE_F32;
     if (activation != FDA_ACT_NONE || (narrow && s.out_features % 8))
         l.g = l.take(total_rows(s) * (narrow ? padded(s.out_features) : s.out_features) * type_size(s.dtype));
+    if (activation != FDA_ACT_NONE && narrow) l.sums = l.take(most_sum_rows(s.batch, s.rows, s.groups) * s.out_features * sizeof(float));
     const Cut c = weight_cut(s);
     l.slots = l.take((size_t)c.slots * s.out_features * s.in_features * sizeof(float));
     l.bias_slots = l.take((size_t)c.slots * s.out_features * sizeof(float));
@@ -604,7 +743,7 @@ int forward(const Shape &s, const Groups &g, const void *x, const void *weight, 
     align_rows(pads, weight, ws + l.w, (size_t)s.groups * s.out_features, s.in_features);
     if (const int rc = pad(pads, st)) return rc;
     const long long in = padded(s.in_features);
-    const MmaRows p{x, weight, bias, residual, y, in, in, s.out_features, s.out_features, s.in_features, s.out_features, s.dtype, activation, g};
+    const MmaRows p{x, weight, bias, residual, y, nullptr, in, in, s.out_features, s.out_features, s.in_features, s.out_features, s.dtype, activation, g};
     return mma_rows(kForward, p, st);
 }
 
@@ -640,16 +779,56 @@ WeightGrad<T> weight_grad_args(const Shape &s, const Groups &g, const Cut &c, co
     return q;
 }
 
+int sum_bias(const Shape &s, const Groups &g, const float *sums, int unit, void *grad_bias, cudaStream_t st) {
+    const unsigned blocks = (unsigned)std::min<long long>(ceil_div(s.out_features, 32) * s.groups, 4 * kSms);
+    if (s.dtype == FDA_DTYPE_F16)
+        return launched(launch_early(linear_bias_sum_kernel<__half>, blocks, 32 * kBiasWarps, 0, st, 1, g, sums, unit, s.out_features,
+                                     static_cast<__half *>(grad_bias)));
+    return launched(launch_early(linear_bias_sum_kernel<__nv_bfloat16>, blocks, 32 * kBiasWarps, 0, st, 1, g, sums, unit, s.out_features,
+                                 static_cast<__nv_bfloat16 *>(grad_bias)));
+}
+
+template <typename T, typename G>
+int few_gradients(const Shape &s, const Groups &g, const void *grad, const void *x, const void *weight, const Gradients &out, cudaStream_t st) {
+    FewGrad<T, G> p;
+    p.grad = static_cast<const G *>(grad);
+    p.x = static_cast<const T *>(x);
+    p.w = static_cast<const T *>(weight);
+    p.grad_x = static_cast<T *>(out.x);
+    p.grad_weight = static_cast<T *>(out.weight);
+    p.grad_bias = static_cast<T *>(out.bias);
+    p.in_features = s.in_features;
+    p.out_features = s.out_features;
+    p.g = g;
+    if (out.x) {
+        const long long items = most_units(s.batch, s.rows, s.groups, kFewRows, true) * ceil_div(s.in_features, kFewInputs);
+        const int rc = launched(launch_early(linear_few_grad_x_kernel<T, G>, (unsigned)std::min<long long>(items, 8 * kSms), 32 * kFewWarps, 0, st, 1, p));
+        if (rc) return rc;
+    }
+    if (!out.weight && !out.bias) return FDA_OK;
+    const long long items = (long long)s.groups * s.out_features * ceil_div(s.in_features, 256);
+    return launched(launch_early(linear_few_weight_grad_kernel<T, G>, (unsigned)std::min<long long>(ceil_div(items, kThreads / 32), 16 * kSms),
+                                 kThreads, 0, st, 1, p));
+}
+
+template <typename T>
+int backward_few(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *grad_output,
+                 const Gradients &out, char *ws, int activation, cudaStream_t st) {
+    if (activation == FDA_ACT_NONE) return few_gradients<T, T>(s, g, grad_output, x, weight, out, st);
+    const Layout l = backward_layout(s, activation);
+    if (const int rc = run_few_rows<T, kPreGrad>(row_product<T>(s, g, x, weight, bias, grad_output, ws + l.g, s.out_features), activation, st))
+        return rc;
+    return few_gradients<T, float>(s, g, ws + l.g, x, weight, out, st);
+}
+
 int backward_f32(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *grad_output,
                  const Gradients &out, char *ws, int activation, cudaStream_t st) {
     const Layout l = backward_layout(s, activation);
     const void *grad = grad_output;
     if (activation != FDA_ACT_NONE) {
         grad = ws + l.g;
-        const int rc = few_rows(s) ? run_few_rows<kPreGrad>(s, g, x, weight, bias, grad_output, ws + l.g, s.out_features, activation, st)
-                                   : run_rows<kPreGrad>(row_product<float>(s, g, x, weight, bias, grad_output, ws + l.g, s.out_features),
-                                                               activation, st);
-        if (rc) return rc;
+        const RowProduct<float> p = row_product<float>(s, g, x, weight, bias, grad_output, ws + l.g, s.out_features);
+        if (const int rc = run_rows<kPreGrad>(p, activation, st)) return rc;
     }
     if (out.x) {
         RowProduct<float> p = row_product<float>(s, g, grad, weight, nullptr, nullptr, out.x, s.in_features);
@@ -667,25 +846,29 @@ int backward_f32(const Shape &s, const Groups &g, const void *x, const void *wei
 }
 
 int backward_narrow(const Shape &s, const Groups &g, const void *x, const void *weight, const void *bias, const void *grad_output,
-                    const Gradients &out, char *ws, int activation, cudaStream_t st) {
+                    Gradients out, char *ws, int activation, cudaStream_t st) {
     const Layout l = backward_layout(s, activation);
-    const bool weights = out.weight || out.bias, few = few_rows(s);
+    bool weights = out.weight || out.bias;
     const long long in = padded(s.in_features), outs = padded(s.out_features);
-    const void *dense_x = x, *dense_weight = weight, *grad = activation != FDA_ACT_NONE ? ws + l.g : grad_output;
+    const void *grad = activation != FDA_ACT_NONE ? ws + l.g : grad_output;
     Padding pads{};
-    if ((activation != FDA_ACT_NONE && !few) || weights) align_rows(pads, x, ws + l.x, total_rows(s), s.in_features);
-    if ((activation != FDA_ACT_NONE && !few) || out.x) align_rows(pads, weight, ws + l.w, (size_t)s.groups * s.out_features, s.in_features);
+    if (activation != FDA_ACT_NONE || weights) align_rows(pads, x, ws + l.x, total_rows(s), s.in_features);
+    if (activation != FDA_ACT_NONE || out.x) align_rows(pads, weight, ws + l.w, (size_t)s.groups * s.out_features, s.in_features);
     if (activation == FDA_ACT_NONE) align_rows(pads, grad, ws + l.g, total_rows(s), s.out_features);
     if (const int rc = pad(pads, st)) return rc;
     if (activation != FDA_ACT_NONE) {
-        const MmaRows p{x, weight, bias, grad_output, ws + l.g, in, in, s.out_features, outs, s.in_features, s.out_features, s.dtype,
+        float *const sums = out.bias ? reinterpret_cast<float *>(ws + l.sums) : nullptr;
+        const MmaRows p{x, weight, bias, grad_output, ws + l.g, sums, in, in, s.out_features, outs, s.in_features, s.out_features, s.dtype,
                         activation, g};
-        const int rc = few ? run_few_rows<kPreGrad>(s, g, dense_x, dense_weight, bias, grad_output, ws + l.g, (int)outs, activation, st)
-                           : mma_rows(kPreGrad, p, st);
-        if (rc) return rc;
+        if (const int rc = mma_rows(kPreGrad, p, st)) return rc;
+        if (out.bias) {
+            if (const int rc = sum_bias(s, g, sums, mma_pre_grad_unit(p), out.bias, st)) return rc;
+            out.bias = nullptr;
+            weights = out.weight;
+        }
     }
     if (out.x) {
-        const MmaRows p{grad, weight, nullptr, nullptr, out.x, outs, in, 0, s.in_features, s.in_features, s.out_features, s.dtype,
+        const MmaRows p{grad, weight, nullptr, nullptr, out.x, nullptr, outs, in, 0, s.in_features, s.in_features, s.out_features, s.dtype,
                         FDA_ACT_NONE, g};
         if (const int rc = mma_rows(kGradX, p, st)) return rc;
     }
@@ -755,8 +938,13 @@ int fda_linear_backward(const void *x, const void *weight, const void *bias, con
     const Groups g{group_start_index, num_starts, groups, batch, rows};
     const Gradients out{grad_x, grad_weight, grad_bias};
     char *ws = static_cast<char *>(workspace);
+    if (dtype != FDA_DTYPE_F32 && (misaligned16(x) || misaligned16(weight) || misaligned16(grad_output))) return FDA_ERR_MISALIGNED;
+    if (few_rows_backward(s)) {
+        if (dtype == FDA_DTYPE_F32) return backward_few<float>(s, g, x, weight, bias, grad_output, out, ws, activation, st);
+        if (dtype == FDA_DTYPE_F16) return backward_few<__half>(s, g, x, weight, bias, grad_output, out, ws, activation, st);
+        return backward_few<__nv_bfloat16>(s, g, x, weight, bias, grad_output, out, ws, activation, st);
+    }
     if (dtype == FDA_DTYPE_F32) return backward_f32(s, g, x, weight, bias, grad_output, out, ws, activation, st);
-    if (misaligned16(x) || misaligned16(weight) || misaligned16(grad_output)) return FDA_ERR_MISALIGNED;
     return backward_narrow(s, g, x, weight, bias, grad_output, out, ws, activation, st);
 }
 

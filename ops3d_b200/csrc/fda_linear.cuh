@@ -299,10 +299,20 @@ enum Mode {
 struct MmaRows {
     const void *a, *w, *bias, *extra;
     void *out;
+    float *sums;  // kPreGrad: the results' sums over 32 rows each, before rounding (BlockSums); may be nullptr
     long long a_pitch, w_pitch, extra_pitch, out_pitch;
     int in_features, out_features, dtype, activation;
     Groups g;
 };
+// Row k of `sums` [..][out_features] for the k-th 32 rows of a unit of `unit` rows, unit / 32 of them for every unit of a row table
+// without rest.  The launch says which unit it took.
+constexpr int kSumRows = 32;
+inline size_t most_sum_rows(int batch, int rows, int groups) {
+    const long long a = most_units(batch, rows, groups, 128, false) * (128 / kSumRows);
+    const long long b = most_units(batch, rows, groups, 256, false) * (256 / kSumRows);
+    return (size_t)(a > b ? a : b);
+}
+int mma_pre_grad_unit(const MmaRows &p);
 int mma_rows_f16(int mode, const MmaRows &p, cudaStream_t st);
 int mma_rows_bf16(int mode, const MmaRows &p, cudaStream_t st);
 

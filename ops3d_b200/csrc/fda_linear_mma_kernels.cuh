@@ -110,6 +110,7 @@ struct RowsArgs {
     unsigned extra_pitch, out_pitch;  // 32 of them fit 32 bits (the host has checked)
     int depth, cols;
     bool resident;
+    float *sums;  // MmaRows::sums
     Groups g;
 };
 
@@ -123,10 +124,31 @@ constexpr int kResidentBytes = kRingBytes - kResidentStages * kBytesA;
 
 constexpr int kForwardPlain = 3;  // kForward without a residual
 
+// Sums over the 32 lanes of 16 values each: lane l returns that of value l / 2 (bits reversed: sum_column).
+__device__ __forceinline__ float sums_over_lanes(float (&v)[16]) {
+    const unsigned lane = threadIdx.x % 32;
+#pragma unroll
+    for (int n = 8; n > 0; n /= 2) {  // lanes 2 n apart share out 2 n values
+        const bool upper = lane & (2 * n);
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+            const float keep = upper ? v[j + n] : v[j], give = upper ? v[j] : v[j + n];
+            v[j] = keep + __shfl_xor_sync(0xffffffffu, give, 2 * n);
+        }
+    }
+    return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
+}
+__device__ __forceinline__ int sum_column() {
+    const int lane = threadIdx.x % 32;
+    return (lane & 16) / 2 + (lane & 8) / 2 + (lane & 4) / 2 + (lane & 2) / 2;
+}
+
 // 16 columns of a lane's row: `row` comes as the extra elements and leaves as the results.  `bias` is in shared memory, the same
-// address for the whole warp.
+// address for the whole warp.  kPreGrad with `sums`: the sums of the results over the first `rows` lanes go there, in fp32: the bias's
+// gradient is made of them, and of results rounded to 16 bits it would be off by up to twice the rounding of the sum itself.
 template <typename T, int kMode, int kAct>
-__device__ __forceinline__ void finish_columns(const uint32_t (&v)[16], const float *bias, uint32_t *row) {
+__device__ __forceinline__ void finish_columns(const uint32_t (&v)[16], const float *bias, uint32_t *row, float *sums, int rows, int columns) {
+    float kept[kMode == kPreGrad ? 16 : 1];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         Pair r(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
@@ -135,6 +157,7 @@ __device__ __forceinline__ void finish_columns(const uint32_t (&v)[16], const fl
             r = r + Pair(b.x, b.y);
             if (kMode == kPreGrad) {
                 r = activate_backward_2<kAct>(r, unpack2<T>(row[j]));
+                if (kMode == kPreGrad) r.split(kept[(2 * j) % (sizeof(kept) / 4)], kept[(2 * j + 1) % (sizeof(kept) / 4)]);
             } else {
                 r = activate_2<kAct>(r);
                 if (kMode == kForward) r = r + unpack2<T>(row[j]);
@@ -142,6 +165,15 @@ __device__ __forceinline__ void finish_columns(const uint32_t (&v)[16], const fl
         }
         row[j] = pack2<T>(r);
     }
+    if constexpr (kMode == kPreGrad)
+        if (sums) {
+            const int lane = threadIdx.x % 32;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) kept[j] = lane < rows ? kept[j] : 0.f;  // what lies beyond may be anything
+            const float sum = sums_over_lanes(kept);
+            const int c = sum_column();
+            if (lane % 2 == 0 && c < columns) sums[c] = sum;
+        }
 }
 
 // kVector: the rows of out and of extra start on 16-byte boundaries.
@@ -336,6 +368,8 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
             if (!__all_sync(0xffffffffu, pipe.sums_full[sums.stage].wait(sums.round, failed))) break;
             fence_after_sync();
             const uint32_t address = pipe.tmem + sums.stage * BN + part * kPart + ((uint32_t)(quarter * 32) << 16);
+            float *const sums_row =
+                kMode == kPreGrad && p.sums && rows > 0 ? p.sums + ((size_t)(tile / columns) * (kTileRows / kSumRows) + quarter) * p.cols + col0 : nullptr;
 #pragma unroll 1
             for (int c = 0; c < kChunks; ++c) {
                 const int count = p.cols - col0 - 32 * c;
@@ -353,7 +387,8 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                     __syncwarp();
                     tmem_load(address + 32 * c + 16 * h, v);
                     tmem_load_wait();
-                    finish_columns<T, kMode, kAct>(v, bias + 32 * c + 16 * h, row + 8 * h);
+                    finish_columns<T, kMode, kAct>(v, bias + 32 * c + 16 * h, row + 8 * h, sums_row ? sums_row + 32 * c + 16 * h : nullptr, rows,
+                                                   count - 16 * h);
                 }
                 store_rows<kVector>(out_rows + 32 * c, p.out_pitch, rows, count, stage, row);
             }
@@ -592,6 +627,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 if (kExtra && !__all_sync(0xffffffffu, pipe.extra_full[mine].wait(loads++ & 1, failed))) break;
                 const uint32_t address = pipe.tmem + sums.stage * kPairColumns + part * 64 + ((uint32_t)(quarter * 32) << 16);
                 T *const out = p.out + (size_t)u.first * p.out_pitch + u.col0;
+                float *const sums_row =
+                    kMode == kPreGrad && p.sums
+                        ? p.sums + ((size_t)(tile / columns) * (kPairRows / kSumRows) + rank * (kTileRows / kSumRows) + quarter) * p.cols + u.col0
+                        : nullptr;
 #pragma unroll 1
                 for (int c = 0; c < 2; ++c) {
                     uint32_t row[16] = {};
@@ -609,7 +648,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                             __syncwarp();
                             tmem_load(address + 32 * c + 16 * h, v);
                             tmem_load_wait();
-                            finish_columns<T, kMode, kAct>(v, bias + 32 * c + 16 * h, row + 8 * h);
+                            finish_columns<T, kMode, kAct>(v, bias + 32 * c + 16 * h, row + 8 * h,
+                                                           sums_row ? sums_row + 32 * c + 16 * h : nullptr, u.rows,
+                                                           p.cols - u.col0 - 32 * c - 16 * h);
                         }
                     store_rows<true>(out + 32 * c, p.out_pitch, u.rows, p.cols - u.col0 - 32 * c, stage, row);
                 }
@@ -1049,6 +1090,16 @@ int launch_pair(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t s
                                2, a, map_a, map_w, map_extra));
 }
 
+// Tiles enough for every pair of blocks, and groups not so short that much of the pairs' units would be empty.
+bool pairs_fit(const Groups &g, int cols, long long pair_units) {
+    return cols > 128 && pair_units * ceil_div(cols, kPairColumns) >= kSms / 2 && (!g.starts || g.rows / g.groups >= 2 * kPairRows);
+}
+
+int pre_grad_unit(const MmaRows &p) {
+    const bool vectors = whole_vectors(p.out, p.out_pitch) && whole_vectors(p.extra, p.extra_pitch);
+    return vectors && pairs_fit(p.g, p.out_features, most_units(p.g.batch, p.g.rows, p.g.groups, kPairRows, false)) ? kPairRows : kTileRows;
+}
+
 template <typename T, int kMode, int kAct>
 int rows_of(const MmaRows &p, cudaStream_t st) {
     RowsArgs<T> a;
@@ -1060,6 +1111,7 @@ int rows_of(const MmaRows &p, cudaStream_t st) {
     if (p.extra_pitch >= (1 << 26) || p.out_pitch >= (1 << 26)) return FDA_ERR_BAD_SHAPE;
     a.depth = kMode == kGradX ? p.out_features : p.in_features;
     a.cols = kMode == kGradX ? p.in_features : p.out_features;
+    a.sums = p.sums;
     a.g = p.g;
     // the widest tile that still gives every SM one
     const long long units = most_units(p.g.batch, p.g.rows, p.g.groups, kTileRows, kMode != kPreGrad && p.g.starts);
@@ -1069,12 +1121,11 @@ int rows_of(const MmaRows &p, cudaStream_t st) {
     }
     // Pairs where they pay: extra rows (73728 x 256 x 1024 with a residual 74 us against 94 by single blocks) or a contraction too long
     // for a resident weight (149504 x 1024 x 256: 78 against 86); else single blocks, whose epilogues wait for no other (598016 x
-    // 256 x 256: 105 against 117).  Groups shorter than two of the pairs' units would leave too much of these empty.
-    const bool ragged = p.g.starts != nullptr, extra = kMode == kForward || kMode == kPreGrad;
+    // 256 x 256: 105 against 117).
+    const bool extra = kMode == kForward || kMode == kPreGrad;
     const bool pays = extra || ceil_div(a.depth, kSliceK) * Shape<256>::kBytesB > kResidentBytes;
-    const long long pair_units = most_units(p.g.batch, p.g.rows, p.g.groups, kPairRows, kMode != kPreGrad && ragged);
-    if (pays && a.cols > 128 && pair_units * ceil_div(a.cols, kPairColumns) >= kSms / 2 && (!ragged || p.g.rows / p.g.groups >= 2 * kPairRows))
-        return launch_pair<T, kMode, kAct>(a, p, pair_units, st);
+    const long long pair_units = most_units(p.g.batch, p.g.rows, p.g.groups, kPairRows, kMode != kPreGrad && p.g.starts);
+    if (pays && pairs_fit(p.g, a.cols, pair_units)) return launch_pair<T, kMode, kAct>(a, p, pair_units, st);
     if (a.cols > 128 && units * ceil_div(a.cols, 256) >= kSms) return launch_rows<T, kMode, kAct, 256, true>(a, p, units, st);
     if (a.cols > 64 && units * ceil_div(a.cols, 128) >= kSms) return launch_rows<T, kMode, kAct, 128, true>(a, p, units, st);
     return launch_rows<T, kMode, kAct, 64, true>(a, p, units, st);

@@ -216,6 +216,47 @@ def test_many_groups_and_long_groups(dtype):
     check(*make((2, 20000), 64, 32, dtype, 3), "none", torch.tensor([0, 15000, 19990], device=DEV))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["none", "gelu", "silu"])
+def test_few_rows_in_groups(act, dtype):
+    """A handful of tokens over many groups, most of them empty, and 64 rows in one: no rounding between the backward's products."""
+    starts = torch.tensor([0, 0, 2, 2, 2, 3, 3, 12, 12, 13], device=DEV)
+    for shape, (K, N) in (((17,), (40, 72)), ((3, 20), (33, 50)), ((2, 17), (256, 520))):
+        x, w, b, r, dy = make(shape, K, N, dtype, 9 if len(shape) == 1 else 10, seed=K)
+        check(x, w, b, r, dy, act, starts)
+        want = reference(x, w, b, r, dy, act, group_of_rows(starts.tolist(), w.shape[0], shape[-1]).repeat(shape[0] if len(shape) > 1 else 1).to(DEV))
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        grads = torch.autograd.grad(grouped_linear(leaves[0], leaves[1], starts, leaves[2], r, act), leaves, dy)
+        for name, g in zip(("x", "weight", "bias"), grads):
+            value = want[name][0].reshape(g.shape)
+            # one rounding, and the fp32 arithmetic: sums of up to 520 products, values of the activations
+            assert ((g.double() - value).abs() <= rounding(value, dtype) * 1.01 + 2e-5 * value.abs().max()).all(), name
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M,K,N", [(65, 40, 72), (500, 33, 50), (3000, 64, 24), (19003, 136, 264), (40000, 64, 136)])
+def test_bias_gradient_is_rounded_once(M, K, N, dtype):
+    """The sums over rows come from the unrounded gradient of the pre-activation: one rounding, and fp32's share of a sum of M terms
+    (in pieces, so far below M steps; 32 + 64 of them bound it here)."""
+    x, w, b, _, dy = make((M,), K, N, dtype, residual=False, seed=M)
+    leaf = b.clone().requires_grad_(True)
+    (g,) = torch.autograd.grad(fused_linear(x, w, leaf, activation="silu"), leaf, dy)
+    pre = x.double() @ w.double().t() + b.double()
+    terms = dy.double() * act64(pre, "silu")[1]
+    value = terms.sum(0)
+    slack = terms.abs().sum(0) * 2.0 ** -23 * 96 + dy.double().abs().sum(0) * 2.0 ** -20 * 4
+    assert ((g.double() - value).abs() <= rounding(value, dtype) * 1.01 + slack).all()
+    starts = torch.tensor([0, M // 3, M // 3 + 40, M - 7], device=DEV)
+    lin = [t.unsqueeze(0).repeat(3, *(1,) * t.dim()).contiguous() for t in (w, b)]
+    leaf = lin[1].requires_grad_(True)
+    (g,) = torch.autograd.grad(grouped_linear(x, lin[0], starts, leaf, activation="silu"), leaf, dy)
+    for e in range(3):
+        rows = slice(int(starts[e]), int(starts[e + 1]))
+        value = terms[rows].sum(0)
+        slack = terms[rows].abs().sum(0) * 2.0 ** -23 * 96 + dy[rows].double().abs().sum(0) * 2.0 ** -20 * 4
+        assert ((g[e].double() - value).abs() <= rounding(value, dtype) * 1.01 + slack).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("act", ACTS)
 def test_enough_tiles_for_every_sm(act, dtype):
