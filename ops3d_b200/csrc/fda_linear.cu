@@ -341,8 +341,8 @@ __global__ void __launch_bounds__(kThreads) linear_few_weight_grad_kernel(const 
 }
 
 // The bias's gradient from the sums over 32 rows that the pre-activation's gradient left behind (MmaRows::sums): a block takes 32 outputs
-// of a group, its warps every 16th of the sums, and adds the warps' in order.
-constexpr int kBiasWarps = 16;
+// of a group, its warps every 32nd of the sums, and adds the warps' in order.
+constexpr int kBiasWarps = 32;
 
 template <typename T>
 __global__ void __launch_bounds__(32 * kBiasWarps) linear_bias_sum_kernel(const Groups g, const float *__restrict__ sums, int unit, int cols,
@@ -674,6 +674,14 @@ Layout forward_layout(const Shape &s) {
 
 bool few_rows_backward(const Shape &s) { return total_rows(s) <= 64; }
 
+// A 16-bit bias's gradient from g as it is (MmaRows::sums) or, by the weight gradient's product with ones, from g rounded.  The second
+// has the rounding's error twice, 1.4 times one rounding in the mean over many outputs and up to twice over few; the first costs
+// the pre-activation's gradient 15 % (73728 x 256 x 1024: 119 instead of 103 us, and 5 to add the sums), too much where the outputs
+// are many.
+bool bias_from_sums(const Shape &s, int activation) {
+    return s.dtype != FDA_DTYPE_F32 && activation != FDA_ACT_NONE && (long long)s.groups * s.out_features < 1024;
+}
+
 // g: the pre-activation's gradient, or a padded copy of grad_output.
 Layout backward_layout(const Shape &s, int activation) {
     Layout l;
@@ -685,7 +693,7 @@ Layout backward_layout(const Shape &s, int activation) {
     const bool narrow = s.dtype != FDA_DTYPE_F32;
     if (activation != FDA_ACT_NONE || (narrow && s.out_features % 8))
         l.g = l.take(total_rows(s) * (narrow ? padded(s.out_features) : s.out_features) * type_size(s.dtype));
-    if (activation != FDA_ACT_NONE && narrow) l.sums = l.take(most_sum_rows(s.batch, s.rows, s.groups) * s.out_features * sizeof(float));
+    if (bias_from_sums(s, activation)) l.sums = l.take(most_sum_rows(s.batch, s.rows, s.groups) * s.out_features * sizeof(float));
     const Cut c = weight_cut(s);
     l.slots = l.take((size_t)c.slots * s.out_features * s.in_features * sizeof(float));
     l.bias_slots = l.take((size_t)c.slots * s.out_features * sizeof(float));
@@ -857,11 +865,11 @@ int backward_narrow(const Shape &s, const Groups &g, const void *x, const void *
     if (activation == FDA_ACT_NONE) align_rows(pads, grad, ws + l.g, total_rows(s), s.out_features);
     if (const int rc = pad(pads, st)) return rc;
     if (activation != FDA_ACT_NONE) {
-        float *const sums = out.bias ? reinterpret_cast<float *>(ws + l.sums) : nullptr;
+        float *const sums = out.bias && bias_from_sums(s, activation) ? reinterpret_cast<float *>(ws + l.sums) : nullptr;
         const MmaRows p{x, weight, bias, grad_output, ws + l.g, sums, in, in, s.out_features, outs, s.in_features, s.out_features, s.dtype,
                         activation, g};
         if (const int rc = mma_rows(kPreGrad, p, st)) return rc;
-        if (out.bias) {
+        if (sums) {
             if (const int rc = sum_bias(s, g, sums, mma_pre_grad_unit(p), out.bias, st)) return rc;
             out.bias = nullptr;
             weights = out.weight;
