@@ -437,7 +437,7 @@ int fda_nms3d_scored(const float *boxes, long long box_stride, long long coord_s
  *
  *   x [batch][rows][in_features]   weight [groups][out_features][in_features]   bias [groups][out_features] or NULL
  *   residual, y, grad_output [batch][rows][out_features]   residual or NULL; its gradient is grad_output
- * all of `dtype`; sums in fp32, one rounding at the end.  Any sizes of at least one feature; rows * batch < 2^31.
+ * all of `dtype`; sums in fp32, one rounding at the end.  Any sizes of 1 .. 2^26 - 1 features; rows * batch < 2^31.
  * 16-bit x, weight and grad_output start on 16-byte boundaries (FDA_ERR_MISALIGNED), the rest anywhere.
  *
  * group_start_index NULL: one group of all rows (groups = 1).  Else int64 on the device, num_starts = groups or groups + 1
@@ -447,8 +447,8 @@ int fda_nms3d_scored(const float *boxes, long long box_stride, long long coord_s
  * groups <= FDA_LINEAR_MAX_GROUPS.
  *
  * The backward computes pre again from x instead of reading it: that is in_features instead of 2 * out_features elements of
- * traffic a row.  For 16-bit types g is rounded to `dtype` between the products.  grad_x, grad_weight and grad_bias may each be
- * NULL.  Sums run in a fixed order: repeated calls give the same bits.
+ * traffic a row.  For 16-bit types and more than 64 rows g is rounded to `dtype` between the products (its sums for fewer than 1024
+ * biases are not).  grad_x, grad_weight and grad_bias may each be NULL.  Sums run in a fixed order: repeated calls give the same bits.
  *
  * The workspaces (256-byte aligned; sizes from the functions, 0 = none) hold intermediate results of the call only; two calls
  * that may overlap need two.  A wait inside a kernel that ran out (2 s: never in a sound run) leaves the outputs undefined and

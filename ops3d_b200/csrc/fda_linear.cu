@@ -528,6 +528,7 @@ int check_shape(const Shape &s) {
     if (s.dtype < 0 || s.dtype > 2) return FDA_ERR_BAD_DTYPE;
     if (s.batch < 0 || s.rows < 0 || s.groups < 1 || s.in_features < 1 || s.out_features < 1) return FDA_ERR_BAD_SHAPE;
     if ((long long)s.batch * s.rows >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
+    if (s.in_features >= (1 << 26) || s.out_features >= (1 << 26)) return FDA_ERR_BAD_SHAPE;
     if (s.groups > FDA_LINEAR_MAX_GROUPS) return FDA_ERR_TOO_LARGE_STATIC;
     return FDA_OK;
 }
@@ -911,7 +912,7 @@ int fda_linear_forward(const void *x, const void *weight, const void *bias, cons
     if (!x || !weight || !y) return FDA_ERR_NULL_POINTER;
     const size_t need = forward_layout(s).total;
     if (need > 0 && (!workspace || workspace_bytes < need)) return FDA_ERR_WORKSPACE;
-    if ((uintptr_t)workspace % 256) return FDA_ERR_MISALIGNED;
+    if (need > 0 && (uintptr_t)workspace % 256) return FDA_ERR_MISALIGNED;
     const Groups g{group_start_index, num_starts, groups, batch, rows};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype != FDA_DTYPE_F32 && (misaligned16(x) || misaligned16(weight))) return FDA_ERR_MISALIGNED;
@@ -942,7 +943,7 @@ int fda_linear_backward(const void *x, const void *weight, const void *bias, con
     if (!x || !weight || !grad_output) return FDA_ERR_NULL_POINTER;
     const size_t need = backward_layout(s, activation).total;
     if (need > 0 && (!workspace || workspace_bytes < need)) return FDA_ERR_WORKSPACE;
-    if ((uintptr_t)workspace % 256) return FDA_ERR_MISALIGNED;
+    if (need > 0 && (uintptr_t)workspace % 256) return FDA_ERR_MISALIGNED;
     const Groups g{group_start_index, num_starts, groups, batch, rows};
     const Gradients out{grad_x, grad_weight, grad_bias};
     char *ws = static_cast<char *>(workspace);

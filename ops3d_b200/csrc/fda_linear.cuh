@@ -48,7 +48,10 @@ __device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)
 template <int kAct>
 __device__ __forceinline__ float activate(float v) {
     if (kAct == FDA_ACT_RELU) return v < 0.f ? 0.f : v;
-    if (kAct == FDA_ACT_GELU) return 0.5f * v * (1.f + erff(v * kSqrtHalf));
+    if (kAct == FDA_ACT_GELU) {
+        const float c = 1.f + erff(v * kSqrtHalf);
+        return c == 0.f ? 0.f : 0.5f * v * c;  // 0 at minus infinity too, as in the paired form
+    }
     if (kAct == FDA_ACT_GELU_TANH) return 0.5f * v * (1.f + tanhf(kTanhScale * (v + kTanhCubic * v * v * v)));
     if (kAct == FDA_ACT_SILU) return v * sigmoid(v);
     return v;

@@ -1108,7 +1108,6 @@ int rows_of(const MmaRows &p, cudaStream_t st) {
     a.out = static_cast<T *>(p.out);
     a.extra_pitch = (unsigned)p.extra_pitch;
     a.out_pitch = (unsigned)p.out_pitch;
-    if (p.extra_pitch >= (1 << 26) || p.out_pitch >= (1 << 26)) return FDA_ERR_BAD_SHAPE;
     a.depth = kMode == kGradX ? p.out_features : p.in_features;
     a.cols = kMode == kGradX ? p.in_features : p.out_features;
     a.sums = p.sums;

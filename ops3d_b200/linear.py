@@ -16,8 +16,9 @@ outside ``0 .. rows`` as the nearer end; an empty group is fine.  Rows of no gro
 Activations: ``"none"``, ``"relu"``, ``"gelu"`` (``v Phi(v)``), ``"gelu_tanh"``, ``"silu"``.  All tensors are CUDA tensors of one dtype --
 float32, float16 or bfloat16 -- of any sizes and strides (an operand that is not contiguous is copied).  Sums are kept in
 fp32 and rounded once.  Nothing but the inputs is kept for the backward, which computes ``x @ weight^T + bias`` again where
-the activation's derivative needs it; between its products ``grad_output * act'`` is rounded to the inputs' dtype.  The results of
-repeated calls are equal bit for bit.  Up to 1024 groups and 2^31 - 1 rows.
+the activation's derivative needs it; beyond 64 rows ``grad_output * act'`` is rounded to the inputs' dtype between the backward's
+products.  The results of repeated calls are equal bit for bit.  Up to 1024 groups, 2^31 - 1 rows and 2^26 - 1 features.
+``gelu`` is 0 at minus infinity.
 
 ``FeedForward`` is a transformer layer's ``x + W2 act(W1 x + b1) + b2``, with a weight pair of its own per group of rows where
 ``n_groups`` is given (one per pyramid level, or one per expert).

@@ -187,6 +187,45 @@ def test_far_values(act):
     assert ((gx.double() - slope).abs() <= 4e-6).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_far_values_in_16_bits(act, dtype):
+    """The same through the tensor-core kernels' paired functions, on every lane of a tile."""
+    v = torch.cat([torch.linspace(-40, 40, 257), torch.tensor([0.0, -0.0, 1e-4, -1e-4, 90, -90, 200, -200, 6e4, -6e4])]).to(DEV)
+    x = torch.zeros(v.numel(), 8, device=DEV)
+    x[:, 3] = v
+    x = x.to(dtype)
+    w = torch.zeros(40, 8, device=DEV, dtype=dtype)
+    w[:, 3] = 1
+    dy = torch.ones(v.numel(), 40, device=DEV, dtype=dtype)
+    leaf = x.clone().requires_grad_(True)
+    y = fused_linear(leaf, w, activation=act)
+    want = reference(x, w[None], None, None, dy, act)
+    compare(y, want["y"], "y")
+    (gx,) = torch.autograd.grad(y, leaf, dy)
+    compare(gx, want["x"], "grad_x")
+    assert torch.equal(y, y[:, :1].expand_as(y))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_infinities_do_not_depend_on_the_number_of_rows(act, dtype):
+    """Plus and minus infinity and NaN as pre-activations: the same class of result for one row, few and many."""
+    inf = float("inf")
+    one = torch.ones(16, 1, device=DEV, dtype=dtype)
+    results = []
+    for rows in (3, 30, 300, 30000):
+        x = torch.tensor([inf, -inf, float("nan")], device=DEV, dtype=dtype).repeat(rows // 3 + 1)[:rows, None].contiguous()
+        y = fused_linear(x, one, activation=act)
+        assert all(torch.equal(y[i::3].isnan(), y[i:i + 1].isnan().expand_as(y[i::3])) for i in range(3))
+        results.append([float(y[i, 0]) for i in range(3)])
+    for r in results:
+        assert r[0] == inf and r[2] != r[2]
+        assert (r[1] == results[0][1]) or (r[1] != r[1] and results[0][1] != results[0][1])
+    if act in ("none", "relu", "gelu"):
+        assert results[0][1] == {"none": -inf, "relu": 0.0, "gelu": 0.0}[act]
+
+
 GROUPS = {
     "one": ([0], 1), "levels": ([0, 300, 375], 3), "ends": ([0, 100, 228, 400], 3), "empty": ([0, 0, 130, 130, 130, 390, 400], 7),
     "late": ([37, 166, 166], 3), "late-ends": ([5, 69, 133, 390], 3), "all-empty": ([9, 9, 9, 9], 3),

@@ -28,6 +28,7 @@ def test_arguments_are_checked_on_the_host(call):
     assert call(lib, dtype=3) == 2 and call(lib, dtype=-1) == 2
     assert call(lib, k=0) == 6 and call(lib, n=0) == 6 and call(lib, groups=0) == 6 and call(lib, rows=-1) == 6 and call(lib, batch=-1) == 6
     assert call(lib, batch=1 << 16, rows=1 << 15) == 6            # rows are counted in 31 bits
+    assert call(lib, k=1 << 26) == 6 and call(lib, n=1 << 26) == 6
     assert call(lib, act=5) == 12 and call(lib, act=-1) == 12
     assert lib.fda_status_string(12) == b"unknown activation"
     assert call(lib, groups=1025, starts=P, num_starts=1025) == 11
@@ -39,6 +40,20 @@ def test_arguments_are_checked_on_the_host(call):
 def test_no_rows_no_launch():
     lib = capi.load()
     assert _forward(lib, rows=0) == 0 and _forward(lib, batch=0) == 0
+
+
+def test_workspaces_hold_what_the_sizes_need():
+    """Odd widths need padded copies, an activation the pre-activation's gradient, few rows only that in fp32, none at all where
+    nothing is kept."""
+    lib = capi.load()
+    fwd, bwd = lib.fda_linear_forward_workspace_bytes, lib.fda_linear_backward_workspace_bytes
+    assert fwd(1, 1000, 1, 64, 64, 2) == 0 and fwd(1, 1000, 1, 63, 64, 0) == 0 and fwd(1, 8, 1, 63, 64, 2) == 0
+    assert fwd(1, 1000, 1, 63, 64, 2) >= 1000 * 64 * 2 + 64 * 64 * 2
+    assert bwd(1, 64, 1, 63, 50, 0, 2) == 0 and 64 * 50 * 4 <= bwd(1, 64, 1, 63, 50, 2, 2) < 64 * 50 * 4 + 256
+    assert bwd(1, 65, 1, 64, 64, 0, 2) == 0                       # one piece: no partial sums
+    assert bwd(1, 65, 1, 64, 50, 0, 2) >= 65 * 56 * 2             # a padded copy of grad_output
+    big = bwd(2, 300000, 3, 256, 256, 0, 2)
+    assert big % (256 * 256 * 4 + 256 * 4) < 512 and big > 30 * 256 * 256 * 4   # slots of partial sums
 
 
 def test_backward_workspace_is_checked():
