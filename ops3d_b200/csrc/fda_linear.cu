@@ -465,11 +465,20 @@ __global__ void __launch_bounds__(32 * kSumWarps) linear_weight_grad_sum_kernel(
             src[j] = weight ? p.slots + first * size + i : p.bias_slots + (size_t)first * p.out_features + (i - size);
             if (i >= both || !(weight ? p.grad_weight : p.grad_bias)) src[j] = nullptr;
         }
-#pragma unroll 4
-        for (int s = kSplit ? warp : 0; s < count; s += kSplit ? kSumWarps : 1)
+        // eight slots on their way at a time, the last round's missing ones left out (not in a loop of single slots)
+        constexpr int kRound = 8, kStep = kSplit ? kSumWarps : 1;
+        for (int s = kSplit ? warp : 0; s < count; s += kRound * kStep) {
+            float v[kRound][kLaneElements];
 #pragma unroll
-            for (int j = 0; j < kLaneElements; ++j)
-                if (src[j]) sum[j] += src[j][s * step[j]];
+            for (int r = 0; r < kRound; ++r)
+#pragma unroll
+                for (int j = 0; j < kLaneElements; ++j)
+                    v[r][j] = src[j] && s + r * kStep < count ? src[j][(size_t)(s + r * kStep) * step[j]] : 0.f;
+#pragma unroll
+            for (int r = 0; r < kRound; ++r)
+#pragma unroll
+                for (int j = 0; j < kLaneElements; ++j) sum[j] += v[r][j];
+        }
         const auto put = [&](size_t i, float total) {
             if (i < size) {
                 if (p.grad_weight) p.grad_weight[e * size + i] = from_f32<T>(total);
