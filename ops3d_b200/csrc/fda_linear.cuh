@@ -302,7 +302,7 @@ enum Mode {
 struct MmaRows {
     const void *a, *w, *bias, *extra;
     void *out;
-    float *sums;  // kPreGrad: the results' sums over 32 rows each, before rounding (BlockSums); may be nullptr
+    float *sums;  // kPreGrad: the results' sums over 32 rows each, before rounding; may be nullptr
     long long a_pitch, w_pitch, extra_pitch, out_pitch;
     int in_features, out_features, dtype, activation;
     Groups g;

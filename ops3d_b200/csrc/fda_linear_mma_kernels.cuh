@@ -1041,6 +1041,11 @@ bool weight_stays(long long tiles, long long columns, int groups, int most) {
     return columns <= most / 8 && (groups == 1 || tiles >= 2ll * groups * most);
 }
 
+template <int BN>
+bool single_keeps(int depth, long long tiles, long long columns, int groups) {
+    return ceil_div(depth, kSliceK) * Shape<BN>::kBytesB <= kResidentBytes && weight_stays(tiles, columns, groups, kSms);
+}
+
 // Blocks (or pairs) for `tiles`: a multiple of the column tiles where the weight is resident.
 unsigned row_grid(long long tiles, long long columns, unsigned most, bool resident) {
     if (tiles <= most) return (unsigned)tiles;
@@ -1063,7 +1068,7 @@ int launch_rows(RowsArgs<T> a, const MmaRows &p, long long units, cudaStream_t s
         map_extra = map_a;
     }
     const long long tiles = units * ceil_div(a.cols, BN);
-    a.resident = ceil_div(a.depth, kSliceK) * Shape<BN>::kBytesB <= kResidentBytes && weight_stays(tiles, ceil_div(a.cols, BN), p.g.groups, kSms);
+    a.resident = single_keeps<BN>(a.depth, tiles, ceil_div(a.cols, BN), p.g.groups);
     if (tiles >= (1ll << 31)) return FDA_ERR_BAD_SHAPE;
     return status(launch_early(kernel, row_grid(tiles, ceil_div(a.cols, BN), kSms, a.resident), Shape<BN>::kThreads, kSmem, st, 1, a, map_a,
                                map_w, map_extra));
@@ -1118,11 +1123,11 @@ int rows_of(const MmaRows &p, cudaStream_t st) {
         if (a.cols > 64 && units * ceil_div(a.cols, 128) >= kSms) return launch_rows<T, kMode, kAct, 128, false>(a, p, units, st);
         return launch_rows<T, kMode, kAct, 64, false>(a, p, units, st);
     }
-    // Pairs where they pay: extra rows (73728 x 256 x 1024 with a residual 74 us against 94 by single blocks) or a contraction too long
-    // for a resident weight (149504 x 1024 x 256: 78 against 86); else single blocks, whose epilogues wait for no other (598016 x
-    // 256 x 256: 105 against 117).
+    // Pairs where they pay: extra rows (73728 x 256 x 1024 with a residual 68 us against 86 by single blocks) or weights that a single
+    // block cannot keep, for their length or because they change with the tile (149504 x 1024 x 256: 74 against 82); else single
+    // blocks, whose epilogues wait for no other (598016 x 256 x 256: 105 against 117).
     const bool extra = kMode == kForward || kMode == kPreGrad;
-    const bool pays = extra || ceil_div(a.depth, kSliceK) * Shape<256>::kBytesB > kResidentBytes;
+    const bool pays = extra || !single_keeps<256>(a.depth, units * ceil_div(a.cols, 256), ceil_div(a.cols, 256), p.g.groups);
     const long long pair_units = most_units(p.g.batch, p.g.rows, p.g.groups, kPairRows, kMode != kPreGrad && p.g.starts);
     if (pays && pairs_fit(p.g, a.cols, pair_units)) return launch_pair<T, kMode, kAct>(a, p, pair_units, st);
     if (a.cols > 128 && units * ceil_div(a.cols, 256) >= kSms) return launch_rows<T, kMode, kAct, 256, true>(a, p, units, st);
