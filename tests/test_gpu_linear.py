@@ -543,6 +543,62 @@ def test_captured_training_pass_follows_its_inputs():
             assert torch.equal(a, e) and torch.equal(a2, e)
 
 
+@pytest.mark.parametrize("M", [3, 200, 20000])
+def test_neighbours_in_the_stream(M):
+    """Copies, fills and kernels right before and after, eager and captured: the operators' kernels are set up early but see what came
+    before, and what comes after sees theirs."""
+    x, w, b, r, dy = make((M,), 64, 136, torch.bfloat16, seed=17)
+    inputs = [make((M,), 64, 136, torch.bfloat16, seed=s)[0] for s in (18, 19, 20)]
+    want = [fused_linear(v, w, b, r, "silu") for v in inputs]
+    torch.cuda.synchronize()
+    buffer, out, mark = torch.empty_like(x), torch.empty_like(r), torch.empty(1 << 20, device=DEV)
+
+    def step(v):
+        mark.zero_()
+        buffer.copy_(v)                                   # a copy, not a kernel
+        y = fused_linear(buffer, w, b, r, "silu")
+        buffer.zero_()                                    # while the product may still be running
+        out.copy_(y)
+        y.fill_(float("nan"))
+        return out
+
+    for _ in range(20):
+        for v, e in zip(inputs, want):
+            assert torch.equal(step(v), e)
+    source = inputs[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(source)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(source)
+    for _ in range(5):
+        for v, e in zip(inputs, want):
+            source.copy_(v)
+            graph.replay()
+            assert torch.equal(out, e)
+
+
+def test_under_autocast_and_checkpointing():
+    """fp32 parameters beside the 16-bit tensors that autocast makes, and the operators inside a recomputed segment."""
+    from torch.utils.checkpoint import checkpoint
+
+    torch.manual_seed(3)
+    ff = FeedForward(32, 64, "gelu").to(DEV)
+    x = torch.randn(100, 32, device=DEV)
+    with torch.autocast("cuda", torch.bfloat16):
+        h = torch.nn.functional.linear(x, torch.eye(32, device=DEV))
+        y = ff(h)
+    assert h.dtype == torch.bfloat16 and y.dtype == torch.bfloat16
+    leaf = x.clone().requires_grad_(True)
+    plain = torch.autograd.grad(ff(leaf).square().sum(), [leaf, *ff.parameters()])
+    again = torch.autograd.grad(checkpoint(ff, leaf, use_reentrant=False).square().sum(), [leaf, *ff.parameters()])
+    for a, e in zip(again, plain):
+        assert torch.equal(a, e)
+
+
 def test_refusals():
     x, w, b, r, dy = make((10,), 16, 24, torch.bfloat16)
     starts = torch.tensor([0], device=DEV)
