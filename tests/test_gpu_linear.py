@@ -10,6 +10,7 @@ Tolerances, from the arithmetic alone (``eps`` of the tensors' type, all quantit
 * for 16-bit types with an activation g is rounded to the type between the products.
 """
 import math
+import threading
 
 import pytest
 import torch
@@ -597,6 +598,53 @@ def test_under_autocast_and_checkpointing():
     again = torch.autograd.grad(checkpoint(ff, leaf, use_reentrant=False).square().sum(), [leaf, *ff.parameters()])
     for a, e in zip(again, plain):
         assert torch.equal(a, e)
+
+
+def test_graphs_and_threads_at_once():
+    """Captured passes replayed on two streams at once, and threads on streams of their own and on a shared one, give what a pass
+    alone gives: no workspace is shared."""
+    starts = torch.tensor([0, 100, 100, 900, 2000, 9000], device="cuda")
+    inputs = []
+    for k in range(2):
+        torch.manual_seed(k)
+        x = torch.randn(9500, 72, device="cuda", dtype=torch.bfloat16).requires_grad_()
+        inputs.append((x, torch.randn(6, 136, 72, device="cuda", dtype=torch.bfloat16).requires_grad_()))
+
+    def grads(k):
+        x, w = inputs[k]
+        return torch.autograd.grad(grouped_linear(x, w, starts, None, None, "gelu").square().sum(), (x, w))
+
+    wants = [grads(k) for k in range(2)]
+    torch.cuda.synchronize()
+    differing = []
+
+    def repeat(stream, k):
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                if not all(torch.equal(a, b) for a, b in zip(grads(k), wants[k])):
+                    differing.append(k)
+
+    threads = [threading.Thread(target=repeat, args=(torch.cuda.Stream() if i % 2 else torch.cuda.default_stream(), i // 2)) for i in range(4)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not differing
+
+    captured = []
+    for k in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results = grads(k)
+        captured.append((graph, results, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, _, stream in captured:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (_, results, _), want in zip(captured, wants):
+        assert all(torch.equal(a, b) for a, b in zip(results, want))
 
 
 def test_refusals():
