@@ -67,6 +67,8 @@ __device__ __forceinline__ void arrive_at(uint32_t cluster_barrier) {
 __device__ __forceinline__ void release_at(uint32_t cluster_barrier) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_barrier) : "memory");
 }
+// Behind a wait for release_at: a barrier's own wait acquires what this block's threads have released, not what the other's have.
+__device__ __forceinline__ void acquire_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
     asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));

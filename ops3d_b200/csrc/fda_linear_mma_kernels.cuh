@@ -869,6 +869,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                     if (count < kSliceK) {
                         sound = __all_sync(0xffffffffu, pipe.mask_go.wait(masks++ & 1, failed));
                         if (!sound) break;
+                        acquire_cluster();  // the copies that the zeros overwrite
                         clear_lines(a, count);
                         if (lane == 0) release_at(cluster_address(&pipe.masked, 0));
                     }
@@ -883,7 +884,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                     if (kPair) {
                         sound = __all_sync(0xffffffffu, pipe.masked.wait(masks++ & 1, failed));
                         if (!sound) break;
-                        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                        acquire_cluster();
                     }
                 }
                 fence_after_sync();

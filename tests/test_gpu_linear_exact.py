@@ -1,0 +1,96 @@
+"""Linear operators over small whole numbers, whose products and sums are exact in fp32 in any order as long as they stay below
+2^24: every result has to be the whole number, rounded once to the tensors' type.  A row, a block or a sum of a piece that is left out,
+taken twice or taken from another group shows in every element that it belongs to, however long the sum.
+
+Values are -2 .. 2, so a sum of n products is at most 4 n: 2^24 is reached from 4 million terms on.
+"""
+import pytest
+import torch
+
+from ops3d_b200 import capi, fused_linear, grouped_linear
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+NARROW = [torch.float16, torch.bfloat16]
+DTYPES = [torch.float32, *NARROW]
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    torch.cuda.synchronize()
+    assert capi.load().fda_linear_timeouts() == 0
+
+
+def whole(gen, *shape):
+    return torch.randint(-2, 3, shape, generator=gen, device=DEV).double()
+
+
+def operands(lead, K, N, groups=None, seed=0):
+    """x, weight, bias, residual and the output's gradient, in 64 bits."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    g = () if groups is None else (groups,)
+    return whole(gen, *lead, K), whole(gen, *g, N, K), whole(gen, *g, N), whole(gen, *lead, N), whole(gen, *lead, N)
+
+
+def expected(x, w, b, r, dy, starts=None, relu=False):
+    """y, grad_x, grad_weight, grad_bias in 64 bits; starts: ascending, one entry more than groups."""
+    K, N = x.shape[-1], w.shape[-2]
+    rows = x.shape[-2]
+    batch = x.numel() // (rows * K)
+    spans = [(0, rows)] if starts is None else list(zip(starts[:-1], starts[1:]))
+    x, dy = x.reshape(batch, rows, K), dy.reshape(batch, rows, N)
+    y = torch.zeros_like(dy) if r is None else r.reshape(batch, rows, N).clone()
+    gx, gw, gb = torch.zeros_like(x), torch.zeros_like(w), torch.zeros_like(b)
+    for e, (lo, hi) in enumerate(spans):
+        we, be = (w, b) if starts is None else (w[e], b[e])
+        xe, ge = x[:, lo:hi].reshape(-1, K), dy[:, lo:hi].reshape(-1, N)
+        pre = xe @ we.t() + be
+        if relu:
+            ge = ge * (pre > 0)
+            pre = pre.clamp_min(0)
+        y[:, lo:hi] += pre.view(batch, hi - lo, N)
+        gx[:, lo:hi] = (ge @ we).view(batch, hi - lo, K)
+        (gw if starts is None else gw[e]).copy_(ge.t() @ xe)
+        (gb if starts is None else gb[e]).copy_(ge.sum(0))
+    return y, gx, gw, gb
+
+
+def run(x, w, b, r, dy, dtype, starts=None, relu=False):
+    leaves = [t.to(dtype).requires_grad_(True) for t in (x, w, b)]
+    r = None if r is None else r.to(dtype)
+    act = "relu" if relu else "none"
+    if starts is None:
+        y = fused_linear(*leaves, r, act)
+    else:
+        y = grouped_linear(leaves[0], leaves[1], torch.tensor(starts, device=DEV), leaves[2], r, act)
+    return (y, *torch.autograd.grad(y, leaves, dy.to(dtype)))
+
+
+def same(got, want, dtype):
+    for name, g, v in zip(("y", "grad_x", "grad_weight", "grad_bias"), got, want):
+        assert v.abs().max().item() < 2 ** 24
+        bad = (g != v.to(dtype).view(g.shape)).sum().item()
+        assert bad == 0, f"{name}: {bad} of {g.numel()} elements"
+
+
+# Weight gradients of which pairs of blocks take 64 rows at a time, and both have to clear the rows behind a group's end: groups that
+# end anywhere inside a block, with every batch element; in pieces whose sums are added, and whole.
+PAIRED = {
+    "pieces": ((2, 20480), 264, 264, [70, 15000, 15001, 15001, 20301]),
+    "whole": ((2, 1500), 2048, 1800, [3, 600, 601, 999, 1400]),
+    "three elements": ((3, 9001), 520, 264, [0, 4001, 4102, 9000]),
+}
+
+
+@pytest.mark.parametrize("dtype", NARROW)
+@pytest.mark.parametrize("kind", PAIRED)
+def test_rows_behind_a_group_stay_out_of_both_blocks(kind, dtype):
+    lead, K, N, starts = PAIRED[kind]
+    x, w, b, r, dy = operands(lead, K, N, len(starts) - 1, seed=1)
+    want = expected(x, w, b, None, dy, starts)
+    for t in (x, dy):   # rows of no group
+        t[..., :starts[0], :], t[..., starts[-1]:, :] = float("nan"), float("inf")
+    for _ in range(5):
+        same(run(x, w, b, None, dy, dtype, starts), want, dtype)
