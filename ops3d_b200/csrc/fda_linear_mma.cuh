@@ -78,6 +78,9 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Between this thread's accesses to shared memory and those of copies and products to the same places, either way round.
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 // A place in a ring, with the parity of its current round.
 struct Ring {
     int stages, stage = 0;

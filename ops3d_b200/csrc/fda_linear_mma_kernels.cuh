@@ -590,8 +590,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             return at;
         };
         const auto works = [&](const Place &at) { return at.rows > 0 && at.col0 < p.cols; };
-        // A place's extra rows into the buffer.  Lanes arrive at extra_empty behind the stores of what they made of the rows before: an
-        // arrival right behind the reads themselves let the copy overtake some of them.
+        // A place's extra rows into the buffer.  Its readers are ordinary loads and its next writer is the copy engine, which no barrier
+        // alone orders behind them: an arrival right behind the reads let the copy overtake some.  So each lane arrives at extra_empty
+        // when it has stored what it made of its rows (its loads have ended) and has put a fence between the two kinds of access.
         unsigned asked = 0, loads = 0;
         const auto request = [&](const Place &at) {
             if (!kExtra || !works(at)) return;
@@ -654,7 +655,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                         }
                     store_rows<true>(out + 32 * c, p.out_pitch, u.rows, p.cols - u.col0 - 32 * c, stage, row);
                 }
-                if (kExtra) pipe.extra_empty[mine].arrive();
+                if (kExtra) {
+                    fence_async();
+                    pipe.extra_empty[mine].arrive();
+                }
             }
             if (more) request(next);
             if (u.group >= 0) {
@@ -736,7 +740,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
     }
     pipeline_begin<kPair>(pipe, kColumns, Shape<BN>::kEpilogueWarps);
     for (int i = threadIdx.x; i < kOnesBytes / 4; i += Shape<BN>::kThreads) reinterpret_cast<uint32_t *>(ones)[i] = pack2<T>(1.f, 1.f);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    fence_async();
     wait_for_previous_kernel();
     build_piece_table(p.g, kSliceK, p.piece, table);
     __syncthreads();
@@ -844,7 +848,7 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                 const int block = l / (lines * 8), rest = l - block * lines * 8;
                 reinterpret_cast<uint4 *>(a + block * (64 * kSliceK * 2) + count * 128)[rest] = make_uint4(0, 0, 0, 0);
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            fence_async();
             __syncwarp();
         };
         constexpr uint32_t kHigh = operand_high(kAtom);

@@ -94,3 +94,17 @@ def test_rows_behind_a_group_stay_out_of_both_blocks(kind, dtype):
         t[..., :starts[0], :], t[..., starts[-1]:, :] = float("nan"), float("inf")
     for _ in range(5):
         same(run(x, w, b, None, dy, dtype, starts), want, dtype)
+
+
+@pytest.mark.parametrize("dtype", NARROW)
+@pytest.mark.parametrize("grouped", [False, True], ids=["one", "groups"])
+def test_extra_rows_of_one_tile_never_reach_another(grouped, dtype):
+    """A residual, and in the backward the output's gradient, pass through a buffer that is filled again while the tile before is still
+    being written: tall inputs, several tiles a pair of blocks, short contractions (the buffer's turn comes soonest)."""
+    starts = [130, 9001, 9001, 30011] if grouped else None
+    lead = (2, 30011) if grouped else (60011,)
+    for K, N in ((16, 520), (200, 264)):
+        ops = operands(lead, K, N, 3 if grouped else None, seed=K)
+        want = expected(*ops, starts, relu=True)
+        for _ in range(5):
+            same(run(*ops, dtype, starts, relu=True), want, dtype)
