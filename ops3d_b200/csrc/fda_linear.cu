@@ -509,6 +509,16 @@ __global__ void __launch_bounds__(32 * kSumWarps) linear_weight_grad_sum_kernel(
 // ---------------------------------------------------------------------------------------------------------------------------
 inline size_t type_size(int dtype) { return dtype == FDA_DTYPE_F32 ? 4 : 2; }
 
+// Upper bound of a piece table's slots, whatever the start indices are.  A group has slots when it has more than `piece` blocks, so more
+// than floor(piece / batch) in each batch element, and all of these but the last are whole: that takes `least` rows of the element.  With k
+// such groups of r rows an element (r >= k in all) there are at most r - k over `block` and one block a group more, times the
+// batch; b blocks of a group are at most (b + piece - 1) / piece pieces.  The bound grows with k and with r.
+long long most_slots(int batch, int rows, int groups, int block, int piece) {
+    if (batch == 0) return 0;
+    const long long least = (long long)block * (piece / batch) + 1, k = std::min<long long>(groups, rows / least);
+    return k == 0 ? 0 : (batch * ((rows - k) / block + k) + k * (piece - 1)) / piece;
+}
+
 // As many pieces as `workers` take at once over `tiles` tiles of the weight, none shorter than `least_piece` blocks.
 Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int least_piece, int workers) {
     Cut c;
@@ -522,12 +532,9 @@ Cut cut_rows(int batch, int rows, int groups, long long tiles, int block, int le
     c.piece = (int)std::max<long long>(least_piece, length);
     if (blocks <= 2 * least_piece) c.piece = (int)blocks;  // the second launch would cost more than it spreads
     c.pieces = ceil_div(blocks, c.piece) + groups;
-    // a group of n > 1 pieces has more than (n - 1) * piece blocks, so at least n / 2 * piece
-    c.slots = blocks <= c.piece ? 0 : std::min(c.pieces, 2 * (blocks / c.piece) + 1);
+    c.slots = most_slots(batch, rows, groups, block, c.piece);
     return c;
 }
-
-
 
 struct Shape {
     int batch, rows, groups, in_features, out_features, dtype;

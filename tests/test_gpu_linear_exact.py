@@ -108,3 +108,21 @@ def test_extra_rows_of_one_tile_never_reach_another(grouped, dtype):
         want = expected(*ops, starts, relu=True)
         for _ in range(5):
             same(run(*ops, dtype, starts, relu=True), want, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_groups_that_just_need_several_pieces(dtype):
+    """As many groups as the rows allow that are one row longer than a piece, the rest hardly any: all partial sums that a call can have.
+    (16-bit: pieces of 512 rows; fp32: 256 rows an element of the batch are a block, and with 9 elements each row is a piece.)"""
+    sizes = [513, 0, 513, 1, 513, 2, *[1] * 40, 0, 513, 3, 513, *[0] * 100]
+    starts = [5]
+    for n in sizes:
+        starts.append(starts[-1] + n)
+    ops = operands((starts[-1] + 20,), 264, 520, len(sizes), seed=2)
+    same(run(*ops[:3], None, ops[4], dtype, starts), expected(*ops[:3], None, ops[4], starts), dtype)
+    sizes = [1, 3, 0, 1, 2, 0, 0, 1]
+    starts = [1]
+    for n in sizes:
+        starts.append(starts[-1] + n)
+    ops = operands((40, starts[-1] + 1), 72, 136, len(sizes), seed=3)
+    same(run(*ops[:3], None, ops[4], dtype, starts), expected(*ops[:3], None, ops[4], starts), dtype)
