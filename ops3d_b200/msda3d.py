@@ -117,6 +117,8 @@ def project_and_pack(query, reference_points, w_offsets, b_offsets, w_logits, b_
 
 
 class MSDeformAttn3D(nn.Module):
+    level_value_proj = False  # of layers pickled before there was a choice
+
     def __init__(self, d_model: int = 256, n_levels: int = 3, n_heads: int = 8, n_points: int = 4, im2col_step: int = 64,
                  fused_projection: bool = True, level_value_proj: bool = False):
         super().__init__()

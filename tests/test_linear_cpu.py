@@ -140,3 +140,12 @@ def test_layer_keeps_its_parameters():
     levels = MSDeformAttn3D(32, 2, 4, 4, level_value_proj=True)
     assert levels.value_proj.weight.shape == (2, 32, 32) and levels.value_proj.bias.shape == (2, 32)
     assert set(levels.state_dict()) == set(plain.state_dict())
+
+
+def test_a_layer_pickled_before_the_level_projections_has_one_for_all():
+    from ops3d_b200.msda3d import MSDeformAttn3D
+
+    layer = MSDeformAttn3D(32, 2, 4, 4)
+    del layer.__dict__["level_value_proj"]
+    assert layer.level_value_proj is False
+    assert MSDeformAttn3D(32, 2, 4, 4, level_value_proj=True).level_value_proj is True
