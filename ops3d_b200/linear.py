@@ -94,6 +94,13 @@ def like(x, parameter):
     return parameter if parameter is None or parameter.dtype == x.dtype else parameter.to(x.dtype)
 
 
+def add_residual(y, residual):
+    """``y + residual`` in the wider of their dtypes, for a residual that the product's epilogue does not take."""
+    if residual.shape != y.shape:
+        raise RuntimeError(f"residual must have the shape of the output, {list(y.shape)}, got {list(residual.shape)}")
+    return y + residual
+
+
 class GroupedLinear(nn.Module):
     """``grouped_linear`` with its parameters: ``n_groups`` linear layers, each for its own rows."""
 

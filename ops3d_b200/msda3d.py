@@ -16,7 +16,7 @@ after the two projections:
 
 Two options take the fused linear operators (``ops3d_b200.linear``): ``level_value_proj=True`` gives each pyramid level a value
 projection of its own, one product over the ragged levels; ``residual`` in ``forward`` is added in the output projection's
-epilogue.
+epilogue, or behind it where it has another dtype than the layer's output (an fp32 stream around a 16-bit layer stays fp32).
 """
 from __future__ import annotations
 
@@ -28,7 +28,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from .flash_deform_attn import FlashDeformAttnFunction
-from .linear import GroupedLinear, fused_linear, like
+from .linear import GroupedLinear, add_residual, fused_linear, like
 
 
 class PackSamplingFunction(Function):
@@ -174,4 +174,7 @@ class MSDeformAttn3D(nn.Module):
         out = FlashDeformAttnFunction.apply(value, spatial_shapes, level_start_index, packed, self.im2col_step, K, True)
         if residual is None:
             return self.output_proj(out)
-        return fused_linear(out, like(out, self.output_proj.weight), like(out, self.output_proj.bias), residual)
+        weight, bias = like(out, self.output_proj.weight), like(out, self.output_proj.bias)
+        if residual.dtype == out.dtype:
+            return fused_linear(out, weight, bias, residual)
+        return add_residual(fused_linear(out, weight, bias), residual)

@@ -149,3 +149,12 @@ def test_a_layer_pickled_before_the_level_projections_has_one_for_all():
     del layer.__dict__["level_value_proj"]
     assert layer.level_value_proj is False
     assert MSDeformAttn3D(32, 2, 4, 4, level_value_proj=True).level_value_proj is True
+
+
+def test_a_residual_of_another_type_keeps_its_bits():
+    from ops3d_b200.linear import add_residual
+
+    y, r = torch.ones(3, 4, dtype=torch.bfloat16), torch.rand(3, 4)
+    assert add_residual(y, r).dtype == torch.float32 and torch.equal(add_residual(y, r), r + 1)
+    with pytest.raises(RuntimeError, match="shape of the output"):
+        add_residual(y, r[:1])
