@@ -20,6 +20,9 @@ the activation's derivative needs it; beyond 64 rows ``grad_output * act'`` is r
 products.  The results of repeated calls are equal bit for bit.  Up to 1024 groups, 2^31 - 1 rows and 2^26 - 1 features.
 ``gelu`` is 0 at minus infinity.
 
+Under ``torch.autocast("cuda")`` x, weight and bias are taken in autocast's dtype, as torch's own linear layers take them.  A residual of
+another dtype (an fp32 stream) is then added behind the product, and the result has the wider of the two.
+
 ``FeedForward`` is a transformer layer's ``x + W2 act(W1 x + b1) + b2``, with a weight pair of its own per group of rows where
 ``n_groups`` is given (one per pyramid level, or one per expert).
 """
@@ -77,21 +80,35 @@ class FusedLinearFunction(Function):
         return super().apply(x, weight, bias, residual, group_start_index, activation)
 
 
+def _product(x, weight, bias, residual, group_start_index, activation):
+    """``FusedLinearFunction.apply``, under autocast with x, weight and bias in its dtype (float64 stays, and is refused) and a residual of
+    another dtype added behind the product."""
+    if not torch.is_autocast_enabled("cuda"):
+        return FusedLinearFunction.apply(x, weight, bias, residual, group_start_index, activation)
+    dtype = torch.get_autocast_dtype("cuda")
+    x, weight, bias = (t if t is None or t.dtype in (dtype, torch.float64) or not t.is_floating_point() else t.to(dtype) for t in (x, weight, bias))
+    if residual is None or residual.dtype == x.dtype:
+        return FusedLinearFunction.apply(x, weight, bias, residual, group_start_index, activation)
+    return add_residual(FusedLinearFunction.apply(x, weight, bias, None, group_start_index, activation), residual)
+
+
 def fused_linear(x, weight, bias=None, residual=None, activation="none"):
     """``act(x @ weight^T + bias) + residual`` in one pass (module docstring)."""
-    return FusedLinearFunction.apply(x, weight, bias, residual, None, activation)
+    return _product(x, weight, bias, residual, None, activation)
 
 
 def grouped_linear(x, weight, group_start_index, bias=None, residual=None, activation="none"):
     """``fused_linear`` with a weight per group of rows (module docstring)."""
     if group_start_index is None:
         raise ValueError("group_start_index is required; fused_linear takes one weight for all rows")
-    return FusedLinearFunction.apply(x, weight, bias, residual, group_start_index, activation)
+    return _product(x, weight, bias, residual, group_start_index, activation)
 
 
 def like(x, parameter):
-    """``parameter`` in the dtype of ``x`` (a 16-bit input beside fp32 parameters, as under autocast)."""
-    return parameter if parameter is None or parameter.dtype == x.dtype else parameter.to(x.dtype)
+    """``parameter`` in the dtype of ``x`` (a 16-bit input beside fp32 parameters); under autocast itself, for the call to cast it once."""
+    if parameter is None or parameter.dtype == x.dtype or torch.is_autocast_enabled("cuda"):
+        return parameter
+    return parameter.to(x.dtype)
 
 
 def add_residual(y, residual):
@@ -149,5 +166,5 @@ class FeedForward(nn.Module):
         if (self.n_groups is None) != (group_start_index is None):
             raise ValueError("group_start_index goes with n_groups")
         w1, b1, w2, b2 = (like(x, p) for p in (self.weight1, self.bias1, self.weight2, self.bias2))
-        hidden = FusedLinearFunction.apply(x, w1, b1, None, group_start_index, self.activation)
-        return FusedLinearFunction.apply(hidden, w2, b2, x if self.residual else None, group_start_index, "none")
+        hidden = _product(x, w1, b1, None, group_start_index, self.activation)
+        return _product(hidden, w2, b2, x if self.residual else None, group_start_index, "none")

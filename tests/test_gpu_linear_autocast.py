@@ -59,3 +59,80 @@ def test_fp32_residual_around_a_16_bit_layer(dtype):
     for g, v in zip(torch.autograd.grad(got, leaves, dy), torch.autograd.grad(want, leaves, dy)):
         assert g.dtype == v.dtype and norm_error(g, v) <= 8 * eps
     assert torch.equal(torch.autograd.grad(layer(src, *rest, residual=stream), stream, dy)[0], dy)
+
+
+@pytest.mark.parametrize("dtype", NARROW)
+@pytest.mark.parametrize("levels", [False, True], ids=["one-projection", "level-projections"])
+def test_layer_under_autocast(levels, dtype):
+    """From an fp32 stream: the projections run in autocast's type, the residual stays fp32, every gradient comes back in fp32."""
+    layer, src, rest = layer_and_inputs()
+    eps = torch.finfo(dtype).eps
+    dy = torch.randn(src.shape, device=DEV)
+    leaves = [src, layer.sampling_offsets.weight, layer.attention_weights.bias, layer.output_proj.weight, layer.output_proj.bias]
+    with torch.autocast("cuda", dtype):
+        want_proj = layer(src, *rest)
+        want = want_proj + src
+    assert want_proj.dtype == dtype
+    wants = torch.autograd.grad(want, leaves, dy)
+    if levels:   # the same weight for every level
+        torch.manual_seed(1)
+        other = MSDeformAttn3D(64, 2, 4, 4, level_value_proj=True).to(DEV)
+        state = layer.state_dict()
+        for k in ("weight", "bias"):
+            state["value_proj." + k] = state["value_proj." + k].expand(2, *state["value_proj." + k].shape).contiguous()
+        other.load_state_dict(state)
+        layer = other
+        leaves = [src, layer.sampling_offsets.weight, layer.attention_weights.bias, layer.output_proj.weight, layer.output_proj.bias]
+    seen = []
+    hook = layer.value_proj.register_forward_hook(lambda m, i, o: seen.append(o.dtype))
+    with torch.autocast("cuda", dtype):
+        got = layer(src, *rest, residual=src)
+    hook.remove()
+    assert seen == [dtype] and got.dtype == torch.float32
+    assert norm_error(got - src, want_proj) <= 8 * eps
+    for g, v in zip(torch.autograd.grad(got, leaves, dy), wants):
+        assert g.dtype == torch.float32 and norm_error(g, v) <= 8 * eps
+
+
+@pytest.mark.parametrize("dtype", NARROW)
+@pytest.mark.parametrize("n_groups", [None, 3])
+def test_feed_forward_under_autocast(n_groups, dtype):
+    """Behind a norm, whose result autocast leaves in fp32: both products in 16 bits, the residual in fp32."""
+    torch.manual_seed(2)
+    ff = FeedForward(72, 136, "gelu", n_groups).to(DEV)
+    starts = None if n_groups is None else torch.tensor([0, 100, 180], device=DEV)
+    x = torch.randn(300, 72, device=DEV, requires_grad=True)
+    dy = torch.randn(300, 72, device=DEV)
+    leaves = [x, *ff.parameters()]
+    with torch.autocast("cuda", dtype):
+        got = ff(x, starts)
+    w1, b1, w2, b2 = (p.to(dtype) for p in (ff.weight1, ff.bias1, ff.weight2, ff.bias2))
+    if n_groups is None:
+        want = fused_linear(fused_linear(x.to(dtype), w1, b1, activation="gelu"), w2, b2) + x
+    else:
+        want = grouped_linear(grouped_linear(x.to(dtype), w1, starts, b1, activation="gelu"), w2, starts, b2) + x
+    assert got.dtype == torch.float32 and torch.equal(got, want)
+    for g, v in zip(torch.autograd.grad(got, leaves, dy), torch.autograd.grad(want, leaves, dy)):
+        assert g.dtype == torch.float32 and torch.equal(g, v)
+
+
+def test_functions_under_autocast():
+    torch.manual_seed(3)
+    x, w, b, r = (torch.randn(*s, device=DEV) for s in ((90, 40), (56, 40), (56,), (90, 56)))
+    low = [t.bfloat16() for t in (x, w, b, r)]
+    starts = torch.tensor([0, 30], device=DEV)
+    with torch.autocast("cuda", torch.bfloat16):
+        assert torch.equal(fused_linear(x, w, b, activation="silu"), fused_linear(*low[:3], activation="silu"))
+        assert torch.equal(fused_linear(low[0], w, low[2], low[3]), fused_linear(*low))
+        assert torch.equal(fused_linear(x, w, b, r), fused_linear(*low[:3]) + r)
+        assert torch.equal(grouped_linear(x, w.expand(2, 56, 40), starts, None, r), grouped_linear(low[0], low[1].expand(2, 56, 40), starts) + r)
+        lin = GroupedLinear(2, 40, 56).to(DEV)
+        assert torch.equal(lin(x, starts), grouped_linear(low[0], lin.weight.bfloat16(), starts, lin.bias.bfloat16()))
+        with pytest.raises(RuntimeError, match="shape of the output"):
+            fused_linear(x, w, b, r[:1])
+        with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
+            fused_linear(x.double(), w.double())
+        with torch.autocast("cuda", enabled=False):
+            assert fused_linear(x, w, b, r).dtype == torch.float32
+    with torch.autocast("cuda", torch.float16):   # tensors of the other 16-bit type too, as torch's own layers
+        assert torch.equal(fused_linear(low[0], w, low[2]), fused_linear(low[0].half(), w.half(), low[2].half()))
