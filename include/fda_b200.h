@@ -447,8 +447,8 @@ int fda_nms3d_scored(const float *boxes, long long box_stride, long long coord_s
  * groups <= FDA_LINEAR_MAX_GROUPS.
  *
  * The backward computes pre again from x instead of reading it: that is in_features instead of 2 * out_features elements of
- * traffic a row.  For 16-bit types and more than 64 rows g is rounded to `dtype` between the products (its sums for fewer than 1024
- * biases are not).  grad_x, grad_weight and grad_bias may each be NULL.  Sums run in a fixed order: repeated calls give the same bits.
+ * traffic a row.  For 16-bit types and more than 64 rows g is rounded to `dtype` between the products (its sums for grad_bias
+ * are not).  grad_x, grad_weight and grad_bias may each be NULL.  Sums run in a fixed order: repeated calls give the same bits.
  *
  * The workspaces (256-byte aligned; sizes from the functions, 0 = none) hold intermediate results of the call only; two calls
  * that may overlap need two.  A wait inside a kernel that ran out (2 s: never in a sound run) leaves the outputs undefined and

@@ -353,8 +353,8 @@ __global__ void __launch_bounds__(32 * kBiasWarps) linear_bias_sum_kernel(const 
     build_row_table(g, unit, false, table);
     __syncthreads();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, steps = (cols + 31) / 32, subs = unit / kSumRows;
-    for (int item = blockIdx.x; item < g.groups * steps; item += gridDim.x) {
-        const int e = item / steps, c = item % steps * 32 + lane;
+    for (long long item = blockIdx.x; item < (long long)g.groups * steps; item += gridDim.x) {
+        const int e = (int)(item / steps), c = (int)(item % steps) * 32 + lane;
         const int each = (table.start[e + 1] - table.start[e] + kSumRows - 1) / kSumRows;  // sums of one batch element
         float sum = 0.f;
         if (c < cols)
@@ -691,13 +691,11 @@ Layout forward_layout(const Shape &s) {
 
 bool few_rows_backward(const Shape &s) { return total_rows(s) <= 64; }
 
-// A 16-bit bias's gradient from g as it is (MmaRows::sums) or, by the weight gradient's product with ones, from g rounded.  The second
-// has the rounding's error twice, 1.4 times one rounding in the mean over many outputs and up to twice over few; the first costs
-// the pre-activation's gradient 15 % (73728 x 256 x 1024: 119 instead of 103 us, and 5 to add the sums), too much where the outputs
-// are many.
-bool bias_from_sums(const Shape &s, int activation) {
-    return s.dtype != FDA_DTYPE_F32 && activation != FDA_ACT_NONE && (long long)s.groups * s.out_features < 1024;
-}
+// A 16-bit bias's gradient behind an activation comes from g as it is (MmaRows::sums), not from g rounded by the weight gradient's product
+// with ones: that would have the rounding's error twice, 1.4 times one rounding in the mean over many outputs and up to twice over few.  The
+// sums cost the pre-activation's gradient 15 % (73728 x 256 x 1024: 119 instead of 103 us, 149504 x 256 x 256: 68 instead of 58),
+// and some us to add them.
+bool bias_from_sums(const Shape &s, int activation) { return s.dtype != FDA_DTYPE_F32 && activation != FDA_ACT_NONE; }
 
 // g: the pre-activation's gradient, or a padded copy of grad_output.
 Layout backward_layout(const Shape &s, int activation) {

@@ -17,6 +17,25 @@ def no_wait_ran_out():
     assert capi.load().fda_linear_timeouts() == 0
 
 
+@pytest.mark.parametrize("dtype", NARROW)
+@pytest.mark.parametrize("groups,M,K,N", [(1, 300, 40, 1024), (1, 3000, 33, 1027), (1, 19003, 72, 1024), (1, 5003, 40, 2056), (16, 9000, 72, 264),
+                                          (70, 4000, 24, 136), (2, 30000, 40, 520)])
+def test_bias_gradient_is_rounded_once_at_every_width(groups, M, K, N, dtype):
+    """The precision of a bias's gradient does not depend on how many biases there are: fp32 sums of unrounded terms, one rounding.  (fp32's
+    share as in test_bias_gradient_is_rounded_once: sums over 32 rows, of which a warp adds every 32nd.)"""
+    x, w, b, _, dy = make((M,), K, N, dtype, groups, residual=False, seed=M)
+    cuts = torch.sort(torch.randint(0, M, (groups - 1,), generator=torch.Generator().manual_seed(groups)))[0].tolist()
+    bounds = [0, *cuts, M]
+    leaf = b.clone().requires_grad_(True)
+    (g,) = torch.autograd.grad(grouped_linear(x, w, torch.tensor(bounds, device=DEV), leaf, activation="silu"), leaf, dy)
+    for e in range(groups):
+        rows = slice(bounds[e], bounds[e + 1])
+        terms = dy[rows].double() * act64(x[rows].double() @ w[e].double().t() + b[e].double(), "silu")[1]
+        value = terms.sum(0)
+        slack = terms.abs().sum(0) * 2.0 ** -23 * 96 + dy[rows].double().abs().sum(0) * 2.0 ** -20 * 4
+        assert ((g[e].double() - value).abs() <= rounding(value, dtype) * 1.01 + slack).all(), e
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_layers_saved_before_the_level_projections(dtype):
     """A whole layer pickled by an earlier version has no attribute for them."""
