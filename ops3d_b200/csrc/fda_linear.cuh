@@ -64,7 +64,9 @@ __device__ __forceinline__ float activate_backward(float v, float dy) {
     if (kAct == FDA_ACT_GELU) return dy * (0.5f * (1.f + erff(v * kSqrtHalf)) + v * kInvSqrt2Pi * expf(-0.5f * v * v));
     if (kAct == FDA_ACT_GELU_TANH) {
         const float t = tanhf(kTanhScale * (v + kTanhCubic * v * v * v));
-        return dy * (0.5f * (1.f + t) + 0.5f * v * (1.f - t * t) * kTanhScale * (1.f + 3.f * kTanhCubic * v * v));
+        // beyond 12 t is 1 or -1 to the last bit, and the slope's polynomial would overflow for very large v
+        const float c = fminf(fmaxf(v, -12.f), 12.f);
+        return dy * (0.5f * (1.f + t) + 0.5f * c * (1.f - t * t) * kTanhScale * (1.f + 3.f * kTanhCubic * c * c));
     }
     if (kAct == FDA_ACT_SILU) {
         const float s = sigmoid(v);

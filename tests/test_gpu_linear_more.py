@@ -17,6 +17,28 @@ def no_wait_ran_out():
     assert capi.load().fda_linear_timeouts() == 0
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_values_and_slopes_up_to_the_types_limit(act, dtype):
+    """Far out the activations are v or 0 and their slopes 1 or 0 exactly, also where v^2 or v^3 overflows: beyond 128 the exponentials
+    are 0 or above every fp32 number, and all that is left is one rounding."""
+    top = torch.finfo(dtype).max
+    v = torch.tensor([s * a for a in (128.0, 3e3, 6e4, 1e7, 1e13, 3e18, 1e20, 1e30, 2e38, top) if a <= top for s in (1, -1)], device=DEV)
+    for copies in (1, 20, 2000):
+        x = torch.zeros(v.numel() * copies, 8, device=DEV, dtype=dtype)
+        x[:, 3] = v.repeat(copies).to(dtype)
+        w = torch.zeros(16, 8, device=DEV, dtype=dtype)
+        w[:, 3] = 1
+        x.requires_grad_(True)
+        y = fused_linear(x, w, activation=act)
+        (gx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+        at = x.detach()[:, 3]
+        want = at if act == "none" else at.clamp_min(0)
+        slope = torch.ones_like(at) if act == "none" else (at > 0).to(dtype)
+        assert torch.equal(y, want[:, None].expand_as(y))
+        assert torch.equal(gx[:, 3], 16 * slope) and not gx[:, :3].any() and not gx[:, 4:].any()
+
+
 @pytest.mark.parametrize("dtype", NARROW)
 @pytest.mark.parametrize("groups,M,K,N", [(1, 300, 40, 1024), (1, 3000, 33, 1027), (1, 19003, 72, 1024), (1, 5003, 40, 2056), (16, 9000, 72, 264),
                                           (70, 4000, 24, 136), (2, 30000, 40, 520)])
