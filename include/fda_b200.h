@@ -452,7 +452,8 @@ int fda_nms3d_scored(const float *boxes, long long box_stride, long long coord_s
  *
  * The workspaces (256-byte aligned; sizes from the functions, 0 = none) hold intermediate results of the call only; two calls
  * that may overlap need two.  A wait inside a kernel that ran out (2 s: never in a sound run) leaves the outputs undefined and
- * counts in fda_linear_timeouts(), which synchronises with the device; the count is per device and never reset.
+ * counts in fda_linear_timeouts(), which synchronises with the device (all its streams, so not while one is being captured); the
+ * count is the current device's and never reset; -1 where the device cannot be asked.
  */
 typedef enum fda_activation {
     FDA_ACT_NONE = 0,

@@ -972,6 +972,8 @@ int fda_linear_backward(const void *x, const void *weight, const void *bias, con
 }
 
 int fda_linear_timeouts(void) {
+    // reading the counts would wait for streams only that wait for the default one
+    if (launched(cudaDeviceSynchronize()) != FDA_OK) return -1;
     const int a = mma_timeouts_f16(), b = mma_timeouts_bf16();
     return a < 0 || b < 0 ? -1 : a + b;
 }

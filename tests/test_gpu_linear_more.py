@@ -58,6 +58,18 @@ def test_bias_gradient_is_rounded_once_at_every_width(groups, M, K, N, dtype):
         assert ((g[e].double() - value).abs() <= rounding(value, dtype) * 1.01 + slack).all(), e
 
 
+def test_counting_waits_waits_for_every_stream():
+    """The count is asked for when nothing runs any more, on streams too that do not wait for the default one."""
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)
+        y = fused_linear(torch.ones(300, 64, device=DEV, dtype=torch.bfloat16), torch.ones(64, 64, device=DEV, dtype=torch.bfloat16))
+    assert not side.query()
+    assert capi.load().fda_linear_timeouts() == 0
+    assert side.query()
+    assert torch.equal(y, torch.full_like(y, 64))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_layers_saved_before_the_level_projections(dtype):
     """A whole layer pickled by an earlier version has no attribute for them."""
