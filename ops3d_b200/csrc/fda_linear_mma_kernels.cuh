@@ -625,7 +625,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 fence_after_sync();
             }
             if (works(u)) {
-                if (kExtra && !__all_sync(0xffffffffu, pipe.extra_full[mine].wait(loads++ & 1, failed))) break;
+                if (kExtra) {
+                    if (!__all_sync(0xffffffffu, pipe.extra_full[mine].wait(loads & 1, failed))) break;
+                    ++loads;
+                }
                 const uint32_t address = pipe.tmem + sums.stage * kPairColumns + part * 64 + ((uint32_t)(quarter * 32) << 16);
                 T *const out = p.out + (size_t)u.first * p.out_pitch + u.col0;
                 float *const sums_row =
@@ -668,7 +671,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 sums.next();
             }
         }
-        if (kExtra && asked != loads && lane == 0) {  // only after a wait that ran out
+        if (kExtra && asked != loads && lane == 0) {  // only after a wait that ran out: a copy may still be on its way
             volatile int again = 0;
             pipe.extra_full[mine].wait((asked - 1) & 1, &again);
         }
