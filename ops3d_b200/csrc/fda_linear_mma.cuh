@@ -12,8 +12,9 @@ static __device__ unsigned int g_timeouts;
 
 __device__ __forceinline__ uint32_t smem_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-// Limit of a wait: about two seconds of the SM's clock.
-constexpr long long kWaitCycles = 4000000000ll;
+// Limit of a wait: about two seconds of the SM's clock.  A stretch between two looks at the clock counts a sixteenth of it at most: what lies
+// beyond is time in which the block was not running (another process had the SM), and no sign of a fault.
+constexpr long long kWaitCycles = 4000000000ll, kMostBetweenLooks = kWaitCycles / 16;
 
 struct Barrier {
     unsigned long long word;
@@ -37,12 +38,15 @@ struct Barrier {
     }
     // False when the phase did not end within two seconds or another wait of the block ran out before: the caller leaves.
     __device__ __noinline__ bool wait_slowly(unsigned parity, volatile int *failed) {
-        const long long begin = clock64();
+        long long waited = 0, last = clock64();
         for (;;) {
             for (int i = 0; i < 64; ++i)
                 if (passed(parity)) return true;
             if (*failed) return false;
-            if (clock64() - begin > kWaitCycles) {
+            const long long now = clock64();
+            waited += min(now - last, kMostBetweenLooks);
+            last = now;
+            if (waited > kWaitCycles) {
                 *failed = 1;
                 return false;
             }
