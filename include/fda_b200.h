@@ -451,7 +451,7 @@ int fda_nms3d_scored(const float *boxes, long long box_stride, long long coord_s
  * are not).  grad_x, grad_weight and grad_bias may each be NULL.  Sums run in a fixed order: repeated calls give the same bits.
  *
  * The workspaces (256-byte aligned; sizes from the functions, 0 = none) hold intermediate results of the call only; two calls
- * that may overlap need two.  A wait inside a kernel that ran out (2 s: never in a sound run) leaves the outputs undefined and
+ * that may overlap need two.  A wait inside a kernel that ran out (2 s: never in a sound run) leaves NaN where the results are missing and
  * counts in fda_linear_timeouts(), which synchronises with the device (all its streams, so not while one is being captured); the
  * count is the current device's and never reset; -1 where the device cannot be asked.
  */

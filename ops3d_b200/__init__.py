@@ -6,8 +6,8 @@ CUDA kernels behind a C ABI (``include/fda_b200.h``, ``libfda_b200.so``), a thin
 """
 from ._extension import _C
 from .flash_deform_attn import FlashDeformAttnFunction, findspec, findspec_bwd
-from .linear import FeedForward, FusedLinearFunction, GroupedLinear, fused_linear, grouped_linear
+from .linear import FeedForward, FusedLinearFunction, GroupedLinear, fused_linear, grouped_linear, linear_timeouts
 
 __all__ = ["FlashDeformAttnFunction", "findspec", "findspec_bwd", "fused_linear", "grouped_linear", "FusedLinearFunction",
-           "GroupedLinear", "FeedForward", "_C"]
+           "GroupedLinear", "FeedForward", "linear_timeouts", "_C"]
 # The layer around the operator lives in ops3d_b200.msda3d (MSDeformAttn3D); imported on demand.

@@ -548,6 +548,12 @@ std::array<OptionalTensor, 3> linear_backward(const at::Tensor &x, const at::Ten
     return out;
 }
 
+int linear_timeouts() {
+    const int n = fda_linear_timeouts();
+    if (n < 0) raise_status(FDA_ERR_CUDA, "linear_timeouts");
+    return n;
+}
+
 // FusedLinearFunction.apply; the residual's gradient is the output's.
 struct FusedLinearBackward : public fda_nodes::SavedNode {
     int activation;
@@ -603,6 +609,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear", &linear, "differentiable linear layer with fused epilogue");
     m.def("linear_forward", &linear_forward, "linear layer with fused epilogue, forward (sm_100a)");
     m.def("linear_backward", &linear_backward, "linear layer with fused epilogue, backward (sm_100a)");
+    m.def("linear_timeouts", &linear_timeouts, "waits of the linear layers' kernels that ran out on the current device");
     m.def("nms_3d", &nms_3d, "non-maximum suppression for 3d boxes (sm_100a)");
     m.def("roi_align_3d_forward", &roi_align_3d_forward, "ROI-Align 3D forward (sm_100a)");
     m.def("roi_align_3d_backward", &roi_align_3d_backward, "ROI-Align 3D backward (sm_100a)");

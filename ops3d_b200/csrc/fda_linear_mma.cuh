@@ -449,4 +449,14 @@ __device__ __forceinline__ void store_rows(T *p, unsigned pitch, int rows, int c
     }
 }
 
+// NaN instead of results that a warp could not wait for: up to 32 rows of `count` elements, and their sums where there are any.
+template <typename T>
+__device__ __noinline__ void store_nan(T *p, unsigned pitch, int rows, int count, float *sums) {
+    const float nan = __int_as_float(0x7fffffff);
+    for (int r = 0; r < min(rows, 32); ++r)
+        for (int c = threadIdx.x % 32; c < count; c += 32) p[(size_t)r * pitch + c] = from_f32<T>(nan);
+    if (sums && rows > 0)
+        for (int c = threadIdx.x % 32; c < count; c += 32) sums[c] = nan;
+}
+
 }  // namespace fda_linear

@@ -3,7 +3,8 @@
 //
 // One block per SM walks the output tiles.  Warp 0 keeps a ring of operand slices filled, warp 1 issues the products, warps 4 and up
 // take finished sums out of tensor memory: accumulators are doubled, so that a tile's epilogue runs beside the next tile's
-// products.  Every wait is bounded: a role that waited in vain leaves, the others follow, and the block counts the event.
+// products.  Every wait is bounded: a role that waited in vain leaves, the others follow, the epilogue writes NaN where it has no sums,
+// and the block counts the event.
 //
 // Included by one translation unit per type.
 #pragma once
@@ -319,6 +320,14 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
             if (kExtra && kVector)
                 fetch_rows(p.extra + (size_t)at.first * p.extra_pitch + at.col0 + 32 * c, p.extra_pitch, at.rows, p.cols - at.col0 - 32 * c, fetched);
         };
+        const auto give_up = [&](unsigned tile) {  // NaN for what the warp still owes
+            for (; tile < tiles; tile += gridDim.x) {
+                const Place at = place(tile);
+                float *const sums_row =
+                    kMode == kPreGrad && p.sums ? p.sums + ((size_t)(tile / columns) * (kTileRows / kSumRows) + quarter) * p.cols + at.col0 : nullptr;
+                store_nan(p.out + (size_t)at.first * p.out_pitch + at.col0, p.out_pitch, at.rows, min(kPart, p.cols - at.col0), sums_row);
+            }
+        };
         Place next;
         if (blockIdx.x < tiles) {
             next = place(blockIdx.x);
@@ -365,7 +374,10 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
                     }
                 continue;
             }
-            if (!__all_sync(0xffffffffu, pipe.sums_full[sums.stage].wait(sums.round, failed))) break;
+            if (!__all_sync(0xffffffffu, pipe.sums_full[sums.stage].wait(sums.round, failed))) {
+                give_up(tile);
+                break;
+            }
             fence_after_sync();
             const uint32_t address = pipe.tmem + sums.stage * BN + part * kPart + ((uint32_t)(quarter * 32) << 16);
             float *const sums_row =
@@ -602,6 +614,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 tma_2d(&map_extra, buffer, &pipe.extra_full[mine], at.col0, (int)at.first);
             }
         };
+        const auto give_up = [&](unsigned tile) {  // NaN for what the warp still owes
+            for (; tile < tiles; tile += pairs) {
+                const Place at = place(tile);
+                float *const sums_row =
+                    kMode == kPreGrad && p.sums
+                        ? p.sums + ((size_t)(tile / columns) * (kPairRows / kSumRows) + rank * (kTileRows / kSumRows) + quarter) * p.cols + at.col0
+                        : nullptr;
+                store_nan(p.out + (size_t)at.first * p.out_pitch + at.col0, p.out_pitch, at.rows, min(64, p.cols - at.col0), sums_row);
+            }
+        };
         Place next;
         if (pair < tiles) {
             next = place(pair);
@@ -621,12 +643,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 __syncwarp();
             }
             if (u.group >= 0) {
-                if (!__all_sync(0xffffffffu, pipe.sums_full[sums.stage].wait(sums.round, failed))) break;
+                if (!__all_sync(0xffffffffu, pipe.sums_full[sums.stage].wait(sums.round, failed))) {
+                    give_up(tile);
+                    break;
+                }
                 fence_after_sync();
             }
             if (works(u)) {
                 if (kExtra) {
-                    if (!__all_sync(0xffffffffu, pipe.extra_full[mine].wait(loads & 1, failed))) break;
+                    if (!__all_sync(0xffffffffu, pipe.extra_full[mine].wait(loads & 1, failed))) {
+                        give_up(tile);
+                        break;
+                    }
                     ++loads;
                 }
                 const uint32_t address = pipe.tmem + sums.stage * kPairColumns + part * 64 + ((uint32_t)(quarter * 32) << 16);
@@ -921,6 +949,26 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
         const int quarter = warp % 4, part = (warp - kFirstEpilogueWarp) / 4;
         Stage &stage = stages[warp - kFirstEpilogueWarp];
         unsigned round = 0;
+        const auto give_up = [&](long long i) {  // NaN for what the warp still owes
+            const float nan = __int_as_float(0x7fffffff);
+            for (; i < items; i += workers) {
+                const Item it = item_at(i);
+                const bool whole = table.slot_begin[it.group + 1] == table.slot_begin[it.group];
+                const size_t slot = whole ? (size_t)it.group : (size_t)table.slot_begin[it.group] + it.piece;
+                const int first = it.out0 + quarter * 32, in0 = it.in0 + part * kPart, count = min(kPart, p.in_features - in0);
+                for (int out = first; out < min(first + 32, p.out_features); ++out) {
+                    const size_t at = slot * p.out_features + out;
+                    for (int k = lane; k < count && p.grad_weight; k += 32) {
+                        if (whole) p.grad_weight[at * p.in_features + in0 + k] = from_f32<T>(nan);
+                        else p.slots[at * p.in_features + in0 + k] = nan;
+                    }
+                    if (lane == 0 && part == 0 && it.in0 == 0 && p.grad_bias) {
+                        if (whole) p.grad_bias[at] = from_f32<T>(nan);
+                        else p.bias_slots[at] = nan;
+                    }
+                }
+            }
+        };
         for (long long i = worker; i < items; i += workers) {
             const Item it = item_at(i);
             const bool none = it.first >= it.last;
@@ -928,7 +976,10 @@ __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
             const size_t slot = whole ? (size_t)it.group : (size_t)table.slot_begin[it.group] + it.piece;
             const int out = it.out0 + quarter * 32 + lane;
             if (!none) {
-                if (!__all_sync(0xffffffffu, pipe.sums_full[0].wait(round, failed))) break;
+                if (!__all_sync(0xffffffffu, pipe.sums_full[0].wait(round, failed))) {
+                    give_up(i);
+                    break;
+                }
                 fence_after_sync();
             }
             const uint32_t address = pipe.tmem + ((uint32_t)(quarter * 32) << 16);

@@ -23,6 +23,9 @@ products.  The results of repeated calls are equal bit for bit.  Up to 1024 grou
 Under ``torch.autocast("cuda")`` x, weight and bias are taken in autocast's dtype, as torch's own linear layers take them.  A residual of
 another dtype (an fp32 stream) is then added behind the product, and the result has the wider of the two.
 
+Blocks of the 16-bit kernels wait for one another, two seconds at most (never in a sound run): results that a wait ran out on are NaN, and
+``linear_timeouts()`` counts it.
+
 ``FeedForward`` is a transformer layer's ``x + W2 act(W1 x + b1) + b2``, with a weight pair of its own per group of rows where
 ``n_groups`` is given (one per pyramid level, or one per expert).
 """
@@ -102,6 +105,11 @@ def grouped_linear(x, weight, group_start_index, bias=None, residual=None, activ
     if group_start_index is None:
         raise ValueError("group_start_index is required; fused_linear takes one weight for all rows")
     return _product(x, weight, bias, residual, group_start_index, activation)
+
+
+def linear_timeouts() -> int:
+    """How many waits inside the operators' kernels have run out on the current device: 0 in a sound process.  Synchronises with the device."""
+    return _ext().linear_timeouts()
 
 
 def like(x, parameter):

@@ -158,3 +158,12 @@ def test_a_residual_of_another_type_keeps_its_bits():
     assert add_residual(y, r).dtype == torch.float32 and torch.equal(add_residual(y, r), r + 1)
     with pytest.raises(RuntimeError, match="shape of the output"):
         add_residual(y, r[:1])
+
+
+def test_waits_that_ran_out_are_counted_in_python(binding, monkeypatch):
+    monkeypatch.setattr(binding, "linear_timeouts", lambda: 3, raising=False)
+    assert ops3d_b200.linear_timeouts() == 3
+    monkeypatch.undo()
+    if not torch.cuda.is_available():
+        with pytest.raises(RuntimeError, match="linear_timeouts"):
+            ops3d_b200.linear_timeouts()
