@@ -126,3 +126,23 @@ def test_groups_that_just_need_several_pieces(dtype):
         starts.append(starts[-1] + n)
     ops = operands((40, starts[-1] + 1), 72, 136, len(sizes), seed=3)
     same(run(*ops[:3], None, ops[4], dtype, starts), expected(*ops[:3], None, ops[4], starts), dtype)
+
+
+# lead, inputs, outputs, groups' start indices, relu.  Chosen so that every form of the products over many rows is met: weights that stay in
+# shared memory and that stream, one block and pairs, pieces and whole groups, odd widths, few rows.
+TALL = [
+    ((40003,), 264, 520, None, False), ((40003,), 264, 1032, None, True), ((70001,), 64, 72, None, True), ((30011,), 131, 99, None, True),
+    ((2, 60000), 64, 72, [300, 20011, 20100, 59000], False), ((2, 60000), 136, 72, [300, 20011, 20100, 59000], True),
+    ((3, 15013), 264, 264, [0, 7001, 7001, 7002, 15013], True), ((2, 30011), 33, 50, [11, 20000, 30011], True),
+    ((2, 4099), 1032, 1800, [0, 1000, 2500, 4001], False), ((9001,), 2056, 1032, None, True), ((61,), 264, 520, None, True),
+    ((2, 31), 72, 136, [1, 2, 2, 25], True), ((1,), 1032, 2056, None, True),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", TALL, ids=lambda c: f"{c[0]}-{c[1]}-{c[2]}-{'groups' if c[3] else 'one'}-{'relu' if c[4] else 'none'}")
+def test_every_element_over_many_rows(case, dtype):
+    """All four gradients and the output, element for element: no row is lost, doubled or taken from elsewhere."""
+    lead, K, N, starts, relu = case
+    ops = operands(lead, K, N, None if starts is None else len(starts) - 1, seed=K + N)
+    same(run(*ops, dtype, starts, relu), expected(*ops, starts, relu), dtype)

@@ -70,6 +70,40 @@ def test_counting_waits_waits_for_every_stream():
     assert torch.equal(y, torch.full_like(y, 64))
 
 
+def test_saved_tensor_hooks_see_what_the_backward_needs():
+    """Tensors that hooks pack away and bring back, to the host for instance, give the same gradients."""
+    x, w, b, r, dy = make((2, 150), 40, 56, torch.bfloat16, 3, seed=4)
+    starts = torch.tensor([0, 20, 90], device=DEV)
+
+    def grads():
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
+        y = grouped_linear(leaves[0], leaves[1], starts, leaves[2], leaves[3], "gelu")
+        return torch.autograd.grad(y, leaves, dy)
+
+    want = grads()
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(t.shape) or t.cpu(), lambda t: t.to(DEV)):
+        got = grads()
+    assert sorted(map(len, packed)) == [1, 2, 3, 3]
+    with torch.autograd.graph.save_on_cpu():
+        again = grads()
+    for a, c, e in zip(got, again, want):
+        assert torch.equal(a, e) and torch.equal(c, e)
+
+
+def test_function_transforms_are_refused():
+    """torch.func has no rule for the operators; it says so, and nothing is computed from a wrapper's storage."""
+    x, w, b, _, _ = make((10,), 16, 24, torch.float32)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: fused_linear(t, w, b).sum())(x)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: fused_linear(t, w, b))(x[None].expand(3, 10, 16))
+    with pytest.raises(RuntimeError):
+        torch.func.jacrev(lambda t: fused_linear(t, w, b))(x)
+    y = fused_linear(x, w, b)                     # and the process is as it was
+    assert torch.isfinite(y).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_layers_saved_before_the_level_projections(dtype):
     """A whole layer pickled by an earlier version has no attribute for them."""
@@ -81,3 +115,11 @@ def test_layers_saved_before_the_level_projections(dtype):
     want = layer(src, ref, src, shapes, lsi)
     del layer.__dict__["level_value_proj"]
     assert torch.equal(layer(src, ref, src, shapes, lsi), want)
+
+
+def test_no_wait_runs_out():
+    """The Python name of the count."""
+    import ops3d_b200
+
+    y = fused_linear(torch.ones(5000, 64, device=DEV, dtype=torch.bfloat16), torch.ones(264, 64, device=DEV, dtype=torch.bfloat16))
+    assert ops3d_b200.linear_timeouts() == 0 and torch.equal(y, torch.full_like(y, 64))
