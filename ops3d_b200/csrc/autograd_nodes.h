@@ -46,7 +46,7 @@ inline bool needs_node(std::initializer_list<std::reference_wrapper<const at::Te
     return false;
 }
 
-// Base: two differentiable inputs saved at most, arguments in the derived class.
+// Base: up to four saved inputs, arguments in the derived class.
 struct SavedNode : public torch::autograd::Node {
     std::array<SavedVariable, 4> saved;
     void save(size_t i, const at::Tensor &t) { saved[i] = SavedVariable(t, /*is_output=*/false); }

@@ -227,7 +227,9 @@ __host__ __device__ constexpr uint32_t instruction(int m, int n, bool a_mn_major
 // A tile of 128 x 256 has 256 elements a lane of an SM, and its bytes pass in about 5500 cycles: more than some 20 instructions
 // an element and the epilogue, not memory, sets the pace (erff, expf and a division took 5.7 us a tile forward and 9.4 backward).
 // So: one exp2 and one reciprocal of the special-function unit each, the rest on pairs of elements where the instruction set has
-// the pair's form.  Errors stay below 1e-6 of 1 + |v|, a two-thousandth of the rounding to bf16 that follows.
+// the pair's form.  Errors stay below 1e-6 of 1 + |v|: an absolute bound, as 1 + erf(v) in fp32 has one.  In gelu's negative tail, where the
+// value itself is small, that can be more than a rounding of it (0.16 % of the value at -5, 0.36 % at -6, 3 % of the 5e-15 at -8; bf16's
+// half step is up to 0.39 %).
 struct Pair {
     unsigned long long bits;
     __device__ __forceinline__ Pair() {}

@@ -158,7 +158,7 @@ __device__ __forceinline__ void finish_columns(const uint32_t (&v)[16], const fl
             r = r + Pair(b.x, b.y);
             if (kMode == kPreGrad) {
                 r = activate_backward_2<kAct>(r, unpack2<T>(row[j]));
-                if (kMode == kPreGrad) r.split(kept[(2 * j) % (sizeof(kept) / 4)], kept[(2 * j + 1) % (sizeof(kept) / 4)]);
+                r.split(kept[(2 * j) % (sizeof(kept) / 4)], kept[(2 * j + 1) % (sizeof(kept) / 4)]);
             } else {
                 r = activate_2<kAct>(r);
                 if (kMode == kForward) r = r + unpack2<T>(row[j]);

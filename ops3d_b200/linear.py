@@ -17,7 +17,7 @@ Activations: ``"none"``, ``"relu"``, ``"gelu"`` (``v Phi(v)``), ``"gelu_tanh"``,
 float32, float16 or bfloat16 -- of any sizes and strides (an operand that is not contiguous is copied).  Sums are kept in
 fp32 and rounded once.  Nothing but the inputs is kept for the backward, which computes ``x @ weight^T + bias`` again where
 the activation's derivative needs it; beyond 64 rows ``grad_output * act'`` is rounded to the inputs' dtype between the backward's
-products.  The results of repeated calls are equal bit for bit.  Up to 1024 groups, 2^31 - 1 rows and 2^26 - 1 features.
+products (not in the sums for the bias).  The results of repeated calls are equal bit for bit.  Up to 1024 groups, 2^31 - 1 rows and 2^26 - 1 features.
 ``gelu`` is 0 at minus infinity.
 
 Under ``torch.autocast("cuda")`` x, weight and bias are taken in autocast's dtype, as torch's own linear layers take them.  A residual of

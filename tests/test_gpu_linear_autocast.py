@@ -136,3 +136,36 @@ def test_functions_under_autocast():
             assert fused_linear(x, w, b, r).dtype == torch.float32
     with torch.autocast("cuda", torch.float16):   # tensors of the other 16-bit type too, as torch's own layers
         assert torch.equal(fused_linear(low[0], w, low[2]), fused_linear(low[0].half(), w.half(), low[2].half()))
+
+
+def test_captured_and_recomputed_under_autocast():
+    """One graph of a training pass from an fp32 stream, whose inputs change between replays, and the same pass inside a checkpoint."""
+    from torch.utils.checkpoint import checkpoint
+
+    torch.manual_seed(4)
+    ff = FeedForward(40, 72, "silu", 3).to(DEV)
+    starts = torch.tensor([0, 50, 130], device=DEV)
+    x, dy = torch.randn(2, 200, 40, device=DEV, requires_grad=True), torch.randn(2, 200, 40, device=DEV)
+    leaves = [x, *ff.parameters()]
+
+    def step(recompute=False):
+        with torch.autocast("cuda", torch.bfloat16):
+            y = checkpoint(ff, x, starts, use_reentrant=False) if recompute else ff(x, starts)
+        return (y, *torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for boundaries in ([0, 50, 130], [10, 10, 200], [0, 0, 0]):
+        with torch.no_grad():
+            starts.copy_(torch.tensor(boundaries))
+            x.copy_(torch.randn(2, 200, 40))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e, r in zip(out, step(), step(recompute=True)):
+            assert a.dtype == torch.float32 and torch.equal(a, e) and torch.equal(r, e)

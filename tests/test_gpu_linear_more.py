@@ -61,9 +61,12 @@ def test_bias_gradient_is_rounded_once_at_every_width(groups, M, K, N, dtype):
 def test_counting_waits_waits_for_every_stream():
     """The count is asked for when nothing runs any more, on streams too that do not wait for the default one."""
     side = torch.cuda.Stream()
+    x, w = (torch.ones(n, 64, device=DEV, dtype=torch.bfloat16) for n in (300, 64))
+    fused_linear(x, w)              # what a first call loads is loaded
+    torch.cuda.synchronize()
     with torch.cuda.stream(side):
         torch.cuda._sleep(400_000_000)
-        y = fused_linear(torch.ones(300, 64, device=DEV, dtype=torch.bfloat16), torch.ones(64, 64, device=DEV, dtype=torch.bfloat16))
+        y = fused_linear(x, w)
     assert not side.query()
     assert capi.load().fda_linear_timeouts() == 0
     assert side.query()
