@@ -43,7 +43,8 @@ __device__ __forceinline__ void copy_slice(float (*dst)[kPitch], const float *a,
 // acc += A B over k in [0, depth); A is 64 x depth, B depth x 64.  A thread owns rows 4 ty .., columns 4 tx ..; with kSumA
 // also sums = its rows of A added over k.  Every thread of the block takes part; the slices are free again at the end.
 // Sums of 128 terms are made by themselves and then added: one chain over all of a long contraction is off by several times
-// as much (a bias's gradient over 46567 rows by 1.5e-6 of its size).
+// as much (a bias's gradient over 46567 rows by 1.5e-6 of its size).  Rows of A, which no product's rounding hides behind, are added
+// slice by slice, 16 terms at a time, and the slices of a call by themselves.
 constexpr int kChainSlices = 8;
 
 template <bool kAK, bool kBK, bool kSumA>
@@ -58,7 +59,7 @@ __device__ __forceinline__ void tile_product(float (&acc)[kOwn][kOwn], float (&s
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    float part[kOwn][kOwn] = {}, part_sums[kOwn] = {};
+    float part[kOwn][kOwn] = {}, slice_sums[kOwn] = {};
 #pragma unroll
     for (int i = 0; i < kAhead - 1; ++i) copy(i);
     for (int i = 0; i < slices; ++i) {
@@ -66,24 +67,24 @@ __device__ __forceinline__ void tile_product(float (&acc)[kOwn][kOwn], float (&s
         __syncthreads();  // slice i has arrived for every thread, and every thread is done with the one that is overwritten next
         copy(i + kAhead - 1);
         const float(*sa)[kPitch] = s.a[i % kAhead], (*sb)[kPitch] = s.b[i % kAhead];
+        float slice_sum[kOwn] = {};
 #pragma unroll
         for (int k = 0; k < kSlice; ++k) {
             const float4 qa = *reinterpret_cast<const float4 *>(&sa[k][kOwn * ty]), qb = *reinterpret_cast<const float4 *>(&sb[k][kOwn * tx]);
             const float ra[kOwn] = {qa.x, qa.y, qa.z, qa.w}, rb[kOwn] = {qb.x, qb.y, qb.z, qb.w};
 #pragma unroll
             for (int r = 0; r < kOwn; ++r) {
-                if (kSumA) part_sums[r] += ra[r];
+                if (kSumA) slice_sum[r] += ra[r];
 #pragma unroll
                 for (int c = 0; c < kOwn; ++c) part[r][c] = fmaf(ra[r], rb[c], part[r][c]);
             }
         }
+        if (kSumA)
+#pragma unroll
+            for (int r = 0; r < kOwn; ++r) slice_sums[r] += slice_sum[r];
         if (i % kChainSlices == kChainSlices - 1 || i + 1 == slices) {
 #pragma unroll
             for (int r = 0; r < kOwn; ++r) {
-                if (kSumA) {
-                    sums[r] += part_sums[r];
-                    part_sums[r] = 0.f;
-                }
 #pragma unroll
                 for (int c = 0; c < kOwn; ++c) {
                     acc[r][c] += part[r][c];
@@ -92,6 +93,9 @@ __device__ __forceinline__ void tile_product(float (&acc)[kOwn][kOwn], float (&s
             }
         }
     }
+    if (kSumA)
+#pragma unroll
+        for (int r = 0; r < kOwn; ++r) sums[r] += slice_sums[r];
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
 }

@@ -126,3 +126,16 @@ def test_no_wait_runs_out():
 
     y = fused_linear(torch.ones(5000, 64, device=DEV, dtype=torch.bfloat16), torch.ones(264, 64, device=DEV, dtype=torch.bfloat16))
     assert ops3d_b200.linear_timeouts() == 0 and torch.equal(y, torch.full_like(y, 64))
+
+
+def test_fp32_bias_gradient_adds_in_short_chains():
+    """A one every 128 rows and terms that a sum of one swallows between them.  fp32 sums over 16 rows, 16 of these, and one addition: off by
+    at most 33 roundings, 2^-24 each, of the sum of the magnitudes.  (A chain of 128 loses 127 terms of 2^-25 for every one: 64 such units.)"""
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    dy = torch.full((256, 70), 2.0 ** -25, device=DEV)
+    dy[::128] = 1
+    x, w = torch.randn(256, 8, generator=gen, device=DEV), torch.randn(70, 8, generator=gen, device=DEV)
+    b = torch.zeros(70, device=DEV, requires_grad=True)
+    (g,) = torch.autograd.grad(fused_linear(x, w, b), b, dy)
+    value = dy.double().sum(0)
+    assert ((g.double() - value).abs() <= 33 * 2.0 ** -24 * value + 2.0 ** -24 * value).all()
