@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) linear_few_weight_grad_kernel(const 
 }
 
 // The bias's gradient from the sums over 32 rows that the pre-activation's gradient left behind (MmaRows::sums): a block takes 32 outputs
-// of a group, its warps every 32nd of the sums, and adds the warps' in order.
+// of a group, its warps every 32nd of an element's sums, or of the elements where there are more, and adds the warps' in order.
 constexpr int kBiasWarps = 32;
 
 template <typename T>
@@ -360,13 +360,20 @@ __global__ void __launch_bounds__(32 * kBiasWarps) linear_bias_sum_kernel(const 
     for (long long item = blockIdx.x; item < (long long)g.groups * steps; item += gridDim.x) {
         const int e = (int)(item / steps), c = (int)(item % steps) * 32 + lane;
         const int each = (table.start[e + 1] - table.start[e] + kSumRows - 1) / kSumRows;  // sums of one batch element
+        const size_t apart = (size_t)table.unit_begin[g.groups + 2] * subs;                // of two elements' sums
+        const float *const first = sums + (size_t)table.unit_begin[e + 1] * subs * cols + c;
         float sum = 0.f;
-        if (c < cols)
-            for (int b = 0; b < g.batch; ++b) {
-                const size_t first = ((size_t)b * table.unit_begin[g.groups + 2] + table.unit_begin[e + 1]) * subs;
+        if (c < cols) {
+            if (each >= kBiasWarps || each >= g.batch) {
+                for (int b = 0; b < g.batch; ++b)
 #pragma unroll 8
-                for (int k = warp; k < each; k += kBiasWarps) sum += sums[(first + k) * cols + c];
+                    for (int k = warp; k < each; k += kBiasWarps) sum += first[(b * apart + k) * cols];
+            } else {  // (one element after the other leaves most warps idle: 512 elements of 3 groups 300 us more)
+#pragma unroll 1
+                for (int b = warp; b < g.batch; b += kBiasWarps)
+                    for (int k = 0; k < each; ++k) sum += first[(b * apart + k) * cols];
             }
+        }
         partial[warp][lane] = sum;
         __syncthreads();
         if (warp == 0 && c < cols) {

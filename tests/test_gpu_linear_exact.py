@@ -135,7 +135,7 @@ TALL = [
     ((2, 60000), 64, 72, [300, 20011, 20100, 59000], False), ((2, 60000), 136, 72, [300, 20011, 20100, 59000], True),
     ((3, 15013), 264, 264, [0, 7001, 7001, 7002, 15013], True), ((2, 30011), 33, 50, [11, 20000, 30011], True),
     ((2, 4099), 1032, 1800, [0, 1000, 2500, 4001], False), ((9001,), 2056, 1032, None, True), ((61,), 264, 520, None, True),
-    ((2, 31), 72, 136, [1, 2, 2, 25], True), ((1,), 1032, 2056, None, True),
+    ((700, 50), 72, 1032, [3, 20, 21, 47], True), ((3000, 9), 40, 264, [0, 4, 4, 9], True), ((2, 31), 72, 136, [1, 2, 2, 25], True), ((1,), 1032, 2056, None, True),
 ]
 
 
