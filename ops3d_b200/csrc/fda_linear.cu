@@ -359,8 +359,8 @@ __global__ void __launch_bounds__(32 * kBiasWarps) linear_bias_sum_kernel(const 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, steps = (cols + 31) / 32, subs = unit / kSumRows;
     for (long long item = blockIdx.x; item < (long long)g.groups * steps; item += gridDim.x) {
         const int e = (int)(item / steps), c = (int)(item % steps) * 32 + lane;
-        const int each = (table.start[e + 1] - table.start[e] + kSumRows - 1) / kSumRows;  // sums of one batch element
-        const size_t apart = (size_t)table.unit_begin[g.groups + 2] * subs;                // of two elements' sums
+        const int each = (int)(((long long)(table.start[e + 1] - table.start[e]) + kSumRows - 1) / kSumRows);  // sums of one batch element
+        const size_t apart = (size_t)table.unit_begin[g.groups + 2] * subs;                                    // of two elements' sums
         const float *const first = sums + (size_t)table.unit_begin[e + 1] * subs * cols + c;
         float sum = 0.f;
         if (c < cols) {

@@ -146,3 +146,24 @@ def test_every_element_over_many_rows(case, dtype):
     lead, K, N, starts, relu = case
     ops = operands(lead, K, N, None if starts is None else len(starts) - 1, seed=K + N)
     same(run(*ops, dtype, starts, relu), expected(*ops, starts, relu), dtype)
+
+
+def test_as_many_rows_as_there_may_be():
+    """2^31 - 1 rows of one feature: a count of them that is rounded up passes 31 bits.  Rows that matter lie at both ends."""
+    M, dtype = 2 ** 31 - 1, torch.bfloat16
+    x, dy = torch.zeros(M, 1, dtype=dtype, device=DEV), torch.zeros(M, 1, dtype=dtype, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    ends = [slice(0, 300), slice(M - 300, M)]
+    for rows in ends:
+        x[rows], dy[rows] = whole(gen, 300, 1).to(dtype), whole(gen, 300, 1).to(dtype)
+    w, b = torch.full((1, 1), 2.0, dtype=dtype, device=DEV), torch.ones(1, dtype=dtype, device=DEV)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = fused_linear(*leaves, activation="relu")
+    gx, gw, gb = torch.autograd.grad(y, leaves, dy)
+    assert (y[300:M - 300] == 1).all() and not gx[300:M - 300].any()
+    xe, ge = (torch.cat([t.detach()[rows].double() for rows in ends]) for t in (x, dy))
+    pre = 2 * xe + 1
+    ge = ge * (pre > 0)
+    assert torch.equal(torch.cat([y[rows] for rows in ends]).double(), pre.clamp_min(0))
+    assert torch.equal(torch.cat([gx[rows] for rows in ends]).double(), 2 * ge)
+    assert gw.item() == (ge * xe).sum().to(dtype).item() and gb.item() == ge.sum().to(dtype).item()
