@@ -55,7 +55,8 @@ typedef enum fda_status {
     FDA_ERR_MISALIGNED = 9,       /* a tensor base address is not 16-byte aligned */
     FDA_ERR_CUDA = 10,            /* a CUDA runtime call or the kernel launch failed; see fda_last_cuda_error() */
     FDA_ERR_TOO_LARGE_STATIC = 11, /* problem exceeds a compiled-in capacity */
-    FDA_ERR_BAD_ACTIVATION = 12   /* unknown activation */
+    FDA_ERR_BAD_ACTIVATION = 12,  /* unknown activation */
+    FDA_ERR_BAD_SCORE = 13        /* unknown score of experts or of their groups */
 } fda_status_t;
 
 /* Human-readable name of a status code (static storage, never NULL). */
@@ -476,6 +477,76 @@ int fda_linear_backward(const void *x, const void *weight, const void *bias, con
                         void *workspace, size_t workspace_bytes, int batch, int rows, int groups, int in_features,
                         int out_features, int activation, int dtype, void *stream);
 int fda_linear_timeouts(void);
+
+/*
+ * Layer norm of a residual sum, per row of `features` elements:
+ *   s = x + residual,   y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias      (var: mean of the squared deviations)
+ * x, y, grad_y, grad_x of `dtype`; weight, bias and their gradients of `param_dtype`, which is `dtype` or f32; residual, sum,
+ * grad_sum, grad_residual of `residual_dtype`, which is `dtype` or f32.  weight, bias and residual may each be NULL (1, 0, 0); sum
+ * (written where not NULL) and grad_sum (the gradient that reaches the sum from elsewhere) need a residual.  Any width of 1 .. 2^26 - 1,
+ * rows < 2^31; the rows' tensors start on 16-byte boundaries (FDA_ERR_MISALIGNED), the parameters anywhere.  fp32 inside, each
+ * output rounded once.  The gradient of the sum is grad_x, and grad_residual where it is wanted in the residual's type.  grad_x,
+ * grad_residual, grad_weight, grad_bias may each be NULL.  Parameter gradients are added in a fixed order: repeated calls give the
+ * same bits.  The workspace (256-byte aligned) holds partial sums of one call.  No counterpart in the reference.
+ */
+int fda_layer_norm_forward(const void *x, const void *weight, const void *bias, const void *residual, void *y, void *sum,
+                           long long rows, int features, float eps, int dtype, int param_dtype, int residual_dtype,
+                           void *stream);
+size_t fda_layer_norm_backward_workspace_bytes(long long rows, int features, int dtype);
+int fda_layer_norm_backward(const void *x, const void *weight, const void *residual, const void *grad_y, const void *grad_sum,
+                            void *grad_x, void *grad_residual, void *grad_weight, void *grad_bias, void *workspace,
+                            size_t workspace_bytes, long long rows, int features, float eps, int dtype, int param_dtype,
+                            int residual_dtype, void *stream);
+
+/*
+ * Routing of tokens to experts.  Per token, from logits [n_experts] of `dtype`:
+ *   score = softmax(logits) or sigmoid(logits);  select = score + bias   (bias [n_experts] fp32 or NULL: chooses, but does not weigh)
+ *   the experts are n_groups runs of n_experts / n_groups; only those of the top_groups best groups are candidates, a group being worth
+ *   its largest select (FDA_GROUP_MAX) or the sum of its two largest (FDA_GROUP_TOP2)
+ *   experts [top_k] int64: the candidates with the largest select, in descending order
+ *   weights [top_k] fp32: scale * score / (sum of the chosen scores) with renormalise, else scale * score
+ * Ties go to the lower index.  Choices are those of exact scores: where fp32 cannot tell two apart they are computed in 64 bits.  NaN
+ * compares as minus infinity and stays NaN in the weights; renormalised softmax weights are the softmax over the chosen logits; scores
+ * that are all 0 (every logit minus infinity) give weights of 0.  n_experts <= 1024, top_k <= 32, n_groups <= 32
+ * (FDA_ERR_TOO_LARGE_STATIC); top_k <= candidates.
+ * Backward: grad_logits [tokens][n_experts] of `dtype` from the gradient of the weights; `experts` is the forward's (an index outside
+ * 0 .. n_experts - 1 gets no gradient).  The choice itself has none.  No counterpart in the reference.
+ */
+#define FDA_SCORE_SOFTMAX 0
+#define FDA_SCORE_SIGMOID 1
+#define FDA_GROUP_MAX 0
+#define FDA_GROUP_TOP2 1
+int fda_route_forward(const void *logits, const float *bias, float *weights, int64_t *experts, long long tokens, int n_experts,
+                      int top_k, int score, int n_groups, int top_groups, int group_score, int renormalise, float scale,
+                      int dtype, void *stream);
+int fda_route_backward(const void *logits, const int64_t *experts, const float *grad_weights, void *grad_logits,
+                       long long tokens, int n_experts, int top_k, int score, int renormalise, float scale, int dtype,
+                       void *stream);
+
+/*
+ * Rows sorted by expert, in the form that fda_linear_forward takes groups of rows, and back.  experts [tokens][top_k] int64; an
+ * entry outside 0 .. n_experts - 1 (a padded token's) belongs to no expert.
+ *   group_start_index [n_experts + 1] int64: first row of each expert, and the end of the last one's
+ *   position [tokens][top_k] int64: the row of each entry, in the entries' order within an expert; -1 for none
+ *   fda_dispatch_rows: rows [tokens * top_k][features]: rows[position] = x[token]; rows behind the last expert's are 0
+ *   fda_combine_rows:  y[token] = sum over its entries of weight * rows[position] + residual
+ *                      weights [tokens][top_k] of `weight_dtype` or NULL (1), residual [tokens][features] or NULL
+ * fda_combine_rows without weights is the gradient of fda_dispatch_rows.  fda_combine_rows_backward: grad_rows[position] = weight *
+ * grad_y[token] (0 in rows from *rows_end on, which is group_start_index + n_experts), grad_weights = <rows[position], grad_y[token]>,
+ * 0 where there is no row; either may be NULL.  `position` and `rows_end` are those of fda_dispatch_rows: no entry leads out of `rows`
+ * whatever they hold, but entries that share a row leave one of their gradients in it.
+ * x, rows, residual, y and their gradients of `dtype`, on 16-byte boundaries; sums in fp32, one rounding.  tokens * top_k < 2^31,
+ * top_k <= 32, n_experts <= 1024, features < 2^26.  No counterpart in the reference.
+ */
+size_t fda_dispatch_workspace_bytes(long long tokens, int top_k, int n_experts);
+int fda_dispatch_rows(const void *x, const int64_t *experts, void *rows, int64_t *group_start_index, int64_t *position,
+                      void *workspace, size_t workspace_bytes, long long tokens, int top_k, int n_experts, int features,
+                      int dtype, void *stream);
+int fda_combine_rows(const void *rows, const int64_t *position, const void *weights, const void *residual, void *y,
+                     long long tokens, int top_k, int features, int dtype, int weight_dtype, void *stream);
+int fda_combine_rows_backward(const void *rows, const int64_t *position, const int64_t *rows_end, const void *weights,
+                              const void *grad_y, void *grad_rows, void *grad_weights, long long tokens, int top_k,
+                              int features, int dtype, int weight_dtype, void *stream);
 
 /*
  * Backward pass that needs no workspace from the caller and allocates nothing: same inputs,

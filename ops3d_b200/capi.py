@@ -25,6 +25,8 @@ EXPORTS = (
     "fda_backward_touched_rows", "fda_cast_grad_value_touched",
     "fda_linear_forward_workspace_bytes", "fda_linear_forward", "fda_linear_backward_workspace_bytes", "fda_linear_backward",
     "fda_linear_timeouts",
+    "fda_layer_norm_forward", "fda_layer_norm_backward_workspace_bytes", "fda_layer_norm_backward", "fda_route_forward", "fda_route_backward",
+    "fda_dispatch_workspace_bytes", "fda_dispatch_rows", "fda_combine_rows", "fda_combine_rows_backward",
 )
 BWD_ZERO_IMAGE, BWD_RESUME, BWD_FINALIZE, BWD_BINNED_DONE, BWD_ZERO_TOUCHED = 1, 2, 4, 8, 16
 NOALLOC_MAX_ELEMENTS = 16 * 1024 * 1024
@@ -131,6 +133,16 @@ def load() -> ctypes.CDLL:
     lib.fda_linear_backward_workspace_bytes.argtypes, lib.fda_linear_backward_workspace_bytes.restype = [i] * 7, sz
     lib.fda_linear_backward.argtypes, lib.fda_linear_backward.restype = [vp] * 5 + [i] + [vp] * 4 + [sz] + [i] * 7 + [vp], i
     lib.fda_linear_timeouts.argtypes, lib.fda_linear_timeouts.restype = [], i
+    ll, f = ctypes.c_longlong, ctypes.c_float
+    lib.fda_layer_norm_forward.argtypes, lib.fda_layer_norm_forward.restype = [vp] * 6 + [ll, i, f] + [i] * 3 + [vp], i
+    lib.fda_layer_norm_backward_workspace_bytes.argtypes, lib.fda_layer_norm_backward_workspace_bytes.restype = [ll, i, i], sz
+    lib.fda_layer_norm_backward.argtypes, lib.fda_layer_norm_backward.restype = [vp] * 10 + [sz, ll, i, f] + [i] * 3 + [vp], i
+    lib.fda_route_forward.argtypes, lib.fda_route_forward.restype = [vp] * 4 + [ll] + [i] * 7 + [f, i, vp], i
+    lib.fda_route_backward.argtypes, lib.fda_route_backward.restype = [vp] * 4 + [ll] + [i] * 4 + [f, i, vp], i
+    lib.fda_dispatch_workspace_bytes.argtypes, lib.fda_dispatch_workspace_bytes.restype = [ll, i, i], sz
+    lib.fda_dispatch_rows.argtypes, lib.fda_dispatch_rows.restype = [vp] * 6 + [sz, ll] + [i] * 4 + [vp], i
+    lib.fda_combine_rows.argtypes, lib.fda_combine_rows.restype = [vp] * 5 + [ll] + [i] * 4 + [vp], i
+    lib.fda_combine_rows_backward.argtypes, lib.fda_combine_rows_backward.restype = [vp] * 7 + [ll] + [i] * 4 + [vp], i
     _lib = lib
     return lib
 

@@ -10,7 +10,8 @@
 // csrc/cuda/flash_deform_attn_cuda.cu:20-179: RuntimeError for CPU / non-contiguous tensors and
 // for batch % min(batch, im2col_step) != 0, ValueError for an unsupported level or point count.
 // linear_forward / linear_backward are the linear layers with a fused epilogue (ops3d_b200/linear.py has the arguments).
-// flash_deform_attn, dcnv4, roi_align_3d and linear are the differentiable forms (autograd_nodes.h), what the Python Functions call.
+// layer_norm, route, dispatch and combine are in binding_experts.h (ops3d_b200/norm.py, ops3d_b200/experts.py).
+// flash_deform_attn, dcnv4, roi_align_3d, linear, layer_norm, route, dispatch and combine are the differentiable forms (autograd_nodes.h), what the Python Functions call.
 // This file only checks tensors, allocates outputs from torch's allocator, and forwards raw
 // pointers plus the current CUDA stream; all arithmetic lives behind the C ABI.
 #include <torch/extension.h>
@@ -597,6 +598,8 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &weight, const OptionalT
     return y;
 }
 
+#include "binding_experts.h"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -610,6 +613,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear_forward", &linear_forward, "linear layer with fused epilogue, forward (sm_100a)");
     m.def("linear_backward", &linear_backward, "linear layer with fused epilogue, backward (sm_100a)");
     m.def("linear_timeouts", &linear_timeouts, "waits of the linear layers' kernels that ran out on the current device");
+    m.def("layer_norm", &layer_norm, "differentiable layer norm of a residual sum");
+    m.def("layer_norm_forward", &layer_norm_forward, "layer norm of a residual sum, forward (sm_100a)");
+    m.def("layer_norm_backward", &layer_norm_backward, "layer norm of a residual sum, backward (sm_100a)");
+    m.def("route", &route, "differentiable routing of tokens to experts");
+    m.def("route_forward", &route_forward, "routing of tokens to experts, forward (sm_100a)");
+    m.def("route_backward", &route_backward, "routing of tokens to experts, backward (sm_100a)");
+    m.def("dispatch", &dispatch, "differentiable rows sorted by expert");
+    m.def("dispatch_forward", &dispatch_forward, "rows sorted by expert (sm_100a)");
+    m.def("combine", &combine, "differentiable weighted sums of rows sorted by expert");
+    m.def("combine_forward", &combine_forward, "weighted sums of rows sorted by expert, forward (sm_100a)");
+    m.def("combine_backward", &combine_backward, "weighted sums of rows sorted by expert, backward (sm_100a)");
     m.def("nms_3d", &nms_3d, "non-maximum suppression for 3d boxes (sm_100a)");
     m.def("roi_align_3d_forward", &roi_align_3d_forward, "ROI-Align 3D forward (sm_100a)");
     m.def("roi_align_3d_backward", &roi_align_3d_backward, "ROI-Align 3D backward (sm_100a)");

@@ -553,6 +553,7 @@ const char *fda_status_string(int status) {
         case FDA_ERR_CUDA: return "CUDA runtime error";
         case FDA_ERR_TOO_LARGE_STATIC: return "problem exceeds a compiled-in capacity";
         case FDA_ERR_BAD_ACTIVATION: return "unknown activation";
+        case FDA_ERR_BAD_SCORE: return "unknown score of experts or of their groups";
         default: return "unknown status";
     }
 }

@@ -1,0 +1,151 @@
+// Row access shared by the kernels around the linear operators (layer norm, routing to experts, rows sorted by expert): 16-byte
+// vectors in the tensors' type, values in fp32, sums over the lanes that share a row.
+#pragma once
+
+#include "fda_linear.cuh"
+
+namespace fda {
+void record_cuda_error(int e);  // fda_api.cu
+}
+
+namespace fda_rows {
+
+using fda_linear::ceil_div;
+using fda_linear::from_f32;
+using fda_linear::kSms;
+using fda_linear::launch_early;
+using fda_linear::to_f32;
+using fda_linear::wait_for_previous_kernel;
+
+inline int launched(cudaError_t e) {
+    if (e == cudaSuccess) return FDA_OK;
+    fda::record_cuda_error((int)e);
+    return FDA_ERR_CUDA;
+}
+
+inline size_t type_size(int dtype) { return dtype == FDA_DTYPE_F32 ? 4 : 2; }
+inline bool known_dtype(int dtype) { return dtype >= FDA_DTYPE_F32 && dtype <= FDA_DTYPE_BF16; }
+inline bool misaligned16(const void *p) { return (uintptr_t)p % 16 != 0; }
+
+// Two 16-bit numbers of a word, the lower one first.
+template <typename T> __device__ __forceinline__ void unpack(unsigned u, float &a, float &b);
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(unsigned u, float &a, float &b) {
+    a = __uint_as_float(u << 16);
+    b = __uint_as_float(u & 0xffff0000u);
+}
+template <> __device__ __forceinline__ void unpack<__half>(unsigned u, float &a, float &b) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u));
+    a = f.x;
+    b = f.y;
+}
+template <typename T> __device__ __forceinline__ unsigned pack(float a, float b);
+template <> __device__ __forceinline__ unsigned pack<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&v);
+}
+template <> __device__ __forceinline__ unsigned pack<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&v);
+}
+
+// kWidth neighbouring elements as they lie in memory: 16 or 32 bytes.
+template <typename T, int kWidth>
+struct Raw {
+    static constexpr int kUnits = kWidth * (int)sizeof(T) / 16;
+    uint4 u[kUnits];
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) u[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) u[i] = reinterpret_cast<const uint4 *>(p)[i];
+    }
+    __device__ __forceinline__ void store(T *p) const {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) reinterpret_cast<uint4 *>(p)[i] = u[i];
+    }
+    __device__ __forceinline__ void get(float *v) const {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const unsigned w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(T) == 4) v[4 * i + j] = __uint_as_float(w[j]);
+                else unpack<T>(w[j], v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
+            }
+        }
+    }
+    __device__ __forceinline__ void set(const float *v) {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            unsigned w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(v[4 * i + j]);
+                else w[j] = pack<T>(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
+            }
+            u[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+};
+
+// A parameter of either type, as fp32.
+__device__ __forceinline__ float load_as_f32(const void *p, int dtype, size_t i) {
+    if (dtype == FDA_DTYPE_F32) return static_cast<const float *>(p)[i];
+    if (dtype == FDA_DTYPE_F16) return __half2float(static_cast<const __half *>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+__device__ __forceinline__ void store_from_f32(void *p, int dtype, size_t i, float v) {
+    if (dtype == FDA_DTYPE_F32) static_cast<float *>(p)[i] = v;
+    else if (dtype == FDA_DTYPE_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
+
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int d = kLanes / 2; d > 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+
+// The threads that share a row: kLanes lanes of a warp, or (0) the block.  sum() leaves the same numbers in all of them.
+template <int kLanes>
+struct Team {
+    __device__ __forceinline__ int lane() const { return threadIdx.x % kLanes; }
+    __device__ __forceinline__ int size() const { return kLanes; }
+    template <int kCount>
+    __device__ __forceinline__ void sum(float (&v)[kCount]) {
+#pragma unroll
+        for (int k = 0; k < kCount; ++k) v[k] = lanes_sum<kLanes>(v[k]);
+    }
+};
+template <>
+struct Team<0> {
+    static constexpr int kMost = 3, kWarps = 16;
+    float (*shared)[kMost][kWarps];  // [2]: a buffer is written again only after everyone has passed the barrier behind the other
+    int buffer = 0;
+    __device__ __forceinline__ int lane() const { return threadIdx.x; }
+    __device__ __forceinline__ int size() const { return blockDim.x; }
+    template <int kCount>
+    __device__ __forceinline__ void sum(float (&v)[kCount]) {
+        static_assert(kCount <= kMost, "");
+        const int warps = blockDim.x / 32;
+#pragma unroll
+        for (int k = 0; k < kCount; ++k) {
+            v[k] = lanes_sum<32>(v[k]);
+            if (threadIdx.x % 32 == 0) shared[buffer][k][threadIdx.x / 32] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kCount; ++k) {
+            float s = shared[buffer][k][0];
+            for (int w = 1; w < warps; ++w) s += shared[buffer][k][w];
+            v[k] = s;
+        }
+        buffer ^= 1;
+    }
+};
+
+}  // namespace fda_rows
