@@ -5,11 +5,14 @@
 //     experts; a group is worth its largest select, or the sum of its two largest); ties go to the lower index
 //     weight_j = scale * score_j / sum of the chosen scores, or scale * score_j
 //
-// A warp takes a token, a lane kPer neighbouring experts, so that of equal values the lowest lane's comes first.  What is chosen is what
-// exact scores choose.  Where select is a monotone function of one logit (no bias, no sum over a group) the logits themselves are
-// compared.  Elsewhere scores in fp32 are compared as long as their distance is beyond what they can be off by; a token for
-// which it is not is decided by scores in 64 bits, so that no choice depends on how an exponential rounds.  A NaN counts as minus
-// infinity in comparisons, and stays one in the weights.
+// What is chosen is what exact scores choose.  Where select is a monotone function of one logit (no bias, no sum over a group) the
+// logits themselves are compared.  Elsewhere scores in fp32 are compared as long as their distance is beyond what they can be off by;
+// a token for which it is not is decided by scores in 64 bits, so that no choice depends on how an exponential rounds.  A NaN
+// counts as minus infinity in comparisons, and stays one in the weights.
+//
+// kLanes (8, or 16 beyond 512 experts) lanes take a token, so that a warp's instructions serve four.  A lane holds octets of
+// neighbouring experts, octet o of the token belonging to lane o mod kLanes.  Their values lie in shared memory, their largest in a
+// register: a step of the choice takes the largest of these over the lanes, and only the lane that has it looks into its octet again.
 #include "fda_rows.cuh"
 
 #include <algorithm>
@@ -19,7 +22,7 @@ namespace {
 using namespace fda_rows;
 
 constexpr unsigned kAll = 0xffffffffu;
-constexpr int kThreads = 256;
+constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kMostExperts = 1024, kMostChoices = 32, kMostExpertGroups = 32;
 
 struct RouteArgs {
@@ -35,17 +38,11 @@ struct RouteArgs {
 };
 
 // Numbers in the order of unsigned integers, all above 0; -0 as 0, NaN as minus infinity.
-__device__ __forceinline__ unsigned order_of(float v) {
-    if (!(v == v)) v = -INFINITY;
-    const unsigned u = __float_as_uint(v + 0.f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
 __device__ __forceinline__ unsigned long long order_of(double v) {
     if (!(v == v)) v = -INFINITY;
     const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
     return u >> 63 ? ~u : u | 1ull << 63;
 }
-__device__ __forceinline__ unsigned warp_max(unsigned v) { return __reduce_max_sync(kAll, v); }
 __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) {
@@ -54,272 +51,444 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
     }
     return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
+template <int kLanes>
+__device__ __forceinline__ float most(float v) {  // NaN only where every lane has one
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2) v = fmaxf(v, __shfl_xor_sync(kAll, v, d));
+    for (int d = kLanes / 2; d > 0; d /= 2) v = fmaxf(v, __shfl_xor_sync(kAll, v, d));
     return v;
 }
-template <typename F>
-__device__ __forceinline__ F warp_sum(F v) {
+template <int kLanes>
+__device__ __forceinline__ int least(int v) {
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(kAll, v, d);
+    for (int d = kLanes / 2; d > 0; d /= 2) v = min(v, __shfl_xor_sync(kAll, v, d));
+    return v;
+}
+template <int kLanes, typename F>
+__device__ __forceinline__ F total(F v) {
+#pragma unroll
+    for (int d = kLanes / 2; d > 0; d /= 2) v += __shfl_xor_sync(kAll, v, d);
     return v;
 }
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
-// 1 / (1 + e^-v)
-template <typename F>
-__device__ __forceinline__ F sigmoid_of(F v) { return (F)1 / ((F)1 + exp_of(-v)); }
+// e^v for comparisons: off by 2^-24 (1.5 |v| + 4) of itself, 0 below the normal range.
+__device__ __forceinline__ float quick_exp(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.44269504088896341f));
+    return r;
+}
 
-// By how much a score in fp32 can be off, relative to itself: e^(l - max) by the rounding of l - max (2^-24 |l - max|, at most 104 before
-// it is 0) and the exponential (2 units), their sum by kPer + 5 additions, the quotient; 1 / (1 + e^-l) by less.
-constexpr float kScoreError = 1.f / 65536.f;
-// The same for the additions, relative to the larger of two values that are compared: the smaller one, where it is below minus that, is
-// further away than it can be off by.
+// By how much a score in fp32 can be off, relative to the token's largest: for a softmax 2^-24 (1.5 |d| + 4) e^d, d = l - max, is at
+// most 5 * 2^-24; the sum of up to 64 + 4 terms adds 2^-24 * 75 at most, the quotient 3.  For a sigmoid, 2^-24 (1.5 |l| + 8) of itself, which is
+// less than this down to l = -80 and below kSmallest beyond.
+constexpr float kScoreError = 1.f / 131072.f;
+// For the addition of the bias, relative to the larger of two values that are compared: a smaller one that is below minus that is further
+// away than it can be off by.
 constexpr float kSumError = 1.f / 2097152.f;
-constexpr float kSmallest = 1e-37f;           // scores below the normal range have an absolute error
-
-// The top_k experts of a token whose select values are v (float or double): lane j gets the j-th.  allowed: bit i of a lane
-// for its expert i.
-template <typename K, int kPer>
-__device__ __forceinline__ int choose(const K (&key)[kPer], unsigned allowed, int top_k) {
-    const int lane = threadIdx.x % 32;
-    int mine = 0;
-    unsigned left = allowed;
-    for (int j = 0; j < top_k; ++j) {
-        K best = 0;
-        int slot = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if ((left >> i & 1) && key[i] > best) { best = key[i]; slot = i; }
-        const K top = warp_max(best);
-        const int winner = __ffs(__ballot_sync(kAll, best == top)) - 1;
-        if (lane == winner) left &= ~(1u << slot);
-        const int expert = __shfl_sync(kAll, lane * kPer + slot, winner);
-        if (lane == j) mine = expert;
-    }
-    return mine;
-}
-
-// Which experts of a lane are in the top_groups best groups.  values [n_experts]: select values of the token in shared memory.
-// unsure: set where the border between the groups is closer than the values' errors (`error` of one value).
-template <typename F, int kPer>
-__device__ __forceinline__ unsigned allowed_experts(const RouteArgs &p, const F *values, F error, bool &unsure) {
-    const int lane = threadIdx.x % 32, size = p.n_experts / p.n_groups;
-    unsigned experts = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-        if (lane * kPer + i < p.n_experts) experts |= 1u << i;
-    if (p.top_groups == p.n_groups) return experts;
-    // 32 / (a power of two of groups) lanes to a group
-    int share = 32;
-    while (32 / share < p.n_groups) share /= 2;
-    const int group = lane / share;
-    F first = -INFINITY, second = -INFINITY;
-    if (group < p.n_groups)
-        for (int i = lane % share; i < size; i += share) {
-            F v = values[group * size + i];
-            if (!(v == v)) v = -INFINITY;
-            if (v > first) { second = first; first = v; }
-            else if (v > second) second = v;
-        }
-    for (int d = 1; d < share; d *= 2) {
-        const F a = __shfl_xor_sync(kAll, first, d), b = __shfl_xor_sync(kAll, second, d);
-        if (a > first) { second = first > b ? first : b; first = a; }
-        else second = a > second ? a : second;
-    }
-    F worth = p.top2 && size > 1 ? first + second : first;
-    if (!(worth == worth)) worth = -INFINITY;
-    // a group's place: how many are better
-    int place = 0;
-    for (int g = 0; g < p.n_groups; ++g) {
-        const F other = __shfl_sync(kAll, worth, g * share);
-        if (other > worth || (other == worth && g < group)) ++place;
-    }
-    const bool chosen = group < p.n_groups && place < p.top_groups;
-    if (error >= 0) {
-        F low = chosen ? worth : (F)INFINITY, high = group < p.n_groups && !chosen ? worth : -(F)INFINITY;
-        for (int d = 16; d > 0; d /= 2) {
-            const F a = __shfl_xor_sync(kAll, low, d), b = __shfl_xor_sync(kAll, high, d);
-            low = a < low ? a : low;
-            high = b > high ? b : high;
-        }
-        if (!(low - high > error) && low > -(F)INFINITY) unsure = true;
-    }
-    const unsigned groups = __ballot_sync(kAll, chosen && lane % share == 0);
-    unsigned allowed = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-        if ((experts >> i & 1) && (groups >> ((lane * kPer + i) / size * share) & 1)) allowed |= 1u << i;
-    return allowed;
-}
+constexpr float kSmallest = 1e-37f;  // scores below the normal range have an absolute error
 
 template <typename T>
 __device__ __forceinline__ float logit(const RouteArgs &p, long long token, int expert) {
     return to_f32(static_cast<const T *>(p.logits)[token * p.n_experts + expert]);
 }
 
-// Softmax's shift and the inverse of its sum; a row without a finite logit has no score.
-template <typename F, int kPer>
-__device__ __forceinline__ void softmax_of(const float (&l)[kPer], int n_experts, F &shift, F &inverse) {
-    const int lane = threadIdx.x % 32;
-    float top = -INFINITY;
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-        if (lane * kPer + i < n_experts) {
-            top = fmaxf(top, l[i]);
-            nan |= !(l[i] == l[i]);
+// ---- in 64 bits, a warp to a token ---------------------------------------------------------------------------------------------
+// Bit i of a lane: its expert kPer * lane + i is in one of the top_groups best groups.  values: the token's in shared memory.
+template <int kPer>
+__device__ unsigned exactly_allowed(const RouteArgs &p, const double *values) {
+    const int lane = threadIdx.x % 32, size = p.n_experts / p.n_groups;
+    unsigned groups = kAll;
+    if (p.top_groups < p.n_groups) {  // a lane takes a group
+        double first = -INFINITY, second = -INFINITY;
+        if (lane < p.n_groups)
+            for (int i = 0; i < size; ++i) {
+                double v = values[lane * size + i];
+                if (!(v == v)) v = -INFINITY;
+                if (v > first) { second = first; first = v; }
+                else if (v > second) second = v;
+            }
+        double worth = p.top2 && size > 1 ? first + second : first;
+        if (!(worth == worth)) worth = -INFINITY;
+        int better = 0;
+        for (int g = 0; g < p.n_groups; ++g) {
+            const double other = __shfl_sync(kAll, worth, g);
+            if (other > worth || (other == worth && g < lane)) ++better;
         }
-    shift = warp_max(top);
-    if (__any_sync(kAll, nan)) shift = NAN;
-    if (shift == -(F)INFINITY) {
-        shift = 0;
-        inverse = 0;
-        return;
+        groups = __ballot_sync(kAll, lane < p.n_groups && better < p.top_groups);
     }
-    F sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-        if (lane * kPer + i < n_experts) sum += exp_of((F)l[i] - shift);
-    inverse = (F)1 / warp_sum(sum);
-}
-
-// A score as every comparison of a token computes it: no contraction with what follows.
-__device__ __forceinline__ float score_of(const RouteArgs &p, float l, float shift, float inverse) {
-    if (p.sigmoid) return sigmoid_of(l);
-    return inverse == 0.f ? 0.f : __fmul_rn(expf(l - shift), inverse);
-}
-
-// The choice by scores in 64 bits; values: [n_experts] numbers of the warp in shared memory.
-template <typename T, int kPer>
-__device__ __noinline__ int choose_exactly(const RouteArgs &p, long long token, double *values) {
-    const int lane = threadIdx.x % 32;
-    float l[kPer];
-    for (int i = 0; i < kPer; ++i) l[i] = lane * kPer + i < p.n_experts ? logit<T>(p, token, lane * kPer + i) : -INFINITY;
-    double shift = 0, inverse = 1;
-    if (!p.sigmoid) softmax_of<double, kPer>(l, p.n_experts, shift, inverse);
-    unsigned long long key[kPer];
-    __syncwarp();
+    unsigned allowed = 0;
     for (int i = 0; i < kPer; ++i) {
         const int e = lane * kPer + i;
-        if (e >= p.n_experts) { key[i] = 0; continue; }
-        double v = p.sigmoid ? sigmoid_of((double)l[i]) : exp((double)l[i] - shift) * inverse;
+        if (e < p.n_experts && (groups >> (e / size) & 1 || p.top_groups == p.n_groups)) allowed |= 1u << i;
+    }
+    return allowed;
+}
+
+// The choice by scores in 64 bits into chosen[top_k]; values: room for [n_experts] numbers.
+template <typename T, int kPer>
+__device__ __noinline__ void choose_exactly(const RouteArgs &p, long long token, double *values, int *chosen) {
+    const int lane = threadIdx.x % 32;
+    double shift = 0, inverse = 1;
+    if (!p.sigmoid) {
+        float top = -INFINITY;
+        bool nan = false;
+        for (int i = 0; i < kPer; ++i)
+            if (lane * kPer + i < p.n_experts) {
+                const float l = logit<T>(p, token, lane * kPer + i);
+                top = fmaxf(top, l);
+                nan |= !(l == l);
+            }
+        shift = most<32>(top);
+        if (__any_sync(kAll, nan)) shift = NAN;
+        if (shift == -INFINITY) {
+            shift = inverse = 0;
+        } else {
+            double sum = 0;
+            for (int i = 0; i < kPer; ++i)
+                if (lane * kPer + i < p.n_experts) sum += exp((double)logit<T>(p, token, lane * kPer + i) - shift);
+            inverse = 1 / total<32>(sum);
+        }
+    }
+    unsigned long long key[kPer];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = lane * kPer + i;
+        key[i] = 0;
+        if (e >= p.n_experts) continue;
+        const double l = logit<T>(p, token, e);
+        double v = p.sigmoid ? 1 / (1 + exp(-l)) : inverse == 0 ? 0 : exp(l - shift) * inverse;
         if (p.bias) v += (double)p.bias[e];
+        else if (p.top2) key[i] = order_of(l);  // groups by their sums, experts by their logits
         values[e] = v;
-        key[i] = order_of(v);
+        if (p.bias || !p.top2) key[i] = order_of(v);
     }
     __syncwarp();
-    bool unsure = false;
-    return choose<unsigned long long, kPer>(key, allowed_experts<double, kPer>(p, values, -1.0, unsure), p.top_k);
-}
-
-// Score of a chosen expert (lane j's), before scaling, and what the weights are divided by.
-struct Chosen {
-    float score, total;
-};
-template <int kPer>
-__device__ __forceinline__ Chosen chosen_scores(const RouteArgs &p, float logit, float shift, float inverse) {
-    const bool there = (int)(threadIdx.x % 32) < p.top_k;
-    Chosen c;
-    if (p.sigmoid) {
-        c.score = there ? sigmoid_of(logit) : 0.f;
-        c.total = p.renormalise ? warp_sum(c.score) : 1.f;
-    } else if (p.renormalise) {  // softmax over the chosen
-        const float nan = there && !(logit == logit) ? logit : 0.f;
-        const float top = warp_max(there ? logit : -INFINITY);
-        c.score = !there ? 0.f : top == -INFINITY && nan == 0.f ? 0.f : expf(logit - top);
-        c.total = warp_sum(c.score);
-    } else {
-        c.score = there ? (inverse == 0.f ? 0.f : expf(logit - shift) * inverse) : 0.f;
-        c.total = 1.f;
+    unsigned left = exactly_allowed<kPer>(p, values);
+    for (int j = 0; j < p.top_k; ++j) {
+        unsigned long long best = 0;
+        int slot = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if ((left >> i & 1) && key[i] > best) { best = key[i]; slot = i; }
+        const unsigned long long top = warp_max(best);
+        const int winner = __ffs(__ballot_sync(kAll, best == top)) - 1;  // neighbouring experts are a lane's: the lowest lane's come first
+        if (lane != winner) continue;
+        left &= ~(1u << slot);
+        chosen[j] = lane * kPer + slot;
     }
-    return c;
+    __syncwarp();
 }
 
-template <typename T, int kPer>
-__global__ void __launch_bounds__(kThreads) route_forward_kernel(const RouteArgs p) {
-    extern __shared__ double shared[];
-    wait_for_previous_kernel();
-    const int lane = threadIdx.x % 32, E = p.n_experts;
-    double *values64 = shared + (threadIdx.x / 32) * E;
-    float *values = reinterpret_cast<float *>(values64);
-    const bool grouped = p.top_groups < p.n_groups;
-    // what is compared: logits, or scores
-    const bool sums = grouped && p.top2 && E > p.n_groups;
-    const bool by_score = p.bias || sums;
-    const bool need_softmax = !p.sigmoid && (by_score || !p.renormalise);
-    for (long long token = (long long)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; token < p.tokens; token += (long long)gridDim.x * (kThreads / 32)) {
-        float l[kPer];
+// ---- in fp32, kLanes lanes to a token ------------------------------------------------------------------------------------------
+// v[q][i] = the logit of expert (q kLanes + lane) 8 + i; minus infinity beyond the last one.
+template <typename T, int kLanes, int kOctets, bool kVector>
+__device__ __forceinline__ void load_logits(const RouteArgs &p, long long token, int lane, float (&v)[kOctets][8]) {
+    const T *row = static_cast<const T *>(p.logits) + token * p.n_experts;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) l[i] = lane * kPer + i < E ? logit<T>(p, token, lane * kPer + i) : -INFINITY;
-        float shift = 0.f, inverse = 1.f;
-        if (need_softmax) softmax_of<float, kPer>(l, E, shift, inverse);
-        unsigned key[kPer];
-        float v[kPer], score[kPer];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = lane * kPer + i;
-            score[i] = 0.f;
-            v[i] = l[i];
-            if (by_score && e < E) {
-                score[i] = score_of(p, l[i], shift, inverse);
-                v[i] = p.bias ? __fadd_rn(score[i], p.bias[e]) : score[i];
-            }
-            key[i] = e < E ? order_of(p.bias ? v[i] : l[i]) : 0;
-        }
-        bool unsure = false;
-        unsigned allowed = kPer == 32 ? kAll : (1u << kPer) - 1;
-        if (grouped) {
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (lane * kPer + i < E) values[lane * kPer + i] = v[i];
-            __syncwarp();
-            // a group is worth up to two values, and two groups are compared
-            float error = 0.f;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (fabsf(v[i]) < INFINITY) error = fmaxf(error, score[i] * kScoreError + fabsf(v[i]) * kSumError);
-            allowed = allowed_experts<float, kPer>(p, values, by_score ? 4.f * (warp_max(error) + kSmallest) : -1.f, unsure);
+    for (int q = 0; q < kOctets; ++q) {
+        const int first = (q * kLanes + lane) * 8;
+        if (kVector && first < p.n_experts) {  // their number is a multiple of 8
+            Raw<T, 8> raw;
+            raw.load(row + first);
+            raw.get(v[q]);
         } else {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (lane * kPer + i >= E) allowed &= ~(1u << i);
+            for (int i = 0; i < 8; ++i) v[q][i] = !kVector && first + i < p.n_experts ? to_f32(row[first + i]) : -INFINITY;
         }
-        int mine = choose<unsigned, kPer>(key, allowed, p.top_k);
-        if (p.bias && !unsure) {
-            // the chosen among themselves, and the rest against the last of them
-            const bool there = lane < p.top_k;
-            const float ml = there ? logit<T>(p, token, mine) : 0.f, mb = there ? p.bias[mine] : 0.f;
-            const float ms = there ? score_of(p, ml, shift, inverse) : 0.f, mv = __fadd_rn(ms, mb);
-            const float nl = __shfl_down_sync(kAll, ml, 1), nb = __shfl_down_sync(kAll, mb, 1), ns = __shfl_down_sync(kAll, ms, 1),
-                        nv = __shfl_down_sync(kAll, mv, 1);
-            bool close = lane + 1 < p.top_k && !(mv - nv > (ms + ns) * kScoreError + fabsf(mv) * kSumError + kSmallest) &&
-                         !(ml == nl && mb == nb);
-            const int last = p.top_k - 1;
-            const float ll = __shfl_sync(kAll, ml, last), lb = __shfl_sync(kAll, mb, last), ls = __shfl_sync(kAll, ms, last),
-                        lv = __shfl_sync(kAll, mv, last);
-            const unsigned lk = order_of(lv);
-            const int le = __shfl_sync(kAll, mine, last);
+    }
+}
+
+// Softmax's shift and the inverse of its sum; a token without a finite logit has no score: inverse 0.
+template <int kLanes, int kOctets>
+__device__ __forceinline__ void softmax_of(const float (&l)[kOctets][8], bool quick, float &shift, float &inverse) {
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int e = lane * kPer + i;
-                // those before the last in the order are chosen
-                if (!(allowed >> i & 1) || key[i] > lk || (key[i] == lk && e <= le)) continue;
-                if (!(lv - v[i] > (ls + score[i]) * kScoreError + fabsf(lv) * kSumError + kSmallest) &&
-                    !(l[i] == ll && p.bias[e] == lb))
-                    close = true;
-            }
-            unsure = __any_sync(kAll, close);
+    for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, l[q][i]);
+    shift = most<kLanes>(top);
+    if (shift == -INFINITY) shift = 0.f;  // every term is 0 then, or NaN
+    if (quick) {
+#pragma unroll
+        for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += quick_exp(l[q][i] - shift);
+    } else {
+#pragma unroll
+        for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += expf(l[q][i] - shift);
+    }
+    sum = total<kLanes>(sum);
+    inverse = sum == 0.f ? 0.f : 1.f / sum;
+}
+
+// Scores of the chosen experts with the logits l (kMine of them in a lane; those that are not there have there[i] false), before
+// scaling, and what the weights are divided by.
+template <int kLanes, int kMine>
+__device__ __forceinline__ float chosen_scores(const RouteArgs &p, const float (&l)[kMine], const bool (&there)[kMine], float shift, float inverse,
+                                               float (&score)[kMine]) {
+    if (!p.sigmoid && p.renormalise) {  // softmax over the chosen
+        shift = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+            if (there[i]) shift = fmaxf(shift, l[i]);
+        shift = most<kLanes>(shift);
+        if (shift == -INFINITY) shift = 0.f;
+        inverse = 1.f;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        score[i] = 0.f;
+        if (there[i]) {
+            if (p.sigmoid) score[i] = 1.f / (1.f + expf(-l[i]));
+            else if (inverse != 0.f) score[i] = expf(l[i] - shift) * inverse;
         }
-        if (unsure) mine = choose_exactly<T, kPer>(p, token, values64);
-        const float ml = lane < p.top_k ? logit<T>(p, token, mine) : -INFINITY;
-        const Chosen c = chosen_scores<kPer>(p, ml, shift, inverse);
-        if (lane < p.top_k) {
-            p.weights[token * p.top_k + lane] = c.total == 0.f ? 0.f : p.scale * c.score / c.total;
-            p.experts[token * p.top_k + lane] = mine;
+        sum += score[i];
+    }
+    return p.renormalise ? total<kLanes>(sum) : 1.f;
+}
+
+// Of a warp, in shared memory.
+template <int kLanes, int kOctets>
+struct WarpShared {
+    static constexpr int kTokens = 32 / kLanes, kExperts = kLanes * kOctets * 8;
+    float values[kTokens][kExperts];
+    float worth[kTokens][kMostExpertGroups];
+    float chosen_value[kTokens][kMostChoices];
+    int chosen[kTokens][kMostChoices];
+};
+
+// Takes the experts of other than the top_groups best groups out of v (NaN).  s.values has them all.  Returns false where the border
+// between the groups is closer than `error`.
+template <int kLanes, int kOctets>
+__device__ __forceinline__ bool keep_best_groups(const RouteArgs &p, const float *values, float *worth, int lane, float error, float (&v)[kOctets][8]) {
+    const int size = p.n_experts / p.n_groups;
+    int share = kLanes;  // lanes to a group
+    while (share > 1 && kLanes / share < p.n_groups) share /= 2;
+    const bool sums = p.top2 && size > 1;
+    for (int base = 0; base < p.n_groups; base += kLanes / share) {
+        const int g = base + lane / share;
+        float first = -INFINITY, second = -INFINITY;
+        if (g < p.n_groups)
+            for (int i = lane % share; i < size; i += share) {
+                const float x = values[g * size + i];
+                second = fmaxf(second, fminf(first, x));
+                first = fmaxf(first, x);
+            }
+        for (int d = 1; d < share; d *= 2) {
+            const float a = __shfl_xor_sync(kAll, first, d), b = __shfl_xor_sync(kAll, second, d);
+            second = fmaxf(fminf(first, a), fmaxf(second, b));
+            first = fmaxf(first, a);
+        }
+        if (g < p.n_groups && lane % share == 0) worth[g] = fmaxf(sums ? first + second : first, -INFINITY);
+    }
+    __syncwarp();
+    unsigned groups = 0;
+    float low = INFINITY, high = -INFINITY;
+    for (int g = lane; g < p.n_groups; g += kLanes) {
+        const float mine = worth[g];
+        int better = 0;
+        for (int o = 0; o < p.n_groups; ++o) {
+            const float other = worth[o];
+            if (other > mine || (other == mine && o < g)) ++better;
+        }
+        if (better < p.top_groups) {
+            groups |= 1u << g;
+            low = fminf(low, mine);
+        } else {
+            high = fmaxf(high, mine);
+        }
+    }
+#pragma unroll
+    for (int d = kLanes / 2; d > 0; d /= 2) groups |= __shfl_xor_sync(kAll, groups, d);
+    low = -most<kLanes>(-low);
+    high = most<kLanes>(high);
+    const unsigned inverse_size = ((1u << 20) + size - 1) / size;  // e / size for e < 1024
+#pragma unroll
+    for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (!(groups >> (((q * kLanes + lane) * 8 + i) * inverse_size >> 20 & 31) & 1)) v[q][i] = NAN;
+    return error < 0.f || low - high > error || low == -INFINITY;
+}
+
+template <typename T, int kLanes, int kOctets, bool kVector>
+__global__ void __launch_bounds__(kThreads) route_forward_kernel(const RouteArgs p) {
+    using Shared = WarpShared<kLanes, kOctets>;
+    __shared__ alignas(16) Shared warps[kWarps];
+    __shared__ alignas(16) float bias[Shared::kExperts];
+    wait_for_previous_kernel();
+    constexpr int kMine = kMostChoices / kLanes;
+    const int lane = threadIdx.x % kLanes, segment = threadIdx.x % 32 / kLanes, E = p.n_experts;
+    Shared &s = warps[threadIdx.x / 32];
+    float *values = s.values[segment];
+    if (p.bias) {
+        for (int e = threadIdx.x; e < Shared::kExperts; e += kThreads) bias[e] = e < E ? p.bias[e] : 0.f;
+        __syncthreads();
+    }
+    const bool grouped = p.top_groups < p.n_groups;
+    const bool by_score = p.bias || (grouped && p.top2 && E > p.n_groups);  // what is compared: scores, or logits
+    const bool need_softmax = !p.sigmoid && (by_score || !p.renormalise);
+    const long long step = (long long)gridDim.x * kWarps * Shared::kTokens;
+    for (long long base = ((long long)blockIdx.x * kWarps + threadIdx.x / 32) * Shared::kTokens; base < p.tokens; base += step) {
+        const long long token = base + segment;
+        const bool active = token < p.tokens;
+        float v[kOctets][8], shift = 0.f, inverse = 1.f, largest = 0.f;
+        load_logits<T, kLanes, kOctets, kVector>(p, active ? token : base, lane, v);
+        if (need_softmax) softmax_of<kLanes, kOctets>(v, p.renormalise, shift, inverse);
+        if (by_score) {  // select values, in the same way for every expert
+#pragma unroll
+            for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (p.sigmoid) v[q][i] = __fdividef(1.f, 1.f + quick_exp(-v[q][i]));
+                    else v[q][i] = __fmul_rn(quick_exp(v[q][i] - shift), inverse);
+                    largest = fmaxf(largest, v[q][i]);
+                }
+            largest = most<kLanes>(largest);
+        }
+        float error = -1.f;  // of a group's worth
+        if (grouped && by_score) error = 0.f;
+        if (grouped && by_score && !p.bias) {
+            // the groups by their scores' sums, experts by their logits
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) values[(q * kLanes + lane) * 8 + i] = v[q][i];
+            __syncwarp();
+            load_logits<T, kLanes, kOctets, kVector>(p, active ? token : base, lane, v);
+        }
+        if (p.bias) {
+#pragma unroll
+            for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[q][i] = __fadd_rn(v[q][i], bias[(q * kLanes + lane) * 8 + i]);
+        }
+#pragma unroll
+        for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[q][i] = (q * kLanes + lane) * 8 + i < E ? fmaxf(v[q][i], -INFINITY) : NAN;
+        bool sure = true;
+        if (grouped) {
+            if (!by_score || p.bias) {
+                float far = 0.f;
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        values[(q * kLanes + lane) * 8 + i] = v[q][i];
+                        if (fabsf(v[q][i]) < INFINITY) far = fmaxf(far, fabsf(v[q][i]));
+                    }
+                __syncwarp();
+                if (by_score) error = 4.f * kSumError * most<kLanes>(far);
+            } else {
+                error = 4.f * kSumError * largest;
+            }
+            // a group is worth up to two values, and two groups are compared
+            if (by_score) error += 4.f * (largest * kScoreError + kSmallest);
+            sure = keep_best_groups<kLanes, kOctets>(p, values, s.worth[segment], lane, error, v);
+        }
+        __syncwarp();
+        float head[kOctets];  // largest of each octet
+#pragma unroll
+        for (int q = 0; q < kOctets; ++q) {
+            float4 *at = reinterpret_cast<float4 *>(values + (q * kLanes + lane) * 8);
+            at[0] = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
+            at[1] = make_float4(v[q][4], v[q][5], v[q][6], v[q][7]);
+            head[q] = NAN;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) head[q] = fmaxf(head[q], v[q][i]);
+        }
+        const auto largest_left = [&]() {
+            float top = head[0];
+#pragma unroll
+            for (int q = 1; q < kOctets; ++q) top = fmaxf(top, head[q]);
+            return most<kLanes>(top);
+        };
+        // the first expert of value `top` leaves; its lane gets the index, others -1
+        const auto take = [&](float top) {
+            int octet = INT32_MAX;
+#pragma unroll
+            for (int q = kOctets - 1; q >= 0; --q)
+                if (head[q] == top) octet = q * kLanes + lane;
+            octet = least<kLanes>(octet);
+            if (octet % kLanes != lane || octet == INT32_MAX) return -1;
+            float4 *at = reinterpret_cast<float4 *>(values + octet * 8);
+            const float4 a = at[0], b = at[1];
+            float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            int slot = 0;
+#pragma unroll
+            for (int i = 7; i >= 0; --i)
+                if (x[i] == top) slot = i;
+            float rest = NAN;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rest = fmaxf(rest, i == slot ? NAN : x[i]);
+            values[octet * 8 + slot] = NAN;
+#pragma unroll
+            for (int q = 0; q < kOctets; ++q)
+                if (octet / kLanes == q) head[q] = rest;
+            return octet * 8 + slot;
+        };
+        for (int j = 0; j < p.top_k; ++j) {
+            const float top = largest_left();
+            const int e = take(top);
+            if (e >= 0) {
+                s.chosen[segment][j] = e;
+                s.chosen_value[segment][j] = top;
+            }
+        }
+        __syncwarp();
+        if (p.bias) {
+            // the chosen among themselves, and the last of them against what is left
+            const float margin = 2.f * largest * kScoreError + kSmallest, last = s.chosen_value[segment][p.top_k - 1];
+            const auto same = [&](int a, int b) {
+                return logit<T>(p, active ? token : base, a) == logit<T>(p, active ? token : base, b) && bias[a] == bias[b];
+            };
+            for (int j = lane; j + 1 < p.top_k; j += kLanes) {
+                const float a = s.chosen_value[segment][j], b = s.chosen_value[segment][j + 1];
+                if (!(a - b > margin + fabsf(a) * kSumError) && !same(s.chosen[segment][j], s.chosen[segment][j + 1])) sure = false;
+            }
+            // of equal experts the lower ones are chosen: what comes behind them counts
+            const int last_chosen = s.chosen[segment][p.top_k - 1];
+            bool open = most<kLanes>(sure ? 0.f : 1.f) == 0.f;
+            while (true) {  // ends: a pass takes an expert out of every token that has one
+                const float next = largest_left();
+                open = open && next == next && !(last - next > margin + fabsf(last) * kSumError);
+                if (!__any_sync(kAll, open)) break;
+                const int e = take(next);
+                if (open && e >= 0 && !same(last_chosen, e)) sure = false;
+                const float settled = most<kLanes>(sure ? 0.f : 1.f);  // every lane takes part
+                open = open && settled == 0.f;
+            }
+        }
+        const unsigned unsure = __ballot_sync(kAll, active && !sure);
+        if (unsure) {
+            for (int t = 0; t < Shared::kTokens; ++t)
+                if (unsure >> (t * kLanes) & ((1ull << kLanes) - 1))
+                    choose_exactly<T, Shared::kExperts / 32>(p, base + t, reinterpret_cast<double *>(s.values), s.chosen[t]);
+            __syncwarp();
+        }
+        int mine[kMine];
+        float l[kMine], score[kMine];
+        bool there[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            there[i] = lane + i * kLanes < p.top_k;
+            mine[i] = there[i] ? s.chosen[segment][lane + i * kLanes] : 0;
+            l[i] = logit<T>(p, active ? token : base, mine[i]);
+        }
+        const float sum = chosen_scores<kLanes, kMine>(p, l, there, shift, inverse, score);
+        if (!active) continue;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            if (!there[i]) continue;
+            const long long at = token * p.top_k + lane + i * kLanes;
+            p.weights[at] = sum == 0.f ? 0.f : p.scale * score[i] / sum;
+            p.experts[at] = mine[i];
         }
     }
 }
@@ -329,72 +498,99 @@ __global__ void __launch_bounds__(kThreads) route_forward_kernel(const RouteArgs
 //     softmax                  dl_i = scale p_i ([i chosen] dw_i - sum of dw p)
 //     sigmoid                  dl_j = ds_j s_j (1 - s_j),  ds_j = scale (dw_j - sum of dw s / S) / S  or  scale dw_j
 // An expert outside 0 .. n_experts - 1 gets none.  No atomics: a row is put together in shared memory.
-template <typename T, int kPer>
+template <typename T, int kLanes, int kOctets, bool kVector>
 __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArgs p) {
-    extern __shared__ float rows[];
+    constexpr int kTokens = 32 / kLanes, kExperts = kLanes * kOctets * 8, kMine = kMostChoices / kLanes;
+    __shared__ alignas(16) float rows[kWarps][kTokens][kExperts];
     wait_for_previous_kernel();
-    const int lane = threadIdx.x % 32, E = p.n_experts;
-    float *row = rows + (threadIdx.x / 32) * E;
+    const int lane = threadIdx.x % kLanes, segment = threadIdx.x % 32 / kLanes, E = p.n_experts;
+    float *row = rows[threadIdx.x / 32][segment];
     const bool dense = !p.sigmoid && !p.renormalise;
-    for (long long token = (long long)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; token < p.tokens; token += (long long)gridDim.x * (kThreads / 32)) {
-        const int64_t chosen = lane < p.top_k ? p.experts[token * p.top_k + lane] : -1;
-        const bool there = chosen >= 0 && chosen < E;
-        const float dw = there ? p.grad_weights[token * p.top_k + lane] * p.scale : 0.f;
-        const float ml = there ? logit<T>(p, token, (int)chosen) : -INFINITY;
-        float l[kPer], shift = 0.f, inverse = 1.f;
-        if (dense) {
+    const long long step = (long long)gridDim.x * kWarps * kTokens;
+    for (long long base = ((long long)blockIdx.x * kWarps + threadIdx.x / 32) * kTokens; base < p.tokens; base += step) {
+        const bool active = base + segment < p.tokens;
+        const long long token = active ? base + segment : base;
+        long long chosen[kMine];
+        float dw[kMine], l[kMine], score[kMine];
+        bool there[kMine];
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) l[i] = lane * kPer + i < E ? logit<T>(p, token, lane * kPer + i) : -INFINITY;
-            softmax_of<float, kPer>(l, E, shift, inverse);
+        for (int i = 0; i < kMine; ++i) {
+            const int j = lane + i * kLanes;
+            chosen[i] = j < p.top_k ? p.experts[token * p.top_k + j] : -1;
+            there[i] = chosen[i] >= 0 && chosen[i] < E;
+            dw[i] = there[i] ? p.grad_weights[token * p.top_k + j] * p.scale : 0.f;
         }
-        const Chosen c = chosen_scores<kPer>(p, ml, shift, inverse);
-        const float s = c.score;
-        float dl = 0.f, along = 0.f;
-        if (p.sigmoid) {
-            along = p.renormalise ? (c.total == 0.f ? 0.f : warp_sum(dw * s) / c.total) : 0.f;
-            dl = c.total == 0.f ? 0.f : (dw - along) / c.total * s * (1.f - s);
-        } else if (p.renormalise) {
-            const float q = c.total == 0.f ? 0.f : s / c.total;
-            dl = q * (dw - warp_sum(dw * q));
-        } else {
-            along = warp_sum(dw * s);
-            dl = s * dw;
+        float v[kOctets][8], shift = 0.f, inverse = 1.f;
+        if (dense) {
+            load_logits<T, kLanes, kOctets, kVector>(p, token, lane, v);
+            softmax_of<kLanes, kOctets>(v, false, shift, inverse);
+        }
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) l[i] = there[i] ? logit<T>(p, token, (int)chosen[i]) : 0.f;
+        const float sum = chosen_scores<kLanes, kMine>(p, l, there, shift, inverse, score);
+        const float over = sum == 0.f ? 0.f : 1.f / sum;
+        float along = 0.f;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) along += dw[i] * score[i] * over;
+        along = total<kLanes>(along);
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < kOctets; ++q) {
+            float4 *at = reinterpret_cast<float4 *>(row + (q * kLanes + lane) * 8);
+            at[0] = at[1] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         __syncwarp();
-        for (int i = lane; i < E; i += 32) row[i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            if (!there[i]) continue;
+            float dl = score[i] * over * (p.renormalise ? dw[i] - along : dw[i]);
+            if (p.sigmoid) dl *= 1.f - score[i];
+            row[chosen[i]] = dl;
+        }
         __syncwarp();
-        if (there) row[chosen] = dl;
-        __syncwarp();
+        if (!active) continue;
         T *out = static_cast<T *>(p.grad_logits) + token * E;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = lane * kPer + i;
-            if (e >= E) continue;
-            float v = row[e];
-            if (dense) v -= inverse == 0.f ? 0.f : expf(l[i] - shift) * inverse * along;
-            out[e] = from_f32<T>(v);
+        for (int q = 0; q < kOctets; ++q) {
+            const int first = (q * kLanes + lane) * 8;
+            if (first >= E) continue;
+            const float4 *at = reinterpret_cast<const float4 *>(row + first);
+            const float4 a = at[0], b = at[1];
+            float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            if (dense && inverse != 0.f) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] -= expf(v[q][i] - shift) * inverse * along;
+            }
+            if (kVector) {
+                Raw<T, 8> raw;
+                raw.set(d);
+                raw.store(out + first);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (first + i < E) out[first + i] = from_f32<T>(d[i]);
+            }
         }
     }
 }
 
-template <typename T, int kPer>
+template <typename T, int kLanes, int kOctets>
 int launch_route(bool backward, const RouteArgs &p, cudaStream_t st) {
-    const unsigned blocks = (unsigned)std::min<long long>(ceil_div(p.tokens, kThreads / 32), 16 * kSms);
-    const int shared = (kThreads / 32) * p.n_experts * (int)(backward ? sizeof(float) : sizeof(double));
-    const auto kernel = backward ? route_backward_kernel<T, kPer> : route_forward_kernel<T, kPer>;
-    if (shared > 48 * 1024)
-        if (const int rc = launched(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared))) return rc;
-    return launched(launch_early(kernel, blocks, kThreads, shared, st, 1, p));
+    const unsigned blocks = (unsigned)std::min<long long>(ceil_div(p.tokens, kWarps * 32 / kLanes), 16 * kSms);
+    // rows of octets that start on 16-byte boundaries
+    const bool vector = p.n_experts % 8 == 0 && !misaligned16(p.logits) && !misaligned16(p.grad_logits);
+    const auto kernel = backward ? (vector ? route_backward_kernel<T, kLanes, kOctets, true> : route_backward_kernel<T, kLanes, kOctets, false>)
+                                 : (vector ? route_forward_kernel<T, kLanes, kOctets, true> : route_forward_kernel<T, kLanes, kOctets, false>);
+    return launched(launch_early(kernel, blocks, kThreads, 0, st, 1, p));
 }
 
 template <typename T>
 int launch_route(bool backward, const RouteArgs &p, cudaStream_t st) {
-    if (p.n_experts <= 32) return launch_route<T, 1>(backward, p, st);
-    if (p.n_experts <= 64) return launch_route<T, 2>(backward, p, st);
-    if (p.n_experts <= 128) return launch_route<T, 4>(backward, p, st);
-    if (p.n_experts <= 256) return launch_route<T, 8>(backward, p, st);
-    if (p.n_experts <= 512) return launch_route<T, 16>(backward, p, st);
-    return launch_route<T, 32>(backward, p, st);
+    if (p.n_experts <= 64) return launch_route<T, 8, 1>(backward, p, st);
+    if (p.n_experts <= 128) return launch_route<T, 8, 2>(backward, p, st);
+    if (p.n_experts <= 256) return launch_route<T, 8, 4>(backward, p, st);
+    if (p.n_experts <= 512) return launch_route<T, 8, 8>(backward, p, st);
+    return launch_route<T, 16, 8>(backward, p, st);
 }
 
 int launch_route(bool backward, const RouteArgs &p, cudaStream_t st) {
