@@ -40,8 +40,9 @@ __device__ __forceinline__ float wide_input(const WideArgs &p, size_t at) {
 }
 __device__ __forceinline__ float wide_weight(const WideArgs &p, int c) { return p.n.weight ? load_as_f32(p.n.weight, p.n.param_dtype, c) : 1.f; }
 
+constexpr int kWideThreads = 512;
 template <bool kBackward>
-__global__ void __launch_bounds__(kBlockThreads) norm_wide_kernel(const WideArgs p) {
+__global__ void __launch_bounds__(kWideThreads) norm_wide_kernel(const WideArgs p) {
     wait_for_previous_kernel();
     Team<0> team = make_team<0>();
     const int width = p.n.width;
@@ -49,11 +50,11 @@ __global__ void __launch_bounds__(kBlockThreads) norm_wide_kernel(const WideArgs
     for (long long row = blockIdx.x; row < p.n.rows; row += gridDim.x) {
         const size_t at = (size_t)row * width;
         float sum[1] = {0.f};
-        for (int c = threadIdx.x; c < width; c += kBlockThreads) sum[0] += wide_input(p, at + c);
+        for (int c = threadIdx.x; c < width; c += kWideThreads) sum[0] += wide_input(p, at + c);
         team.sum(sum);
         const float mean = sum[0] * inverse;
         float sums[3] = {0.f, 0.f, 0.f};
-        for (int c = threadIdx.x; c < width; c += kBlockThreads) {
+        for (int c = threadIdx.x; c < width; c += kWideThreads) {
             const float d = wide_input(p, at + c) - mean;
             sums[0] += d * d;
             if (kBackward) {
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(kBlockThreads) norm_wide_kernel(const WideArgs
             p.statistics[2 * row + 1] = q;
         }
         const float along = q * q * sums[1] * inverse, level = sums[2] * inverse;
-        for (int c = threadIdx.x; c < width; c += kBlockThreads) {
+        for (int c = threadIdx.x; c < width; c += kWideThreads) {
             const float s = wide_input(p, at + c), d = s - mean;
             if (!kBackward) {
                 if (p.n.sum) store_from_f32(p.n.sum, p.residual_dtype, at + c, s);
@@ -105,13 +106,8 @@ __global__ void __launch_bounds__(256) norm_wide_columns_kernel(const WideArgs p
 
 constexpr int kWideParts = 64;
 
-bool is_wide(int width, int dtype) { return width > most_fast_width(dtype); }
-
-// Blocks of the backward, each of which leaves sums of its own: two to an SM are what registers allow (one of 512 threads).
-unsigned backward_blocks(long long rows, int width, int dtype) {
-    const NormShape s = norm_shape(width, dtype);
-    return norm_blocks(s, rows, s.lanes ? 2 : std::max(1, 2048 / s.threads / 4));
-}
+// Blocks of the backward, each of which leaves sums of its own.
+unsigned backward_blocks(long long rows, int width, int dtype) { return norm_blocks(norm_shape(width, dtype), rows, true); }
 
 struct Workspace {
     size_t partial, statistics, total;
@@ -161,10 +157,10 @@ int fda_layer_norm_forward(const void *x, const void *weight, const void *bias, 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (is_wide(features, dtype)) {
         WideArgs w{p, dtype, residual_dtype, nullptr, 0};
-        return launched(launch_early(norm_wide_kernel<false>, (unsigned)std::min<long long>(rows, 4 * kSms), kBlockThreads, 0, st, 1, w));
+        return launched(launch_early(norm_wide_kernel<false>, (unsigned)std::min<long long>(rows, 4 * kSms), kWideThreads, 0, st, 1, w));
     }
     const NormShape s = norm_shape(features, dtype);
-    return run_fast(false, p, dtype, residual_dtype, norm_blocks(s, rows, s.lanes ? 4 : std::max(1, 2048 / s.threads / 2)), st);
+    return run_fast(false, p, dtype, residual_dtype, norm_blocks(s, rows, false), st);
 }
 
 size_t fda_layer_norm_backward_workspace_bytes(long long rows, int features, int dtype) {
@@ -206,7 +202,7 @@ int fda_layer_norm_backward(const void *x, const void *weight, const void *resid
         parts = (int)std::min<long long>(rows, kWideParts);
         w.rows_per_part = (int)ceil_div(rows, parts);
         parts = (int)ceil_div(rows, w.rows_per_part);
-        if (const int rc = launched(launch_early(norm_wide_kernel<true>, (unsigned)std::min<long long>(rows, 4 * kSms), kBlockThreads, 0, st, 1, w)))
+        if (const int rc = launched(launch_early(norm_wide_kernel<true>, (unsigned)std::min<long long>(rows, 4 * kSms), kWideThreads, 0, st, 1, w)))
             return rc;
         if (!parameters) return FDA_OK;
         norm_wide_columns_kernel<<<dim3((unsigned)ceil_div(features, 256), parts), 256, 0, st>>>(w);

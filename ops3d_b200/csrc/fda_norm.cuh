@@ -3,8 +3,8 @@
 //     s = x + residual,   mu = mean(s),   d = s - mu,   q = 1 / sqrt(mean(d d) + eps),   y = d q weight + bias          per row
 //     g = dy weight,   ds = q (g - mean(g) - d q^2 mean(g d)) + dsum,   dweight = sum over rows of dy d q,   dbias = sum of dy
 //
-// One pass over memory in each direction: a row stays in the registers of the threads that share it (8 or 32 lanes of a warp, or a
-// block), while its mean and then the sums of the deviations are taken, so the variance has no cancellation.  Nothing is kept for
+// One pass over memory in each direction: a row stays in the registers of the threads that share it (4 to 32 lanes of a warp, or
+// a block), while its mean and then the sums of the deviations are taken, so the variance has no cancellation.  Nothing is kept for
 // the backward but x and residual: the statistics come from the row again, which is there anyway.  Bound by DRAM traffic.
 //
 // Rows of any width are read in aligned 16-byte vectors.  Row r starts r * width elements into the tensor, that is at element
@@ -30,73 +30,145 @@ struct NormArgs {
     float eps;
 };
 
-constexpr int kTeamThreads = 256;   // of a block whose teams are lanes of a warp
-constexpr int kBlockThreads = 512;  // most threads of a block that is a team
+constexpr int kTeamThreads = 256;    // of a block whose teams are lanes of a warp
+constexpr int kBlockThreads = 1024;  // most threads of a block that is a team
 
 template <typename T> constexpr int kWidthOf = 16 / (int)sizeof(T);
 
-// Vectors of one row that belong to a lane: columns, and whether they are all inside.
-template <int kWidth, int kVectors, int kLanes, bool kRagged>
+// Vectors of a row that belong to a lane.
+template <int kWidth, int kVectors, bool kRagged>
 struct Columns {
-    int first[kVectors];  // may be negative where kRagged
     int width;
+    int first[kVectors];                // column of the first element; may be negative where kRagged
+    int count[kVectors];                // elements from the first to the row's end, at most kWidth; 0 where the row has none
+    unsigned bits[kVectors];            // bit j: element j is one of the row's
+    float valid[kVectors][kRagged ? kWidth : 1];  // the same as factors
+    unsigned keep[kVectors][kRagged ? 4 : 1];     // and as a mask of the vector's words
     __device__ __forceinline__ Columns(int width, long long row, int lane, int size) : width(width) {
         const int shift = kRagged ? (int)((row * width) % kWidth) : 0;
 #pragma unroll
-        for (int i = 0; i < kVectors; ++i) first[i] = (i * size + lane) * kWidth - shift;
+        for (int i = 0; i < kVectors; ++i) {
+            first[i] = (i * size + lane) * kWidth - shift;
+            count[i] = max(0, min(kWidth, width - first[i]));
+            bits[i] = (1u << count[i]) - 1;
+            if constexpr (kRagged) {
+                if (first[i] < 0) bits[i] &= ~((1u << -first[i]) - 1);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) keep[i][k] = 0;
+#pragma unroll
+                for (int j = 0; j < kWidth; ++j) {
+                    valid[i][j] = has(i, j) ? 1.f : 0.f;
+                    if (has(i, j)) keep[i][j * 4 / kWidth] |= kWidth == 4 ? 0xffffffffu : 0xffffu << (j % 2 * 16);
+                }
+            } else {
+                valid[i][0] = count[i] ? 1.f : 0.f;
+            }
+        }
     }
-    __device__ __forceinline__ bool any(int i) const { return first[i] < width; }
-    __device__ __forceinline__ bool whole(int i) const { return !kRagged || (first[i] >= 0 && first[i] + kWidth <= width); }
-    __device__ __forceinline__ bool has(int i, int j) const { return kRagged ? first[i] + j >= 0 && first[i] + j < width : first[i] < width; }
+    __device__ __forceinline__ bool any(int i) const { return count[i] != 0; }
+    __device__ __forceinline__ bool whole(int i) const { return !kRagged || bits[i] == (1u << kWidth) - 1; }
+    __device__ __forceinline__ bool has(int i, int j) const { return bits[i] >> j & 1; }
+    __device__ __forceinline__ float one(int i, int j) const { return valid[i][kRagged ? j : 0]; }
 };
 
-template <typename T, int kWidth, bool kRagged>
-__device__ __forceinline__ void load_vector(Raw<T, kWidth> &raw, const T *tensor, long long at, long long total) {
-    if (kRagged && at + kWidth > total) {  // the tensor ends inside the vector
-        alignas(16) T v[kWidth];
-        for (int j = 0; j < kWidth; ++j) v[j] = at + j < total ? tensor[at + j] : from_f32<T>(0.f);
-        raw.load(v);
-        return;
-    }
-    raw.load(tensor + at);
+// Rows on their way: every lane copies its own vectors into its own places of a ring in shared memory, kStages - 1 rows ahead of the one
+// that it works on, so that nothing has to wait for another lane.
+__device__ __forceinline__ void copy16(unsigned to, const void *from, int bytes) {  // the rest of the 16 becomes 0
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
-template <typename T, int kWidth, int kVectors, int kLanes, bool kRagged>
-__device__ __forceinline__ void load_row(Raw<T, kWidth> (&raw)[kVectors], const void *tensor, const Columns<kWidth, kVectors, kLanes, kRagged> &c,
-                                         long long row, long long rows) {
+// at: where the row's first vector of the lane starts in the tensor; left: rows from this one on, of which only the last may end inside a
+// vector at the tensor's end.
+template <typename E, int kWidth, int kVectors, bool kRagged>
+__device__ __forceinline__ void copy_row(unsigned slot, unsigned pitch, const void *tensor, const Columns<kWidth, kVectors, kRagged> &c,
+                                         long long at, long long left) {
+    constexpr int kUnits = kWidth * (int)sizeof(E) / 16, kEach = 16 / (int)sizeof(E);
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
-        if (row < rows && c.any(i)) load_vector<T, kWidth, kRagged>(raw[i], static_cast<const T *>(tensor), row * c.width + c.first[i], rows * c.width);
-        else raw[i].clear();
+        const E *from = static_cast<const E *>(tensor) + at + (c.first[i] - c.first[0]);
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            const int last = kRagged ? max(0, min(kEach, c.count[i] - u * kEach)) * (int)sizeof(E) : 16;
+            const int bytes = !c.any(i) || left <= 0 ? 0 : kRagged && left == 1 ? last : 16;
+            copy16(slot + (i * kUnits + u) * pitch, bytes ? from + u * kEach : tensor, bytes);
+        }
     }
 }
 
-template <typename T, int kWidth, int kVectors, int kLanes, bool kRagged>
-__device__ __forceinline__ void store_vector(void *tensor, const float *v, const Columns<kWidth, kVectors, kLanes, kRagged> &c, int i, long long row) {
-    T *at = static_cast<T *>(tensor) + row * c.width + c.first[i];
+// A lane's vector i from its place, elements of neighbouring rows as 0.
+template <typename E, int kWidth, int kVectors, bool kRagged>
+__device__ __forceinline__ void read_vector(const char *slot, unsigned pitch, const Columns<kWidth, kVectors, kRagged> &c, int i, float *v) {
+    constexpr int kUnits = kWidth * (int)sizeof(E) / 16;
+    Raw<E, kWidth> raw;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) raw.u[u] = *reinterpret_cast<const uint4 *>(slot + (i * kUnits + u) * pitch);
+    if (kRagged && kUnits == 1) {
+        raw.u[0].x &= c.keep[i][0];
+        raw.u[0].y &= c.keep[i][kRagged ? 1 : 0];
+        raw.u[0].z &= c.keep[i][kRagged ? 2 : 0];
+        raw.u[0].w &= c.keep[i][kRagged ? 3 : 0];
+    }
+    raw.get(v);
+    if (kRagged && kUnits > 1) {
+#pragma unroll
+        for (int j = 0; j < kWidth; ++j) v[j] = c.one(i, j) != 0.f ? v[j] : 0.f;
+    }
+}
+
+// at: as above, of the row that is stored.
+template <typename E, int kWidth, int kVectors, bool kRagged>
+__device__ __forceinline__ void store_vector(void *tensor, const float *v, const Columns<kWidth, kVectors, kRagged> &c, int i, long long at) {
+    E *to = static_cast<E *>(tensor) + at + (c.first[i] - c.first[0]);
+    Raw<E, kWidth> raw;
+    raw.set(v);
     if (c.whole(i)) {
-        Raw<T, kWidth> raw;
-        raw.set(v);
-        raw.store(at);
+        raw.store(to);
         return;
     }
 #pragma unroll
     for (int j = 0; j < kWidth; ++j)
-        if (c.has(i, j)) at[j] = from_f32<T>(v[j]);
+        if (c.has(i, j)) to[j] = raw.element(j);
+}
+
+// A parameter's numbers for a lane's columns, `otherwise` where there is none.
+template <typename E, int kWidth, int kVectors, bool kRagged>
+__device__ __forceinline__ void load_parameter(const E *tensor, const Columns<kWidth, kVectors, kRagged> &c, float (&v)[kVectors][kWidth]) {
+    const bool vector = !kRagged && (uintptr_t)tensor % 16 == 0;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+        if (vector && c.any(i)) {
+            Raw<E, kWidth> raw;
+            raw.load(tensor + c.first[i]);
+            raw.get(v[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kWidth; ++j)
+                if (c.has(i, j)) v[i][j] = to_f32(tensor[c.first[i] + j]);
+        }
+    }
+}
+template <typename T, int kWidth, int kVectors, bool kRagged>
+__device__ __forceinline__ void load_parameter(const void *tensor, int dtype, float otherwise, const Columns<kWidth, kVectors, kRagged> &c,
+                                               float (&v)[kVectors][kWidth]) {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+        for (int j = 0; j < kWidth; ++j) v[i][j] = otherwise;
+    if (!tensor) return;
+    if (dtype == FDA_DTYPE_F32) load_parameter(static_cast<const float *>(tensor), c, v);
+    else load_parameter(static_cast<const T *>(tensor), c, v);
 }
 
 // Which rows a team takes: the first one, and how far apart they are (a multiple of kWidth, because a grid's blocks are where a block
 // is a team, and a block's teams are otherwise).
 template <int kLanes>
 __device__ __forceinline__ void team_rows(long long &first, long long &step) {
-    if (kLanes == 0) {
-        first = blockIdx.x;
-        step = gridDim.x;
-    } else {
-        constexpr int kTeams = kTeamThreads / (kLanes ? kLanes : 1);
-        first = (long long)blockIdx.x * kTeams + threadIdx.x / (kLanes ? kLanes : 1);
-        step = (long long)gridDim.x * kTeams;
-    }
+    constexpr int kTeams = kLanes ? kTeamThreads / (kLanes ? kLanes : 1) : 1;
+    first = (long long)blockIdx.x * kTeams + (kLanes ? threadIdx.x / (kLanes ? kLanes : 1) : 0);
+    step = (long long)gridDim.x * kTeams;
 }
 
 // Shared memory of the sums over a block.
@@ -104,56 +176,74 @@ template <int kLanes>
 __device__ __forceinline__ Team<kLanes> make_team() {
     Team<kLanes> team;
     if constexpr (kLanes == 0) {
-        __shared__ float sums[2][Team<0>::kMost][Team<0>::kWarps];
+        __shared__ alignas(16) float sums[2][Team<0>::kMost][Team<0>::kWarps];
+        for (int i = threadIdx.x; i < 2 * Team<0>::kMost * Team<0>::kWarps; i += blockDim.x) (&sums[0][0][0])[i] = 0.f;
+        __syncthreads();
         team.shared = sums;
     }
     return team;
 }
 
+// 16-byte places of a lane for one row, and rows of the ring: as many bytes on their way as DRAM's latency takes (40 KB to an SM and more),
+// and no more than two blocks (one of 1024 threads) have room for.
+template <typename T, typename R, bool kResidual, int kVectors, bool kBackward>
+constexpr int kUnitsOf = kVectors * ((kBackward ? 2 : 1) + (kResidual ? (int)(sizeof(R) / sizeof(T)) : 0));
+template <int kUnits, int kLanes>
+constexpr int kStagesOf = kLanes || kUnits <= 2 ? 4 : kUnits <= 4 ? 3 : 2;
+
 // R: the residual's type; kResidual false: there is none.
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes, bool kRagged>
 __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_forward_kernel(const NormArgs p) {
-    constexpr int W = kWidthOf<T>;
+    constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, false>, kStages = kStagesOf<kUnits, kLanes>;
+    extern __shared__ uint4 ring[];
     wait_for_previous_kernel();
     Team<kLanes> team = make_team<kLanes>();
     long long row, step;
     team_rows<kLanes>(row, step);
-    const Columns<W, kVectors, kLanes, kRagged> c(p.width, row, team.lane(), team.size());
-    Raw<T, W> x[kVectors];
-    Raw<R, W> r[kVectors];
-    load_row<T>(x, p.x, c, row, p.rows);
-    if (kResidual) load_row<R>(r, p.residual, c, row, p.rows);
+    const Columns<W, kVectors, kRagged> c(p.width, row, team.lane(), team.size());
+    const unsigned pitch = blockDim.x * 16, stage = pitch * kUnits;
+    const char *const mine = reinterpret_cast<const char *>(ring + threadIdx.x);
+    const unsigned slots = (unsigned)__cvta_generic_to_shared(mine);
+    long long at = row * p.width + c.first[0], left = p.rows - row;  // of the next row to be copied, then of the one that is worked on
+    const long long stride = step * p.width;
+    const auto issue = [&](int s) {
+        copy_row<T>(slots + s * stage, pitch, p.x, c, at, left);
+        if (kResidual) copy_row<R>(slots + s * stage + kVectors * pitch, pitch, p.residual, c, at, left);
+        copies_issued();
+        at += stride;
+        left -= step;
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) issue(s);
     float weight[kVectors][W], bias[kVectors][W];
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-            weight[i][j] = p.weight && c.has(i, j) ? load_as_f32(p.weight, p.param_dtype, c.first[i] + j) : 1.f;
-            bias[i][j] = p.bias && c.has(i, j) ? load_as_f32(p.bias, p.param_dtype, c.first[i] + j) : 0.f;
-        }
+    load_parameter<T>(p.weight, p.param_dtype, 1.f, c, weight);
+    load_parameter<T>(p.bias, p.param_dtype, 0.f, c, bias);
     const float inverse = 1.f / (float)p.width;
     // every lane of a warp stays to the end: they exchange sums
-    const long long lanes_first = kLanes ? row - threadIdx.x % 32 / (kLanes ? kLanes : 1) : row;
-    for (long long base = lanes_first; base < p.rows; base += step, row += step) {
-        float s[kVectors][W], sums[1] = {0.f};
+    int s = 0;
+    for (long long base = row - (kLanes ? threadIdx.x % 32 / (kLanes ? kLanes : 1) : 0); base < p.rows; base += step, row += step) {
+        float d[kVectors][W], sums[1] = {0.f};
+        wait_copies<kStages - 2>();
+        const char *const slot = mine + s * stage;
 #pragma unroll
         for (int i = 0; i < kVectors; ++i) {
-            x[i].get(s[i]);
+            read_vector<T>(slot, pitch, c, i, d[i]);
             if (kResidual) {
                 float extra[W];
-                r[i].get(extra);
+                read_vector<R>(slot + kVectors * pitch, pitch, c, i, extra);
 #pragma unroll
-                for (int j = 0; j < W; ++j) s[i][j] += extra[j];
+                for (int j = 0; j < W; ++j) d[i][j] += extra[j];
             }
 #pragma unroll
-            for (int j = 0; j < W; ++j) sums[0] += c.has(i, j) ? s[i][j] : 0.f;
+            for (int j = 0; j < W; ++j) sums[0] += d[i][j];
         }
-        load_row<T>(x, p.x, c, row + step, p.rows);
-        if (kResidual) load_row<R>(r, p.residual, c, row + step, p.rows);
+        issue(s == 0 ? kStages - 1 : s - 1);
+        const long long here = at - kStages * stride;
+        s = s == kStages - 1 ? 0 : s + 1;
         if (kResidual && p.sum && row < p.rows) {
 #pragma unroll
             for (int i = 0; i < kVectors; ++i)
-                if (c.any(i)) store_vector<R>(p.sum, s[i], c, i, row);
+                if (c.any(i)) store_vector<R>(p.sum, d[i], c, i, here);
         }
         team.sum(sums);
         const float mean = sums[0] * inverse;
@@ -162,8 +252,8 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
         for (int i = 0; i < kVectors; ++i)
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                s[i][j] = c.has(i, j) ? s[i][j] - mean : 0.f;
-                sums[0] += s[i][j] * s[i][j];
+                d[i][j] = fmaf(-mean, c.one(i, j), d[i][j]);
+                sums[0] = fmaf(d[i][j], d[i][j], sums[0]);
             }
         team.sum(sums);
         const float q = __frsqrt_rn(sums[0] * inverse + p.eps);
@@ -172,53 +262,65 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
         for (int i = 0; i < kVectors; ++i) {
             if (!c.any(i)) continue;
 #pragma unroll
-            for (int j = 0; j < W; ++j) s[i][j] = s[i][j] * q * weight[i][j] + bias[i][j];
-            store_vector<T>(p.y, s[i], c, i, row);
+            for (int j = 0; j < W; ++j) d[i][j] = fmaf(d[i][j] * q, weight[i][j], bias[i][j]);
+            store_vector<T>(p.y, d[i], c, i, here);
         }
     }
+    wait_copies<0>();
 }
 
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes, bool kRagged>
 __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_backward_kernel(const NormArgs p) {
-    constexpr int W = kWidthOf<T>;
+    constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, true>, kStages = kStagesOf<kUnits, kLanes>;
+    extern __shared__ uint4 ring[];
     wait_for_previous_kernel();
     Team<kLanes> team = make_team<kLanes>();
     long long row, step;
     team_rows<kLanes>(row, step);
-    const Columns<W, kVectors, kLanes, kRagged> c(p.width, row, team.lane(), team.size());
-    Raw<T, W> x[kVectors], dy[kVectors];
-    Raw<R, W> r[kVectors];
-    load_row<T>(x, p.x, c, row, p.rows);
-    load_row<T>(dy, p.grad_y, c, row, p.rows);
-    if (kResidual) load_row<R>(r, p.residual, c, row, p.rows);
+    const Columns<W, kVectors, kRagged> c(p.width, row, team.lane(), team.size());
+    const unsigned pitch = blockDim.x * 16, stage = pitch * kUnits;
+    const char *const mine = reinterpret_cast<const char *>(ring + threadIdx.x);
+    const unsigned slots = (unsigned)__cvta_generic_to_shared(mine);
+    long long at = row * p.width + c.first[0], left = p.rows - row;
+    const long long stride = step * p.width;
+    const auto issue = [&](int s) {
+        copy_row<T>(slots + s * stage, pitch, p.x, c, at, left);
+        copy_row<T>(slots + s * stage + kVectors * pitch, pitch, p.grad_y, c, at, left);
+        if (kResidual) copy_row<R>(slots + s * stage + 2 * kVectors * pitch, pitch, p.residual, c, at, left);
+        copies_issued();
+        at += stride;
+        left -= step;
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) issue(s);
     float weight[kVectors][W], grad_weight[kVectors][W], grad_bias[kVectors][W];
+    load_parameter<T>(p.weight, p.param_dtype, 1.f, c, weight);
 #pragma unroll
     for (int i = 0; i < kVectors; ++i)
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            weight[i][j] = p.weight && c.has(i, j) ? load_as_f32(p.weight, p.param_dtype, c.first[i] + j) : 1.f;
-            grad_weight[i][j] = grad_bias[i][j] = 0.f;
-        }
+        for (int j = 0; j < W; ++j) grad_weight[i][j] = grad_bias[i][j] = 0.f;
     const float inverse = 1.f / (float)p.width;
-    const long long lanes_first = kLanes ? row - threadIdx.x % 32 / (kLanes ? kLanes : 1) : row;
-    for (long long base = lanes_first; base < p.rows; base += step, row += step) {
-        float d[kVectors][W], g[kVectors][W], mean[1] = {0.f};
+    int s = 0;
+    for (long long base = row - (kLanes ? threadIdx.x % 32 / (kLanes ? kLanes : 1) : 0); base < p.rows; base += step, row += step) {
+        float d[kVectors][W], dy[kVectors][W], mean[1] = {0.f};
+        wait_copies<kStages - 2>();
+        const char *const slot = mine + s * stage;
 #pragma unroll
         for (int i = 0; i < kVectors; ++i) {
-            x[i].get(d[i]);
-            dy[i].get(g[i]);
+            read_vector<T>(slot, pitch, c, i, d[i]);
+            read_vector<T>(slot + kVectors * pitch, pitch, c, i, dy[i]);
             if (kResidual) {
                 float extra[W];
-                r[i].get(extra);
+                read_vector<R>(slot + 2 * kVectors * pitch, pitch, c, i, extra);
 #pragma unroll
                 for (int j = 0; j < W; ++j) d[i][j] += extra[j];
             }
 #pragma unroll
-            for (int j = 0; j < W; ++j) mean[0] += c.has(i, j) ? d[i][j] : 0.f;
+            for (int j = 0; j < W; ++j) mean[0] += d[i][j];
         }
-        load_row<T>(x, p.x, c, row + step, p.rows);
-        load_row<T>(dy, p.grad_y, c, row + step, p.rows);
-        if (kResidual) load_row<R>(r, p.residual, c, row + step, p.rows);
+        issue(s == 0 ? kStages - 1 : s - 1);
+        const long long here = at - kStages * stride;
+        s = s == kStages - 1 ? 0 : s + 1;
         team.sum(mean);
         mean[0] *= inverse;
         float sums[3] = {0.f, 0.f, 0.f};  // of d d, g d, g
@@ -226,11 +328,11 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
         for (int i = 0; i < kVectors; ++i)
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                d[i][j] = c.has(i, j) ? d[i][j] - mean[0] : 0.f;
-                const float gw = c.has(i, j) ? g[i][j] * weight[i][j] : 0.f;
-                sums[0] += d[i][j] * d[i][j];
-                sums[1] += gw * d[i][j];
-                sums[2] += gw;
+                d[i][j] = fmaf(-mean[0], c.one(i, j), d[i][j]);
+                const float g = dy[i][j] * weight[i][j];
+                sums[0] = fmaf(d[i][j], d[i][j], sums[0]);
+                sums[1] = fmaf(g, d[i][j], sums[1]);
+                sums[2] += g;
             }
         team.sum(sums);
         const float q = __frsqrt_rn(sums[0] * inverse + p.eps);
@@ -242,23 +344,29 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
             float ds[W];
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                const float dyv = c.has(i, j) ? g[i][j] : 0.f;
-                ds[j] = q * (dyv * weight[i][j] - level - d[i][j] * along);
-                grad_weight[i][j] += dyv * (d[i][j] * q);
-                grad_bias[i][j] += dyv;
+                ds[j] = q * (fmaf(dy[i][j], weight[i][j], -level) - d[i][j] * along);
+                grad_weight[i][j] = fmaf(dy[i][j], d[i][j] * q, grad_weight[i][j]);
+                grad_bias[i][j] += dy[i][j];
             }
             if (kResidual && p.grad_sum) {
-                Raw<R, W> raw;
-                load_vector<R, W, kRagged>(raw, static_cast<const R *>(p.grad_sum), row * p.width + c.first[i], p.rows * p.width);
+                const R *from = static_cast<const R *>(p.grad_sum) + here + (c.first[i] - c.first[0]);
                 float extra[W];
-                raw.get(extra);
+                if (c.whole(i)) {
+                    Raw<R, W> raw;
+                    raw.load(from);
+                    raw.get(extra);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) extra[j] = c.has(i, j) ? to_f32(from[j]) : 0.f;
+                }
 #pragma unroll
                 for (int j = 0; j < W; ++j) ds[j] += extra[j];
             }
-            if (p.grad_x) store_vector<T>(p.grad_x, ds, c, i, row);
-            if (kResidual && p.grad_residual) store_vector<R>(p.grad_residual, ds, c, i, row);
+            if (p.grad_x) store_vector<T>(p.grad_x, ds, c, i, here);
+            if (kResidual && p.grad_residual) store_vector<R>(p.grad_residual, ds, c, i, here);
         }
     }
+    wait_copies<0>();
     if (!p.partial) return;
     // the block's sums, column by column; with several teams in a fixed order
     float *out = p.partial + (size_t)blockIdx.x * 2 * p.width;
@@ -272,11 +380,26 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
                     out[p.width + c.first[i] + j] = grad_bias[i][j];
                 }
     } else {
-        extern __shared__ float columns[];  // [2][width]
+        // teams of a warp have the same columns unless rows are ragged
+        constexpr int kSteps = kRagged ? kTeamThreads / (kLanes ? kLanes : 1) : kTeamThreads / 32;
+        if (!kRagged) {
+#pragma unroll
+            for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    for (int o = kLanes; o < 32; o *= 2) {
+                        grad_weight[i][j] += __shfl_xor_sync(0xffffffffu, grad_weight[i][j], o);
+                        grad_bias[i][j] += __shfl_xor_sync(0xffffffffu, grad_bias[i][j], o);
+                    }
+        }
+        __syncthreads();
+        float *columns = reinterpret_cast<float *>(ring);  // [2][width]
         for (int i = threadIdx.x; i < 2 * p.width; i += kTeamThreads) columns[i] = 0.f;
-        for (int t = 0; t < kTeamThreads / (kLanes ? kLanes : 1); ++t) {
+        const int turn = kRagged ? (int)threadIdx.x / (kLanes ? kLanes : 1)
+                                 : (int)threadIdx.x % 32 < kLanes ? (int)threadIdx.x / 32 : -1;
+        for (int t = 0; t < kSteps; ++t) {
             __syncthreads();
-            if ((int)threadIdx.x / (kLanes ? kLanes : 1) != t) continue;
+            if (turn != t) continue;
 #pragma unroll
             for (int i = 0; i < kVectors; ++i)
 #pragma unroll
@@ -292,36 +415,38 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
-// Threads that share a row, and vectors of each.
+// Threads that share a row, and 16-byte vectors of each.
 struct NormShape {
     int lanes, vectors, threads;
     bool ragged;
 };
-// Up to 16 values of a row in a lane: twice as many spill in the backward (its sums take as many registers again).
-constexpr int kMostValues = 16;
-inline int most_fast_width(int) { return kBlockThreads * kMostValues - 16; }
+// 8 values of a row to a lane; 16 where that still lets a warp take the row, which saves the barriers of a block.
+constexpr int kMostValues = 8;
 
 inline NormShape norm_shape(int width, int dtype) {
     const int W = dtype == FDA_DTYPE_F32 ? 4 : 8;
     NormShape s;
     s.ragged = width % W != 0;
     const int vectors = (width + (s.ragged ? W - 1 : 0) + W - 1) / W;
-    s.lanes = vectors <= 8 ? 8 : 32;
+    s.vectors = kMostValues / W;
     s.threads = kTeamThreads;
-    s.vectors = 1;
-    while (s.vectors * W < kMostValues && s.lanes * s.vectors < vectors) s.vectors *= 2;
-    if (s.lanes * s.vectors < vectors) {
-        s.lanes = 0;
-        s.threads = (int)ceil_div(ceil_div(vectors, s.vectors), 32) * 32;
-    }
+    for (s.lanes = 4; s.lanes <= 32; s.lanes *= 2)
+        if (s.lanes * s.vectors >= vectors) return s;
+    s.lanes = 32;
+    s.vectors *= 2;
+    if (s.lanes * s.vectors >= vectors) return s;
+    s.vectors /= 2;
+    s.lanes = 0;
+    s.threads = (int)ceil_div(ceil_div(vectors, s.vectors), 32) * 32;
     return s;
 }
+inline bool is_wide(int width, int dtype) { return norm_shape(width, dtype).threads > kBlockThreads; }  // for a block's registers
 
 // Blocks: as many as rows need, at most what fills the device; a multiple of 8 where a block is a team (rows 8 apart).
-inline unsigned norm_blocks(const NormShape &s, long long rows, int most_per_sm) {
-    const long long per_block = s.lanes ? s.threads / s.lanes : 1;
-    const long long needed = ceil_div(rows, per_block);
-    const long long room = (long long)kSms * most_per_sm;
+inline unsigned norm_blocks(const NormShape &s, long long rows, bool backward) {
+    const long long needed = ceil_div(rows, s.lanes ? s.threads / s.lanes : 1);
+    const int per_sm = s.lanes ? (backward ? 2 : 4) : (backward ? 1024 : 2048) / s.threads;
+    const long long room = (long long)kSms * (per_sm > 0 ? per_sm : 1);
     long long blocks = needed < room ? needed : room;
     if (!s.lanes) blocks = ceil_div(blocks, 8) * 8;
     return (unsigned)blocks;
@@ -334,27 +459,27 @@ int norm_bf16(bool backward, const NormArgs &p, const NormShape &s, int residual
 
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes>
 int run_norm(bool backward, const NormArgs &p, const NormShape &s, unsigned blocks, cudaStream_t st) {
-    if (backward) {
-        const int shared = kLanes && p.partial ? 2 * p.width * (int)sizeof(float) : 0;
-        return launched(launch_early(s.ragged ? norm_backward_kernel<T, R, kResidual, kVectors, kLanes, true>
-                                              : norm_backward_kernel<T, R, kResidual, kVectors, kLanes, false>,
-                                     blocks, s.threads, shared, st, 1, p));
-    }
-    return launched(launch_early(s.ragged ? norm_forward_kernel<T, R, kResidual, kVectors, kLanes, true>
-                                          : norm_forward_kernel<T, R, kResidual, kVectors, kLanes, false>,
-                                 blocks, s.threads, 0, st, 1, p));
+    constexpr int kForward = kUnitsOf<T, R, kResidual, kVectors, false>, kBackward = kUnitsOf<T, R, kResidual, kVectors, true>;
+    const int units = backward ? kBackward * kStagesOf<kBackward, kLanes> : kForward * kStagesOf<kForward, kLanes>;
+    const int shared = units * s.threads * 16;
+    const auto kernel = backward ? (s.ragged ? norm_backward_kernel<T, R, kResidual, kVectors, kLanes, true>
+                                             : norm_backward_kernel<T, R, kResidual, kVectors, kLanes, false>)
+                                 : (s.ragged ? norm_forward_kernel<T, R, kResidual, kVectors, kLanes, true>
+                                             : norm_forward_kernel<T, R, kResidual, kVectors, kLanes, false>);
+    if (shared > 40 * 1024)  // with the static part beyond what every launch may have; the attribute belongs to the current device
+        if (const int rc = launched(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared))) return rc;
+    return launched(launch_early(kernel, blocks, s.threads, shared, st, 1, p));
 }
 
 template <typename T, typename R, bool kResidual>
 int run_norm(bool backward, const NormArgs &p, const NormShape &s, unsigned blocks, cudaStream_t st) {
-    constexpr int kMost = kMostValues / kWidthOf<T>;
-    if (s.lanes == 8) return run_norm<T, R, kResidual, 1, 8>(backward, p, s, blocks, st);
-    if (s.lanes == 32) {
-        if (s.vectors == 1) return run_norm<T, R, kResidual, 1, 32>(backward, p, s, blocks, st);
-        if (s.vectors == 2) return run_norm<T, R, kResidual, 2, 32>(backward, p, s, blocks, st);
-        return run_norm<T, R, kResidual, kMost, 32>(backward, p, s, blocks, st);
-    }
-    return run_norm<T, R, kResidual, kMost, 0>(backward, p, s, blocks, st);
+    constexpr int kEach = kMostValues / kWidthOf<T>;
+    if (s.lanes == 4) return run_norm<T, R, kResidual, kEach, 4>(backward, p, s, blocks, st);
+    if (s.lanes == 8) return run_norm<T, R, kResidual, kEach, 8>(backward, p, s, blocks, st);
+    if (s.lanes == 16) return run_norm<T, R, kResidual, kEach, 16>(backward, p, s, blocks, st);
+    if (s.lanes == 0) return run_norm<T, R, kResidual, kEach, 0>(backward, p, s, blocks, st);
+    if (s.vectors == kEach) return run_norm<T, R, kResidual, kEach, 32>(backward, p, s, blocks, st);
+    return run_norm<T, R, kResidual, 2 * kEach, 32>(backward, p, s, blocks, st);
 }
 
 template <typename T>

@@ -66,6 +66,17 @@ struct Raw {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) reinterpret_cast<uint4 *>(p)[i] = u[i];
     }
+    // Element j, known when this is compiled.
+    __device__ __forceinline__ T element(int j) const {
+        const uint4 &a = u[j * (int)sizeof(T) / 16];
+        const int k = j * (int)sizeof(T) / 4 % 4;
+        const unsigned w = k == 0 ? a.x : k == 1 ? a.y : k == 2 ? a.z : a.w;
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+        else {
+            const unsigned short h = (unsigned short)(j % 2 ? w >> 16 : w);
+            return *reinterpret_cast<const T *>(&h);
+        }
+    }
     __device__ __forceinline__ void get(float *v) const {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
@@ -123,27 +134,32 @@ struct Team {
 };
 template <>
 struct Team<0> {
-    static constexpr int kMost = 3, kWarps = 16;
-    float (*shared)[kMost][kWarps];  // [2]: a buffer is written again only after everyone has passed the barrier behind the other
+    static constexpr int kMost = 3, kWarps = 32;
+    float (*shared)[kMost][kWarps];  // [2], 0 for warps that are not there; a buffer is written again only after everyone has passed the barrier
+                                     // behind the other
     int buffer = 0;
     __device__ __forceinline__ int lane() const { return threadIdx.x; }
     __device__ __forceinline__ int size() const { return blockDim.x; }
     template <int kCount>
     __device__ __forceinline__ void sum(float (&v)[kCount]) {
         static_assert(kCount <= kMost, "");
-        const int warps = blockDim.x / 32;
 #pragma unroll
         for (int k = 0; k < kCount; ++k) {
             v[k] = lanes_sum<32>(v[k]);
             if (threadIdx.x % 32 == 0) shared[buffer][k][threadIdx.x / 32] = v[k];
         }
         __syncthreads();
+        float4 s[kCount];
 #pragma unroll
-        for (int k = 0; k < kCount; ++k) {
-            float s = shared[buffer][k][0];
-            for (int w = 1; w < warps; ++w) s += shared[buffer][k][w];
-            v[k] = s;
-        }
+        for (int k = 0; k < kCount; ++k) s[k] = *reinterpret_cast<const float4 *>(shared[buffer][k]);
+        for (int w = 4; w < (int)blockDim.x / 32; w += 4)
+#pragma unroll
+            for (int k = 0; k < kCount; ++k) {
+                const float4 o = *reinterpret_cast<const float4 *>(shared[buffer][k] + w);
+                s[k].x += o.x; s[k].y += o.y; s[k].z += o.z; s[k].w += o.w;
+            }
+#pragma unroll
+        for (int k = 0; k < kCount; ++k) v[k] = (s[k].x + s[k].y) + (s[k].z + s[k].w);
         buffer ^= 1;
     }
 };
