@@ -42,8 +42,8 @@ struct Columns {
     int first[kVectors];                // column of the first element; may be negative where kRagged
     int count[kVectors];                // elements from the first to the row's end, at most kWidth; 0 where the row has none
     unsigned bits[kVectors];            // bit j: element j is one of the row's
-    float valid[kVectors][kRagged ? kWidth : 1];  // the same as factors
-    unsigned keep[kVectors][kRagged ? 4 : 1];     // and as a mask of the vector's words
+    Pair valid[kVectors][kRagged ? kWidth / 2 : 1];  // the same as factors
+    unsigned keep[kVectors][kRagged ? 4 : 1];        // and as a mask of the vector's words
     __device__ __forceinline__ Columns(int width, long long row, int lane, int size) : width(width) {
         const int shift = kRagged ? (int)((row * width) % kWidth) : 0;
 #pragma unroll
@@ -56,19 +56,20 @@ struct Columns {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) keep[i][k] = 0;
 #pragma unroll
+                for (int j = 0; j < kWidth / 2; ++j) valid[i][j] = Pair(has(i, 2 * j) ? 1.f : 0.f, has(i, 2 * j + 1) ? 1.f : 0.f);
+#pragma unroll
                 for (int j = 0; j < kWidth; ++j) {
-                    valid[i][j] = has(i, j) ? 1.f : 0.f;
                     if (has(i, j)) keep[i][j * 4 / kWidth] |= kWidth == 4 ? 0xffffffffu : 0xffffu << (j % 2 * 16);
                 }
             } else {
-                valid[i][0] = count[i] ? 1.f : 0.f;
+                valid[i][0] = Pair(count[i] ? 1.f : 0.f);
             }
         }
     }
     __device__ __forceinline__ bool any(int i) const { return count[i] != 0; }
     __device__ __forceinline__ bool whole(int i) const { return !kRagged || bits[i] == (1u << kWidth) - 1; }
     __device__ __forceinline__ bool has(int i, int j) const { return bits[i] >> j & 1; }
-    __device__ __forceinline__ float one(int i, int j) const { return valid[i][kRagged ? j : 0]; }
+    __device__ __forceinline__ Pair ones(int i, int j) const { return valid[i][kRagged ? j : 0]; }  // of elements 2 j and 2 j + 1
 };
 
 // Rows on their way: every lane copies its own vectors into its own places of a ring in shared memory, kStages - 1 rows ahead of the one
@@ -100,27 +101,32 @@ __device__ __forceinline__ void copy_row(unsigned slot, unsigned pitch, const vo
 
 // A lane's vector i from its place, elements of neighbouring rows as 0.
 template <typename E, int kWidth, int kVectors, bool kRagged>
-__device__ __forceinline__ void read_vector(const char *slot, unsigned pitch, const Columns<kWidth, kVectors, kRagged> &c, int i, float *v) {
+__device__ __forceinline__ void read_vector(const char *slot, unsigned pitch, const Columns<kWidth, kVectors, kRagged> &c, int i, Pair *v) {
     constexpr int kUnits = kWidth * (int)sizeof(E) / 16;
     Raw<E, kWidth> raw;
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) raw.u[u] = *reinterpret_cast<const uint4 *>(slot + (i * kUnits + u) * pitch);
-    if (kRagged && kUnits == 1) {
+    if constexpr (kRagged && kUnits == 1) {
         raw.u[0].x &= c.keep[i][0];
-        raw.u[0].y &= c.keep[i][kRagged ? 1 : 0];
-        raw.u[0].z &= c.keep[i][kRagged ? 2 : 0];
-        raw.u[0].w &= c.keep[i][kRagged ? 3 : 0];
+        raw.u[0].y &= c.keep[i][1];
+        raw.u[0].z &= c.keep[i][2];
+        raw.u[0].w &= c.keep[i][3];
     }
-    raw.get(v);
-    if (kRagged && kUnits > 1) {
+    if constexpr (kRagged && kUnits > 1) {
+        float f[kWidth];
+        raw.get(f);
 #pragma unroll
-        for (int j = 0; j < kWidth; ++j) v[j] = c.one(i, j) != 0.f ? v[j] : 0.f;
+        for (int j = 0; j < kWidth; ++j) f[j] = c.has(i, j) ? f[j] : 0.f;
+#pragma unroll
+        for (int j = 0; j < kWidth / 2; ++j) v[j] = Pair(f[2 * j], f[2 * j + 1]);
+    } else {
+        raw.get(v);
     }
 }
 
 // at: as above, of the row that is stored.
 template <typename E, int kWidth, int kVectors, bool kRagged>
-__device__ __forceinline__ void store_vector(void *tensor, const float *v, const Columns<kWidth, kVectors, kRagged> &c, int i, long long at) {
+__device__ __forceinline__ void store_vector(void *tensor, const Pair *v, const Columns<kWidth, kVectors, kRagged> &c, int i, long long at) {
     E *to = static_cast<E *>(tensor) + at + (c.first[i] - c.first[0]);
     Raw<E, kWidth> raw;
     raw.set(v);
@@ -152,14 +158,20 @@ __device__ __forceinline__ void load_parameter(const E *tensor, const Columns<kW
 }
 template <typename T, int kWidth, int kVectors, bool kRagged>
 __device__ __forceinline__ void load_parameter(const void *tensor, int dtype, float otherwise, const Columns<kWidth, kVectors, kRagged> &c,
-                                               float (&v)[kVectors][kWidth]) {
+                                               Pair (&pairs)[kVectors][kWidth / 2]) {
+    float v[kVectors][kWidth];
 #pragma unroll
     for (int i = 0; i < kVectors; ++i)
 #pragma unroll
         for (int j = 0; j < kWidth; ++j) v[i][j] = otherwise;
-    if (!tensor) return;
-    if (dtype == FDA_DTYPE_F32) load_parameter(static_cast<const float *>(tensor), c, v);
-    else load_parameter(static_cast<const T *>(tensor), c, v);
+    if (tensor) {
+        if (dtype == FDA_DTYPE_F32) load_parameter(static_cast<const float *>(tensor), c, v);
+        else load_parameter(static_cast<const T *>(tensor), c, v);
+    }
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+        for (int j = 0; j < kWidth / 2; ++j) pairs[i][j] = Pair(v[i][2 * j], v[i][2 * j + 1]);
 }
 
 // Which rows a team takes: the first one, and how far apart they are (a multiple of kWidth, because a grid's blocks are where a block
@@ -215,27 +227,29 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
     };
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) issue(s);
-    float weight[kVectors][W], bias[kVectors][W];
+    constexpr int H = W / 2;
+    Pair weight[kVectors][H], bias[kVectors][H];
     load_parameter<T>(p.weight, p.param_dtype, 1.f, c, weight);
     load_parameter<T>(p.bias, p.param_dtype, 0.f, c, bias);
     const float inverse = 1.f / (float)p.width;
     // every lane of a warp stays to the end: they exchange sums
     int s = 0;
     for (long long base = row - (kLanes ? threadIdx.x % 32 / (kLanes ? kLanes : 1) : 0); base < p.rows; base += step, row += step) {
-        float d[kVectors][W], sums[1] = {0.f};
+        Pair d[kVectors][H], add(0.f);
+        float sums[1];
         wait_copies<kStages - 2>();
         const char *const slot = mine + s * stage;
 #pragma unroll
         for (int i = 0; i < kVectors; ++i) {
             read_vector<T>(slot, pitch, c, i, d[i]);
             if (kResidual) {
-                float extra[W];
+                Pair extra[H];
                 read_vector<R>(slot + kVectors * pitch, pitch, c, i, extra);
 #pragma unroll
-                for (int j = 0; j < W; ++j) d[i][j] += extra[j];
+                for (int j = 0; j < H; ++j) d[i][j] = d[i][j] + extra[j];
             }
 #pragma unroll
-            for (int j = 0; j < W; ++j) sums[0] += d[i][j];
+            for (int j = 0; j < H; ++j) add = add + d[i][j];
         }
         issue(s == 0 ? kStages - 1 : s - 1);
         const long long here = at - kStages * stride;
@@ -245,24 +259,26 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
             for (int i = 0; i < kVectors; ++i)
                 if (c.any(i)) store_vector<R>(p.sum, d[i], c, i, here);
         }
+        sums[0] = add.sum();
         team.sum(sums);
-        const float mean = sums[0] * inverse;
-        sums[0] = 0.f;
+        const Pair minus_mean(-sums[0] * inverse);
+        Pair square(0.f);
 #pragma unroll
         for (int i = 0; i < kVectors; ++i)
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                d[i][j] = fmaf(-mean, c.one(i, j), d[i][j]);
-                sums[0] = fmaf(d[i][j], d[i][j], sums[0]);
+            for (int j = 0; j < H; ++j) {
+                d[i][j] = fma2(minus_mean, c.ones(i, j), d[i][j]);
+                square = fma2(d[i][j], d[i][j], square);
             }
+        sums[0] = square.sum();
         team.sum(sums);
-        const float q = __frsqrt_rn(sums[0] * inverse + p.eps);
+        const Pair q(__frsqrt_rn(sums[0] * inverse + p.eps));
         if (row >= p.rows) continue;
 #pragma unroll
         for (int i = 0; i < kVectors; ++i) {
             if (!c.any(i)) continue;
 #pragma unroll
-            for (int j = 0; j < W; ++j) d[i][j] = fmaf(d[i][j] * q, weight[i][j], bias[i][j]);
+            for (int j = 0; j < H; ++j) d[i][j] = fma2(d[i][j] * q, weight[i][j], bias[i][j]);
             store_vector<T>(p.y, d[i], c, i, here);
         }
     }
@@ -293,16 +309,17 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
     };
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) issue(s);
-    float weight[kVectors][W], grad_weight[kVectors][W], grad_bias[kVectors][W];
+    constexpr int H = W / 2;
+    Pair weight[kVectors][H], weight_sum[kVectors][H], bias_sum[kVectors][H];
     load_parameter<T>(p.weight, p.param_dtype, 1.f, c, weight);
 #pragma unroll
     for (int i = 0; i < kVectors; ++i)
 #pragma unroll
-        for (int j = 0; j < W; ++j) grad_weight[i][j] = grad_bias[i][j] = 0.f;
+        for (int j = 0; j < H; ++j) weight_sum[i][j] = bias_sum[i][j] = Pair(0.f);
     const float inverse = 1.f / (float)p.width;
     int s = 0;
     for (long long base = row - (kLanes ? threadIdx.x % 32 / (kLanes ? kLanes : 1) : 0); base < p.rows; base += step, row += step) {
-        float d[kVectors][W], dy[kVectors][W], mean[1] = {0.f};
+        Pair d[kVectors][H], dy[kVectors][H], add(0.f);
         wait_copies<kStages - 2>();
         const char *const slot = mine + s * stage;
 #pragma unroll
@@ -310,43 +327,45 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
             read_vector<T>(slot, pitch, c, i, d[i]);
             read_vector<T>(slot + kVectors * pitch, pitch, c, i, dy[i]);
             if (kResidual) {
-                float extra[W];
+                Pair extra[H];
                 read_vector<R>(slot + 2 * kVectors * pitch, pitch, c, i, extra);
 #pragma unroll
-                for (int j = 0; j < W; ++j) d[i][j] += extra[j];
+                for (int j = 0; j < H; ++j) d[i][j] = d[i][j] + extra[j];
             }
 #pragma unroll
-            for (int j = 0; j < W; ++j) mean[0] += d[i][j];
+            for (int j = 0; j < H; ++j) add = add + d[i][j];
         }
         issue(s == 0 ? kStages - 1 : s - 1);
         const long long here = at - kStages * stride;
         s = s == kStages - 1 ? 0 : s + 1;
+        float mean[1] = {add.sum()};
         team.sum(mean);
-        mean[0] *= inverse;
-        float sums[3] = {0.f, 0.f, 0.f};  // of d d, g d, g
+        const Pair minus_mean(-mean[0] * inverse);
+        Pair dd(0.f), gd(0.f), gg(0.f);
 #pragma unroll
         for (int i = 0; i < kVectors; ++i)
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                d[i][j] = fmaf(-mean[0], c.one(i, j), d[i][j]);
-                const float g = dy[i][j] * weight[i][j];
-                sums[0] = fmaf(d[i][j], d[i][j], sums[0]);
-                sums[1] = fmaf(g, d[i][j], sums[1]);
-                sums[2] += g;
+            for (int j = 0; j < H; ++j) {
+                d[i][j] = fma2(minus_mean, c.ones(i, j), d[i][j]);
+                const Pair g = dy[i][j] * weight[i][j];
+                dd = fma2(d[i][j], d[i][j], dd);
+                gd = fma2(g, d[i][j], gd);
+                gg = gg + g;
             }
+        float sums[3] = {dd.sum(), gd.sum(), gg.sum()};
         team.sum(sums);
-        const float q = __frsqrt_rn(sums[0] * inverse + p.eps);
-        const float along = q * q * sums[1] * inverse, level = sums[2] * inverse;
+        const float scale = __frsqrt_rn(sums[0] * inverse + p.eps);
         if (row >= p.rows) continue;
+        const Pair q(scale), level(-scale * (sums[2] * inverse)), along(-scale * (scale * scale * (sums[1] * inverse)));
 #pragma unroll
         for (int i = 0; i < kVectors; ++i) {
             if (!c.any(i)) continue;
-            float ds[W];
+            Pair ds[H];
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                ds[j] = q * (fmaf(dy[i][j], weight[i][j], -level) - d[i][j] * along);
-                grad_weight[i][j] = fmaf(dy[i][j], d[i][j] * q, grad_weight[i][j]);
-                grad_bias[i][j] += dy[i][j];
+            for (int j = 0; j < H; ++j) {
+                ds[j] = fma2(dy[i][j] * weight[i][j], q, fma2(d[i][j], along, level));
+                weight_sum[i][j] = fma2(dy[i][j], d[i][j] * q, weight_sum[i][j]);
+                bias_sum[i][j] = bias_sum[i][j] + dy[i][j];
             }
             if (kResidual && p.grad_sum) {
                 const R *from = static_cast<const R *>(p.grad_sum) + here + (c.first[i] - c.first[0]);
@@ -360,7 +379,7 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
                     for (int j = 0; j < W; ++j) extra[j] = c.has(i, j) ? to_f32(from[j]) : 0.f;
                 }
 #pragma unroll
-                for (int j = 0; j < W; ++j) ds[j] += extra[j];
+                for (int j = 0; j < H; ++j) ds[j] = ds[j] + Pair(extra[2 * j], extra[2 * j + 1]);
             }
             if (p.grad_x) store_vector<T>(p.grad_x, ds, c, i, here);
             if (kResidual && p.grad_residual) store_vector<R>(p.grad_residual, ds, c, i, here);
@@ -369,6 +388,14 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
     wait_copies<0>();
     if (!p.partial) return;
     // the block's sums, column by column; with several teams in a fixed order
+    float grad_weight[kVectors][W], grad_bias[kVectors][W];
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+            weight_sum[i][j].get(grad_weight[i][2 * j], grad_weight[i][2 * j + 1]);
+            bias_sum[i][j].get(grad_bias[i][2 * j], grad_bias[i][2 * j + 1]);
+        }
     float *out = p.partial + (size_t)blockIdx.x * 2 * p.width;
     if constexpr (kLanes == 0) {
 #pragma unroll

@@ -48,6 +48,35 @@ template <> __device__ __forceinline__ unsigned pack<__half>(float a, float b) {
     return *reinterpret_cast<const unsigned *>(&v);
 }
 
+// Two fp32 numbers that one instruction works on.
+struct Pair {
+    unsigned long long bits;
+    __device__ __forceinline__ Pair() {}
+    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ explicit Pair(float a) : Pair(a, a) {}
+    __device__ __forceinline__ void get(float &a, float &b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(bits)); }
+    __device__ __forceinline__ float sum() const {
+        float a, b;
+        get(a, b);
+        return a + b;
+    }
+};
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+    return r;
+}
+
 // kWidth neighbouring elements as they lie in memory: 16 or 32 bytes.
 template <typename T, int kWidth>
 struct Raw {
@@ -87,6 +116,18 @@ struct Raw {
                 else unpack<T>(w[j], v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
             }
         }
+    }
+    __device__ __forceinline__ void get(Pair *v) const {
+        float f[kWidth];
+        get(f);
+#pragma unroll
+        for (int j = 0; j < kWidth / 2; ++j) v[j] = Pair(f[2 * j], f[2 * j + 1]);
+    }
+    __device__ __forceinline__ void set(const Pair *v) {
+        float f[kWidth];
+#pragma unroll
+        for (int j = 0; j < kWidth / 2; ++j) v[j].get(f[2 * j], f[2 * j + 1]);
+        set(f);
     }
     __device__ __forceinline__ void set(const float *v) {
 #pragma unroll
@@ -149,17 +190,16 @@ struct Team<0> {
             if (threadIdx.x % 32 == 0) shared[buffer][k][threadIdx.x / 32] = v[k];
         }
         __syncthreads();
-        float4 s[kCount];
-#pragma unroll
-        for (int k = 0; k < kCount; ++k) s[k] = *reinterpret_cast<const float4 *>(shared[buffer][k]);
-        for (int w = 4; w < (int)blockDim.x / 32; w += 4)
+        if (blockDim.x <= 128) {
 #pragma unroll
             for (int k = 0; k < kCount; ++k) {
-                const float4 o = *reinterpret_cast<const float4 *>(shared[buffer][k] + w);
-                s[k].x += o.x; s[k].y += o.y; s[k].z += o.z; s[k].w += o.w;
+                const float4 s = *reinterpret_cast<const float4 *>(shared[buffer][k]);
+                v[k] = (s.x + s.y) + (s.z + s.w);
             }
+        } else {
 #pragma unroll
-        for (int k = 0; k < kCount; ++k) v[k] = (s[k].x + s[k].y) + (s[k].z + s[k].w);
+            for (int k = 0; k < kCount; ++k) v[k] = lanes_sum<32>(shared[buffer][k][threadIdx.x % 32]);
+        }
         buffer ^= 1;
     }
 };
