@@ -530,7 +530,7 @@ int fda_route_backward(const void *logits, const int64_t *experts, const float *
  *   position [tokens][top_k] int64: the row of each entry, in the entries' order within an expert; -1 for none
  *   fda_dispatch_rows: rows [tokens * top_k][features]: rows[position] = x[token]; rows behind the last expert's are 0
  *   fda_combine_rows:  y[token] = sum over its entries of weight * rows[position] + residual
- *                      weights [tokens][top_k] of `weight_dtype` or NULL (1), residual [tokens][features] or NULL
+ *                      weights [tokens][top_k] of `weight_dtype` (`dtype` or f32) or NULL (1), residual [tokens][features] or NULL
  * fda_combine_rows without weights is the gradient of fda_dispatch_rows.  fda_combine_rows_backward: grad_rows[position] = weight *
  * grad_y[token] (0 in rows from *rows_end on, which is group_start_index + n_experts), grad_weights = <rows[position], grad_y[token]>,
  * 0 where there is no row; either may be NULL.  `position` and `rows_end` are those of fda_dispatch_rows: no entry leads out of `rows`

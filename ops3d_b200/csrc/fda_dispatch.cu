@@ -31,25 +31,12 @@ struct MoveArgs {
     const void *rows, *x, *weights, *residual, *grad;
     const int64_t *position, *end;  // end: where the last expert's rows end
     void *out, *grad_weights;
-    long long tokens;
-    int top_k, width, weight_dtype;
-    int slots, passes;  // vectors that a row can touch, and how often a team of lanes takes some of them
+    long long tokens, entries;
+    int top_k, width, passes;  // passes: how often a team of lanes takes vectors of a row
+    bool wide_weights;         // fp32, else in the rows' type
 };
 
 template <typename T> constexpr int kWidthOf = 16 / (int)sizeof(T);
-
-// Vector number `at` of a tensor of `total` elements; 0 outside.
-template <typename T, bool kRagged>
-__device__ __forceinline__ uint4 load_vector(const T *tensor, long long at, long long total) {
-    constexpr int W = kWidthOf<T>;
-    if (kRagged && (at < 0 || at * W + W > total)) {
-        alignas(16) T v[W];
-#pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = at >= 0 && at * W + j < total ? tensor[at * W + j] : from_f32<T>(0.f);
-        return *reinterpret_cast<const uint4 *>(v);
-    }
-    return reinterpret_cast<const uint4 *>(tensor)[at];
-}
 
 // Elements by, by + 1, ... of the vectors a and b, one behind the other.
 template <typename T>
@@ -72,58 +59,104 @@ __device__ __forceinline__ uint4 next_lane(uint4 v) {
     return make_uint4(__shfl_down_sync(kAll, v.x, 1), __shfl_down_sync(kAll, v.y, 1), __shfl_down_sync(kAll, v.z, 1), __shfl_down_sync(kAll, v.w, 1));
 }
 
-// A row that vectors of one tensor are aligned to: slot i holds its elements first, first + 1, ...
-template <typename T, bool kRagged>
-struct Slot {
-    long long vector;  // in the tensor
-    int first, width;
-    __device__ __forceinline__ Slot(long long row, int width, int i) : width(width) {
-        constexpr int W = kWidthOf<T>;
-        const long long start = row * width;
-        const int lead = kRagged ? (int)(start % W) : 0;
-        vector = start / W + i;
-        first = i * W - lead;
+// A tensor of rows.  Row numbers and offsets inside a row have 31 bits, their products 64.
+template <typename T>
+struct Rows {
+    static constexpr int W = kWidthOf<T>;
+    T *base;
+    const T *end;
+    unsigned width;
+    __device__ __forceinline__ Rows(const void *tensor, long long rows, int width)
+        : base(const_cast<T *>(static_cast<const T *>(tensor))), end(base + rows * width), width(width) {}
+    // Where a row starts in its first vector.
+    __device__ __forceinline__ int lead(int row) const { return (int)((unsigned)row * width % W); }
+    __device__ __forceinline__ T *at(int row, int column) const { return base + ((unsigned long long)(unsigned)row * width + (long long)column); }
+    // The vector that starts on a boundary; outside the tensor 0.
+    template <bool kRagged>
+    __device__ __forceinline__ uint4 load(const T *from) const {
+        if (kRagged && (from < base || from + W > end)) {
+            alignas(16) T v[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[j] = from + j >= base && from + j < end ? from[j] : from_f32<T>(0.f);
+            return *reinterpret_cast<const uint4 *>(v);
+        }
+        return *reinterpret_cast<const uint4 *>(from);
     }
-    __device__ __forceinline__ bool any() const { return first < width; }
-    __device__ __forceinline__ bool whole() const { return !kRagged || (first >= 0 && first + kWidthOf<T> <= width); }
-    __device__ __forceinline__ bool has(int j) const { return !kRagged || (first + j >= 0 && first + j < width); }
-    __device__ __forceinline__ void store(T *tensor, uint4 v) const {
-        if (!any()) return;
-        if (whole()) {
-            reinterpret_cast<uint4 *>(tensor)[vector] = v;
+    // Elements column .. column + W - 1 of a row, -W < column; what is not in the row may be anything.  Where rows are ragged every lane
+    // of the warp takes part, and a lane needs the next one to have the next W columns.  `there` false: 0, nothing is read.
+    template <bool kRagged>
+    __device__ __forceinline__ uint4 fetch(int row, int column, bool there) const {
+        const uint4 none = make_uint4(0, 0, 0, 0);
+        if (!kRagged) return there && column < (int)width ? load<false>(at(row, column)) : none;
+        const T *from = at(row, column);
+        const int by = (int)((uintptr_t)from % 16) / (int)sizeof(T);
+        const uint4 a = there && column < (int)width + W ? load<true>(from - by) : none;
+        return shifted<T>(a, next_lane(a), by);
+    }
+    // Columns column .. of a row at a vector's boundary; those outside the row stay as they are.
+    template <bool kRagged>
+    __device__ __forceinline__ void store(int row, int column, uint4 v) const {
+        if (column >= (int)width) return;
+        T *to = at(row, column);
+        if (!kRagged || (column >= 0 && column + W <= (int)width)) {
+            *reinterpret_cast<uint4 *>(to) = v;
             return;
         }
-        Raw<T, kWidthOf<T>> raw;
+        Raw<T, W> raw;
         raw.u[0] = v;
+        const unsigned bits = ((1u << min(W, (int)width - column)) - 1) & ~((1u << max(0, -column)) - 1);
 #pragma unroll
-        for (int j = 0; j < kWidthOf<T>; ++j)
-            if (has(j)) tensor[vector * kWidthOf<T> + j] = raw.element(j);
-    }
-    // The same elements of the row `row` of a tensor of rows as wide; with elements of its neighbours where has(j) is false.  Every
-    // lane of the warp takes part; `there` false: 0.
-    __device__ __forceinline__ uint4 fetch(const T *tensor, long long row, long long rows, bool there) const {
-        constexpr int W = kWidthOf<T>;
-        there = there && any();
-        if (!kRagged) return there ? reinterpret_cast<const uint4 *>(tensor)[row * (width / W) + first / W] : make_uint4(0, 0, 0, 0);
-        const long long from = row * width + first;
-        const long long at = from >= 0 ? from / W : -1;  // above -W
-        const uint4 a = row >= 0 && first - W < width ? load_vector<T, true>(tensor, at, rows * width) : make_uint4(0, 0, 0, 0);
-        const uint4 v = shifted<T>(a, next_lane(a), (int)(from - at * W));
-        return there ? v : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < W; ++j)
+            if (bits >> j & 1) to[j] = raw.element(j);
     }
 };
 
-// A position that leads nowhere counts as none.
-__device__ __forceinline__ long long row_of(const MoveArgs &p, long long entry) {
-    const int64_t at = p.position[entry];
-    return at >= 0 && at < p.tokens * p.top_k ? at : -1;
+// A vector of a row that starts at `column`: elements outside the row as 0.
+template <typename T>
+__device__ __forceinline__ uint4 inside(uint4 v, int column, int width) {
+    constexpr int kBits = (int)sizeof(T) * 8;
+    const int low = max(0, -column) * kBits, high = max(0, min(kWidthOf<T>, width - column)) * kBits;
+    unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int from = min(max(low - 32 * i, 0), 32), to = min(max(high - 32 * i, 0), 32);
+        w[i] &= (unsigned)((0xffffffffull << from) & (0xffffffffull >> (32 - to)));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
+
+// Positions and weights of kAtOnce choices of a token, as they are read; a choice beyond the last has none.
+template <int kAtOnce>
+struct Choices {
+    int64_t position[kAtOnce];
+    float weight[kAtOnce];
+    template <typename T>
+    __device__ __forceinline__ void load(const MoveArgs &p, long long token, int j, bool there) {
+        const long long entry = token * p.top_k + j;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const bool one = there && j + i < p.top_k;
+            position[i] = one ? p.position[entry + i] : -1;
+            weight[i] = 1.f;
+        }
+        if (!p.weights) return;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const bool one = there && j + i < p.top_k;
+            if (one) weight[i] = p.wide_weights ? static_cast<const float *>(p.weights)[entry + i] : to_f32(static_cast<const T *>(p.weights)[entry + i]);
+        }
+    }
+    // The row; -1 for a position that leads nowhere.
+    __device__ __forceinline__ int row(const MoveArgs &p, int i) const {
+        return (unsigned long long)position[i] < (unsigned long long)p.entries ? (int)position[i] : -1;
+    }
+};
 
 // Rows first .. last - 1 are 0.
 template <typename T, bool kRagged>
-__device__ __forceinline__ void clear_rows(const MoveArgs &p, T *rows, long long first, long long last, long long thread, long long threads) {
+__device__ __forceinline__ void clear_rows(T *rows, int width, long long first, long long last, long long thread, long long threads) {
     constexpr int W = kWidthOf<T>;
-    const long long begin = first * p.width, end = last * p.width;
+    const long long begin = first * width, end = last * width;
     for (long long v = begin / W + thread; v * W < end; v += threads) {
         if (!kRagged || (v * W >= begin && v * W + W <= end)) {
             reinterpret_cast<uint4 *>(rows)[v] = make_uint4(0, 0, 0, 0);
@@ -133,62 +166,62 @@ __device__ __forceinline__ void clear_rows(const MoveArgs &p, T *rows, long long
     }
 }
 
-// Slots that a team of kLanes lanes (0: the block) takes in a pass: a ragged row's last lane only has the vector that the one before needs.
+// Vectors that a team of kLanes lanes (0: the block, warp by warp) takes in a pass: a ragged row's last lane only has the vector that the
+// one before needs.
 template <int kLanes, bool kRagged>
 __device__ __forceinline__ int slot_of(int pass, int lane) {
-    constexpr int kTake = kRagged ? 31 : 32;
     if (kLanes != 0) return pass * (kRagged ? kLanes - 1 : kLanes) + lane;
-    return (pass * kWarps + (int)threadIdx.x / 32) * kTake + lane;  // warp by warp
+    return (pass * kWarps + (int)threadIdx.x / 32) * (kRagged ? 31 : 32) + lane;
 }
 template <int kLanes, bool kRagged>
 __device__ __forceinline__ bool takes(int lane) {
     return !kRagged || lane + 1 < (kLanes ? kLanes : 32);
 }
 
-// kLanes lanes take a token's slots of one pass.
-template <typename T, int kLanes, bool kRagged>
+// kLanes lanes take a token's vectors of one pass.  Positions and weights of the next choices are on their way while rows are added up.
+template <typename T, int kLanes, bool kRagged, int kAtOnce>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const MoveArgs p) {
-    constexpr int W = kWidthOf<T>, H = W / 2, kTeams = kThreads / kLanes, kAtOnce = 4;
+    constexpr int W = kWidthOf<T>, H = W / 2, kTeams = kThreads / kLanes;
     wait_for_previous_kernel();
     const int lane = threadIdx.x % kLanes;
-    const T *rows = static_cast<const T *>(p.rows);
-    const long long units = p.tokens * p.passes, all = p.tokens * p.top_k;
-    const long long own = (long long)blockIdx.x * kTeams + threadIdx.x / kLanes;
-    for (long long unit = own; unit - own % (32 / kLanes) < units; unit += (long long)gridDim.x * kTeams) {
-        const bool active = unit < units;
-        const long long token = !active ? 0 : p.passes == 1 ? unit : unit / p.passes;
-        const Slot<T, kRagged> slot(token, p.width, slot_of<kLanes, kRagged>((int)(unit - token * p.passes), lane));
-        Pair sum[H];
+    const Rows<T> rows(p.rows, p.entries, p.width), out(p.out, p.tokens, p.width), residual(p.residual, p.tokens, p.width);
+    const long long units = p.tokens * p.passes, step = (long long)gridDim.x * kTeams;
+    long long unit = (long long)blockIdx.x * kTeams + threadIdx.x / kLanes;
+    const long long warp = threadIdx.x % 32 / kLanes;  // the warp's first team decides when it ends
+    const auto token_of = [&](long long u) { return p.passes == 1 ? u : u / p.passes; };
+    int j = 0;
+    Pair sum[H];
 #pragma unroll
-        for (int i = 0; i < H; ++i) sum[i] = Pair(0.f);
-        uint4 extra = make_uint4(0, 0, 0, 0);
-        const bool mine = active && slot.any() && takes<kLanes, kRagged>(lane);
-        if (p.residual && mine) extra = load_vector<T, kRagged>(static_cast<const T *>(p.residual), slot.vector, p.tokens * p.width);
-        for (int j = 0; j < p.top_k; j += kAtOnce) {
-            long long at[kAtOnce];
-            float weight[kAtOnce];
-            uint4 v[kAtOnce];
+    for (int h = 0; h < H; ++h) sum[h] = Pair(0.f);
+    Choices<kAtOnce> next;
+    next.template load<T>(p, token_of(unit), 0, unit < units);
+    while (unit - warp < units) {
+        const bool active = unit < units, last = j + kAtOnce >= p.top_k;
+        const int token = active ? (int)token_of(unit) : 0, pass = active ? (int)(unit - (long long)token * p.passes) : 0;
+        const int column = slot_of<kLanes, kRagged>(pass, lane) * W - (kRagged ? out.lead(token) : 0);
+        const bool mine = active && column < p.width && takes<kLanes, kRagged>(lane);
+        uint4 v[kAtOnce], extra = make_uint4(0, 0, 0, 0);
+        float weight[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) {
-                const long long entry = token * p.top_k + j + i;
-                const bool there = active && j + i < p.top_k;
-                at[i] = there ? row_of(p, entry) : -1;
-                weight[i] = there && p.weights ? load_as_f32(p.weights, p.weight_dtype, entry) : 1.f;
-            }
-#pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) v[i] = slot.fetch(rows, at[i], all, at[i] >= 0);
-#pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) {
-                if (at[i] < 0) continue;  // the weight of no row may be anything
-                Raw<T, W> raw;
-                Pair e[H];
-                raw.u[0] = v[i];
-                raw.get(e);
-#pragma unroll
-                for (int h = 0; h < H; ++h) sum[h] = fma2(e[h], Pair(weight[i]), sum[h]);
-            }
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int row = next.row(p, i);
+            v[i] = rows.template fetch<kRagged>(max(row, 0), column, row >= 0);
+            weight[i] = row >= 0 ? next.weight[i] : 0.f;  // that of no row may be anything
         }
-        if (!mine) continue;
+        if (p.residual && last && mine) extra = residual.template load<kRagged>(residual.at(token, column));
+        j = last ? 0 : j + kAtOnce;
+        if (last) unit += step;
+        next.template load<T>(p, token_of(unit), j, unit < units);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            Raw<T, W> raw;
+            Pair e[H];
+            raw.u[0] = v[i];
+            raw.get(e);
+#pragma unroll
+            for (int h = 0; h < H; ++h) sum[h] = fma2(e[h], Pair(weight[i]), sum[h]);
+        }
+        if (!last) continue;
         Raw<T, W> raw;
         if (p.residual) {
             Pair e[H];
@@ -198,109 +231,101 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const MoveArgs p) {
             for (int h = 0; h < H; ++h) sum[h] = sum[h] + e[h];
         }
         raw.set(sum);
-        slot.store(static_cast<T *>(p.out), raw.u[0]);
+        if (mine) out.template store<kRagged>(token, column, raw.u[0]);
+#pragma unroll
+        for (int h = 0; h < H; ++h) sum[h] = Pair(0.f);
     }
 }
 
 // kLanes lanes, or (0) a block, take a token.
-template <typename T, int kLanes, bool kRagged>
+template <typename T, int kLanes, bool kRagged, int kAtOnce>
 __global__ void __launch_bounds__(kThreads) combine_backward_kernel(const MoveArgs p) {
-    constexpr int W = kWidthOf<T>, H = W / 2, kLine = kLanes ? kLanes : 32, kTeams = kLanes ? kThreads / kLine : 1, kAtOnce = 4;
+    constexpr int W = kWidthOf<T>, H = W / 2, kLine = kLanes ? kLanes : 32, kTeams = kLanes ? kThreads / kLine : 1;
     __shared__ float dots[kWarps][kAtOnce];
     wait_for_previous_kernel();
     const int lane = threadIdx.x % kLine;
-    const T *rows = static_cast<const T *>(p.rows), *grad = static_cast<const T *>(p.grad);
-    T *out = static_cast<T *>(p.out);
-    const long long all = p.tokens * p.top_k;
-    const long long own = (long long)blockIdx.x * kTeams + (kLanes ? threadIdx.x / kLine : 0), step = (long long)gridDim.x * kTeams;
-    for (long long unit = own; unit - (kLanes ? own % (32 / kLine) : 0) < p.tokens; unit += step) {
+    const Rows<T> rows(p.rows, p.entries, p.width), grad(p.grad, p.tokens, p.width), out(p.out, p.entries, p.width);
+    const long long step = (long long)gridDim.x * kTeams, warp = kLanes ? threadIdx.x % 32 / kLine : 0;
+    long long unit = (long long)blockIdx.x * kTeams + (kLanes ? threadIdx.x / kLine : 0);
+    int j = 0;
+    Choices<kAtOnce> next;
+    next.template load<T>(p, unit, 0, unit < p.tokens);
+    while (unit - warp < p.tokens) {
         const bool active = unit < p.tokens;
-        const long long token = active ? unit : 0;
-        for (int j = 0; j < p.top_k; j += kAtOnce) {
-            long long at[kAtOnce];
-            float weight[kAtOnce];
-            Pair dot[kAtOnce];
+        const int token = active ? (int)unit : 0, first = j;
+        int row[kAtOnce];
+        Pair weight[kAtOnce], dot[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            row[i] = next.row(p, i);
+            weight[i] = Pair(next.weight[i]);
+            dot[i] = Pair(0.f);
+        }
+        const bool last = j + kAtOnce >= p.top_k;
+        j = last ? 0 : j + kAtOnce;
+        if (last) unit += step;
+        next.template load<T>(p, unit, j, unit < p.tokens);
+        for (int pass = 0; pass < p.passes; ++pass) {
+            const int start = slot_of<kLanes, kRagged>(pass, lane) * W;
+            uint4 dy[kRagged ? kAtOnce : 1], v[kAtOnce];
+            int column[kAtOnce];
+            if constexpr (!kRagged) dy[0] = grad.template fetch<false>(token, start, active);
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i) {
-                const long long entry = token * p.top_k + j + i;
-                const bool there = active && j + i < p.top_k;
-                at[i] = there ? row_of(p, entry) : -1;
-                weight[i] = there && p.weights ? load_as_f32(p.weights, p.weight_dtype, entry) : 1.f;
-                dot[i] = Pair(0.f);
+                column[i] = start - (kRagged ? rows.lead(max(row[i], 0)) : 0);
+                if constexpr (kRagged) dy[i] = grad.template fetch<true>(token, column[i], row[i] >= 0);
+                v[i] = make_uint4(0, 0, 0, 0);
+                if (p.grad_weights && row[i] >= 0 && column[i] < p.width) v[i] = rows.template load<kRagged>(rows.at(row[i], column[i]));
             }
-            for (int pass = 0; pass < p.passes; ++pass) {
-                const int number = slot_of<kLanes, kRagged>(pass, lane);
-                uint4 dy[kAtOnce], v[kAtOnce];
-                if (!kRagged) {
-                    const Slot<T, kRagged> slot(token, p.width, number);
-                    dy[0] = slot.fetch(grad, token, p.tokens, active);
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                if (row[i] < 0 || !takes<kLanes, kRagged>(lane)) continue;
+                Raw<T, W> raw;
+                Pair g[H], e[H];
+                raw.u[0] = kRagged ? inside<T>(dy[kRagged ? i : 0], column[i], p.width) : dy[0];
+                raw.get(g);
+                if (p.grad_weights) {
+                    raw.u[0] = kRagged ? inside<T>(v[i], column[i], p.width) : v[i];
+                    raw.get(e);
+#pragma unroll
+                    for (int h = 0; h < H; ++h) dot[i] = fma2(g[h], e[h], dot[i]);
                 }
+                if (p.out) {
 #pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    const Slot<T, kRagged> slot(max(at[i], 0ll), p.width, number);
-                    if (kRagged) dy[i] = slot.fetch(grad, token, p.tokens, at[i] >= 0);
-                    else dy[i] = dy[0];
-                    v[i] = make_uint4(0, 0, 0, 0);
-                    if (p.grad_weights && at[i] >= 0 && slot.any() && takes<kLanes, kRagged>(lane))
-                        v[i] = load_vector<T, kRagged>(rows, slot.vector, all * p.width);
-                }
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    if (at[i] < 0 || !takes<kLanes, kRagged>(lane)) continue;
-                    const Slot<T, kRagged> slot(at[i], p.width, number);
-                    Raw<T, W> raw;
-                    Pair g[H], e[H];
-                    raw.u[0] = dy[i];
-                    raw.get(g);
-                    if (p.grad_weights) {
-                        raw.u[0] = v[i];
-                        raw.get(e);
-                        if (slot.whole()) {  // beyond the row's end both are 0
-#pragma unroll
-                            for (int h = 0; h < H; ++h) dot[i] = fma2(g[h], e[h], dot[i]);
-                        } else {
-#pragma unroll
-                            for (int h = 0; h < H; ++h) {
-                                float a, b, c, d;
-                                g[h].get(a, b);
-                                e[h].get(c, d);
-                                const float first = slot.has(2 * h) ? a * c : 0.f, second = slot.has(2 * h + 1) ? b * d : 0.f;
-                                dot[i] = dot[i] + Pair(first, second);
-                            }
-                        }
-                    }
-                    if (out) {
-#pragma unroll
-                        for (int h = 0; h < H; ++h) g[h] = g[h] * Pair(weight[i]);
-                        raw.set(g);
-                        slot.store(out, raw.u[0]);
-                    }
+                    for (int h = 0; h < H; ++h) g[h] = g[h] * weight[i];
+                    raw.set(g);
+                    out.template store<kRagged>(row[i], column[i], raw.u[0]);
                 }
             }
-            if (!p.grad_weights) continue;
-            float sums[kAtOnce];
+        }
+        if (!p.grad_weights) continue;
+        float sums[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) sums[i] = lanes_sum<kLine>(dot[i].sum());
-            if constexpr (kLanes == 0) {
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i)
-                    if (lane == 0) dots[threadIdx.x / 32][i] = sums[i];
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    sums[i] = dots[0][i];
-                    for (int w = 1; w < kWarps; ++w) sums[i] += dots[w][i];
-                }
-            }
+        for (int i = 0; i < kAtOnce; ++i) sums[i] = lanes_sum<kLine>(dot[i].sum());
+        if constexpr (kLanes == 0) {
+            __syncthreads();
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i)
-                if (active && j + i < p.top_k && (kLanes ? lane : (int)threadIdx.x) == 0)
-                    store_from_f32(p.grad_weights, p.weight_dtype, token * p.top_k + j + i, at[i] < 0 ? 0.f : sums[i]);
+                if (lane == 0) dots[threadIdx.x / 32][i] = sums[i];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                sums[i] = dots[0][i];
+                for (int w = 1; w < kWarps; ++w) sums[i] += dots[w][i];
+            }
+        }
+        if (!active || (kLanes ? lane : (int)threadIdx.x) != 0) continue;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (first + i >= p.top_k) continue;
+            const long long entry = (long long)token * p.top_k + first + i;
+            const float g = row[i] < 0 ? 0.f : sums[i];
+            if (p.wide_weights) static_cast<float *>(p.grad_weights)[entry] = g;
+            else static_cast<T *>(p.grad_weights)[entry] = from_f32<T>(g);
         }
     }
-    if (out) clear_rows<T, kRagged>(p, out, min(max((long long)*p.end, 0ll), all), all, (long long)blockIdx.x * kThreads + threadIdx.x,
-                                    (long long)gridDim.x * kThreads);
+    if (p.out) clear_rows<T, kRagged>(static_cast<T *>(p.out), p.width, min(max((long long)*p.end, 0ll), p.entries), p.entries,
+                                      (long long)blockIdx.x * kThreads + threadIdx.x, (long long)gridDim.x * kThreads);
 }
 
 // ---- sorting, and the rows with it -------------------------------------------------------------------------------------------
@@ -370,6 +395,8 @@ enum Counted {
 constexpr int kPart = 2048;  // entries of a block that are placed at a time
 constexpr int kMoveThreads = 512, kMoveWarps = kMoveThreads / 32;
 
+constexpr int kAheadBytes = 256 * 1024;  // of a block: together they fit L2
+
 // Dynamic shared memory: next[kMoveWarps][n_experts], then total[n_experts], then start[n_experts + 1], then place[kPart].
 inline int move_shared(int n_experts) { return ((kMoveWarps + 2) * n_experts + 1 + kPart) * (int)sizeof(int); }
 
@@ -382,6 +409,12 @@ __global__ void __launch_bounds__(kMoveThreads, 2) dispatch_kernel(const SortArg
     const int E = p.n_experts, warp = threadIdx.x / 32;
     int *next = shared, *total = shared + kMoveWarps * E, *start = total + E, *place = start + E + 1;
     const long long first = (long long)blockIdx.x * p.chunk, last = min(first + p.chunk, p.entries);
+    if (kCounted != kByItself) {  // the rows of the first entries come to L2 while these are placed
+        const char *from = static_cast<const char *>(m.x) + first / m.top_k * m.width * sizeof(T);
+        const long long bytes = (min(last, first + kPart) - first) / m.top_k * m.width * (long long)sizeof(T);
+        for (long long i = threadIdx.x * 128ll; i < min(bytes, (long long)kAheadBytes); i += kMoveThreads * 128)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(from + i));
+    }
     // next[0][e]: entries of expert e before the block's; total[e]: all
     for (int i = threadIdx.x; i < (kMoveWarps + 1) * E; i += kMoveThreads) next[i] = 0;
     __syncthreads();
@@ -401,7 +434,7 @@ __global__ void __launch_bounds__(kMoveThreads, 2) dispatch_kernel(const SortArg
             const int e = E >= kMoveThreads ? base + threadIdx.x : threadIdx.x % E, row = E >= kMoveThreads ? 0 : threadIdx.x / E;
             int all = 0, before = 0;
             if (e < E && row < rows) {
-#pragma unroll 4
+#pragma unroll 8
                 for (int c = row; c < p.chunks; c += rows) {
                     const int n = p.counts[(size_t)c * E + e];
                     all += n;
@@ -449,8 +482,8 @@ __global__ void __launch_bounds__(kMoveThreads, 2) dispatch_kernel(const SortArg
     for (int e = threadIdx.x; e < E; e += kMoveThreads) total[e] = start[e] + next[e];  // where the block's first entry of e goes
     __syncthreads();
 
-    T *rows = static_cast<T *>(m.out);
-    const T *x = static_cast<const T *>(m.x);
+    constexpr int W = kWidthOf<T>;
+    const Rows<T> x(m.x, m.tokens, m.width), rows(m.out, p.entries, m.width);
     const int part_size = kPart / m.top_k * m.top_k;
     for (long long part = first; part < last; part += part_size) {
         const long long end = min(part + part_size, last);
@@ -495,37 +528,34 @@ __global__ void __launch_bounds__(kMoveThreads, 2) dispatch_kernel(const SortArg
         __syncthreads();
         // the rows of the part's tokens: kLanes lanes to a token and pass
         constexpr int kTeams = kMoveThreads / kLanes, kAtOnce = 4;
-        const long long token0 = part / m.top_k;
-        const int tokens = (int)((end - part) / m.top_k), tl = threadIdx.x % kLanes, team = threadIdx.x / kLanes;
+        const int token0 = (int)(part / m.top_k), tokens = (int)((end - part) / m.top_k), tl = threadIdx.x % kLanes, team = threadIdx.x / kLanes;
         for (int pass = blockIdx.y; pass < m.passes; pass += gridDim.y) {
-            const int number = slot_of<kLanes, kRagged>(pass, tl);
+            const int column = slot_of<kLanes, kRagged>(pass, tl) * W;
             for (int base = 0; base < tokens; base += kTeams * kAtOnce) {
-                if (!kRagged) {
+                if constexpr (!kRagged) {
                     uint4 v[kAtOnce];
 #pragma unroll
                     for (int i = 0; i < kAtOnce; ++i) {
                         const int t = base + i * kTeams + team;
-                        const Slot<T, kRagged> slot(token0 + t, m.width, number);
-                        v[i] = slot.fetch(x, token0 + t, m.tokens, t < tokens);
+                        v[i] = x.template fetch<false>(token0 + t, column, t < tokens);
                     }
+                    for (int j = 0; j < m.top_k; ++j) {
 #pragma unroll
-                    for (int i = 0; i < kAtOnce; ++i) {
-                        const int t = base + i * kTeams + team;
-                        if (t >= tokens) continue;
-                        for (int j = 0; j < m.top_k; ++j) {
-                            const int at = place[t * m.top_k + j];
-                            if (at >= 0) Slot<T, kRagged>(at, m.width, number).store(rows, v[i]);
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            const int t = base + i * kTeams + team;
+                            const int at = t < tokens ? place[t * m.top_k + j] : -1;
+                            if (at >= 0) rows.template store<false>(at, column, v[i]);
                         }
                     }
                 } else {
+                    for (int j = 0; j < m.top_k; ++j) {
 #pragma unroll
-                    for (int i = 0; i < kAtOnce; ++i) {
-                        const int t = base + i * kTeams + team;
-                        for (int j = 0; j < m.top_k; ++j) {
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            const int t = base + i * kTeams + team;
                             const int at = t < tokens ? place[t * m.top_k + j] : -1;
-                            const Slot<T, kRagged> slot(max(at, 0), m.width, number);
-                            const uint4 v = slot.fetch(x, token0 + t, m.tokens, at >= 0);
-                            if (at >= 0 && takes<kLanes, kRagged>(tl)) slot.store(rows, v);
+                            const int own = column - rows.lead(max(at, 0));
+                            const uint4 v = x.template fetch<true>(token0 + (at >= 0 ? t : 0), own, at >= 0);
+                            if (at >= 0 && takes<kLanes, kRagged>(tl)) rows.template store<true>(at, own, v);
                         }
                     }
                 }
@@ -533,54 +563,61 @@ __global__ void __launch_bounds__(kMoveThreads, 2) dispatch_kernel(const SortArg
         }
         __syncthreads();
     }
-    clear_rows<T, kRagged>(m, rows, start[E], p.entries, ((long long)blockIdx.y * gridDim.x + blockIdx.x) * kMoveThreads + threadIdx.x,
+    clear_rows<T, kRagged>(rows.base, m.width, start[E], p.entries, ((long long)blockIdx.y * gridDim.x + blockIdx.x) * kMoveThreads + threadIdx.x,
                            (long long)gridDim.x * gridDim.y * kMoveThreads);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------
-// Lanes that take a token, and passes over its vectors.
+// Lanes that take a token, and passes over its vectors: the fewest lanes' turns, wider teams where these are nearly as few.
 template <typename T>
-void set_slots(MoveArgs &p, int &lanes, bool &ragged) {
+void set_passes(MoveArgs &p, int &lanes, bool &ragged) {
     constexpr int W = kWidthOf<T>;
     ragged = p.width % W != 0;
-    p.slots = ragged ? (p.width + 2 * W - 2) / W : p.width / W;
-    const int extra = ragged ? 1 : 0;
-    lanes = 32;
-    while (lanes > 4 && lanes / 2 - extra >= p.slots) lanes /= 2;
-    p.passes = (int)ceil_div(p.slots, lanes - extra);
-}
-
-template <typename T, int kLanes, bool kRagged>
-int run_combine(const MoveArgs &p, cudaStream_t st) {
-    const long long blocks = ceil_div(p.tokens * p.passes, kThreads / kLanes);
-    return launched(launch_early(combine_kernel<T, kLanes, kRagged>, (unsigned)std::min<long long>(blocks, 32 * kSms), kThreads, 0, st, 1, p));
-}
-template <typename T, int kLanes, bool kRagged>
-int run_combine_backward(const MoveArgs &p, cudaStream_t st) {
-    const long long blocks = kLanes ? ceil_div(p.tokens, kThreads / (kLanes ? kLanes : 1)) : p.tokens;
-    return launched(launch_early(combine_backward_kernel<T, kLanes, kRagged>, (unsigned)std::min<long long>(blocks, 32 * kSms), kThreads, 0, st, 1, p));
-}
-
-template <typename T, bool kRagged>
-int run_combine(const MoveArgs &p, int lanes, bool backward, cudaStream_t st) {
-    // wide rows of few tokens: a block to a token
-    if (backward && p.passes > 1 && p.tokens < 8 * kSms * kWarps) {
-        MoveArgs q = p;
-        q.passes = (int)ceil_div(p.slots, kWarps * (kRagged ? 31 : 32));
-        return run_combine_backward<T, 0, kRagged>(q, st);
+    const long long slots = ragged ? (p.width + 2 * W - 2) / W : p.width / W;  // vectors that a row can touch
+    long long least = 0;
+    for (int l = 32; l >= 4; l /= 2) {
+        const long long passes = ceil_div(slots, l - (ragged ? 1 : 0)), turns = passes * l;
+        if (l < 32 && turns * 8 > least * 7) continue;
+        least = turns;
+        lanes = l;
+        p.passes = (int)passes;
     }
-    if (lanes == 4) return backward ? run_combine_backward<T, 4, kRagged>(p, st) : run_combine<T, 4, kRagged>(p, st);
-    if (lanes == 8) return backward ? run_combine_backward<T, 8, kRagged>(p, st) : run_combine<T, 8, kRagged>(p, st);
-    if (lanes == 16) return backward ? run_combine_backward<T, 16, kRagged>(p, st) : run_combine<T, 16, kRagged>(p, st);
-    return backward ? run_combine_backward<T, 32, kRagged>(p, st) : run_combine<T, 32, kRagged>(p, st);
+}
+
+template <typename T, int kLanes, bool kRagged, int kAtOnce>
+int run_combine(const MoveArgs &p, bool backward, cudaStream_t st) {
+    long long units = p.tokens * p.passes;
+    auto kernel = combine_kernel<T, kLanes, kRagged, kAtOnce>;
+    MoveArgs q = p;
+    if (backward) {
+        units = p.tokens;
+        kernel = combine_backward_kernel<T, kLanes, kRagged, kAtOnce>;
+        // wide rows of few tokens: a block to a token
+        if (p.passes > 1 && p.tokens < 8 * kSms * kWarps) {
+            q.passes = (int)ceil_div((long long)p.passes * kLanes, kThreads - (kRagged ? kWarps : 0));
+            units *= kThreads / kLanes;
+            kernel = combine_backward_kernel<T, 0, kRagged, kAtOnce>;
+        }
+    }
+    const unsigned blocks = (unsigned)std::min<long long>(ceil_div(units, kThreads / kLanes), 8 * kSms);
+    return launched(launch_early(kernel, blocks, kThreads, 0, st, 1, q));
+}
+
+template <typename T, bool kRagged, int kAtOnce>
+int run_combine(const MoveArgs &p, int lanes, bool backward, cudaStream_t st) {
+    if (lanes == 4) return run_combine<T, 4, kRagged, kAtOnce>(p, backward, st);
+    if (lanes == 8) return run_combine<T, 8, kRagged, kAtOnce>(p, backward, st);
+    if (lanes == 16) return run_combine<T, 16, kRagged, kAtOnce>(p, backward, st);
+    return run_combine<T, 32, kRagged, kAtOnce>(p, backward, st);
 }
 
 template <typename T>
 int run_combine(MoveArgs p, bool backward, cudaStream_t st) {
     int lanes;
     bool ragged;
-    set_slots<T>(p, lanes, ragged);
-    return ragged ? run_combine<T, true>(p, lanes, backward, st) : run_combine<T, false>(p, lanes, backward, st);
+    set_passes<T>(p, lanes, ragged);
+    if (p.top_k <= 2) return ragged ? run_combine<T, true, 2>(p, lanes, backward, st) : run_combine<T, false, 2>(p, lanes, backward, st);
+    return ragged ? run_combine<T, true, 4>(p, lanes, backward, st) : run_combine<T, false, 4>(p, lanes, backward, st);
 }
 
 int run_combine(const MoveArgs &p, int dtype, bool backward, cudaStream_t st) {
@@ -640,7 +677,7 @@ int run_dispatch(SortArgs s, MoveArgs p, cudaStream_t st) {
     int lanes;
     bool ragged;
     unsigned slices;
-    set_slots<T>(p, lanes, ragged);
+    set_passes<T>(p, lanes, ragged);
     set_chunks(s, p.top_k, p.passes, slices);
     const Counted c = counted(s);
     if (c != kByItself)
@@ -690,7 +727,7 @@ int fda_dispatch_rows(const void *x, const int64_t *experts, void *rows, int64_t
         s.total = reinterpret_cast<int *>(static_cast<char *>(workspace) + counts_bytes(n_experts));
     }
     MoveArgs p{};
-    p.x = x; p.out = rows; p.tokens = tokens; p.top_k = top_k; p.width = features;
+    p.x = x; p.out = rows; p.tokens = tokens; p.top_k = top_k; p.entries = s.entries; p.width = features;
     if (dtype == FDA_DTYPE_F32) return run_dispatch<float>(s, p, st);
     if (dtype == FDA_DTYPE_F16) return run_dispatch<__half>(s, p, st);
     return run_dispatch<__nv_bfloat16>(s, p, st);
@@ -699,13 +736,13 @@ int fda_dispatch_rows(const void *x, const int64_t *experts, void *rows, int64_t
 int fda_combine_rows(const void *rows, const int64_t *position, const void *weights, const void *residual, void *y, long long tokens, int top_k,
                      int features, int dtype, int weight_dtype, void *stream) {
     if (const int rc = check_rows(tokens, top_k, features, dtype)) return rc;
-    if (weights && !known_dtype(weight_dtype)) return FDA_ERR_BAD_DTYPE;
+    if (weights && weight_dtype != dtype && weight_dtype != FDA_DTYPE_F32) return FDA_ERR_BAD_DTYPE;
     if (tokens == 0) return FDA_OK;
     if (!rows || !position || !y) return FDA_ERR_NULL_POINTER;
     if (misaligned16(rows) || misaligned16(residual) || misaligned16(y)) return FDA_ERR_MISALIGNED;
     MoveArgs p{};
     p.rows = rows; p.position = position; p.weights = weights; p.residual = residual; p.out = y; p.tokens = tokens; p.top_k = top_k;
-    p.width = features; p.weight_dtype = weight_dtype;
+    p.entries = tokens * top_k; p.width = features; p.wide_weights = weight_dtype == FDA_DTYPE_F32;
     return run_combine(p, dtype, false, static_cast<cudaStream_t>(stream));
 }
 
@@ -713,13 +750,13 @@ int fda_combine_rows_backward(const void *rows, const int64_t *position, const i
                               void *grad_rows, void *grad_weights, long long tokens, int top_k, int features, int dtype, int weight_dtype,
                               void *stream) {
     if (const int rc = check_rows(tokens, top_k, features, dtype)) return rc;
-    if ((weights || grad_weights) && !known_dtype(weight_dtype)) return FDA_ERR_BAD_DTYPE;
+    if ((weights || grad_weights) && weight_dtype != dtype && weight_dtype != FDA_DTYPE_F32) return FDA_ERR_BAD_DTYPE;
     if (tokens == 0 || (!grad_rows && !grad_weights)) return FDA_OK;
     if (!position || !rows_end || !grad_y || (grad_weights && !rows)) return FDA_ERR_NULL_POINTER;
     if (misaligned16(rows) || misaligned16(grad_y) || misaligned16(grad_rows)) return FDA_ERR_MISALIGNED;
     MoveArgs p{};
     p.rows = rows; p.position = position; p.end = rows_end; p.weights = weights; p.grad = grad_y; p.out = grad_rows; p.grad_weights = grad_weights;
-    p.tokens = tokens; p.top_k = top_k; p.width = features; p.weight_dtype = weight_dtype;
+    p.tokens = tokens; p.top_k = top_k; p.entries = tokens * top_k; p.width = features; p.wide_weights = weight_dtype == FDA_DTYPE_F32;
     return run_combine(p, dtype, true, static_cast<cudaStream_t>(stream));
 }
 
