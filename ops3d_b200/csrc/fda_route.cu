@@ -70,17 +70,17 @@ __device__ __forceinline__ F total(F v) {
     return v;
 }
 
-// e^v for comparisons: off by 2^-24 (1.5 |v| + 4) of itself, 0 below the normal range.
-__device__ __forceinline__ float quick_exp(float v) {
+// 2^v for comparisons: off by 2^-22 of itself, 0 below the normal range.
+__device__ __forceinline__ float quick_exp2(float v) {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.44269504088896341f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
 
-// By how much a score in fp32 can be off, relative to the token's largest: for a softmax 2^-24 (1.5 |d| + 4) e^d, d = l - max, is at
-// most 5 * 2^-24; the sum of up to 64 + 4 terms adds 2^-24 * 75 at most, the quotient 3.  For a sigmoid, 2^-24 (1.5 |l| + 8) of itself, which is
-// less than this down to l = -80 and below kSmallest beyond.
-constexpr float kScoreError = 1.f / 131072.f;
+// By how much a score in fp32 can be off.  A softmax's, relative to the token's largest: 2^-24 (1.5 |d| + 4) e^d, d = l - max, is at most
+// 5 * 2^-24; the sum, by octets and then over up to 8 of them and 16 lanes, adds 20 * 2^-24, quotient and product 4.  A sigmoid's: (1.5 |l| + 4)
+// s (1 - s) 2^-24 is at most 1.1 * 2^-24, sum and quotient add 3.
+constexpr float kSoftmaxError = 1.f / 524288.f, kSigmoidError = 1.f / 2097152.f;
 // For the addition of the bias, relative to the larger of two values that are compared: a smaller one that is below minus that is further
 // away than it can be off by.
 constexpr float kSumError = 1.f / 2097152.f;
@@ -158,9 +158,8 @@ __device__ __noinline__ void choose_exactly(const RouteArgs &p, long long token,
         const double l = logit<T>(p, token, e);
         double v = p.sigmoid ? 1 / (1 + exp(-l)) : inverse == 0 ? 0 : exp(l - shift) * inverse;
         if (p.bias) v += (double)p.bias[e];
-        else if (p.top2) key[i] = order_of(l);  // groups by their sums, experts by their logits
         values[e] = v;
-        if (p.bias || !p.top2) key[i] = order_of(v);
+        key[i] = order_of(p.bias ? v : l);  // without a bias experts are compared by their logits, only groups by sums of scores
     }
     __syncwarp();
     unsigned left = exactly_allowed<kPer>(p, values);
@@ -198,26 +197,36 @@ __device__ __forceinline__ void load_logits(const RouteArgs &p, long long token,
     }
 }
 
-// Softmax's shift and the inverse of its sum; a token without a finite logit has no score: inverse 0.
+// e^(l - shift) in place of the logits, `quick` for comparisons; shift is the largest logit.  The inverse of their sum; 0 for a token without
+// a finite logit, which has no score.
 template <int kLanes, int kOctets>
-__device__ __forceinline__ void softmax_of(const float (&l)[kOctets][8], bool quick, float &shift, float &inverse) {
+__device__ __forceinline__ void softmax_of(float (&v)[kOctets][8], bool quick, float &shift, float &inverse) {
     float top = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int q = 0; q < kOctets; ++q)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, l[q][i]);
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, v[q][i]);
     shift = most<kLanes>(top);
     if (shift == -INFINITY) shift = 0.f;  // every term is 0 then, or NaN
-    if (quick) {
+    const Pair minus(-shift), scale(1.44269504088896341f);
 #pragma unroll
-        for (int q = 0; q < kOctets; ++q)
+    for (int q = 0; q < kOctets; ++q) {
+        if (quick) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += quick_exp(l[q][i] - shift);
-    } else {
+            for (int i = 0; i < 8; i += 2) {
+                const Pair d = (Pair(v[q][i], v[q][i + 1]) + minus) * scale;
+                d.get(v[q][i], v[q][i + 1]);
+                v[q][i] = quick_exp2(v[q][i]);
+                v[q][i + 1] = quick_exp2(v[q][i + 1]);
+            }
+        } else {
 #pragma unroll
-        for (int q = 0; q < kOctets; ++q)
+            for (int i = 0; i < 8; ++i) v[q][i] = expf(v[q][i] - shift);
+        }
+        Pair half[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += expf(l[q][i] - shift);
+        for (int i = 0; i < 4; ++i) half[i] = Pair(v[q][2 * i], v[q][2 * i + 1]);
+        sum += ((half[0] + half[1]) + (half[2] + half[3])).sum();
     }
     sum = total<kLanes>(sum);
     inverse = sum == 0.f ? 0.f : 1.f / sum;
@@ -241,6 +250,7 @@ __device__ __forceinline__ float chosen_scores(const RouteArgs &p, const float (
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
         score[i] = 0.f;
+        if (i * kLanes >= p.top_k) continue;
         if (there[i]) {
             if (p.sigmoid) score[i] = 1.f / (1.f + expf(-l[i]));
             else if (inverse != 0.f) score[i] = expf(l[i] - shift) * inverse;
@@ -255,34 +265,55 @@ template <int kLanes, int kOctets>
 struct WarpShared {
     static constexpr int kTokens = 32 / kLanes, kExperts = kLanes * kOctets * 8;
     float values[kTokens][kExperts];
+    float2 largest[kTokens][kExperts / 8];  // two of each octet
     float worth[kTokens][kMostExpertGroups];
     float chosen_value[kTokens][kMostChoices];
     int chosen[kTokens][kMostChoices];
 };
 
-// Takes the experts of other than the top_groups best groups out of v (NaN).  s.values has them all.  Returns false where the border
-// between the groups is closer than `error`.
+__device__ __forceinline__ float2 two_largest(float2 a, float2 b) {  // of two pairs, each largest first
+    return make_float2(fmaxf(a.x, b.x), fmaxf(fminf(a.x, b.x), fmaxf(a.y, b.y)));
+}
+
+// Takes the experts of other than the top_groups best groups out of v (NaN).  `worths` are the values that groups are compared by, v those of
+// experts.  Returns false where the border between the groups is closer than `error`.
 template <int kLanes, int kOctets>
-__device__ __forceinline__ bool keep_best_groups(const RouteArgs &p, const float *values, float *worth, int lane, float error, float (&v)[kOctets][8]) {
+__device__ __forceinline__ bool keep_best_groups(const RouteArgs &p, WarpShared<kLanes, kOctets> &s, int segment, int lane, float error,
+                                                 const float (&worths)[kOctets][8], float (&v)[kOctets][8]) {
     const int size = p.n_experts / p.n_groups;
+    const bool sums = p.top2 && size > 1, octets = size % 8 == 0;  // octets: groups are runs of whole octets
+    float *worth = s.worth[segment];
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < kOctets; ++q) {
+        if (octets) {
+            float2 best[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                best[i] = make_float2(fmaxf(worths[q][2 * i], worths[q][2 * i + 1]), fminf(worths[q][2 * i], worths[q][2 * i + 1]));
+            s.largest[segment][q * kLanes + lane] = two_largest(two_largest(best[0], best[1]), two_largest(best[2], best[3]));
+        } else {
+            float4 *at = reinterpret_cast<float4 *>(s.values[segment] + (q * kLanes + lane) * 8);
+            at[0] = make_float4(worths[q][0], worths[q][1], worths[q][2], worths[q][3]);
+            at[1] = make_float4(worths[q][4], worths[q][5], worths[q][6], worths[q][7]);
+        }
+    }
+    __syncwarp();
     int share = kLanes;  // lanes to a group
     while (share > 1 && kLanes / share < p.n_groups) share /= 2;
-    const bool sums = p.top2 && size > 1;
     for (int base = 0; base < p.n_groups; base += kLanes / share) {
         const int g = base + lane / share;
-        float first = -INFINITY, second = -INFINITY;
-        if (g < p.n_groups)
-            for (int i = lane % share; i < size; i += share) {
-                const float x = values[g * size + i];
-                second = fmaxf(second, fminf(first, x));
-                first = fmaxf(first, x);
+        float2 best = make_float2(-INFINITY, -INFINITY);
+        if (g < p.n_groups) {
+            if (octets) {
+                for (int i = lane % share; i < size / 8; i += share) best = two_largest(best, s.largest[segment][g * (size / 8) + i]);
+            } else {
+                for (int i = lane % share; i < size; i += share) best = two_largest(best, make_float2(s.values[segment][g * size + i], -INFINITY));
             }
-        for (int d = 1; d < share; d *= 2) {
-            const float a = __shfl_xor_sync(kAll, first, d), b = __shfl_xor_sync(kAll, second, d);
-            second = fmaxf(fminf(first, a), fmaxf(second, b));
-            first = fmaxf(first, a);
         }
-        if (g < p.n_groups && lane % share == 0) worth[g] = fmaxf(sums ? first + second : first, -INFINITY);
+        for (int d = 1; d < share; d *= 2)
+            best = two_largest(best, make_float2(__shfl_xor_sync(kAll, best.x, d), __shfl_xor_sync(kAll, best.y, d)));
+        if (g < p.n_groups && lane % share == 0) worth[g] = fmaxf(sums ? best.x + best.y : best.x, -INFINITY);
     }
     __syncwarp();
     unsigned groups = 0;
@@ -307,15 +338,41 @@ __device__ __forceinline__ bool keep_best_groups(const RouteArgs &p, const float
     high = most<kLanes>(high);
     const unsigned inverse_size = ((1u << 20) + size - 1) / size;  // e / size for e < 1024
 #pragma unroll
-    for (int q = 0; q < kOctets; ++q)
+    for (int q = 0; q < kOctets; ++q) {
+        const unsigned e = (q * kLanes + lane) * 8;
+        if (octets) {
+            const bool keep = groups >> (e * inverse_size >> 20 & 31) & 1;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (!(groups >> (((q * kLanes + lane) * 8 + i) * inverse_size >> 20 & 31) & 1)) v[q][i] = NAN;
+            for (int i = 0; i < 8; ++i) v[q][i] = keep ? v[q][i] : NAN;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!(groups >> ((e + i) * inverse_size >> 20 & 31) & 1)) v[q][i] = NAN;
+        }
+    }
     return error < 0.f || low - high > error || low == -INFINITY;
 }
 
+// NaN for experts beyond the last, which are no candidates; minus infinity for other NaN.
+template <int kLanes, int kOctets>
+__device__ __forceinline__ void only_candidates(int n_experts, int lane, bool has_nan, float (&v)[kOctets][8]) {
+    if (has_nan) {
+#pragma unroll
+        for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[q][i] = fmaxf(v[q][i], -INFINITY);
+    }
+    if (n_experts < kLanes * kOctets * 8) {
+#pragma unroll
+        for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if ((q * kLanes + lane) * 8 + i >= n_experts) v[q][i] = NAN;
+    }
+}
+
 template <typename T, int kLanes, int kOctets, bool kVector>
-__global__ void __launch_bounds__(kThreads) route_forward_kernel(const RouteArgs p) {
+__global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 6 : 3) route_forward_kernel(const RouteArgs p) {
     using Shared = WarpShared<kLanes, kOctets>;
     __shared__ alignas(16) Shared warps[kWarps];
     __shared__ alignas(16) float bias[Shared::kExperts];
@@ -325,72 +382,72 @@ __global__ void __launch_bounds__(kThreads) route_forward_kernel(const RouteArgs
     Shared &s = warps[threadIdx.x / 32];
     float *values = s.values[segment];
     if (p.bias) {
-        for (int e = threadIdx.x; e < Shared::kExperts; e += kThreads) bias[e] = e < E ? p.bias[e] : 0.f;
+        for (int e = threadIdx.x; e < Shared::kExperts; e += kThreads) bias[e] = e < E ? fmaxf(p.bias[e], -INFINITY) : 0.f;
         __syncthreads();
     }
-    const bool grouped = p.top_groups < p.n_groups;
-    const bool by_score = p.bias || (grouped && p.top2 && E > p.n_groups);  // what is compared: scores, or logits
+    const bool grouped = p.top_groups < p.n_groups, sums = grouped && p.top2 && E > p.n_groups;
+    const bool by_score = p.bias || sums;  // what is compared: scores, or logits
     const bool need_softmax = !p.sigmoid && (by_score || !p.renormalise);
     const long long step = (long long)gridDim.x * kWarps * Shared::kTokens;
     for (long long base = ((long long)blockIdx.x * kWarps + threadIdx.x / 32) * Shared::kTokens; base < p.tokens; base += step) {
-        const long long token = base + segment;
-        const bool active = token < p.tokens;
-        float v[kOctets][8], shift = 0.f, inverse = 1.f, largest = 0.f;
-        load_logits<T, kLanes, kOctets, kVector>(p, active ? token : base, lane, v);
-        if (need_softmax) softmax_of<kLanes, kOctets>(v, p.renormalise, shift, inverse);
-        if (by_score) {  // select values, in the same way for every expert
-#pragma unroll
-            for (int q = 0; q < kOctets; ++q)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (p.sigmoid) v[q][i] = __fdividef(1.f, 1.f + quick_exp(-v[q][i]));
-                    else v[q][i] = __fmul_rn(quick_exp(v[q][i] - shift), inverse);
-                    largest = fmaxf(largest, v[q][i]);
-                }
-            largest = most<kLanes>(largest);
-        }
-        float error = -1.f;  // of a group's worth
-        if (grouped && by_score) error = 0.f;
-        if (grouped && by_score && !p.bias) {
-            // the groups by their scores' sums, experts by their logits
-            __syncwarp();
-#pragma unroll
-            for (int q = 0; q < kOctets; ++q)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) values[(q * kLanes + lane) * 8 + i] = v[q][i];
-            __syncwarp();
-            load_logits<T, kLanes, kOctets, kVector>(p, active ? token : base, lane, v);
-        }
-        if (p.bias) {
-#pragma unroll
-            for (int q = 0; q < kOctets; ++q)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[q][i] = __fadd_rn(v[q][i], bias[(q * kLanes + lane) * 8 + i]);
-        }
-#pragma unroll
-        for (int q = 0; q < kOctets; ++q)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[q][i] = (q * kLanes + lane) * 8 + i < E ? fmaxf(v[q][i], -INFINITY) : NAN;
-        bool sure = true;
-        if (grouped) {
-            if (!by_score || p.bias) {
-                float far = 0.f;
-                __syncwarp();
+        const bool active = base + segment < p.tokens;
+        const long long token = active ? base + segment : base;
+        float v[kOctets][8], shift = 0.f, inverse = 1.f, largest = 1.f;
+        load_logits<T, kLanes, kOctets, kVector>(p, token, lane, v);
+        bool has_nan = true;  // perhaps
+        if (need_softmax) {
+            softmax_of<kLanes, kOctets>(v, p.renormalise, shift, inverse);
+            largest = inverse;
+            if (by_score) {
+                has_nan = !(inverse == inverse);  // then every score is
 #pragma unroll
                 for (int q = 0; q < kOctets; ++q)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        values[(q * kLanes + lane) * 8 + i] = v[q][i];
-                        if (fabsf(v[q][i]) < INFINITY) far = fmaxf(far, fabsf(v[q][i]));
-                    }
-                __syncwarp();
-                if (by_score) error = 4.f * kSumError * most<kLanes>(far);
+                    for (int i = 0; i < 8; ++i) v[q][i] *= inverse;
             } else {
-                error = 4.f * kSumError * largest;
+                load_logits<T, kLanes, kOctets, kVector>(p, token, lane, v);
             }
-            // a group is worth up to two values, and two groups are compared
-            if (by_score) error += 4.f * (largest * kScoreError + kSmallest);
-            sure = keep_best_groups<kLanes, kOctets>(p, values, s.worth[segment], lane, error, v);
+        } else if (by_score) {
+#pragma unroll
+            for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[q][i] = __fdividef(1.f, 1.f + quick_exp2(v[q][i] * -1.44269504088896341f));
+        }
+        const float score_error = p.sigmoid ? kSigmoidError : largest * kSoftmaxError;
+        if (p.bias) {
+#pragma unroll
+            for (int q = 0; q < kOctets; ++q) {
+                const float4 *at = reinterpret_cast<const float4 *>(bias + (q * kLanes + lane) * 8);
+                const float4 a = at[0], b = at[1];
+                const float add[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[q][i] = __fadd_rn(v[q][i], add[i]);
+            }
+        }
+        only_candidates<kLanes, kOctets>(E, lane, __any_sync(kAll, has_nan), v);
+        bool sure = true;
+        if (grouped) {
+            float error = -1.f;
+            if (by_score) {  // a group is worth up to two values, and two groups are compared
+                float far = 0.f;
+#pragma unroll
+                for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) far = fabsf(v[q][i]) < INFINITY ? fmaxf(far, fabsf(v[q][i])) : far;
+                error = 4.f * (score_error + kSmallest + kSumError * most<kLanes>(far));
+            }
+            if (by_score && !p.bias) {  // the groups by sums of scores, experts by their logits
+                float l[kOctets][8];
+                load_logits<T, kLanes, kOctets, kVector>(p, token, lane, l);
+                only_candidates<kLanes, kOctets>(E, lane, true, l);
+                sure = keep_best_groups<kLanes, kOctets>(p, s, segment, lane, error, v, l);
+#pragma unroll
+                for (int q = 0; q < kOctets; ++q)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[q][i] = l[q][i];
+            } else {
+                sure = keep_best_groups<kLanes, kOctets>(p, s, segment, lane, error, v, v);
+            }
         }
         __syncwarp();
         float head[kOctets];  // largest of each octet
@@ -403,23 +460,31 @@ __global__ void __launch_bounds__(kThreads) route_forward_kernel(const RouteArgs
 #pragma unroll
             for (int i = 0; i < 8; ++i) head[q] = fmaxf(head[q], v[q][i]);
         }
-        const auto largest_left = [&]() {
+        const auto largest_of_lane = [&]() {
             float top = head[0];
 #pragma unroll
             for (int q = 1; q < kOctets; ++q) top = fmaxf(top, head[q]);
-            return most<kLanes>(top);
+            return top;
         };
-        // the first expert of value `top` leaves; its lane gets the index, others -1
-        const auto take = [&](float top) {
+        // The first expert of the largest value leaves (value in `top`, NaN where none is left); its lane gets the index, others -1.
+        const auto take = [&](float &top) {
+            const float own = largest_of_lane();
+            top = most<kLanes>(own);
+            const unsigned have = __ballot_sync(kAll, own == top) >> (segment * kLanes) & ((1ull << kLanes) - 1);
             int octet = INT32_MAX;
+            if (own == top) {
 #pragma unroll
-            for (int q = kOctets - 1; q >= 0; --q)
-                if (head[q] == top) octet = q * kLanes + lane;
-            octet = least<kLanes>(octet);
-            if (octet % kLanes != lane || octet == INT32_MAX) return -1;
+                for (int q = kOctets - 1; q >= 0; --q)
+                    if (head[q] == top) octet = q * kLanes + lane;
+            }
+            if (__any_sync(kAll, have & (have - 1))) {  // several lanes: the lowest octet's
+                const int first = least<kLanes>(octet);
+                if (octet != first) octet = INT32_MAX;
+            }
+            if (octet == INT32_MAX) return -1;
             float4 *at = reinterpret_cast<float4 *>(values + octet * 8);
             const float4 a = at[0], b = at[1];
-            float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
             int slot = 0;
 #pragma unroll
             for (int i = 7; i >= 0; --i)
@@ -434,7 +499,7 @@ __global__ void __launch_bounds__(kThreads) route_forward_kernel(const RouteArgs
             return octet * 8 + slot;
         };
         for (int j = 0; j < p.top_k; ++j) {
-            const float top = largest_left();
+            float top;
             const int e = take(top);
             if (e >= 0) {
                 s.chosen[segment][j] = e;
@@ -444,10 +509,8 @@ __global__ void __launch_bounds__(kThreads) route_forward_kernel(const RouteArgs
         __syncwarp();
         if (p.bias) {
             // the chosen among themselves, and the last of them against what is left
-            const float margin = 2.f * largest * kScoreError + kSmallest, last = s.chosen_value[segment][p.top_k - 1];
-            const auto same = [&](int a, int b) {
-                return logit<T>(p, active ? token : base, a) == logit<T>(p, active ? token : base, b) && bias[a] == bias[b];
-            };
+            const float margin = 2.f * score_error + kSmallest, last = s.chosen_value[segment][p.top_k - 1];
+            const auto same = [&](int a, int b) { return logit<T>(p, token, a) == logit<T>(p, token, b) && bias[a] == bias[b]; };
             for (int j = lane; j + 1 < p.top_k; j += kLanes) {
                 const float a = s.chosen_value[segment][j], b = s.chosen_value[segment][j + 1];
                 if (!(a - b > margin + fabsf(a) * kSumError) && !same(s.chosen[segment][j], s.chosen[segment][j + 1])) sure = false;
@@ -456,7 +519,7 @@ __global__ void __launch_bounds__(kThreads) route_forward_kernel(const RouteArgs
             const int last_chosen = s.chosen[segment][p.top_k - 1];
             bool open = most<kLanes>(sure ? 0.f : 1.f) == 0.f;
             while (true) {  // ends: a pass takes an expert out of every token that has one
-                const float next = largest_left();
+                float next = most<kLanes>(largest_of_lane());
                 open = open && next == next && !(last - next > margin + fabsf(last) * kSumError);
                 if (!__any_sync(kAll, open)) break;
                 const int e = take(next);
@@ -478,8 +541,12 @@ __global__ void __launch_bounds__(kThreads) route_forward_kernel(const RouteArgs
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             there[i] = lane + i * kLanes < p.top_k;
-            mine[i] = there[i] ? s.chosen[segment][lane + i * kLanes] : 0;
-            l[i] = logit<T>(p, active ? token : base, mine[i]);
+            mine[i] = 0;
+            l[i] = 0.f;
+            if (there[i]) {
+                mine[i] = s.chosen[segment][lane + i * kLanes];
+                l[i] = logit<T>(p, token, mine[i]);
+            }
         }
         const float sum = chosen_scores<kLanes, kMine>(p, l, there, shift, inverse, score);
         if (!active) continue;
@@ -557,9 +624,10 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArg
             const float4 *at = reinterpret_cast<const float4 *>(row + first);
             const float4 a = at[0], b = at[1];
             float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            if (dense && inverse != 0.f) {
+            if (dense) {
+                const float each = inverse * along;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] -= expf(v[q][i] - shift) * inverse * along;
+                for (int i = 0; i < 8; ++i) d[i] -= v[q][i] * each;
             }
             if (kVector) {
                 Raw<T, 8> raw;
