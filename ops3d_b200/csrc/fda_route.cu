@@ -12,7 +12,8 @@
 //
 // kLanes (8, or 16 beyond 512 experts) lanes take a token, so that a warp's instructions serve four.  A lane holds octets of
 // neighbouring experts, octet o of the token belonging to lane o mod kLanes.  Their values lie in shared memory, their largest in a
-// register: a step of the choice takes the largest of these over the lanes, and only the lane that has it looks into its octet again.
+// register: a step of the choice takes the largest of these over the lanes, then a lane looks at each value of the octet that has it.
+// Bound by the pipe of comparisons and selections.
 #include "fda_rows.cuh"
 
 #include <algorithm>
@@ -372,7 +373,7 @@ __device__ __forceinline__ void only_candidates(int n_experts, int lane, bool ha
 }
 
 template <typename T, int kLanes, int kOctets, bool kVector>
-__global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 6 : 3) route_forward_kernel(const RouteArgs p) {
+__global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_kernel(const RouteArgs p) {
     using Shared = WarpShared<kLanes, kOctets>;
     __shared__ alignas(16) Shared warps[kWarps];
     __shared__ alignas(16) float bias[Shared::kExperts];
@@ -426,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 6 : 3) route_forward_
         }
         only_candidates<kLanes, kOctets>(E, lane, __any_sync(kAll, has_nan), v);
         bool sure = true;
+        __syncwarp();
         if (grouped) {
             float error = -1.f;
             if (by_score) {  // a group is worth up to two values, and two groups are compared
@@ -449,7 +451,6 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 6 : 3) route_forward_
                 sure = keep_best_groups<kLanes, kOctets>(p, s, segment, lane, error, v, v);
             }
         }
-        __syncwarp();
         float head[kOctets];  // largest of each octet
 #pragma unroll
         for (int q = 0; q < kOctets; ++q) {
@@ -460,48 +461,41 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 6 : 3) route_forward_
 #pragma unroll
             for (int i = 0; i < 8; ++i) head[q] = fmaxf(head[q], v[q][i]);
         }
+        __syncwarp();
         const auto largest_of_lane = [&]() {
             float top = head[0];
 #pragma unroll
             for (int q = 1; q < kOctets; ++q) top = fmaxf(top, head[q]);
             return top;
         };
-        // The first expert of the largest value leaves (value in `top`, NaN where none is left); its lane gets the index, others -1.
+        // The first expert of the largest value leaves: every lane of the token gets its value (NaN where none is left) and its number (-1).
+        // The octet that it is in is looked at by a lane an expert, always the same one, so that no lane reads what another has written.
         const auto take = [&](float &top) {
             const float own = largest_of_lane();
             top = most<kLanes>(own);
-            const unsigned have = __ballot_sync(kAll, own == top) >> (segment * kLanes) & ((1ull << kLanes) - 1);
+            constexpr unsigned kSegment = (unsigned)((1ull << kLanes) - 1);
+            const unsigned have = __ballot_sync(kAll, own == top) >> (segment * kLanes) & kSegment;
             int octet = INT32_MAX;
-            if (own == top) {
 #pragma unroll
-                for (int q = kOctets - 1; q >= 0; --q)
-                    if (head[q] == top) octet = q * kLanes + lane;
-            }
-            if (__any_sync(kAll, have & (have - 1))) {  // several lanes: the lowest octet's
-                const int first = least<kLanes>(octet);
-                if (octet != first) octet = INT32_MAX;
-            }
-            if (octet == INT32_MAX) return -1;
-            float4 *at = reinterpret_cast<float4 *>(values + octet * 8);
-            const float4 a = at[0], b = at[1];
-            const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            int slot = 0;
-#pragma unroll
-            for (int i = 7; i >= 0; --i)
-                if (x[i] == top) slot = i;
-            float rest = NAN;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) rest = fmaxf(rest, i == slot ? NAN : x[i]);
-            values[octet * 8 + slot] = NAN;
+            for (int q = kOctets - 1; q >= 0; --q)
+                if (head[q] == top) octet = q * kLanes + lane;
+            if (__any_sync(kAll, have & (have - 1))) octet = least<kLanes>(octet);  // several lanes have it
+            else octet = __shfl_sync(kAll, octet, __ffs(have) - 1, kLanes);
+            const bool any = have != 0;
+            const float x = any && (kLanes == 8 || lane < 8) ? values[octet * 8 + lane] : NAN;
+            const int slot = __ffs(__ballot_sync(kAll, x == top) >> (segment * kLanes) & kSegment) - 1;
+            const float rest = most<kLanes>(lane == slot ? NAN : x);
+            if (!any) return -1;
+            if (lane == slot) values[octet * 8 + lane] = NAN;
 #pragma unroll
             for (int q = 0; q < kOctets; ++q)
-                if (octet / kLanes == q) head[q] = rest;
+                if (octet == q * kLanes + lane) head[q] = rest;
             return octet * 8 + slot;
         };
         for (int j = 0; j < p.top_k; ++j) {
             float top;
             const int e = take(top);
-            if (e >= 0) {
+            if (lane == 0) {
                 s.chosen[segment][j] = e;
                 s.chosen_value[segment][j] = top;
             }
@@ -515,17 +509,15 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 6 : 3) route_forward_
                 const float a = s.chosen_value[segment][j], b = s.chosen_value[segment][j + 1];
                 if (!(a - b > margin + fabsf(a) * kSumError) && !same(s.chosen[segment][j], s.chosen[segment][j + 1])) sure = false;
             }
+            sure = most<kLanes>(sure ? 0.f : 1.f) == 0.f;
             // of equal experts the lower ones are chosen: what comes behind them counts
             const int last_chosen = s.chosen[segment][p.top_k - 1];
-            bool open = most<kLanes>(sure ? 0.f : 1.f) == 0.f;
             while (true) {  // ends: a pass takes an expert out of every token that has one
                 float next = most<kLanes>(largest_of_lane());
-                open = open && next == next && !(last - next > margin + fabsf(last) * kSumError);
+                const bool open = sure && next == next && !(last - next > margin + fabsf(last) * kSumError);
                 if (!__any_sync(kAll, open)) break;
                 const int e = take(next);
-                if (open && e >= 0 && !same(last_chosen, e)) sure = false;
-                const float settled = most<kLanes>(sure ? 0.f : 1.f);  // every lane takes part
-                open = open && settled == 0.f;
+                if (open && !same(last_chosen, e)) sure = false;
             }
         }
         const unsigned unsure = __ballot_sync(kAll, active && !sure);
