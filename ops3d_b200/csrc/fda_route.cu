@@ -354,10 +354,10 @@ __device__ __forceinline__ bool keep_best_groups(const RouteArgs &p, WarpShared<
     return error < 0.f || low - high > error || low == -INFINITY;
 }
 
-// NaN for experts beyond the last, which are no candidates; minus infinity for other NaN.
+// NaN for experts beyond the last, which are no candidates; with `sanitise` minus infinity for other NaN.
 template <int kLanes, int kOctets>
-__device__ __forceinline__ void only_candidates(int n_experts, int lane, bool has_nan, float (&v)[kOctets][8]) {
-    if (has_nan) {
+__device__ __forceinline__ void only_candidates(int n_experts, int lane, bool sanitise, float (&v)[kOctets][8]) {
+    if (sanitise) {
 #pragma unroll
         for (int q = 0; q < kOctets; ++q)
 #pragma unroll
@@ -395,16 +395,14 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
         const long long token = active ? base + segment : base;
         float v[kOctets][8], shift = 0.f, inverse = 1.f, largest = 1.f;
         load_logits<T, kLanes, kOctets, kVector>(p, token, lane, v);
-        bool has_nan = true;  // perhaps
         if (need_softmax) {
             softmax_of<kLanes, kOctets>(v, p.renormalise, shift, inverse);
             largest = inverse;
             if (by_score) {
-                has_nan = !(inverse == inverse);  // then every score is
 #pragma unroll
                 for (int q = 0; q < kOctets; ++q)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[q][i] *= inverse;
+                    for (int i = 0; i < 8; i += 2) (Pair(v[q][i], v[q][i + 1]) * Pair(inverse)).get(v[q][i], v[q][i + 1]);
             } else {
                 load_logits<T, kLanes, kOctets, kVector>(p, token, lane, v);
             }
@@ -420,12 +418,13 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
             for (int q = 0; q < kOctets; ++q) {
                 const float4 *at = reinterpret_cast<const float4 *>(bias + (q * kLanes + lane) * 8);
                 const float4 a = at[0], b = at[1];
-                const float add[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                const Pair add[4] = {Pair(a.x, a.y), Pair(a.z, a.w), Pair(b.x, b.y), Pair(b.z, b.w)};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[q][i] = __fadd_rn(v[q][i], add[i]);
+                for (int i = 0; i < 4; ++i) (Pair(v[q][2 * i], v[q][2 * i + 1]) + add[i]).get(v[q][2 * i], v[q][2 * i + 1]);
             }
         }
-        only_candidates<kLanes, kOctets>(E, lane, __any_sync(kAll, has_nan), v);
+        // a NaN is never the largest; where nothing else is left the choice is made again below
+        only_candidates<kLanes, kOctets>(E, lane, grouped, v);
         bool sure = true;
         __syncwarp();
         if (grouped) {
@@ -495,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
         for (int j = 0; j < p.top_k; ++j) {
             float top;
             const int e = take(top);
+            if (e < 0) sure = false;
             if (lane == 0) {
                 s.chosen[segment][j] = e;
                 s.chosen_value[segment][j] = top;
@@ -504,7 +504,9 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
         if (p.bias) {
             // the chosen among themselves, and the last of them against what is left
             const float margin = 2.f * score_error + kSmallest, last = s.chosen_value[segment][p.top_k - 1];
-            const auto same = [&](int a, int b) { return logit<T>(p, token, a) == logit<T>(p, token, b) && bias[a] == bias[b]; };
+            const auto same = [&](int a, int b) {
+                return min(a, b) >= 0 && logit<T>(p, token, a) == logit<T>(p, token, b) && bias[a] == bias[b];
+            };
             for (int j = lane; j + 1 < p.top_k; j += kLanes) {
                 const float a = s.chosen_value[segment][j], b = s.chosen_value[segment][j + 1];
                 if (!(a - b > margin + fabsf(a) * kSumError) && !same(s.chosen[segment][j], s.chosen[segment][j + 1])) sure = false;
@@ -557,14 +559,13 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
 //     softmax                  dl_i = scale p_i ([i chosen] dw_i - sum of dw p)
 //     sigmoid                  dl_j = ds_j s_j (1 - s_j),  ds_j = scale (dw_j - sum of dw s / S) / S  or  scale dw_j
 // An expert outside 0 .. n_experts - 1 gets none.  No atomics: a row is put together in shared memory.
-template <typename T, int kLanes, int kOctets, bool kVector>
+template <typename T, int kLanes, int kOctets, bool kVector, bool kDense>
 __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArgs p) {
     constexpr int kTokens = 32 / kLanes, kExperts = kLanes * kOctets * 8, kMine = kMostChoices / kLanes;
     __shared__ alignas(16) float rows[kWarps][kTokens][kExperts];
     wait_for_previous_kernel();
     const int lane = threadIdx.x % kLanes, segment = threadIdx.x % 32 / kLanes, E = p.n_experts;
     float *row = rows[threadIdx.x / 32][segment];
-    const bool dense = !p.sigmoid && !p.renormalise;
     const long long step = (long long)gridDim.x * kWarps * kTokens;
     for (long long base = ((long long)blockIdx.x * kWarps + threadIdx.x / 32) * kTokens; base < p.tokens; base += step) {
         const bool active = base + segment < p.tokens;
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArg
             dw[i] = there[i] ? p.grad_weights[token * p.top_k + j] * p.scale : 0.f;
         }
         float v[kOctets][8], shift = 0.f, inverse = 1.f;
-        if (dense) {
+        if (kDense) {  // softmax without renormalising: every expert's logit has a gradient
             load_logits<T, kLanes, kOctets, kVector>(p, token, lane, v);
             softmax_of<kLanes, kOctets>(v, false, shift, inverse);
         }
@@ -616,7 +617,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArg
             const float4 *at = reinterpret_cast<const float4 *>(row + first);
             const float4 a = at[0], b = at[1];
             float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            if (dense) {
+            if (kDense) {
                 const float each = inverse * along;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) d[i] -= v[q][i] * each;
@@ -639,8 +640,10 @@ int launch_route(bool backward, const RouteArgs &p, cudaStream_t st) {
     const unsigned blocks = (unsigned)std::min<long long>(ceil_div(p.tokens, kWarps * 32 / kLanes), 16 * kSms);
     // rows of octets that start on 16-byte boundaries
     const bool vector = p.n_experts % 8 == 0 && !misaligned16(p.logits) && !misaligned16(p.grad_logits);
-    const auto kernel = backward ? (vector ? route_backward_kernel<T, kLanes, kOctets, true> : route_backward_kernel<T, kLanes, kOctets, false>)
-                                 : (vector ? route_forward_kernel<T, kLanes, kOctets, true> : route_forward_kernel<T, kLanes, kOctets, false>);
+    const bool dense = !p.sigmoid && !p.renormalise;
+    const auto kernel = !backward ? (vector ? route_forward_kernel<T, kLanes, kOctets, true> : route_forward_kernel<T, kLanes, kOctets, false>)
+                        : dense   ? (vector ? route_backward_kernel<T, kLanes, kOctets, true, true> : route_backward_kernel<T, kLanes, kOctets, false, true>)
+                                  : (vector ? route_backward_kernel<T, kLanes, kOctets, true, false> : route_backward_kernel<T, kLanes, kOctets, false, false>);
     return launched(launch_early(kernel, blocks, kThreads, 0, st, 1, p));
 }
 
