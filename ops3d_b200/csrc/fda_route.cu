@@ -266,10 +266,16 @@ template <int kLanes, int kOctets>
 struct WarpShared {
     static constexpr int kTokens = 32 / kLanes, kExperts = kLanes * kOctets * 8;
     float values[kTokens][kExperts];
-    float2 largest[kTokens][kExperts / 8];  // two of each octet
-    float worth[kTokens][kMostExpertGroups];
-    float chosen_value[kTokens][kMostChoices];
-    int chosen[kTokens][kMostChoices];
+    union {
+        struct {  // while groups are chosen
+            float2 largest[kTokens][kExperts / 8];  // two of each octet
+            float worth[kTokens][kMostExpertGroups];
+        };
+        struct {  // after it
+            float chosen_value[kTokens][kMostChoices];
+            int chosen[kTokens][kMostChoices];
+        };
+    };
 };
 
 __device__ __forceinline__ float2 two_largest(float2 a, float2 b) {  // of two pairs, each largest first
@@ -481,11 +487,21 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
             if (__any_sync(kAll, have & (have - 1))) octet = least<kLanes>(octet);  // several lanes have it
             else octet = __shfl_sync(kAll, octet, __ffs(have) - 1, kLanes);
             const bool any = have != 0;
-            const float x = any && (kLanes == 8 || lane < 8) ? values[octet * 8 + lane] : NAN;
-            const int slot = __ffs(__ballot_sync(kAll, x == top) >> (segment * kLanes) & kSegment) - 1;
-            const float rest = most<kLanes>(lane == slot ? NAN : x);
+            // a lane looks at one or two of its experts
+            constexpr int kLooks = kLanes >= 8 ? 1 : 8 / kLanes;
+            float x[kLooks], rest = NAN;
+            int slot = -1;
+#pragma unroll
+            for (int i = 0; i < kLooks; ++i) {
+                x[i] = any && (kLanes <= 8 || lane < 8) ? values[octet * 8 + i * kLanes + lane] : NAN;
+                const unsigned equal = __ballot_sync(kAll, x[i] == top) >> (segment * kLanes) & kSegment;
+                if (slot < 0 && equal) slot = i * kLanes + __ffs(equal) - 1;
+            }
+#pragma unroll
+            for (int i = 0; i < kLooks; ++i) rest = fmaxf(rest, slot == i * kLanes + lane ? NAN : x[i]);
+            rest = most<kLanes>(rest);
             if (!any) return -1;
-            if (lane == slot) values[octet * 8 + lane] = NAN;
+            if (slot % kLanes == lane) values[octet * 8 + slot] = NAN;
 #pragma unroll
             for (int q = 0; q < kOctets; ++q)
                 if (octet == q * kLanes + lane) head[q] = rest;
@@ -558,14 +574,14 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
 //     softmax, renormalised    dl_j = w_j (dw_j - sum of dw w / scale)           (a softmax over the chosen alone)
 //     softmax                  dl_i = scale p_i ([i chosen] dw_i - sum of dw p)
 //     sigmoid                  dl_j = ds_j s_j (1 - s_j),  ds_j = scale (dw_j - sum of dw s / S) / S  or  scale dw_j
-// An expert outside 0 .. n_experts - 1 gets none.  No atomics: a row is put together in shared memory.
+// An expert outside 0 .. n_experts - 1 gets none.  A token's row is one team's, so there are no atomics.
 template <typename T, int kLanes, int kOctets, bool kVector, bool kDense>
 __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArgs p) {
     constexpr int kTokens = 32 / kLanes, kExperts = kLanes * kOctets * 8, kMine = kMostChoices / kLanes;
-    __shared__ alignas(16) float rows[kWarps][kTokens][kExperts];
+    __shared__ alignas(16) float rows[kDense ? kWarps : 1][kTokens][kDense ? kExperts : 1];
     wait_for_previous_kernel();
     const int lane = threadIdx.x % kLanes, segment = threadIdx.x % 32 / kLanes, E = p.n_experts;
-    float *row = rows[threadIdx.x / 32][segment];
+    float *row = rows[kDense ? threadIdx.x / 32 : 0][segment];
     const long long step = (long long)gridDim.x * kWarps * kTokens;
     for (long long base = ((long long)blockIdx.x * kWarps + threadIdx.x / 32) * kTokens; base < p.tokens; base += step) {
         const bool active = base + segment < p.tokens;
@@ -593,43 +609,65 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArg
 #pragma unroll
         for (int i = 0; i < kMine; ++i) along += dw[i] * score[i] * over;
         along = total<kLanes>(along);
-        __syncwarp();
-#pragma unroll
-        for (int q = 0; q < kOctets; ++q) {
-            float4 *at = reinterpret_cast<float4 *>(row + (q * kLanes + lane) * 8);
-            at[0] = at[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        __syncwarp();
+        T *out = static_cast<T *>(p.grad_logits) + token * E;
+        float dl[kMine];
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
-            if (!there[i]) continue;
-            float dl = score[i] * over * (p.renormalise ? dw[i] - along : dw[i]);
-            if (p.sigmoid) dl *= 1.f - score[i];
-            row[chosen[i]] = dl;
+            dl[i] = score[i] * over * (p.renormalise ? dw[i] - along : dw[i]);
+            if (p.sigmoid) dl[i] *= 1.f - score[i];
         }
-        __syncwarp();
-        if (!active) continue;
-        T *out = static_cast<T *>(p.grad_logits) + token * E;
+        if constexpr (!kDense) {  // zeros, and the chosen behind them
+            if (active) {
 #pragma unroll
-        for (int q = 0; q < kOctets; ++q) {
-            const int first = (q * kLanes + lane) * 8;
-            if (first >= E) continue;
-            const float4 *at = reinterpret_cast<const float4 *>(row + first);
-            const float4 a = at[0], b = at[1];
-            float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            if (kDense) {
-                const float each = inverse * along;
+                for (int q = 0; q < kOctets; ++q) {
+                    const int first = (q * kLanes + lane) * 8;
+                    if (kVector && first < E) {
+                        Raw<T, 8> raw;
+                        raw.clear();
+                        raw.store(out + first);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (first + i < E) out[first + i] = from_f32<T>(0.f);
+                    }
+                }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kMine; ++i)
+                if (active && there[i]) out[chosen[i]] = from_f32<T>(dl[i]);
+        } else {
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < kOctets; ++q) {
+                float4 *at = reinterpret_cast<float4 *>(row + (q * kLanes + lane) * 8);
+                at[0] = at[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kMine; ++i)
+                if (there[i]) row[chosen[i]] = dl[i];
+            __syncwarp();
+            if (!active) continue;
+            const float each = inverse * along;
+#pragma unroll
+            for (int q = 0; q < kOctets; ++q) {
+                const int first = (q * kLanes + lane) * 8;
+                if (first >= E) continue;
+                const float4 *at = reinterpret_cast<const float4 *>(row + first);
+                const float4 a = at[0], b = at[1];
+                float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
                 for (int i = 0; i < 8; ++i) d[i] -= v[q][i] * each;
-            }
-            if (kVector) {
-                Raw<T, 8> raw;
-                raw.set(d);
-                raw.store(out + first);
-            } else {
+                if (kVector) {
+                    Raw<T, 8> raw;
+                    raw.set(d);
+                    raw.store(out + first);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (first + i < E) out[first + i] = from_f32<T>(d[i]);
+                    for (int i = 0; i < 8; ++i)
+                        if (first + i < E) out[first + i] = from_f32<T>(d[i]);
+                }
             }
         }
     }
@@ -649,7 +687,8 @@ int launch_route(bool backward, const RouteArgs &p, cudaStream_t st) {
 
 template <typename T>
 int launch_route(bool backward, const RouteArgs &p, cudaStream_t st) {
-    if (p.n_experts <= 64) return launch_route<T, 8, 1>(backward, p, st);
+    if (p.n_experts <= 32) return launch_route<T, 4, 1>(backward, p, st);
+    if (p.n_experts <= 64) return launch_route<T, 4, 2>(backward, p, st);
     if (p.n_experts <= 128) return launch_route<T, 8, 2>(backward, p, st);
     if (p.n_experts <= 256) return launch_route<T, 8, 4>(backward, p, st);
     if (p.n_experts <= 512) return launch_route<T, 8, 8>(backward, p, st);
