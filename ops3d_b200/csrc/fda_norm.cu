@@ -6,22 +6,22 @@
 namespace fda_norm {
 namespace {
 
-// grad_weight and grad_bias from the blocks' partial sums [count][2][width], added in a fixed order: 32 columns a block, 8 threads a
-// column, each taking every eighth partial sum.
-constexpr int kSumThreads = 256;
-__global__ void __launch_bounds__(kSumThreads) norm_sum_kernel(const float *partial, int count, int width, void *grad_weight, void *grad_bias,
-                                                               int dtype) {
+// grad_weight and grad_bias from the blocks' partial sums [count][2][width], added in a fixed order: 32 columns a block, its warps
+// (as many as there are sums for, up to 32) taking turns over them.
+__global__ void __launch_bounds__(1024) norm_sum_kernel(const float *partial, int count, int width, void *grad_weight, void *grad_bias, int dtype) {
     wait_for_previous_kernel();
-    __shared__ float sums[8][33];
-    const int lane = threadIdx.x % 32, part = threadIdx.x / 32;
+    __shared__ float sums[32][32];
+    const int lane = threadIdx.x % 32, part = threadIdx.x / 32, parts = blockDim.x / 32;
     const long long column = (long long)blockIdx.x * 32 + lane;
     float s = 0.f;
-    if (column < 2ll * width)
-        for (int i = part; i < count; i += 8) s += partial[(size_t)i * 2 * width + column];
+    if (column < 2ll * width) {
+#pragma unroll 8
+        for (int i = part; i < count; i += parts) s += partial[(size_t)i * 2 * width + column];
+    }
     sums[part][lane] = s;
     __syncthreads();
     if (part != 0 || column >= 2ll * width) return;
-    for (int k = 1; k < 8; ++k) s += sums[k][lane];
+    for (int k = 1; k < parts; ++k) s += sums[k][lane];
     void *out = column < width ? grad_weight : grad_bias;
     if (out) store_from_f32(out, dtype, column < width ? column : column - width, s);
 }
@@ -106,15 +106,12 @@ __global__ void __launch_bounds__(256) norm_wide_columns_kernel(const WideArgs p
 
 constexpr int kWideParts = 64;
 
-// Blocks of the backward, each of which leaves sums of its own.
-unsigned backward_blocks(long long rows, int width, int dtype) { return norm_blocks(norm_shape(width, dtype), rows, true); }
-
 struct Workspace {
     size_t partial, statistics, total;
 };
 Workspace workspace_of(long long rows, int width, int dtype) {
     const bool wide = is_wide(width, dtype);
-    const size_t parts = wide ? (size_t)std::min<long long>(rows, kWideParts) : backward_blocks(rows, width, dtype);
+    const size_t parts = wide ? (size_t)std::min<long long>(rows, kWideParts) : norm_backward_blocks(norm_shape(width, dtype, true), rows, dtype);
     Workspace w;
     w.partial = fda_linear::round256(parts * 2 * width * sizeof(float));
     w.statistics = wide ? fda_linear::round256((size_t)rows * 2 * sizeof(float)) : 0;
@@ -122,11 +119,11 @@ Workspace workspace_of(long long rows, int width, int dtype) {
     return w;
 }
 
-int run_fast(bool backward, const NormArgs &p, int dtype, int residual_dtype, unsigned blocks, cudaStream_t st) {
-    const NormShape s = norm_shape(p.width, dtype);
-    if (dtype == FDA_DTYPE_F32) return norm_f32(backward, p, s, residual_dtype, blocks, st);
-    if (dtype == FDA_DTYPE_F16) return norm_f16(backward, p, s, residual_dtype, blocks, st);
-    return norm_bf16(backward, p, s, residual_dtype, blocks, st);
+int run_fast(bool backward, const NormArgs &p, int dtype, int residual_dtype, cudaStream_t st) {
+    const NormShape s = norm_shape(p.width, dtype, backward);
+    if (dtype == FDA_DTYPE_F32) return norm_f32(backward, p, s, residual_dtype, st);
+    if (dtype == FDA_DTYPE_F16) return norm_f16(backward, p, s, residual_dtype, st);
+    return norm_bf16(backward, p, s, residual_dtype, st);
 }
 
 int check(long long rows, int width, int dtype, int param_dtype, int residual_dtype, bool residual) {
@@ -159,8 +156,7 @@ int fda_layer_norm_forward(const void *x, const void *weight, const void *bias, 
         WideArgs w{p, dtype, residual_dtype, nullptr, 0};
         return launched(launch_early(norm_wide_kernel<false>, (unsigned)std::min<long long>(rows, 4 * kSms), kWideThreads, 0, st, 1, w));
     }
-    const NormShape s = norm_shape(features, dtype);
-    return run_fast(false, p, dtype, residual_dtype, norm_blocks(s, rows, false), st);
+    return run_fast(false, p, dtype, residual_dtype, st);
 }
 
 size_t fda_layer_norm_backward_workspace_bytes(long long rows, int features, int dtype) {
@@ -208,11 +204,12 @@ int fda_layer_norm_backward(const void *x, const void *weight, const void *resid
         norm_wide_columns_kernel<<<dim3((unsigned)ceil_div(features, 256), parts), 256, 0, st>>>(w);
         if (const int rc = launched(cudaGetLastError())) return rc;
     } else {
-        parts = (int)backward_blocks(rows, features, dtype);
-        if (const int rc = run_fast(true, p, dtype, residual_dtype, parts, st)) return rc;
+        parts = (int)norm_backward_blocks(norm_shape(features, dtype, true), rows, dtype);
+        if (const int rc = run_fast(true, p, dtype, residual_dtype, st)) return rc;
         if (!parameters) return FDA_OK;
     }
-    return launched(launch_early(norm_sum_kernel, (unsigned)ceil_div(2ll * features, 32), kSumThreads, 0, st, 1, static_cast<const float *>(p.partial),
+    const unsigned threads = 32 * (unsigned)std::min<long long>(32, ceil_div(parts, 4));
+    return launched(launch_early(norm_sum_kernel, (unsigned)ceil_div(2ll * features, 32), threads, 0, st, 1, static_cast<const float *>(p.partial),
                                  parts, features, grad_weight, grad_bias, param_dtype));
 }
 

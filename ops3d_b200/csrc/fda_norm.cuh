@@ -15,6 +15,8 @@
 
 #include "fda_rows.cuh"
 
+#include <algorithm>
+
 namespace fda_norm {
 
 using namespace fda_rows;
@@ -196,17 +198,28 @@ __device__ __forceinline__ Team<kLanes> make_team() {
     return team;
 }
 
-// 16-byte places of a lane for one row, and rows of the ring: as many bytes on their way as DRAM's latency takes (40 KB to an SM and more),
-// and no more than two blocks (one of 1024 threads) have room for.
+// 16-byte places of a lane for one row, rows of the ring, and (where teams are lanes) blocks to an SM.  They are so many that 48 KB or so are
+// on their way to an SM: that covers DRAM's latency, and more makes it slower (598016 x 256 bf16 forward with a residual: 32 KB 144 us, 48 KB
+// 138, 72 KB 185).
 template <typename T, typename R, bool kResidual, int kVectors, bool kBackward>
 constexpr int kUnitsOf = kVectors * ((kBackward ? 2 : 1) + (kResidual ? (int)(sizeof(R) / sizeof(T)) : 0));
-template <int kUnits, int kLanes>
-constexpr int kStagesOf = kLanes || kUnits <= 2 ? 4 : kUnits <= 4 ? 3 : 2;
+#ifndef KB2
+#define KB2 4
+#define KB3 4
+#define BT2 3
+#define BT3 2
+#endif
+template <int kUnits, int kLanes, bool kBackward>
+constexpr int kStagesOf = kLanes == 0  ? (kUnits == 1 ? 4 : kUnits == 2 ? BT2 : BT3)
+                          : kBackward ? (kUnits == 2 ? KB2 : kUnits == 3 ? KB3 : 2)
+                                      : (kUnits <= 2 ? 4 : kUnits == 3 ? 3 : 2);
+template <int kUnits>
+constexpr int kForwardBlocks = kUnits == 1 ? 4 : kUnits == 4 ? 3 : 2;
 
 // R: the residual's type; kResidual false: there is none.
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes, bool kRagged>
 __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_forward_kernel(const NormArgs p) {
-    constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, false>, kStages = kStagesOf<kUnits, kLanes>;
+    constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, false>, kStages = kStagesOf<kUnits, kLanes, false>;
     extern __shared__ uint4 ring[];
     wait_for_previous_kernel();
     Team<kLanes> team = make_team<kLanes>();
@@ -287,7 +300,7 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
 
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes, bool kRagged>
 __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_backward_kernel(const NormArgs p) {
-    constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, true>, kStages = kStagesOf<kUnits, kLanes>;
+    constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, true>, kStages = kStagesOf<kUnits, kLanes, true>;
     extern __shared__ uint4 ring[];
     wait_for_previous_kernel();
     Team<kLanes> team = make_team<kLanes>();
@@ -408,7 +421,7 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
                 }
     } else {
         // teams of a warp have the same columns unless rows are ragged
-        constexpr int kSteps = kRagged ? kTeamThreads / (kLanes ? kLanes : 1) : kTeamThreads / 32;
+        constexpr int kTeams = kRagged ? kTeamThreads / (kLanes ? kLanes : 1) : kTeamThreads / 32;
         if (!kRagged) {
 #pragma unroll
             for (int i = 0; i < kVectors; ++i)
@@ -420,24 +433,25 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
                     }
         }
         __syncthreads();
-        float *columns = reinterpret_cast<float *>(ring);  // [2][width]
-        for (int i = threadIdx.x; i < 2 * p.width; i += kTeamThreads) columns[i] = 0.f;
-        const int turn = kRagged ? (int)threadIdx.x / (kLanes ? kLanes : 1)
-                                 : (int)threadIdx.x % 32 < kLanes ? (int)threadIdx.x / 32 : -1;
-        for (int t = 0; t < kSteps; ++t) {
-            __syncthreads();
-            if (turn != t) continue;
+        float *columns = reinterpret_cast<float *>(ring);  // [kTeams][2][width]
+        const int t = kRagged ? (int)threadIdx.x / (kLanes ? kLanes : 1) : (int)threadIdx.x / 32;
+        if (kRagged || threadIdx.x % 32 < kLanes) {
 #pragma unroll
             for (int i = 0; i < kVectors; ++i)
 #pragma unroll
                 for (int j = 0; j < W; ++j)
                     if (c.has(i, j)) {
-                        columns[c.first[i] + j] += grad_weight[i][j];
-                        columns[p.width + c.first[i] + j] += grad_bias[i][j];
+                        columns[t * 2 * p.width + c.first[i] + j] = grad_weight[i][j];
+                        columns[(t * 2 + 1) * p.width + c.first[i] + j] = grad_bias[i][j];
                     }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < 2 * p.width; i += kTeamThreads) out[i] = columns[i];
+        for (int i = threadIdx.x; i < 2 * p.width; i += kTeamThreads) {
+            float sum = 0.f;
+#pragma unroll 8
+            for (int k = 0; k < kTeams; ++k) sum += columns[k * 2 * p.width + i];
+            out[i] = sum;
+        }
     }
 }
 
@@ -447,10 +461,11 @@ struct NormShape {
     int lanes, vectors, threads;
     bool ragged;
 };
-// 8 values of a row to a lane; 16 where that still lets a warp take the row, which saves the barriers of a block.
+// 8 values of a row to a lane; 16 where that still lets a warp take the row, which saves the barriers of a block.  Not in the backward of
+// ragged rows: masks and sums beside 16 values leave one block to an SM (100000 x 259 bf16: 130 us, by 64 threads 117; forward 49 and 58).
 constexpr int kMostValues = 8;
 
-inline NormShape norm_shape(int width, int dtype) {
+inline NormShape norm_shape(int width, int dtype, bool backward) {
     const int W = dtype == FDA_DTYPE_F32 ? 4 : 8;
     NormShape s;
     s.ragged = width % W != 0;
@@ -461,33 +476,36 @@ inline NormShape norm_shape(int width, int dtype) {
         if (s.lanes * s.vectors >= vectors) return s;
     s.lanes = 32;
     s.vectors *= 2;
-    if (s.lanes * s.vectors >= vectors) return s;
+    if (!(s.ragged && backward) && s.lanes * s.vectors >= vectors) return s;
     s.vectors /= 2;
     s.lanes = 0;
     s.threads = (int)ceil_div(ceil_div(vectors, s.vectors), 32) * 32;
     return s;
 }
-inline bool is_wide(int width, int dtype) { return norm_shape(width, dtype).threads > kBlockThreads; }  // for a block's registers
+inline bool is_wide(int width, int dtype) { return norm_shape(width, dtype, true).threads > kBlockThreads; }  // for a block's registers
 
-// Blocks: as many as rows need, at most what fills the device; a multiple of 8 where a block is a team (rows 8 apart).
-inline unsigned norm_blocks(const NormShape &s, long long rows, bool backward) {
+// Blocks: as many as rows need, at most what is on the device at once (blocks that are teams have 64 registers a thread); a multiple of 8
+// where a block is a team (rows 8 apart).
+inline unsigned norm_blocks(const NormShape &s, long long rows, int per_sm) {
     const long long needed = ceil_div(rows, s.lanes ? s.threads / s.lanes : 1);
-    const int per_sm = s.lanes ? (backward ? 2 : 4) : (backward ? 1024 : 2048) / s.threads;
-    const long long room = (long long)kSms * (per_sm > 0 ? per_sm : 1);
-    long long blocks = needed < room ? needed : room;
-    if (!s.lanes) blocks = ceil_div(blocks, 8) * 8;
-    return (unsigned)blocks;
+    if (s.lanes) return (unsigned)std::min<long long>(needed, kSms * per_sm);
+    const long long room = (long long)kSms * (kBlockThreads / s.threads) / 8 * 8;
+    return (unsigned)std::min(ceil_div(needed, 8) * 8, room);
+}
+// Of the backward, whose blocks leave sums each.
+inline unsigned norm_backward_blocks(const NormShape &s, long long rows, int dtype) {
+    return norm_blocks(s, rows, s.vectors * (dtype == FDA_DTYPE_F32 ? 4 : 8) > kMostValues ? 2 : 3);
 }
 
 // The kernels of one type (fda_norm_f32.cu and so on).
-int norm_f32(bool backward, const NormArgs &p, const NormShape &s, int residual_dtype, unsigned blocks, cudaStream_t st);
-int norm_f16(bool backward, const NormArgs &p, const NormShape &s, int residual_dtype, unsigned blocks, cudaStream_t st);
-int norm_bf16(bool backward, const NormArgs &p, const NormShape &s, int residual_dtype, unsigned blocks, cudaStream_t st);
+int norm_f32(bool backward, const NormArgs &p, const NormShape &s, int residual_dtype, cudaStream_t st);
+int norm_f16(bool backward, const NormArgs &p, const NormShape &s, int residual_dtype, cudaStream_t st);
+int norm_bf16(bool backward, const NormArgs &p, const NormShape &s, int residual_dtype, cudaStream_t st);
 
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes>
-int run_norm(bool backward, const NormArgs &p, const NormShape &s, unsigned blocks, cudaStream_t st) {
+int run_norm(bool backward, const NormArgs &p, const NormShape &s, cudaStream_t st) {
     constexpr int kForward = kUnitsOf<T, R, kResidual, kVectors, false>, kBackward = kUnitsOf<T, R, kResidual, kVectors, true>;
-    const int units = backward ? kBackward * kStagesOf<kBackward, kLanes> : kForward * kStagesOf<kForward, kLanes>;
+    const int units = backward ? kBackward * kStagesOf<kBackward, kLanes, true> : kForward * kStagesOf<kForward, kLanes, false>;
     const int shared = units * s.threads * 16;
     const auto kernel = backward ? (s.ragged ? norm_backward_kernel<T, R, kResidual, kVectors, kLanes, true>
                                              : norm_backward_kernel<T, R, kResidual, kVectors, kLanes, false>)
@@ -495,25 +513,27 @@ int run_norm(bool backward, const NormArgs &p, const NormShape &s, unsigned bloc
                                              : norm_forward_kernel<T, R, kResidual, kVectors, kLanes, false>);
     if (shared > 40 * 1024)  // with the static part beyond what every launch may have; the attribute belongs to the current device
         if (const int rc = launched(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared))) return rc;
+    const unsigned blocks = backward ? norm_backward_blocks(s, p.rows, sizeof(T) == 4 ? FDA_DTYPE_F32 : FDA_DTYPE_F16)
+                                     : norm_blocks(s, p.rows, kForwardBlocks<kForward>);
     return launched(launch_early(kernel, blocks, s.threads, shared, st, 1, p));
 }
 
 template <typename T, typename R, bool kResidual>
-int run_norm(bool backward, const NormArgs &p, const NormShape &s, unsigned blocks, cudaStream_t st) {
+int run_norm(bool backward, const NormArgs &p, const NormShape &s, cudaStream_t st) {
     constexpr int kEach = kMostValues / kWidthOf<T>;
-    if (s.lanes == 4) return run_norm<T, R, kResidual, kEach, 4>(backward, p, s, blocks, st);
-    if (s.lanes == 8) return run_norm<T, R, kResidual, kEach, 8>(backward, p, s, blocks, st);
-    if (s.lanes == 16) return run_norm<T, R, kResidual, kEach, 16>(backward, p, s, blocks, st);
-    if (s.lanes == 0) return run_norm<T, R, kResidual, kEach, 0>(backward, p, s, blocks, st);
-    if (s.vectors == kEach) return run_norm<T, R, kResidual, kEach, 32>(backward, p, s, blocks, st);
-    return run_norm<T, R, kResidual, 2 * kEach, 32>(backward, p, s, blocks, st);
+    if (s.lanes == 4) return run_norm<T, R, kResidual, kEach, 4>(backward, p, s, st);
+    if (s.lanes == 8) return run_norm<T, R, kResidual, kEach, 8>(backward, p, s, st);
+    if (s.lanes == 16) return run_norm<T, R, kResidual, kEach, 16>(backward, p, s, st);
+    if (s.lanes == 0) return run_norm<T, R, kResidual, kEach, 0>(backward, p, s, st);
+    if (s.vectors == kEach) return run_norm<T, R, kResidual, kEach, 32>(backward, p, s, st);
+    return run_norm<T, R, kResidual, 2 * kEach, 32>(backward, p, s, st);
 }
 
 template <typename T>
-int run_norm(bool backward, const NormArgs &p, const NormShape &s, int residual_dtype, unsigned blocks, cudaStream_t st) {
-    if (!p.residual) return run_norm<T, T, false>(backward, p, s, blocks, st);
-    if (sizeof(T) == 2 && residual_dtype == FDA_DTYPE_F32) return run_norm<T, float, true>(backward, p, s, blocks, st);
-    return run_norm<T, T, true>(backward, p, s, blocks, st);
+int run_norm(bool backward, const NormArgs &p, const NormShape &s, int residual_dtype, cudaStream_t st) {
+    if (!p.residual) return run_norm<T, T, false>(backward, p, s, st);
+    if (sizeof(T) == 2 && residual_dtype == FDA_DTYPE_F32) return run_norm<T, float, true>(backward, p, s, st);
+    return run_norm<T, T, true>(backward, p, s, st);
 }
 
 }  // namespace fda_norm
