@@ -74,8 +74,9 @@ struct Columns {
     __device__ __forceinline__ Pair ones(int i, int j) const { return valid[i][kRagged ? j : 0]; }  // of elements 2 j and 2 j + 1
 };
 
-// Rows on their way: every lane copies its own vectors into its own places of a ring in shared memory, kStages - 1 rows ahead of the one
-// that it works on, so that nothing has to wait for another lane.
+// Rows on their way: every lane copies vectors into its own places of a ring in shared memory, kStages - 1 rows ahead of the one that it
+// works on.  They are its own vectors, so that nothing has to wait for another lane; where a vector has 32 bytes (an fp32 residual beside 16-bit
+// rows) lanes of a warp share them, so that their copies still cover whole lines (598016 x 256 forward 271 us without, 181 with).
 __device__ __forceinline__ void copy16(unsigned to, const void *from, int bytes) {  // the rest of the 16 becomes 0
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
@@ -84,45 +85,56 @@ template <int kLeft>
 __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
 // at: where the row's first vector of the lane starts in the tensor; left: rows from this one on, of which only the last may end inside a
-// vector at the tensor's end.
-template <typename E, int kWidth, int kVectors, bool kRagged>
+// vector at the tensor's end.  kLanes: neighbouring lanes that share the row.
+template <typename E, int kLanes, int kWidth, int kVectors, bool kRagged>
 __device__ __forceinline__ void copy_row(unsigned slot, unsigned pitch, const void *tensor, const Columns<kWidth, kVectors, kRagged> &c,
                                          long long at, long long left) {
     constexpr int kUnits = kWidth * (int)sizeof(E) / 16, kEach = 16 / (int)sizeof(E);
+    const int lane = threadIdx.x % kLanes;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
-        const E *from = static_cast<const E *>(tensor) + at + (c.first[i] - c.first[0]);
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
-            const int last = kRagged ? max(0, min(kEach, c.count[i] - u * kEach)) * (int)sizeof(E) : 16;
-            const int bytes = !c.any(i) || left <= 0 ? 0 : kRagged && left == 1 ? last : 16;
-            copy16(slot + (i * kUnits + u) * pitch, bytes ? from + u * kEach : tensor, bytes);
+            // elements from the lane's own vector to what it copies
+            const int ahead = kUnits == 1 ? 0 : (u * kLanes + lane) * kEach - lane * kWidth;
+            const int rest = kUnits == 1 ? c.count[i] : c.width - (c.first[i] + ahead);
+            const int last = kRagged ? max(0, min(kEach, rest)) * (int)sizeof(E) : 16;
+            const int bytes = rest <= 0 || left <= 0 ? 0 : kRagged && left == 1 ? last : 16;
+            const E *from = static_cast<const E *>(tensor) + at + (c.first[i] - c.first[0]) + ahead;
+            copy16(slot + (i * kUnits + u) * pitch, bytes ? from : tensor, bytes);
         }
     }
 }
 
 // A lane's vector i from its place, elements of neighbouring rows as 0.
-template <typename E, int kWidth, int kVectors, bool kRagged>
+template <typename E, int kLanes, int kWidth, int kVectors, bool kRagged>
 __device__ __forceinline__ void read_vector(const char *slot, unsigned pitch, const Columns<kWidth, kVectors, kRagged> &c, int i, Pair *v) {
     constexpr int kUnits = kWidth * (int)sizeof(E) / 16;
     Raw<E, kWidth> raw;
+    if constexpr (kUnits == 1) {
+        raw.u[0] = *reinterpret_cast<const uint4 *>(slot + i * pitch);
+        if constexpr (kRagged) {
+            raw.u[0].x &= c.keep[i][0];
+            raw.u[0].y &= c.keep[i][1];
+            raw.u[0].z &= c.keep[i][2];
+            raw.u[0].w &= c.keep[i][3];
+        }
+        raw.get(v);
+    } else {
+        const int lane = threadIdx.x % kLanes;
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) raw.u[u] = *reinterpret_cast<const uint4 *>(slot + (i * kUnits + u) * pitch);
-    if constexpr (kRagged && kUnits == 1) {
-        raw.u[0].x &= c.keep[i][0];
-        raw.u[0].y &= c.keep[i][1];
-        raw.u[0].z &= c.keep[i][2];
-        raw.u[0].w &= c.keep[i][3];
-    }
-    if constexpr (kRagged && kUnits > 1) {
+        for (int u = 0; u < kUnits; ++u) {
+            const int chunk = lane * kUnits + u;
+            raw.u[u] = *reinterpret_cast<const uint4 *>(slot + (i * kUnits + chunk / kLanes) * pitch + (chunk % kLanes - lane) * 16);
+        }
         float f[kWidth];
         raw.get(f);
+        if (kRagged) {
 #pragma unroll
-        for (int j = 0; j < kWidth; ++j) f[j] = c.has(i, j) ? f[j] : 0.f;
+            for (int j = 0; j < kWidth; ++j) f[j] = c.has(i, j) ? f[j] : 0.f;
+        }
 #pragma unroll
         for (int j = 0; j < kWidth / 2; ++j) v[j] = Pair(f[2 * j], f[2 * j + 1]);
-    } else {
-        raw.get(v);
     }
 }
 
@@ -203,15 +215,9 @@ __device__ __forceinline__ Team<kLanes> make_team() {
 // 138, 72 KB 185).
 template <typename T, typename R, bool kResidual, int kVectors, bool kBackward>
 constexpr int kUnitsOf = kVectors * ((kBackward ? 2 : 1) + (kResidual ? (int)(sizeof(R) / sizeof(T)) : 0));
-#ifndef KB2
-#define KB2 4
-#define KB3 4
-#define BT2 3
-#define BT3 2
-#endif
 template <int kUnits, int kLanes, bool kBackward>
-constexpr int kStagesOf = kLanes == 0  ? (kUnits == 1 ? 4 : kUnits == 2 ? BT2 : BT3)
-                          : kBackward ? (kUnits == 2 ? KB2 : kUnits == 3 ? KB3 : 2)
+constexpr int kStagesOf = kLanes == 0  ? (kUnits == 1 ? 4 : kUnits == 2 && !kBackward ? 3 : 2)
+                          : kBackward ? (kUnits == 2 ? 4 : kUnits == 3 ? 3 : 2)
                                       : (kUnits <= 2 ? 4 : kUnits == 3 ? 3 : 2);
 template <int kUnits>
 constexpr int kForwardBlocks = kUnits == 1 ? 4 : kUnits == 4 ? 3 : 2;
@@ -220,6 +226,7 @@ constexpr int kForwardBlocks = kUnits == 1 ? 4 : kUnits == 4 ? 3 : 2;
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes, bool kRagged>
 __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_forward_kernel(const NormArgs p) {
     constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, false>, kStages = kStagesOf<kUnits, kLanes, false>;
+    constexpr int kLine = kLanes ? kLanes : 32;  // of a warp, that share a row
     extern __shared__ uint4 ring[];
     wait_for_previous_kernel();
     Team<kLanes> team = make_team<kLanes>();
@@ -232,8 +239,8 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
     long long at = row * p.width + c.first[0], left = p.rows - row;  // of the next row to be copied, then of the one that is worked on
     const long long stride = step * p.width;
     const auto issue = [&](int s) {
-        copy_row<T>(slots + s * stage, pitch, p.x, c, at, left);
-        if (kResidual) copy_row<R>(slots + s * stage + kVectors * pitch, pitch, p.residual, c, at, left);
+        copy_row<T, kLine>(slots + s * stage, pitch, p.x, c, at, left);
+        if (kResidual) copy_row<R, kLine>(slots + s * stage + kVectors * pitch, pitch, p.residual, c, at, left);
         copies_issued();
         at += stride;
         left -= step;
@@ -251,13 +258,14 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
         Pair d[kVectors][H], add(0.f);
         float sums[1];
         wait_copies<kStages - 2>();
+        if (kResidual && sizeof(R) > sizeof(T)) __syncwarp();  // other lanes' copies are there too, and the places of the row before are free
         const char *const slot = mine + s * stage;
 #pragma unroll
         for (int i = 0; i < kVectors; ++i) {
-            read_vector<T>(slot, pitch, c, i, d[i]);
+            read_vector<T, kLine>(slot, pitch, c, i, d[i]);
             if (kResidual) {
                 Pair extra[H];
-                read_vector<R>(slot + kVectors * pitch, pitch, c, i, extra);
+                read_vector<R, kLine>(slot + kVectors * pitch, pitch, c, i, extra);
 #pragma unroll
                 for (int j = 0; j < H; ++j) d[i][j] = d[i][j] + extra[j];
             }
@@ -301,6 +309,7 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes, bool kRagged>
 __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_backward_kernel(const NormArgs p) {
     constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, true>, kStages = kStagesOf<kUnits, kLanes, true>;
+    constexpr int kLine = kLanes ? kLanes : 32;  // of a warp, that share a row
     extern __shared__ uint4 ring[];
     wait_for_previous_kernel();
     Team<kLanes> team = make_team<kLanes>();
@@ -313,9 +322,9 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
     long long at = row * p.width + c.first[0], left = p.rows - row;
     const long long stride = step * p.width;
     const auto issue = [&](int s) {
-        copy_row<T>(slots + s * stage, pitch, p.x, c, at, left);
-        copy_row<T>(slots + s * stage + kVectors * pitch, pitch, p.grad_y, c, at, left);
-        if (kResidual) copy_row<R>(slots + s * stage + 2 * kVectors * pitch, pitch, p.residual, c, at, left);
+        copy_row<T, kLine>(slots + s * stage, pitch, p.x, c, at, left);
+        copy_row<T, kLine>(slots + s * stage + kVectors * pitch, pitch, p.grad_y, c, at, left);
+        if (kResidual) copy_row<R, kLine>(slots + s * stage + 2 * kVectors * pitch, pitch, p.residual, c, at, left);
         copies_issued();
         at += stride;
         left -= step;
@@ -334,14 +343,15 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
     for (long long base = row - (kLanes ? threadIdx.x % 32 / (kLanes ? kLanes : 1) : 0); base < p.rows; base += step, row += step) {
         Pair d[kVectors][H], dy[kVectors][H], add(0.f);
         wait_copies<kStages - 2>();
+        if (kResidual && sizeof(R) > sizeof(T)) __syncwarp();  // other lanes' copies are there too, and the places of the row before are free
         const char *const slot = mine + s * stage;
 #pragma unroll
         for (int i = 0; i < kVectors; ++i) {
-            read_vector<T>(slot, pitch, c, i, d[i]);
-            read_vector<T>(slot + kVectors * pitch, pitch, c, i, dy[i]);
+            read_vector<T, kLine>(slot, pitch, c, i, d[i]);
+            read_vector<T, kLine>(slot + kVectors * pitch, pitch, c, i, dy[i]);
             if (kResidual) {
                 Pair extra[H];
-                read_vector<R>(slot + 2 * kVectors * pitch, pitch, c, i, extra);
+                read_vector<R, kLine>(slot + 2 * kVectors * pitch, pitch, c, i, extra);
 #pragma unroll
                 for (int j = 0; j < H; ++j) d[i][j] = d[i][j] + extra[j];
             }
