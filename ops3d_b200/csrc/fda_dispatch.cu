@@ -25,6 +25,7 @@ using namespace fda_rows;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMostExperts = 1024, kMostChoices = 32;
+constexpr int kMostChunks = 2 * kSms;  // blocks along the entries where they are many
 
 // ---- rows --------------------------------------------------------------------------------------------------------------------
 struct MoveArgs {
@@ -359,30 +360,35 @@ __global__ void __launch_bounds__(kThreads) sort_count_kernel(const SortArgs p) 
     for (int e = threadIdx.x; e < p.n_experts; e += kThreads) p.counts[(size_t)blockIdx.x * p.n_experts + e] = count[e];
 }
 
-// Over the blocks, 32 experts at a time: 32 runs of blocks side by side.
+// Over the blocks, 32 experts at a time: 32 runs of blocks side by side, a run's counts in registers.
 __global__ void __launch_bounds__(1024) sort_scan_kernel(const SortArgs p) {
     __shared__ int sums[32][33];
     wait_for_previous_kernel();
+    constexpr int kRun = (kMostChunks + 31) / 32;
     const int lane = threadIdx.x % 32, run = threadIdx.x / 32, e = blockIdx.x * 32 + lane;
-    const int length = (p.chunks + 31) / 32, first = min(run * length, p.chunks), last = min(first + length, p.chunks);
-    int s = 0;
-    if (e < p.n_experts)
-        for (int c = first; c < last; ++c) s += p.counts[(size_t)c * p.n_experts + e];
+    int n[kRun], s = 0;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const int c = run * kRun + i;
+        n[i] = e < p.n_experts && c < p.chunks ? p.counts[(size_t)c * p.n_experts + e] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) s += n[i];
     sums[run][lane] = s;
     __syncthreads();
-    int before = 0, all = 0;
-    for (int k = 0; k < 32; ++k) {
-        if (k == run) before = all;
-        all += sums[k][lane];
+    // a warp adds up an expert's runs, then each run has those before it
+    const int own = sums[lane][run], upto = fda_linear::warp_scan_sum(own);
+    if (lane == 31 && blockIdx.x * 32 + run < p.n_experts) p.total[blockIdx.x * 32 + run] = upto;
+    __syncthreads();
+    sums[lane][run] = upto - own;
+    __syncthreads();
+    int before = sums[run][lane];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const int c = run * kRun + i;
+        if (e < p.n_experts && c < p.chunks) p.counts[(size_t)c * p.n_experts + e] = before;
+        before += n[i];
     }
-    if (e >= p.n_experts) return;
-    for (int c = first; c < last; ++c) {
-        const size_t at = (size_t)c * p.n_experts + e;
-        const int n = p.counts[at];
-        p.counts[at] = before;
-        before += n;
-    }
-    if (run == 0) p.total[e] = all;
 }
 
 // How a block of the moving kernel learns how many entries of each expert there are, and how many before its own.
@@ -626,21 +632,25 @@ int run_combine(const MoveArgs &p, int dtype, bool backward, cudaStream_t st) {
     return run_combine<__nv_bfloat16>(p, backward, st);
 }
 
-constexpr long long kFewEntries = 4096;  // that every block counts by itself
+// Entries that every block counts by itself.  9003 by 131 experts take 10.7 us so and 13.9 by the launches before (16 experts: 10.4 and 11.5);
+// 16000 by 64 take longer.
+constexpr long long kFewEntries = 10240;
 
 // Entries of a block, and blocks along them.
 void set_chunks(SortArgs &s, int top_k, int passes, unsigned &slices) {
     const long long tokens = s.entries / top_k;
     const bool few = s.entries <= kFewEntries;
-    // few: a token to a warp and pass, and slices of columns until every SM has a block; many: two blocks to an SM
-    long long per = few ? std::max<long long>(1, kMoveWarps / passes) : ceil_div(tokens, 2 * kSms);
+    // few: a token to a warp and pass, and slices of columns until every SM has a block; never more than two blocks to an SM along the tokens
+    const long long per = std::max<long long>(ceil_div(tokens, kMostChunks), few ? std::max(1, kMoveWarps / passes) : 1);
     s.chunk = (int)(per * top_k);
     s.chunks = (int)ceil_div(tokens, per);
     slices = few ? (unsigned)std::min<long long>(passes, std::max<long long>(1, kSms / s.chunks)) : 1;
 }
 Counted counted(const SortArgs &s) {
     if (s.entries <= kFewEntries) return kByItself;
-    return s.n_experts <= 64 ? kPerBlock : kScanned;
+    // blocks add up a few experts' counts while a third launch would start: 147456 entries by 16 experts 25.6 us so and 27.4 with a scan, 80000
+    // by 64 experts 19.5 and 18.7
+    return s.n_experts <= 32 ? kPerBlock : kScanned;
 }
 
 template <typename T, int kLanes, bool kRagged>
@@ -696,7 +706,7 @@ int check_rows(long long tokens, int top_k, int width, int dtype) {
 }
 
 // Counts of the blocks; there are at most two to an SM.
-size_t counts_bytes(int n_experts) { return fda_linear::round256((size_t)2 * kSms * n_experts * sizeof(int)); }
+size_t counts_bytes(int n_experts) { return fda_linear::round256((size_t)kMostChunks * n_experts * sizeof(int)); }
 
 }  // namespace
 

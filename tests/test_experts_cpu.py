@@ -73,9 +73,9 @@ def test_row_arguments():
     assert _dispatch(lib, k=33) == 11 and _dispatch(lib, experts=1025) == 11
     assert all(_dispatch(lib, **{n: None}) == 1 for n in ("x", "e", "rows", "starts", "pos"))
     assert lib.fda_dispatch_workspace_bytes(4, 2, 8) == 0         # few entries are counted where they are placed
-    need = lib.fda_dispatch_workspace_bytes(4000, 2, 8)
-    assert need > 0 and _dispatch(lib, tokens=4000, ws=None) == 8 and _dispatch(lib, tokens=4000, ws_bytes=need - 1) == 8
-    assert _dispatch(lib, tokens=4000, ws=ODD) == 9
+    need = lib.fda_dispatch_workspace_bytes(40000, 2, 8)
+    assert need > 0 and _dispatch(lib, tokens=400000, ws=None) == 8 and _dispatch(lib, tokens=40000, ws_bytes=need - 1) == 8
+    assert _dispatch(lib, tokens=400000, ws=ODD) == 9
     assert lib.fda_dispatch_workspace_bytes(1 << 29, 2, 1024) < 4 << 20
     assert _dispatch(lib, x=ODD) == 9 and _dispatch(lib, rows=ODD) == 9
     assert lib.fda_dispatch_workspace_bytes(0, 2, 8) == 0 and lib.fda_dispatch_workspace_bytes(4, 2, 1025) == 0

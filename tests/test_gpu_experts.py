@@ -225,6 +225,23 @@ def test_masked_experts():
             assert not grad.any()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("experts", [24, 64, 128, 256, 512, 1000])
+def test_rows_of_one_value(dtype, experts):
+    """Every logit the same, the types' extremes among them: the first experts, equal weights, and no gradient through a softmax of all."""
+    fi = torch.finfo(dtype)
+    for value in (0.0, -3.0, fi.min, fi.max, fi.tiny):
+        logits = torch.full((5, experts), value, dtype=dtype, device=DEV)
+        for bias in (None, torch.full((experts,), 0.25, device=DEV)):
+            for renormalise in (True, False):
+                weights, chosen_ = route_experts(logits, 4, bias=bias, renormalise=renormalise)
+                assert torch.equal(chosen_, torch.arange(4, device=DEV).expand(5, 4))
+                assert (weights - 1 / (4 if renormalise else experts)).abs().max() <= 60 * U / (4 if renormalise else experts)
+            weights, chosen_ = route_experts(logits, 4, bias=bias, score="sigmoid", renormalise=False)
+            want = torch.sigmoid(torch.tensor(value, dtype=torch.float64)).item()
+            assert torch.equal(chosen_, torch.arange(4, device=DEV).expand(5, 4)) and (weights - want).abs().max() <= 8 * U * want + 2.0 ** -148
+
+
 def test_choices_of_less_than_all_that_is_left():
     """Two experts are left of which four are wanted: the others follow by index, with weights of 0."""
     logits = torch.full((2, 10), -INF, device=DEV)
@@ -378,6 +395,8 @@ def test_the_same_expert_twice():
 def test_many_rows():
     check_rows(experts_of(70001, 4, 64, 0.02), 64, 64, BF16)
     check_rows(experts_of(30001, 2, 16, 0.02), 16, 259, F16)
+    for n_experts in (7, 500):      # blocks that place their entries in several parts
+        check_rows(experts_of(90001, 8, n_experts, 0.02), n_experts, 8, BF16, residual=False)
 
 
 def test_row_strides():
