@@ -13,17 +13,22 @@ __global__ void __launch_bounds__(1024) norm_sum_kernel(const float *partial, in
     __shared__ float sums[32][32];
     const int lane = threadIdx.x % 32, part = threadIdx.x / 32, parts = blockDim.x / 32;
     const long long column = (long long)blockIdx.x * 32 + lane;
-    float s = 0.f;
+    // short chains of additions: eight sums side by side, then pairs of them
+    float s[8] = {};
     if (column < 2ll * width) {
-#pragma unroll 8
-        for (int i = part; i < count; i += parts) s += partial[(size_t)i * 2 * width + column];
+        for (int i = part; i < count; i += 8 * parts)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i + k * parts < count) s[k] += partial[(size_t)(i + k * parts) * 2 * width + column];
     }
-    sums[part][lane] = s;
-    __syncthreads();
+    sums[part][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+    for (int half = 16; half > 0; half /= 2) {
+        __syncthreads();
+        if (part < half && part + half < parts) sums[part][lane] += sums[part + half][lane];
+    }
     if (part != 0 || column >= 2ll * width) return;
-    for (int k = 1; k < parts; ++k) s += sums[k][lane];
     void *out = column < width ? grad_weight : grad_bias;
-    if (out) store_from_f32(out, dtype, column < width ? column : column - width, s);
+    if (out) store_from_f32(out, dtype, column < width ? column : column - width, sums[0][lane]);
 }
 
 // ---- rows that no block keeps in registers: a pass over the row for each step -----------------------------------------------
