@@ -435,6 +435,31 @@ def test_rows_of_nan_stay_where_they_are():
     assert torch.isfinite(gr).all() and torch.isfinite(gw).all() and not gr[98:].any() and not gw[7].any()
 
 
+def test_row_gradients_against_differences():
+    """Of dispatch and combine together, along a direction of everything that has a gradient; the sums are of products of two, so central
+    differences in 64 bits have no error but rounding."""
+    experts = experts_of(40, 3, 5, 0.2)
+    leaves = [rows_of((40, 24), F32).requires_grad_(True), rows_of((40, 3), F32, 1).requires_grad_(True), rows_of((40, 24), F32, 2).requires_grad_(True)]
+    factor, dy = rows_of((120, 24), F32, 3), rows_of((40, 24), F32, 4)
+    rows, order = dispatch_rows(leaves[0], experts, 5)
+    grads = torch.autograd.grad(combine_rows(rows * factor, order, leaves[1], residual=leaves[2]), leaves, dy)
+    position = order_of(experts, 5)[1]
+    there, at = (position >= 0)[..., None], position.clamp_min(0)
+
+    def value(x, w, r):
+        return (((x[:, None] * factor.double()[at]) * there * w[..., None]).sum(1) + r).mul(dy.double()).sum()
+
+    moves = [torch.randn(t.shape, dtype=torch.float64, device=DEV, generator=torch.Generator(device=DEV).manual_seed(i)) for i, t in enumerate(leaves)]
+    up, down = (value(*(t.detach().double() + h * v for t, v in zip(leaves, moves))).item() for h in (0.5, -0.5))
+    got = sum((g.double() * v).sum().item() for g, v in zip(grads, moves))
+    # each gradient is a sum of at most 24 products of three factors, rounded at each
+    size = sum((g.double().abs() * v.abs()).sum().item() for g, v in zip(grads, moves))
+    terms = ((leaves[0].abs().double()[:, None] * factor.abs().double()[at]) * there * dy.abs().double()[:, None]).sum(-1)
+    slack = 32 * U * (size + (terms * moves[1].abs()).sum().item())
+    slack += 32 * U * ((factor.abs().double()[at] * there * leaves[1].detach().abs().double()[..., None]).sum(1) * dy.abs().double() * moves[0].abs()).sum().item()
+    assert abs(got - (up - down)) <= slack + 1e-12 * size
+
+
 def test_positions_that_lead_nowhere():
     """An order put together by hand with indices outside the rows: they count as none."""
     rows = rows_of((12, 16), F32).requires_grad_(True)
@@ -529,6 +554,17 @@ def test_block_of_experts(options):
     ref = torch.autograd.grad(want, [x64, *m.parameters()], dy.double())
     for name, a, b in zip(names, got, ref):
         assert (a - b).abs().max() <= 12 * 2.0 ** -16 * b.abs().max(), name
+
+
+def test_block_without_tokens():
+    m = ExpertFeedForward(32, 64, 8, 2).to(DEV)
+    x = torch.zeros(2, 0, 32, device=DEV, requires_grad=True)
+    y, order = m(x, return_order=True)
+    assert y.shape == x.shape and not order.group_start_index.any()
+    y.sum().backward()
+    assert all(not p.grad.any() for p in m.parameters())
+    y, order = m(torch.randn(5, 32, device=DEV), torch.ones(5, dtype=torch.bool, device=DEV), return_order=True)    # padding only
+    assert not order.group_start_index.any() and (order.position == -1).all()
 
 
 @pytest.mark.parametrize("tokens", [1, 3, 300])
