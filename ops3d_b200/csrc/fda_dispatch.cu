@@ -181,8 +181,9 @@ __device__ __forceinline__ bool takes(int lane) {
 
 // kLanes lanes take a token's vectors of one pass.  Positions and weights of the next choices are on their way while rows are added up.  Bound
 // by DRAM (149504 x 4 x 256 bf16 77 us, 6.0 TB/s); read as data that is not used again rows come faster (73728 x 2 x 256: 27 -> 22 us).
+constexpr int kCombineBlocks = 4;  // to an SM, all there at once
 template <typename T, int kLanes, bool kRagged, int kAtOnce>
-__global__ void __launch_bounds__(kThreads) combine_kernel(const MoveArgs p) {
+__global__ void __launch_bounds__(kThreads, kCombineBlocks) combine_kernel(const MoveArgs p) {
     constexpr int W = kWidthOf<T>, H = W / 2, kTeams = kThreads / kLanes;
     wait_for_previous_kernel();
     const int lane = threadIdx.x % kLanes;
@@ -239,9 +240,13 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const MoveArgs p) {
     }
 }
 
-// kLanes lanes, or (0) a block, take a token.
+// kLanes lanes, or (0) a block, take a token.  Bound by DRAM: 149504 x 4 x 256 bf16 124 us, 5.6 TB/s.
+// Blocks that registers leave room for on an SM: where rows are aligned as many as are launched (149504 x 4: 132 us with more blocks than fit,
+// 124 so), shifted rows need twice the registers.
+template <bool kRagged, int kAtOnce>
+constexpr int kCombineBackwardBlocks = kAtOnce == 2 ? (kRagged ? 3 : 4) : kRagged ? 2 : 3;
 template <typename T, int kLanes, bool kRagged, int kAtOnce>
-__global__ void __launch_bounds__(kThreads) combine_backward_kernel(const MoveArgs p) {
+__global__ void __launch_bounds__(kThreads, kCombineBackwardBlocks<kRagged, kAtOnce>) combine_backward_kernel(const MoveArgs p) {
     constexpr int W = kWidthOf<T>, H = W / 2, kLine = kLanes ? kLanes : 32, kTeams = kLanes ? kThreads / kLine : 1;
     __shared__ float dots[kWarps][kAtOnce];
     wait_for_previous_kernel();
@@ -593,11 +598,12 @@ void set_passes(MoveArgs &p, int &lanes, bool &ragged) {
 
 template <typename T, int kLanes, bool kRagged, int kAtOnce>
 int run_combine(const MoveArgs &p, bool backward, cudaStream_t st) {
-    long long units = p.tokens * p.passes;
+    long long units = p.tokens * p.passes, most = kCombineBlocks * kSms;
     auto kernel = combine_kernel<T, kLanes, kRagged, kAtOnce>;
     MoveArgs q = p;
     if (backward) {
         units = p.tokens;
+        most = (kRagged ? 8 : kCombineBackwardBlocks<kRagged, kAtOnce>) * kSms;
         kernel = combine_backward_kernel<T, kLanes, kRagged, kAtOnce>;
         // wide rows of few tokens: a block to a token
         if (p.passes > 1 && p.tokens < 8 * kSms * kWarps) {
@@ -606,7 +612,7 @@ int run_combine(const MoveArgs &p, bool backward, cudaStream_t st) {
             kernel = combine_backward_kernel<T, 0, kRagged, kAtOnce>;
         }
     }
-    const unsigned blocks = (unsigned)std::min<long long>(ceil_div(units, kThreads / kLanes), 8 * kSms);
+    const unsigned blocks = (unsigned)std::min<long long>(ceil_div(units, kThreads / kLanes), most);
     return launched(launch_early(kernel, blocks, kThreads, 0, st, 1, q));
 }
 

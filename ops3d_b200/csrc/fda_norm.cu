@@ -49,7 +49,7 @@ constexpr int kWideThreads = 512;
 template <bool kBackward>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_kernel(const WideArgs p) {
     wait_for_previous_kernel();
-    Team<0> team = make_team<0>();
+    Team<0> team = block_team();
     const int width = p.n.width;
     const float inverse = 1.f / (float)width;
     for (long long row = blockIdx.x; row < p.n.rows; row += gridDim.x) {

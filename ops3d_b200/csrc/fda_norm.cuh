@@ -153,6 +153,23 @@ __device__ __forceinline__ void store_vector(void *tensor, const Pair *v, const 
         if (c.has(i, j)) to[j] = raw.element(j);
 }
 
+// ds += the gradient that reaches the sum from elsewhere.
+template <typename E, int kWidth, int kVectors, bool kRagged>
+__device__ __forceinline__ void add_sum_gradient(const void *tensor, Pair *ds, const Columns<kWidth, kVectors, kRagged> &c, int i, long long at) {
+    const E *from = static_cast<const E *>(tensor) + at + (c.first[i] - c.first[0]);
+    float v[kWidth];
+    if (c.whole(i)) {
+        Raw<E, kWidth> raw;
+        raw.load(from);
+        raw.get(v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kWidth; ++j) v[j] = c.has(i, j) ? to_f32(from[j]) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < kWidth / 2; ++j) ds[j] = ds[j] + Pair(v[2 * j], v[2 * j + 1]);
+}
+
 // A parameter's numbers for a lane's columns, `otherwise` where there is none.
 template <typename E, int kWidth, int kVectors, bool kRagged>
 __device__ __forceinline__ void load_parameter(const E *tensor, const Columns<kWidth, kVectors, kRagged> &c, float (&v)[kVectors][kWidth]) {
@@ -188,25 +205,21 @@ __device__ __forceinline__ void load_parameter(const void *tensor, int dtype, fl
         for (int j = 0; j < kWidth / 2; ++j) pairs[i][j] = Pair(v[i][2 * j], v[i][2 * j + 1]);
 }
 
-// Which rows a team takes: the first one, and how far apart they are (a multiple of kWidth, because a grid's blocks are where a block
-// is a team, and a block's teams are otherwise).
+// Which rows a team of lanes takes: the first one, and how far apart they are (a multiple of kWidth, because a block's teams are).
 template <int kLanes>
 __device__ __forceinline__ void team_rows(long long &first, long long &step) {
-    constexpr int kTeams = kLanes ? kTeamThreads / (kLanes ? kLanes : 1) : 1;
-    first = (long long)blockIdx.x * kTeams + (kLanes ? threadIdx.x / (kLanes ? kLanes : 1) : 0);
+    constexpr int kTeams = kTeamThreads / kLanes;
+    first = (long long)blockIdx.x * kTeams + threadIdx.x / kLanes;
     step = (long long)gridDim.x * kTeams;
 }
 
-// Shared memory of the sums over a block.
-template <int kLanes>
-__device__ __forceinline__ Team<kLanes> make_team() {
-    Team<kLanes> team;
-    if constexpr (kLanes == 0) {
-        __shared__ alignas(16) float sums[2][Team<0>::kMost][Team<0>::kWarps];
-        for (int i = threadIdx.x; i < 2 * Team<0>::kMost * Team<0>::kWarps; i += blockDim.x) (&sums[0][0][0])[i] = 0.f;
-        __syncthreads();
-        team.shared = sums;
-    }
+// The block as a team, with shared memory for its sums.
+__device__ __forceinline__ Team<0> block_team() {
+    __shared__ alignas(16) float sums[2][Team<0>::kMost][Team<0>::kWarps];
+    for (int i = threadIdx.x; i < 2 * Team<0>::kMost * Team<0>::kWarps; i += blockDim.x) (&sums[0][0][0])[i] = 0.f;
+    __syncthreads();
+    Team<0> team;
+    team.shared = sums;
     return team;
 }
 
@@ -224,12 +237,11 @@ constexpr int kForwardBlocks = kUnits == 1 ? 4 : kUnits == 4 ? 3 : 2;
 
 // R: the residual's type; kResidual false: there is none.
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes, bool kRagged>
-__global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_forward_kernel(const NormArgs p) {
+__global__ void __launch_bounds__(kTeamThreads) norm_forward_kernel(const NormArgs p) {
     constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, false>, kStages = kStagesOf<kUnits, kLanes, false>;
-    constexpr int kLine = kLanes ? kLanes : 32;  // of a warp, that share a row
     extern __shared__ uint4 ring[];
     wait_for_previous_kernel();
-    Team<kLanes> team = make_team<kLanes>();
+    Team<kLanes> team;
     long long row, step;
     team_rows<kLanes>(row, step);
     const Columns<W, kVectors, kRagged> c(p.width, row, team.lane(), team.size());
@@ -239,8 +251,8 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
     long long at = row * p.width + c.first[0], left = p.rows - row;  // of the next row to be copied, then of the one that is worked on
     const long long stride = step * p.width;
     const auto issue = [&](int s) {
-        copy_row<T, kLine>(slots + s * stage, pitch, p.x, c, at, left);
-        if (kResidual) copy_row<R, kLine>(slots + s * stage + kVectors * pitch, pitch, p.residual, c, at, left);
+        copy_row<T, kLanes>(slots + s * stage, pitch, p.x, c, at, left);
+        if (kResidual) copy_row<R, kLanes>(slots + s * stage + kVectors * pitch, pitch, p.residual, c, at, left);
         copies_issued();
         at += stride;
         left -= step;
@@ -254,7 +266,7 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
     const float inverse = 1.f / (float)p.width;
     // every lane of a warp stays to the end: they exchange sums
     int s = 0;
-    for (long long base = row - (kLanes ? threadIdx.x % 32 / (kLanes ? kLanes : 1) : 0); base < p.rows; base += step, row += step) {
+    for (long long base = row - threadIdx.x % 32 / kLanes; base < p.rows; base += step, row += step) {
         Pair d[kVectors][H], add(0.f);
         float sums[1];
         wait_copies<kStages - 2>();
@@ -262,10 +274,10 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
         const char *const slot = mine + s * stage;
 #pragma unroll
         for (int i = 0; i < kVectors; ++i) {
-            read_vector<T, kLine>(slot, pitch, c, i, d[i]);
+            read_vector<T, kLanes>(slot, pitch, c, i, d[i]);
             if (kResidual) {
                 Pair extra[H];
-                read_vector<R, kLine>(slot + kVectors * pitch, pitch, c, i, extra);
+                read_vector<R, kLanes>(slot + kVectors * pitch, pitch, c, i, extra);
 #pragma unroll
                 for (int j = 0; j < H; ++j) d[i][j] = d[i][j] + extra[j];
             }
@@ -307,12 +319,11 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_fo
 }
 
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes, bool kRagged>
-__global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_backward_kernel(const NormArgs p) {
+__global__ void __launch_bounds__(kTeamThreads) norm_backward_kernel(const NormArgs p) {
     constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, true>, kStages = kStagesOf<kUnits, kLanes, true>;
-    constexpr int kLine = kLanes ? kLanes : 32;  // of a warp, that share a row
     extern __shared__ uint4 ring[];
     wait_for_previous_kernel();
-    Team<kLanes> team = make_team<kLanes>();
+    Team<kLanes> team;
     long long row, step;
     team_rows<kLanes>(row, step);
     const Columns<W, kVectors, kRagged> c(p.width, row, team.lane(), team.size());
@@ -322,9 +333,9 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
     long long at = row * p.width + c.first[0], left = p.rows - row;
     const long long stride = step * p.width;
     const auto issue = [&](int s) {
-        copy_row<T, kLine>(slots + s * stage, pitch, p.x, c, at, left);
-        copy_row<T, kLine>(slots + s * stage + kVectors * pitch, pitch, p.grad_y, c, at, left);
-        if (kResidual) copy_row<R, kLine>(slots + s * stage + 2 * kVectors * pitch, pitch, p.residual, c, at, left);
+        copy_row<T, kLanes>(slots + s * stage, pitch, p.x, c, at, left);
+        copy_row<T, kLanes>(slots + s * stage + kVectors * pitch, pitch, p.grad_y, c, at, left);
+        if (kResidual) copy_row<R, kLanes>(slots + s * stage + 2 * kVectors * pitch, pitch, p.residual, c, at, left);
         copies_issued();
         at += stride;
         left -= step;
@@ -340,18 +351,18 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
         for (int j = 0; j < H; ++j) weight_sum[i][j] = bias_sum[i][j] = Pair(0.f);
     const float inverse = 1.f / (float)p.width;
     int s = 0;
-    for (long long base = row - (kLanes ? threadIdx.x % 32 / (kLanes ? kLanes : 1) : 0); base < p.rows; base += step, row += step) {
+    for (long long base = row - threadIdx.x % 32 / kLanes; base < p.rows; base += step, row += step) {
         Pair d[kVectors][H], dy[kVectors][H], add(0.f);
         wait_copies<kStages - 2>();
         if (kResidual && sizeof(R) > sizeof(T)) __syncwarp();  // other lanes' copies are there too, and the places of the row before are free
         const char *const slot = mine + s * stage;
 #pragma unroll
         for (int i = 0; i < kVectors; ++i) {
-            read_vector<T, kLine>(slot, pitch, c, i, d[i]);
-            read_vector<T, kLine>(slot + kVectors * pitch, pitch, c, i, dy[i]);
+            read_vector<T, kLanes>(slot, pitch, c, i, d[i]);
+            read_vector<T, kLanes>(slot + kVectors * pitch, pitch, c, i, dy[i]);
             if (kResidual) {
                 Pair extra[H];
-                read_vector<R, kLine>(slot + 2 * kVectors * pitch, pitch, c, i, extra);
+                read_vector<R, kLanes>(slot + 2 * kVectors * pitch, pitch, c, i, extra);
 #pragma unroll
                 for (int j = 0; j < H; ++j) d[i][j] = d[i][j] + extra[j];
             }
@@ -390,20 +401,7 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
                 weight_sum[i][j] = fma2(dy[i][j], d[i][j] * q, weight_sum[i][j]);
                 bias_sum[i][j] = bias_sum[i][j] + dy[i][j];
             }
-            if (kResidual && p.grad_sum) {
-                const R *from = static_cast<const R *>(p.grad_sum) + here + (c.first[i] - c.first[0]);
-                float extra[W];
-                if (c.whole(i)) {
-                    Raw<R, W> raw;
-                    raw.load(from);
-                    raw.get(extra);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < W; ++j) extra[j] = c.has(i, j) ? to_f32(from[j]) : 0.f;
-                }
-#pragma unroll
-                for (int j = 0; j < H; ++j) ds[j] = ds[j] + Pair(extra[2 * j], extra[2 * j + 1]);
-            }
+            if (kResidual && p.grad_sum) add_sum_gradient<R>(p.grad_sum, ds, c, i, here);
             if (p.grad_x) store_vector<T>(p.grad_x, ds, c, i, here);
             if (kResidual && p.grad_residual) store_vector<R>(p.grad_residual, ds, c, i, here);
         }
@@ -420,49 +418,230 @@ __global__ void __launch_bounds__(kLanes ? kTeamThreads : kBlockThreads) norm_ba
             bias_sum[i][j].get(grad_bias[i][2 * j], grad_bias[i][2 * j + 1]);
         }
     float *out = p.partial + (size_t)blockIdx.x * 2 * p.width;
-    if constexpr (kLanes == 0) {
+    // teams of a warp have the same columns unless rows are ragged
+    constexpr int kTeams = kRagged ? kTeamThreads / kLanes : kTeamThreads / 32;
+    if (!kRagged) {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                for (int o = kLanes; o < 32; o *= 2) {
+                    grad_weight[i][j] += __shfl_xor_sync(0xffffffffu, grad_weight[i][j], o);
+                    grad_bias[i][j] += __shfl_xor_sync(0xffffffffu, grad_bias[i][j], o);
+                }
+    }
+    __syncthreads();
+    float *columns = reinterpret_cast<float *>(ring);  // [kTeams][2][width]
+    const int t = kRagged ? (int)threadIdx.x / kLanes : (int)threadIdx.x / 32;
+    if (kRagged || threadIdx.x % 32 < kLanes) {
 #pragma unroll
         for (int i = 0; i < kVectors; ++i)
 #pragma unroll
             for (int j = 0; j < W; ++j)
                 if (c.has(i, j)) {
-                    out[c.first[i] + j] = grad_weight[i][j];
-                    out[p.width + c.first[i] + j] = grad_bias[i][j];
+                    columns[t * 2 * p.width + c.first[i] + j] = grad_weight[i][j];
+                    columns[(t * 2 + 1) * p.width + c.first[i] + j] = grad_bias[i][j];
                 }
-    } else {
-        // teams of a warp have the same columns unless rows are ragged
-        constexpr int kTeams = kRagged ? kTeamThreads / (kLanes ? kLanes : 1) : kTeamThreads / 32;
-        if (!kRagged) {
-#pragma unroll
-            for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-                for (int j = 0; j < W; ++j)
-                    for (int o = kLanes; o < 32; o *= 2) {
-                        grad_weight[i][j] += __shfl_xor_sync(0xffffffffu, grad_weight[i][j], o);
-                        grad_bias[i][j] += __shfl_xor_sync(0xffffffffu, grad_bias[i][j], o);
-                    }
-        }
-        __syncthreads();
-        float *columns = reinterpret_cast<float *>(ring);  // [kTeams][2][width]
-        const int t = kRagged ? (int)threadIdx.x / (kLanes ? kLanes : 1) : (int)threadIdx.x / 32;
-        if (kRagged || threadIdx.x % 32 < kLanes) {
-#pragma unroll
-            for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-                for (int j = 0; j < W; ++j)
-                    if (c.has(i, j)) {
-                        columns[t * 2 * p.width + c.first[i] + j] = grad_weight[i][j];
-                        columns[(t * 2 + 1) * p.width + c.first[i] + j] = grad_bias[i][j];
-                    }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 2 * p.width; i += kTeamThreads) {
-            float sum = 0.f;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * p.width; i += kTeamThreads) {
+        float sum = 0.f;
 #pragma unroll 8
-            for (int k = 0; k < kTeams; ++k) sum += columns[k * 2 * p.width + i];
-            out[i] = sum;
+        for (int k = 0; k < kTeams; ++k) sum += columns[k * 2 * p.width + i];
+        out[i] = sum;
+    }
+}
+
+// ---- a block to a row ----------------------------------------------------------------------------------------------------------
+// As above, for rows that a warp has no registers for.  A row's mean is taken together with the sums of the row before it, so that the block
+// meets once for a row: a row's time is that of the barrier and the exchange around it (100000 x 640 bf16 forward: two meetings 76 us, one 58).
+template <typename T, typename R, bool kResidual, int kVectors, bool kRagged>
+__global__ void __launch_bounds__(kBlockThreads) norm_forward_block_kernel(const NormArgs p) {
+    constexpr int W = kWidthOf<T>, H = W / 2, kUnits = kUnitsOf<T, R, kResidual, kVectors, false>, kStages = kStagesOf<kUnits, 0, false>;
+    extern __shared__ uint4 ring[];
+    wait_for_previous_kernel();
+    Team<0> team = block_team();
+    const Columns<W, kVectors, kRagged> c(p.width, blockIdx.x, team.lane(), team.size());
+    const unsigned pitch = blockDim.x * 16, stage = pitch * kUnits;
+    const char *const mine = reinterpret_cast<const char *>(ring + threadIdx.x);
+    const unsigned slots = (unsigned)__cvta_generic_to_shared(mine);
+    long long at = (long long)blockIdx.x * p.width + c.first[0], left = p.rows - blockIdx.x;  // of the next row to be copied
+    const long long stride = (long long)gridDim.x * p.width;
+    const auto issue = [&](int s) {
+        copy_row<T, 32>(slots + s * stage, pitch, p.x, c, at, left);
+        if (kResidual) copy_row<R, 32>(slots + s * stage + kVectors * pitch, pitch, p.residual, c, at, left);
+        copies_issued();
+        at += stride;
+        left -= gridDim.x;
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) issue(s);
+    Pair weight[kVectors][H], bias[kVectors][H];
+    load_parameter<T>(p.weight, p.param_dtype, 1.f, c, weight);
+    load_parameter<T>(p.bias, p.param_dtype, 0.f, c, bias);
+    const float inverse = 1.f / (float)p.width;
+    int s = 0;
+    // the row of place s, whose sum is returned; the place of the row before it is filled again
+    const auto read_row = [&](Pair (&d)[kVectors][H], bool there) {
+        wait_copies<kStages - 2>();
+        if (kResidual && sizeof(R) > sizeof(T)) __syncwarp();
+        const char *const slot = mine + s * stage;
+        Pair add(0.f);
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            read_vector<T, 32>(slot, pitch, c, i, d[i]);
+            if (kResidual) {
+                Pair extra[H];
+                read_vector<R, 32>(slot + kVectors * pitch, pitch, c, i, extra);
+#pragma unroll
+                for (int j = 0; j < H; ++j) d[i][j] = d[i][j] + extra[j];
+            }
+#pragma unroll
+            for (int j = 0; j < H; ++j) add = add + d[i][j];
+        }
+        issue(s == 0 ? kStages - 1 : s - 1);
+        s = s == kStages - 1 ? 0 : s + 1;
+        if (kResidual && p.sum && there) {
+#pragma unroll
+            for (int i = 0; i < kVectors; ++i)
+                if (c.any(i)) store_vector<R>(p.sum, d[i], c, i, at - kStages * stride);
+        }
+        return add.sum();
+    };
+    Pair d[kVectors][H], ahead[kVectors][H];
+    float sums[2] = {0.f, read_row(d, blockIdx.x < p.rows)};
+    team.sum(sums);
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const Pair minus_mean(-sums[1] * inverse);
+        Pair square(0.f);
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+                d[i][j] = fma2(minus_mean, c.ones(i, j), d[i][j]);
+                square = fma2(d[i][j], d[i][j], square);
+            }
+        sums[1] = read_row(ahead, row + gridDim.x < p.rows);
+        sums[0] = square.sum();
+        team.sum(sums);
+        const Pair q(__frsqrt_rn(sums[0] * inverse + p.eps));
+        const long long here = at - (kStages + 1) * stride;
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            if (c.any(i)) {
+#pragma unroll
+                for (int j = 0; j < H; ++j) d[i][j] = fma2(d[i][j] * q, weight[i][j], bias[i][j]);
+                store_vector<T>(p.y, d[i], c, i, here);
+            }
+#pragma unroll
+            for (int j = 0; j < H; ++j) d[i][j] = ahead[i][j];
         }
     }
+    wait_copies<0>();
+}
+
+// The backward has no registers for a second row: its block meets twice (73728 x 1024 f16 108 us, with the next row's mean ahead 120).
+template <typename T, typename R, bool kResidual, int kVectors, bool kRagged>
+__global__ void __launch_bounds__(kBlockThreads) norm_backward_block_kernel(const NormArgs p) {
+    constexpr int W = kWidthOf<T>, H = W / 2, kUnits = kUnitsOf<T, R, kResidual, kVectors, true>, kStages = kStagesOf<kUnits, 0, true>;
+    extern __shared__ uint4 ring[];
+    wait_for_previous_kernel();
+    Team<0> team = block_team();
+    const Columns<W, kVectors, kRagged> c(p.width, blockIdx.x, team.lane(), team.size());
+    const unsigned pitch = blockDim.x * 16, stage = pitch * kUnits;
+    const char *const mine = reinterpret_cast<const char *>(ring + threadIdx.x);
+    const unsigned slots = (unsigned)__cvta_generic_to_shared(mine);
+    long long at = (long long)blockIdx.x * p.width + c.first[0], left = p.rows - blockIdx.x;
+    const long long stride = (long long)gridDim.x * p.width;
+    const auto issue = [&](int s) {
+        copy_row<T, 32>(slots + s * stage, pitch, p.x, c, at, left);
+        copy_row<T, 32>(slots + s * stage + kVectors * pitch, pitch, p.grad_y, c, at, left);
+        if (kResidual) copy_row<R, 32>(slots + s * stage + 2 * kVectors * pitch, pitch, p.residual, c, at, left);
+        copies_issued();
+        at += stride;
+        left -= gridDim.x;
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) issue(s);
+    Pair weight[kVectors][H], weight_sum[kVectors][H], bias_sum[kVectors][H];
+    load_parameter<T>(p.weight, p.param_dtype, 1.f, c, weight);
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+        for (int j = 0; j < H; ++j) weight_sum[i][j] = bias_sum[i][j] = Pair(0.f);
+    const float inverse = 1.f / (float)p.width;
+    int s = 0;
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        wait_copies<kStages - 2>();
+        if (kResidual && sizeof(R) > sizeof(T)) __syncwarp();
+        const char *const slot = mine + s * stage;
+        Pair d[kVectors][H], dy[kVectors][H], add(0.f);
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            read_vector<T, 32>(slot, pitch, c, i, d[i]);
+            read_vector<T, 32>(slot + kVectors * pitch, pitch, c, i, dy[i]);
+            if (kResidual) {
+                Pair extra[H];
+                read_vector<R, 32>(slot + 2 * kVectors * pitch, pitch, c, i, extra);
+#pragma unroll
+                for (int j = 0; j < H; ++j) d[i][j] = d[i][j] + extra[j];
+            }
+#pragma unroll
+            for (int j = 0; j < H; ++j) add = add + d[i][j];
+        }
+        issue(s == 0 ? kStages - 1 : s - 1);
+        const long long here = at - kStages * stride;
+        s = s == kStages - 1 ? 0 : s + 1;
+        float mean[1] = {add.sum()};
+        team.sum(mean);
+        const Pair minus_mean(-mean[0] * inverse);
+        Pair dd(0.f), gd(0.f), gg(0.f);
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+                d[i][j] = fma2(minus_mean, c.ones(i, j), d[i][j]);
+                const Pair g = dy[i][j] * weight[i][j];
+                dd = fma2(d[i][j], d[i][j], dd);
+                gd = fma2(g, d[i][j], gd);
+                gg = gg + g;
+            }
+        float sums[3] = {dd.sum(), gd.sum(), gg.sum()};
+        team.sum(sums);
+        const float scale = __frsqrt_rn(sums[0] * inverse + p.eps);
+        const Pair q(scale), level(-scale * (sums[2] * inverse)), along(-scale * (scale * scale * (sums[1] * inverse)));
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            Pair ds[H];
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+                ds[j] = fma2(dy[i][j] * weight[i][j], q, fma2(d[i][j], along, level));
+                weight_sum[i][j] = fma2(dy[i][j], d[i][j] * q, weight_sum[i][j]);
+                bias_sum[i][j] = bias_sum[i][j] + dy[i][j];
+            }
+            if (!c.any(i)) continue;
+            if (kResidual && p.grad_sum) add_sum_gradient<R>(p.grad_sum, ds, c, i, here);
+            if (p.grad_x) store_vector<T>(p.grad_x, ds, c, i, here);
+            if (kResidual && p.grad_residual) store_vector<R>(p.grad_residual, ds, c, i, here);
+        }
+    }
+    wait_copies<0>();
+    if (!p.partial) return;
+    float *out = p.partial + (size_t)blockIdx.x * 2 * p.width;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+            float w[2], b[2];
+            weight_sum[i][j].get(w[0], w[1]);
+            bias_sum[i][j].get(b[0], b[1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (c.has(i, 2 * j + k)) {
+                    out[c.first[i] + 2 * j + k] = w[k];
+                    out[p.width + c.first[i] + 2 * j + k] = b[k];
+                }
+        }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
@@ -517,10 +696,17 @@ int run_norm(bool backward, const NormArgs &p, const NormShape &s, cudaStream_t 
     constexpr int kForward = kUnitsOf<T, R, kResidual, kVectors, false>, kBackward = kUnitsOf<T, R, kResidual, kVectors, true>;
     const int units = backward ? kBackward * kStagesOf<kBackward, kLanes, true> : kForward * kStagesOf<kForward, kLanes, false>;
     const int shared = units * s.threads * 16;
-    const auto kernel = backward ? (s.ragged ? norm_backward_kernel<T, R, kResidual, kVectors, kLanes, true>
-                                             : norm_backward_kernel<T, R, kResidual, kVectors, kLanes, false>)
-                                 : (s.ragged ? norm_forward_kernel<T, R, kResidual, kVectors, kLanes, true>
-                                             : norm_forward_kernel<T, R, kResidual, kVectors, kLanes, false>);
+    void (*kernel)(NormArgs);
+    if constexpr (kLanes == 0)
+        kernel = backward ? (s.ragged ? norm_backward_block_kernel<T, R, kResidual, kVectors, true>
+                                      : norm_backward_block_kernel<T, R, kResidual, kVectors, false>)
+                          : (s.ragged ? norm_forward_block_kernel<T, R, kResidual, kVectors, true>
+                                      : norm_forward_block_kernel<T, R, kResidual, kVectors, false>);
+    else
+        kernel = backward ? (s.ragged ? norm_backward_kernel<T, R, kResidual, kVectors, kLanes, true>
+                                      : norm_backward_kernel<T, R, kResidual, kVectors, kLanes, false>)
+                          : (s.ragged ? norm_forward_kernel<T, R, kResidual, kVectors, kLanes, true>
+                                      : norm_forward_kernel<T, R, kResidual, kVectors, kLanes, false>);
     if (shared > 40 * 1024)  // with the static part beyond what every launch may have; the attribute belongs to the current device
         if (const int rc = launched(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared))) return rc;
     const unsigned blocks = backward ? norm_backward_blocks(s, p.rows, sizeof(T) == 4 ? FDA_DTYPE_F32 : FDA_DTYPE_F16)
