@@ -351,6 +351,7 @@ __device__ __forceinline__ int expert_of(const SortArgs &p, long long i, long lo
     return e >= 0 && e < p.n_experts ? (int)e : -1;
 }
 
+// 7 us for 598016 entries: latency of two rounds of loads and of the launch.
 __global__ void __launch_bounds__(kThreads) sort_count_kernel(const SortArgs p) {
     __shared__ int count[kMostExperts];
     wait_for_previous_kernel();
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(kThreads) sort_count_kernel(const SortArgs p) 
     for (int e = threadIdx.x; e < p.n_experts; e += kThreads) p.counts[(size_t)blockIdx.x * p.n_experts + e] = count[e];
 }
 
-// Over the blocks, 32 experts at a time: 32 runs of blocks side by side, a run's counts in registers.
+// Over the blocks, 32 experts at a time: 32 runs of blocks side by side, a run's counts in registers (6 us, latency; 7.6 with two passes).
 __global__ void __launch_bounds__(1024) sort_scan_kernel(const SortArgs p) {
     __shared__ int sums[32][33];
     wait_for_previous_kernel();
@@ -412,7 +413,10 @@ constexpr int kAheadBytes = 256 * 1024;  // of a block: together they fit L2
 // Dynamic shared memory: next[kMoveWarps][n_experts], then total[n_experts], then start[n_experts + 1], then place[kPart].
 inline int move_shared(int n_experts) { return ((kMoveWarps + 2) * n_experts + 1 + kPart) * (int)sizeof(int); }
 
-// A block takes a chunk of entries (tokens), and of their rows the columns of one of gridDim.y slices.
+// A block takes a chunk of entries (tokens), and of their rows the columns of one of gridDim.y slices.  Two blocks to an SM, a part of 2048
+// entries at a time: smaller chunks learn their place more often (80000 entries of 256 bf16: 19 us, with twice the blocks 24).  Four tokens of a
+// team are on their way at once.  149504 x 4 x 256 bf16: 81 us of 90 with the launches before, 4.7 TB/s, four fifths of it writes; while entries
+// are placed, some 10 us, DRAM idles.
 template <typename T, int kLanes, bool kRagged, int kCounted>
 __global__ void __launch_bounds__(kMoveThreads, 2) dispatch_kernel(const SortArgs p, const MoveArgs m) {
     extern __shared__ int shared[];

