@@ -438,11 +438,10 @@ __global__ void __launch_bounds__(kMoveThreads, 2) dispatch_kernel(const SortArg
 #pragma unroll 4
         for (long long i = threadIdx.x; i < p.entries; i += kMoveThreads) {
             const int e = expert_of(p, i, p.entries);
-            if (e >= 0) {
-                atomicAdd(&total[e], 1);
-                if (i < first) atomicAdd(&next[e], 1);
-            }
+            if (e >= 0) atomicAdd(i < first ? &next[e] : &total[e], 1);
         }
+        __syncthreads();
+        for (int e = threadIdx.x; e < E; e += kMoveThreads) total[e] += next[e];
     } else if (kCounted == kPerBlock) {
         // threads side by side take neighbouring experts of one block
         const int rows = max(1, kMoveThreads / E);
