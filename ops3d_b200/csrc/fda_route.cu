@@ -126,30 +126,39 @@ __device__ unsigned exactly_allowed(const RouteArgs &p, const double *values) {
     return allowed;
 }
 
-// The choice by scores in 64 bits into chosen[top_k]; values: room for [n_experts] numbers.
+// The choice by scores in 64 bits into chosen[top_k]; values: room for [n_experts] numbers.  One token of a call is enough to wait for it, so
+// logits and bias are read once and each exponential is taken once.
 template <typename T, int kPer>
 __device__ __noinline__ void choose_exactly(const RouteArgs &p, long long token, double *values, int *chosen) {
     const int lane = threadIdx.x % 32;
-    double shift = 0, inverse = 1;
-    if (!p.sigmoid) {
-        float top = -INFINITY;
-        bool nan = false;
-        for (int i = 0; i < kPer; ++i)
-            if (lane * kPer + i < p.n_experts) {
-                const float l = logit<T>(p, token, lane * kPer + i);
-                top = fmaxf(top, l);
-                nan |= !(l == l);
-            }
-        shift = most<32>(top);
+    float l[kPer], bias[kPer], top = -INFINITY;
+    double v[kPer], inverse = 1;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = lane * kPer + i;
+        l[i] = e < p.n_experts ? logit<T>(p, token, e) : -INFINITY;
+        bias[i] = e < p.n_experts && p.bias ? p.bias[e] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        top = fmaxf(top, l[i]);
+        nan |= !(l[i] == l[i]);
+    }
+    if (p.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[i] = 1 / (1 + exp(-(double)l[i]));
+    } else {
+        double shift = most<32>(top), sum = 0;
         if (__any_sync(kAll, nan)) shift = NAN;
-        if (shift == -INFINITY) {
-            shift = inverse = 0;
-        } else {
-            double sum = 0;
-            for (int i = 0; i < kPer; ++i)
-                if (lane * kPer + i < p.n_experts) sum += exp((double)logit<T>(p, token, lane * kPer + i) - shift);
-            inverse = 1 / total<32>(sum);
+        if (shift == -INFINITY) shift = 0;  // every score is 0
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            v[i] = exp((double)l[i] - shift);
+            sum += v[i];
         }
+        sum = total<32>(sum);
+        inverse = sum == 0 ? 0 : 1 / sum;
     }
     unsigned long long key[kPer];
     __syncwarp();
@@ -158,11 +167,10 @@ __device__ __noinline__ void choose_exactly(const RouteArgs &p, long long token,
         const int e = lane * kPer + i;
         key[i] = 0;
         if (e >= p.n_experts) continue;
-        const double l = logit<T>(p, token, e);
-        double v = p.sigmoid ? 1 / (1 + exp(-l)) : inverse == 0 ? 0 : exp(l - shift) * inverse;
-        if (p.bias) v += (double)p.bias[e];
-        values[e] = v;
-        key[i] = order_of(p.bias ? v : l);  // without a bias experts are compared by their logits, only groups by sums of scores
+        if (!p.sigmoid) v[i] *= inverse;
+        if (p.bias) v[i] += (double)bias[i];
+        values[e] = v[i];
+        key[i] = order_of(p.bias ? v[i] : (double)l[i]);  // without a bias experts are compared by their logits, only groups by sums of scores
     }
     __syncwarp();
     unsigned left = exactly_allowed<kPer>(p, values);
@@ -476,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
             return top;
         };
         // The first expert of the largest value leaves: every lane of the token gets its value (NaN where none is left) and its number (-1).
-        // The octet that it is in is looked at by a lane an expert, always the same one, so that no lane reads what another has written.
+        // The octet that it is in is looked at by a lane an expert, always the same one, so that no lane reads here what another has written.
         const auto take = [&](float &top) {
             const float own = largest_of_lane();
             top = most<kLanes>(own);
@@ -529,15 +537,15 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
                 const float a = s.chosen_value[segment][j], b = s.chosen_value[segment][j + 1];
                 if (!(a - b > margin + fabsf(a) * kSumError) && !same(s.chosen[segment][j], s.chosen[segment][j + 1])) sure = false;
             }
-            sure = most<kLanes>(sure ? 0.f : 1.f) == 0.f;
-            // of equal experts the lower ones are chosen: what comes behind them counts
+            // of equal experts the lower ones are chosen: all that is left within the margin has to be equal to the last
             const int last_chosen = s.chosen[segment][p.top_k - 1];
-            while (true) {  // ends: a pass takes an expert out of every token that has one
-                float next = most<kLanes>(largest_of_lane());
-                const bool open = sure && next == next && !(last - next > margin + fabsf(last) * kSumError);
-                if (!__any_sync(kAll, open)) break;
-                const int e = take(next);
-                if (open && !same(last_chosen, e)) sure = false;
+            const float next = most<kLanes>(largest_of_lane()), reach = margin + fabsf(last) * kSumError;
+            const bool open = next == next && !(last - next > reach);
+            if (__any_sync(kAll, open)) {
+                for (int e = lane; e < E; e += kLanes) {  // what is taken or no candidate is NaN
+                    const float x = values[e];
+                    if (open && x == x && !(last - x > reach) && !same(last_chosen, e)) sure = false;
+                }
             }
         }
         const unsigned unsure = __ballot_sync(kAll, active && !sure);
