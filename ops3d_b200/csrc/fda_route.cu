@@ -14,7 +14,7 @@
 // neighbouring experts, octet o of the token belonging to lane o mod kLanes.  Their values lie in shared memory, their largest in a
 // register: a step of the choice takes the largest of these over the lanes, then a lane looks at each value of the octet that has it.
 // Bound by instructions, no pipe of which is full (comparisons and selections 50 %, shuffles and shared memory 56 %, issue slots 61 %):
-// 149504 tokens x 256 experts, 8 chosen, bf16: 61 us by logits, 87 by biased softmax scores, of which the bytes would take 14; 37376 x 64 in 8 groups
+// 149504 tokens x 256 experts, 8 chosen, bf16: 60 us by logits, 84 by biased softmax scores, of which the bytes would take 14; 37376 x 64 in 8 groups
 // 17 us.
 #include "fda_rows.cuh"
 
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArg
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             dl[i] = score[i] * over * (p.renormalise ? dw[i] - along : dw[i]);
-            if (p.sigmoid) dl[i] *= 1.f - score[i];
+            if (p.sigmoid) dl[i] *= 1.f / (1.f + expf(l[i]));  // 1 - s, without its cancellation near 1
         }
         if constexpr (!kDense) {  // zeros, and the chosen behind them
             if (active) {
