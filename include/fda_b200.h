@@ -532,9 +532,9 @@ int fda_route_backward(const void *logits, const int64_t *experts, const float *
  *   fda_combine_rows:  y[token] = sum over its entries of weight * rows[position] + residual
  *                      weights [tokens][top_k] of `weight_dtype` (`dtype` or f32) or NULL (1), residual [tokens][features] or NULL
  * fda_combine_rows without weights is the gradient of fda_dispatch_rows.  fda_combine_rows_backward: grad_rows[position] = weight *
- * grad_y[token] (0 in rows from *rows_end on, which is group_start_index + n_experts), grad_weights = <rows[position], grad_y[token]>,
- * 0 where there is no row; either may be NULL.  `position` and `rows_end` are those of fda_dispatch_rows: no entry leads out of `rows`
- * whatever they hold, but entries that share a row leave one of their gradients in it.
+ * grad_y[token], 0 in rows that are no entry's, grad_weights = <rows[position], grad_y[token]>, 0 where there is no row; either may be
+ * NULL, and without grad_rows the workspace too.  `position` is that of fda_dispatch_rows, or with entries taken out of it (-1).  No
+ * entry leads out of `rows` whatever it holds, but where entries share a row its gradient is put together from theirs, not their sum.
  * x, rows, residual, y and their gradients of `dtype`, on 16-byte boundaries; sums in fp32, one rounding.  tokens * top_k < 2^31,
  * top_k <= 32, n_experts <= 1024, features < 2^26.  No counterpart in the reference.
  */
@@ -544,9 +544,10 @@ int fda_dispatch_rows(const void *x, const int64_t *experts, void *rows, int64_t
                       int dtype, void *stream);
 int fda_combine_rows(const void *rows, const int64_t *position, const void *weights, const void *residual, void *y,
                      long long tokens, int top_k, int features, int dtype, int weight_dtype, void *stream);
-int fda_combine_rows_backward(const void *rows, const int64_t *position, const int64_t *rows_end, const void *weights,
-                              const void *grad_y, void *grad_rows, void *grad_weights, long long tokens, int top_k,
-                              int features, int dtype, int weight_dtype, void *stream);
+size_t fda_combine_rows_backward_workspace_bytes(long long tokens, int top_k);
+int fda_combine_rows_backward(const void *rows, const int64_t *position, const void *weights, const void *grad_y,
+                              void *grad_rows, void *grad_weights, void *workspace, size_t workspace_bytes, long long tokens,
+                              int top_k, int features, int dtype, int weight_dtype, void *stream);
 
 /*
  * Backward pass that needs no workspace from the caller and allocates nothing: same inputs,

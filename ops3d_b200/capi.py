@@ -26,7 +26,8 @@ EXPORTS = (
     "fda_linear_forward_workspace_bytes", "fda_linear_forward", "fda_linear_backward_workspace_bytes", "fda_linear_backward",
     "fda_linear_timeouts",
     "fda_layer_norm_forward", "fda_layer_norm_backward_workspace_bytes", "fda_layer_norm_backward", "fda_route_forward", "fda_route_backward",
-    "fda_dispatch_workspace_bytes", "fda_dispatch_rows", "fda_combine_rows", "fda_combine_rows_backward",
+    "fda_dispatch_workspace_bytes", "fda_dispatch_rows", "fda_combine_rows", "fda_combine_rows_backward_workspace_bytes",
+    "fda_combine_rows_backward",
 )
 BWD_ZERO_IMAGE, BWD_RESUME, BWD_FINALIZE, BWD_BINNED_DONE, BWD_ZERO_TOUCHED = 1, 2, 4, 8, 16
 NOALLOC_MAX_ELEMENTS = 16 * 1024 * 1024
@@ -142,7 +143,8 @@ def load() -> ctypes.CDLL:
     lib.fda_dispatch_workspace_bytes.argtypes, lib.fda_dispatch_workspace_bytes.restype = [ll, i, i], sz
     lib.fda_dispatch_rows.argtypes, lib.fda_dispatch_rows.restype = [vp] * 6 + [sz, ll] + [i] * 4 + [vp], i
     lib.fda_combine_rows.argtypes, lib.fda_combine_rows.restype = [vp] * 5 + [ll] + [i] * 4 + [vp], i
-    lib.fda_combine_rows_backward.argtypes, lib.fda_combine_rows_backward.restype = [vp] * 7 + [ll] + [i] * 4 + [vp], i
+    lib.fda_combine_rows_backward_workspace_bytes.argtypes, lib.fda_combine_rows_backward_workspace_bytes.restype = [ll, i], sz
+    lib.fda_combine_rows_backward.argtypes, lib.fda_combine_rows_backward.restype = [vp] * 7 + [sz, ll] + [i] * 4 + [vp], i
     _lib = lib
     return lib
 

@@ -381,16 +381,14 @@ at::Tensor combine_forward_impl(const at::Tensor &rows, const at::Tensor &positi
 }
 
 // Gradients of rows and weights.  `rows` may be undefined where the weights need none.
-std::array<at::Tensor, 2> combine_backward_impl(const at::Tensor &rows, const at::Tensor &position, const at::Tensor &starts,
-                                                const at::Tensor &weights, const at::Tensor &grad_y, bool need_rows, bool need_weights) {
+std::array<at::Tensor, 2> combine_backward_impl(const at::Tensor &rows, const at::Tensor &position, const at::Tensor &weights,
+                                                const at::Tensor &grad_y, bool need_rows, bool need_weights) {
     std::array<at::Tensor, 2> out;
     need_weights = need_weights && weights.defined();
     if (!need_rows && !need_weights) return out;
     const CombineTensors c = check_combine(grad_y, "grad_output", position, weights);
     TORCH_CHECK(grad_y.sizes() == at::IntArrayRef(c.out_size), "grad_output must have the shape of the output, ", at::IntArrayRef(c.out_size),
                 ", got ", grad_y.sizes());
-    check_device(starts, grad_y, "group_start_index", "grad_output");
-    TORCH_CHECK(starts.scalar_type() == at::kLong && starts.dim() == 1 && starts.size(0) >= 1, "group_start_index must be a one-dimensional int64 tensor");
     c10::cuda::CUDAGuard guard(grad_y.device());
     at::Tensor r;
     if (need_weights) {
@@ -399,11 +397,13 @@ std::array<at::Tensor, 2> combine_backward_impl(const at::Tensor &rows, const at
         check_combined_rows(rows, c);
         r = dense(rows);
     }
-    const at::Tensor dy = dense(grad_y), s = starts.contiguous();
+    const at::Tensor dy = dense(grad_y);
     if (need_rows) out[0] = empty_on(grad_y, {c.position.numel(), c.features}, grad_y.scalar_type());
     if (need_weights) out[1] = empty_on(grad_y, weights.sizes(), weights.scalar_type());
-    raise_status(fda_combine_rows_backward(ptr_of(r), c.position.data_ptr<int64_t>(), s.data_ptr<int64_t>() + (s.numel() - 1), ptr_of(c.weights),
-                                           dy.data_ptr(), ptr_of(out[0]), ptr_of(out[1]), c.tokens, c.top_k, c.features, c.dtype, c.weight_dtype,
+    const size_t bytes = need_rows ? fda_combine_rows_backward_workspace_bytes(c.tokens, c.top_k) : 0;
+    const at::Tensor ws = linear_workspace(grad_y, bytes);
+    raise_status(fda_combine_rows_backward(ptr_of(r), c.position.data_ptr<int64_t>(), ptr_of(c.weights), dy.data_ptr(), ptr_of(out[0]),
+                                           ptr_of(out[1]), ptr_of(ws), bytes, c.tokens, c.top_k, c.features, c.dtype, c.weight_dtype,
                                            current_stream()),
                  "combine_rows backward");
     return out;
@@ -413,9 +413,9 @@ at::Tensor combine_forward(const at::Tensor &rows, const at::Tensor &position, c
     return combine_forward_impl(rows, position, or_undefined(weights), or_undefined(residual));
 }
 
-std::array<OptionalTensor, 2> combine_backward(const OptionalTensor &rows, const at::Tensor &position, const at::Tensor &starts,
-                                               const OptionalTensor &weights, const at::Tensor &grad_y, bool need_rows, bool need_weights) {
-    const auto grads = combine_backward_impl(or_undefined(rows), position, starts, or_undefined(weights), grad_y, need_rows, need_weights);
+std::array<OptionalTensor, 2> combine_backward(const OptionalTensor &rows, const at::Tensor &position, const OptionalTensor &weights,
+                                               const at::Tensor &grad_y, bool need_rows, bool need_weights) {
+    const auto grads = combine_backward_impl(or_undefined(rows), position, or_undefined(weights), grad_y, need_rows, need_weights);
     std::array<OptionalTensor, 2> out;
     for (int i = 0; i < 2; ++i)
         if (grads[i].defined()) out[i] = grads[i];
@@ -432,8 +432,7 @@ struct CombineRowsBackward : public fda_nodes::SavedNode {
         {
             at::NoGradGuard no_grad;
             const at::Tensor g = grad_output(grads);
-            const auto r = combine_backward_impl(unpack(0), unpack(1), unpack(2), unpack(3), g, task_should_compute_output(0),
-                                                 task_should_compute_output(1));
+            const auto r = combine_backward_impl(unpack(0), unpack(1), unpack(2), g, task_should_compute_output(0), task_should_compute_output(1));
             results[0] = r[0];
             results[1] = r[1];
             if (task_should_compute_output(2)) results[2] = g;
@@ -442,8 +441,7 @@ struct CombineRowsBackward : public fda_nodes::SavedNode {
     }
 };
 
-at::Tensor combine(const at::Tensor &rows, const at::Tensor &position, const at::Tensor &starts, const OptionalTensor &weights,
-                   const OptionalTensor &residual) {
+at::Tensor combine(const at::Tensor &rows, const at::Tensor &position, const OptionalTensor &weights, const OptionalTensor &residual) {
     const at::Tensor w = or_undefined(weights), r = or_undefined(residual);
     at::Tensor y;
     {
@@ -454,8 +452,7 @@ at::Tensor combine(const at::Tensor &rows, const at::Tensor &position, const at:
         auto node = std::make_shared<CombineRowsBackward>();
         if (w.defined() && w.requires_grad()) node->save(0, rows);  // only the weights' gradient reads them
         node->save(1, position);
-        node->save(2, starts);
-        node->save(3, w);
+        node->save(2, w);
         fda_nodes::connect(node, y, torch::autograd::collect_next_edges(rows, w, r));
     }
     return y;

@@ -28,8 +28,9 @@ read on the host, so everything may be captured into a graph.  Sums are fp32 in 
 equal bit for bit.  Weights of ``combine_rows`` are float32 or in the dtype of the rows; a residual of another dtype than the rows' is
 added behind the sum, in the wider of the two.  Up to 1024 experts, 32 entries a token, 32 groups, 2^31 - 1 entries.
 
-``order`` comes from ``dispatch_rows``; an order put together by hand leads out of no tensor, but entries that share a row leave one of
-their gradients in it.
+``order`` comes from ``dispatch_rows``; entries may be taken out of it (``order._replace(position=...)`` with -1 for those beyond an
+expert's capacity, say): their rows get a gradient of 0.  One put together by hand leads out of no tensor, but where entries share a row
+its gradient is put together from theirs, not their sum.
 
 ``ExpertFeedForward`` is a transformer layer's feed-forward block with experts: norm, router, experts, sum and residual.
 """
@@ -132,34 +133,34 @@ def dispatch_rows(x, experts, n_experts):
 
 
 class CombineRowsFunction(Function):
-    """``apply(rows, position, group_start_index, weights, residual)``."""
+    """``apply(rows, position, weights, residual)``."""
 
     @staticmethod
-    def forward(ctx, rows, position, group_start_index, weights, residual):
-        needs_rows = weights is not None and ctx.needs_input_grad[3]  # only the weights' gradient reads them
-        ctx.save_for_backward(rows if needs_rows else None, position, group_start_index, weights)
+    def forward(ctx, rows, position, weights, residual):
+        needs_rows = weights is not None and ctx.needs_input_grad[2]  # only the weights' gradient reads them
+        ctx.save_for_backward(rows if needs_rows else None, position, weights)
         return _ext().combine_forward(rows, position, weights, residual)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output):
         need = ctx.needs_input_grad
-        grad_rows, grad_weights = _ext().combine_backward(*ctx.saved_tensors, grad_output, need[0], need[3])
-        return grad_rows, None, None, grad_weights, grad_output if need[4] else None
+        grad_rows, grad_weights = _ext().combine_backward(*ctx.saved_tensors, grad_output, need[0], need[2])
+        return grad_rows, None, grad_weights, grad_output if need[3] else None
 
     @classmethod
-    def apply(cls, rows, position, group_start_index, weights=None, residual=None):
+    def apply(cls, rows, position, weights=None, residual=None):
         if cls is CombineRowsFunction and takes_node():
-            return _ext().combine(rows, position, group_start_index, weights, residual)
-        return super().apply(rows, position, group_start_index, weights, residual)
+            return _ext().combine(rows, position, weights, residual)
+        return super().apply(rows, position, weights, residual)
 
 
 def combine_rows(rows, order, weights=None, residual=None):
     """Each token's weighted sum of its rows (module docstring)."""
-    starts, position = order
+    _, position = order
     if residual is None or residual.dtype == rows.dtype:
-        return CombineRowsFunction.apply(rows, position, starts, weights, residual)
-    return add_residual(CombineRowsFunction.apply(rows, position, starts, weights, None), residual)
+        return CombineRowsFunction.apply(rows, position, weights, residual)
+    return add_residual(CombineRowsFunction.apply(rows, position, weights, None), residual)
 
 
 class ExpertFeedForward(nn.Module):

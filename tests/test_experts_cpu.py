@@ -82,9 +82,12 @@ def test_row_arguments():
     comb = lambda rows=P, pos=P, w=P, r=P, y=P, t=4, k=2, c=8, dt=BF16, wdt=F32: lib.fda_combine_rows(rows, pos, w, r, y, t, k, c, dt, wdt, None)  # noqa: E731
     assert comb(dt=3) == 2 and comb(wdt=3) == 2 and comb(t=-1) == 6 and comb(k=33) == 11 and comb(rows=None) == 1 and comb(pos=None) == 1
     assert comb(rows=ODD) == 9 and comb(r=ODD) == 9 and comb(y=ODD) == 9 and comb(t=0, rows=None) == 0
-    back = lambda rows=P, pos=P, end=P, w=P, dy=P, dr=P, dw=P, t=4, dt=BF16, wdt=F32: lib.fda_combine_rows_backward(  # noqa: E731
-        rows, pos, end, w, dy, dr, dw, t, 2, 8, dt, wdt, None)
-    assert back(dt=3) == 2 and back(wdt=3) == 2 and back(rows=None) == 1 and back(end=None) == 1 and back(dy=None) == 1
+    need = lib.fda_combine_rows_backward_workspace_bytes(4, 2)
+    assert need >= 32 and lib.fda_combine_rows_backward_workspace_bytes(0, 2) == 0 == lib.fda_combine_rows_backward_workspace_bytes(1 << 30, 2)
+    back = lambda rows=P, pos=P, w=P, dy=P, dr=P, dw=P, ws=P, ws_bytes=need, t=4, dt=BF16, wdt=F32: lib.fda_combine_rows_backward(  # noqa: E731
+        rows, pos, w, dy, dr, dw, ws, ws_bytes, t, 2, 8, dt, wdt, None)
+    assert back(dt=3) == 2 and back(wdt=3) == 2 and back(rows=None) == 1 and back(pos=None) == 1 and back(dy=None) == 1
+    assert back(ws=None) == 8 and back(ws_bytes=need - 1) == 8 and back(ws=ODD) == 9
     assert back(dr=ODD) == 9 and back(dy=ODD) == 9 and back(dr=None, dw=None, dy=None) == 0 and back(t=0) == 0
 
 
@@ -149,13 +152,13 @@ class Binding:
     def dispatch_forward(self, x, experts, n):
         return [self._first(x, (experts.numel(), x.shape[-1])), *self._order(experts, n)]
 
-    def combine(self, rows, position, starts, weights, residual):
+    def combine(self, rows, position, weights, residual):
         return self._node(rows, (*position.shape[:-1], rows.shape[-1]))
 
     def combine_forward(self, rows, position, weights, residual):
         return rows.sum() * torch.ones(*position.shape[:-1], rows.shape[-1])
 
-    def combine_backward(self, rows, position, starts, weights, grad, need_rows, need_weights):
+    def combine_backward(self, rows, position, weights, grad, need_rows, need_weights):
         return [grad.sum() * torch.ones(position.numel(), grad.shape[-1]) if need_rows else None, None]
 
 
@@ -168,12 +171,11 @@ def binding(monkeypatch):
 
 
 EXPERTS = torch.zeros(3, 2, dtype=torch.int64)
-STARTS = torch.zeros(5, dtype=torch.int64)
 OPS = {
     "norm": (norm_mod.LayerNormFunction, torch.rand(3, 4), lambda f, v: f(v, None, None, None, 1e-5, False)[0]),
     "route": (experts_mod.RouteExpertsFunction, torch.rand(3, 4), lambda f, v: f(v, None, 2, 0, 1, 1, 0, True, 1.0)[0]),
     "dispatch": (experts_mod.DispatchRowsFunction, torch.rand(3, 4), lambda f, v: f(v, EXPERTS, 4)[0]),
-    "combine": (experts_mod.CombineRowsFunction, torch.rand(6, 4), lambda f, v: f(v, EXPERTS, STARTS, None, None)),
+    "combine": (experts_mod.CombineRowsFunction, torch.rand(6, 4), lambda f, v: f(v, EXPERTS, None, None)),
 }
 
 

@@ -470,8 +470,30 @@ def test_positions_that_lead_nowhere():
     at = torch.where((position >= 0) & (position < 12), position, -1)
     e = rows.detach().double()[at.clamp_min(0)] * (at >= 0)[..., None] * w.detach().double()[..., None]
     close(y, e.sum(1), 4 * U * e.abs().sum(1))
-    _, gw = torch.autograd.grad(y, (rows, w), torch.ones_like(y))
+    gr, gw = torch.autograd.grad(y, (rows, w), torch.ones_like(y))
     assert torch.equal(gw == 0, at < 0)
+    expected = torch.zeros(12, device=DEV).index_add_(0, at[at >= 0], w.detach()[at >= 0])  # no row twice: nothing is rounded
+    assert torch.equal(gr, expected[:, None].expand(12, 16))
+
+
+@pytest.mark.parametrize("tokens,k,width,dtype", [(1, 1, 8, F32), (40, 3, 24, BF16), (700, 2, 99, F32), (60, 4, 1031, F16), (60, 4, 4096, BF16),
+                                                  (30000, 4, 64, BF16), (30000, 4, 35, BF16)])
+def test_entries_taken_out_of_an_order(tokens, k, width, dtype):
+    """Beyond an expert's capacity: the rows that no entry leads to any more get a gradient of 0 wherever they lie, the others theirs."""
+    experts = experts_of(tokens, k, 7, 0.1)
+    rows, order = dispatch_rows(rows_of((tokens, width), dtype), experts, 7)
+    capacity = max(1, tokens * k // 11)
+    beyond = order.position - order.group_start_index[experts.clamp(0, 6)] >= capacity
+    kept = order._replace(position=order.position.masked_fill(beyond, -1))
+    leaf, w, dy = rows.detach().requires_grad_(True), rows_of((tokens, k), F32, 1).requires_grad_(True), rows_of((tokens, width), dtype, 2)
+    junk = [torch.full_like(rows, NAN) for _ in range(2)]  # what the gradient's memory may hold
+    del junk
+    gr, gw = torch.autograd.grad(combine_rows(leaf, kept, w), (leaf, w), dy)
+    all_r, all_w = torch.autograd.grad(combine_rows(leaf, order, w), (leaf, w), dy)
+    there = torch.zeros(tokens * k, dtype=torch.bool, device=DEV)
+    there[kept.position[kept.position >= 0]] = True
+    assert torch.equal(gr, torch.where(there[:, None], all_r, torch.zeros_like(all_r)))
+    assert torch.equal(gw, all_w.masked_fill(kept.position < 0, 0.0))
 
 
 def test_residual_of_another_type_keeps_its_bits():
@@ -500,7 +522,7 @@ def test_functions_are_the_nodes():
         leaves = [t.detach().requires_grad_(True) for t in (logits, x)]
         w, e = route.apply(leaves[0], None, 3, 0, 1, 1, 0, False, 1.0)
         rows, starts, position = dispatch.apply(leaves[1], e, 24)
-        y = combine.apply(rows, position, starts, w, leaves[1])
+        y = combine.apply(rows, position, w, leaves[1])
         assert not e.requires_grad and not starts.requires_grad and not position.requires_grad
         out.append([w, e, rows, starts, position, y, *torch.autograd.grad(y, leaves, dy)])
     assert all(torch.equal(a, b) for a, b in zip(*out))
