@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kTeamThreads) norm_forward_kernel(const NormAr
     wait_copies<0>();
 }
 
-// 598016 x 256 bf16: 163 us (5.6 TB/s), with a residual 188 (6.5); 300000 x 64 with one 30 (5.1).  Two rounds of sums over the lanes, the second of
+// 598016 x 256 bf16: 157 us (5.8 TB/s), with a residual 185 (6.6); 300000 x 64 with one 30 (5.1).  Two rounds of sums over the lanes, the second of
 // three numbers; issue slots are 73 % busy.
 template <typename T, typename R, bool kResidual, int kVectors, int kLanes, bool kRagged>
 __global__ void __launch_bounds__(kTeamThreads) norm_backward_kernel(const NormArgs p) {
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(kBlockThreads) norm_forward_block_kernel(const
     wait_copies<0>();
 }
 
-// The backward has no registers for a second row: its block meets twice (73728 x 1024 f16 108 us, with the next row's mean ahead 120).
+// The backward has no registers for a second row: its block meets twice (73728 x 1024 f16 103 us; before its sums took fewer exchanges 108, and then 120 with the next row's mean ahead).
 template <typename T, typename R, bool kResidual, int kVectors, bool kRagged>
 __global__ void __launch_bounds__(kBlockThreads) norm_backward_block_kernel(const NormArgs p) {
     constexpr int W = kWidthOf<T>, H = W / 2, kUnits = kUnitsOf<T, R, kResidual, kVectors, true>, kStages = kStagesOf<kUnits, 0, true>;

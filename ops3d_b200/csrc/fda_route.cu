@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArg
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             dl[i] = score[i] * over * (p.renormalise ? dw[i] - along : dw[i]);
-            if (p.sigmoid) dl[i] *= 1.f / (1.f + expf(l[i]));  // 1 - s, without its cancellation near 1
+            if (p.sigmoid && there[i]) dl[i] *= 1.f / (1.f + expf(l[i]));  // 1 - s, without its cancellation near 1
         }
         if constexpr (!kDense) {  // zeros, and the chosen behind them
             if (active) {
