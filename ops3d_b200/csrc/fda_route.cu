@@ -580,23 +580,37 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
     }
 }
 
+// A warp sets n <= kMost elements to 0, in vectors but for the ends.
+template <int kMost, typename T>
+__device__ __forceinline__ void clear_run(T *begin, int n, int lane) {
+    constexpr int W = 16 / (int)sizeof(T);
+    const int head = min((int)(-(reinterpret_cast<uintptr_t>(begin) / sizeof(T)) % W), n), vectors = (n - head) / W, tail = head + vectors * W;
+    if (lane < head) begin[lane] = from_f32<T>(0.f);
+#pragma unroll
+    for (int i = 0; i < kMost / W; i += 32)
+        if (i + lane < vectors) reinterpret_cast<uint4 *>(begin + head)[i + lane] = make_uint4(0, 0, 0, 0);
+    if (tail + lane < n) begin[tail + lane] = from_f32<T>(0.f);
+}
+
 // grad_logits from grad_weights: with s the scores of the chosen and S their sum,
 //     softmax, renormalised    dl_j = w_j (dw_j - sum of dw w / scale)           (a softmax over the chosen alone)
 //     softmax                  dl_i = scale p_i ([i chosen] dw_i - sum of dw p)
 //     sigmoid                  dl_j = ds_j s_j (1 - s_j),  ds_j = scale (dw_j - sum of dw s / S) / S  or  scale dw_j
-// An expert outside 0 .. n_experts - 1 gets none.  A token's row is one team's, so there are no atomics.  149504 x 256 bf16: 30 us (2.9 TB/s)
-// renormalised, 45 for the dense softmax; bound by the chain from a choice to its logit.
-template <typename T, int kLanes, int kOctets, bool kVector, bool kDense>
+// An expert outside 0 .. n_experts - 1 gets none.  A token's row is one team's, so there are no atomics.  149504 x 256 bf16: 27 us (3.4 TB/s)
+// renormalised, 39 (4.3 TB/s) for the dense softmax; bound by the chain from a choice to its logit.  A lane has kMine choices, no more than top_k
+// needs (149504 x 64 f32, 2 chosen: 11 us, with room for 32 18).  The rows of a warp's tokens lie one behind the other and are zeroed as one run
+// (100000 x 131 bf16 10.5 us, row by row 45; 20000 x 1000 f32 16 and 21; 149504 x 256 bf16 26.7 and 26.0).
+template <typename T, int kLanes, int kOctets, bool kVector, bool kDense, int kMine>
 __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArgs p) {
-    constexpr int kTokens = 32 / kLanes, kExperts = kLanes * kOctets * 8, kMine = kMostChoices / kLanes;
+    constexpr int kTokens = 32 / kLanes, kExperts = kLanes * kOctets * 8;
     __shared__ alignas(16) float rows[kDense ? kWarps : 1][kTokens][kDense ? kExperts : 1];
     wait_for_previous_kernel();
     const int lane = threadIdx.x % kLanes, segment = threadIdx.x % 32 / kLanes, E = p.n_experts;
     float *row = rows[kDense ? threadIdx.x / 32 : 0][segment];
     const long long step = (long long)gridDim.x * kWarps * kTokens;
-    // Choices and their weights' gradients of the next token are on their way while one is worked on; four lanes, with eight choices each,
-    // have no registers for that (149504 x 64: 18 us with, 14 without; 149504 x 256 by eight lanes 29.5 with, 32.4 without).
-    constexpr bool kAhead = kLanes >= 8;
+    // Choices and their weights' gradients of the next token are on their way while one is worked on; eight of them in a lane have no registers
+    // for that (149504 x 64: 18 us with, 14 without; four, 149504 x 256 29.5 with, 32.4 without).
+    constexpr bool kAhead = kMine <= 4;
     long long next_chosen[kMine];
     float next_dw[kMine];
     const auto read_choices = [&](long long t) {
@@ -648,21 +662,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArg
             if (p.sigmoid && there[i]) dl[i] *= 1.f / (1.f + expf(l[i]));  // 1 - s, without its cancellation near 1
         }
         if constexpr (!kDense) {  // zeros, and the chosen behind them
-            if (active) {
-#pragma unroll
-                for (int q = 0; q < kOctets; ++q) {
-                    const int first = (q * kLanes + lane) * 8;
-                    if (kVector && first < E) {
-                        Raw<T, 8> raw;
-                        raw.clear();
-                        raw.store(out + first);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (first + i < E) out[first + i] = from_f32<T>(0.f);
-                    }
-                }
-            }
+            clear_run<kTokens * kExperts>(static_cast<T *>(p.grad_logits) + base * E, (int)min((long long)kTokens, p.tokens - base) * E, threadIdx.x % 32);
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < kMine; ++i)
@@ -704,21 +704,30 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(const RouteArg
     }
 }
 
+template <typename T, int kLanes, int kOctets, int kMine>
+auto route_backward_kernel_of(bool vector, bool dense) {
+    if (!dense) return route_backward_kernel<T, kLanes, kOctets, false, false, kMine>;  // without vectors of a token's row
+    return vector ? route_backward_kernel<T, kLanes, kOctets, true, true, kMine> : route_backward_kernel<T, kLanes, kOctets, false, true, kMine>;
+}
+
 template <typename T, int kLanes, int kOctets>
 int launch_route(bool backward, const RouteArgs &p, cudaStream_t st) {
     const unsigned blocks = (unsigned)std::min<long long>(ceil_div(p.tokens, kWarps * 32 / kLanes), 16 * kSms);
     // rows of octets that start on 16-byte boundaries
     const bool vector = p.n_experts % 8 == 0 && !misaligned16(p.logits) && !misaligned16(p.grad_logits);
     const bool dense = !p.sigmoid && !p.renormalise;
-    const auto kernel = !backward ? (vector ? route_forward_kernel<T, kLanes, kOctets, true> : route_forward_kernel<T, kLanes, kOctets, false>)
-                        : dense   ? (vector ? route_backward_kernel<T, kLanes, kOctets, true, true> : route_backward_kernel<T, kLanes, kOctets, false, true>)
-                                  : (vector ? route_backward_kernel<T, kLanes, kOctets, true, false> : route_backward_kernel<T, kLanes, kOctets, false, false>);
+    auto kernel = vector ? route_forward_kernel<T, kLanes, kOctets, true> : route_forward_kernel<T, kLanes, kOctets, false>;
+    if (backward) {
+        kernel = p.top_k <= kLanes       ? route_backward_kernel_of<T, kLanes, kOctets, 1>(vector, dense)
+                 : p.top_k <= 2 * kLanes ? route_backward_kernel_of<T, kLanes, kOctets, 2>(vector, dense)
+                                         : route_backward_kernel_of<T, kLanes, kOctets, kMostChoices / kLanes>(vector, dense);
+    }
     return launched(launch_early(kernel, blocks, kThreads, 0, st, 1, p));
 }
 
 template <typename T>
 int launch_route(bool backward, const RouteArgs &p, cudaStream_t st) {
-    // four lanes up to 64 experts (149504 x 64 f32: 20 + 14 us, eight lanes 25 + 18), not beyond (x 256 bf16: 95 + 51 us, eight lanes 88 + 33)
+    // four lanes up to 64 experts (149504 x 64 f32 forward: 20 us, eight lanes 25), not beyond (x 256 bf16: 95 us, eight lanes 88)
     if (p.n_experts <= 32) return launch_route<T, 4, 1>(backward, p, st);
     if (p.n_experts <= 64) return launch_route<T, 4, 2>(backward, p, st);
     if (p.n_experts <= 128) return launch_route<T, 8, 2>(backward, p, st);
