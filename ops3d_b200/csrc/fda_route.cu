@@ -388,6 +388,17 @@ __device__ __forceinline__ void only_candidates(int n_experts, int lane, bool sa
     }
 }
 
+// Whether a lane finds a NaN among its share of a token's logits.  Few tokens ask: not inlined, so that others keep their registers.
+template <typename T>
+__device__ __noinline__ bool has_nan(const RouteArgs &p, long long token, int lane, int lanes) {
+    bool nan = false;
+    for (int e = lane; e < p.n_experts; e += lanes) {
+        const float x = logit<T>(p, token, e);
+        nan |= x != x;
+    }
+    return nan;
+}
+
 template <typename T, int kLanes, int kOctets, bool kVector>
 __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_kernel(const RouteArgs p) {
     using Shared = WarpShared<kLanes, kOctets>;
@@ -527,6 +538,9 @@ __global__ void __launch_bounds__(kThreads, kOctets <= 4 ? 8 : 4) route_forward_
             }
         }
         __syncwarp();
+        // A NaN counts as minus infinity, of which the lower index is chosen; without groups it is no candidate here, and one before the last
+        // chosen minus infinity is a choice.
+        if (!grouped && s.chosen_value[segment][p.top_k - 1] == -INFINITY && has_nan<T>(p, token, lane, kLanes)) sure = false;
         if (p.bias) {
             // the chosen among themselves, and the last of them against what is left
             const float margin = 2.f * score_error + kSmallest, last = s.chosen_value[segment][p.top_k - 1];
