@@ -244,18 +244,24 @@ __device__ __forceinline__ void softmax_of(float (&v)[kOctets][8], bool quick, f
 }
 
 // Scores of the chosen experts with the logits l (kMine of them in a lane; those that are not there have there[i] false), before
-// scaling, and what the weights are divided by.
+// scaling, and what the weights are divided by.  Renormalised scores are ratios, which stay what they are where the scores themselves leave fp32's
+// range: a softmax is taken over the chosen alone, and with m = min(0, largest chosen logit) a sigmoid's share of them is
+//     e^(l - m) / (1 + e^(l - m) e^m)   for l < 0,     1 / (1 + e^-l)   else (m is 0 then)
+// which is the score divided by e^m.
 template <int kLanes, int kMine>
 __device__ __forceinline__ float chosen_scores(const RouteArgs &p, const float (&l)[kMine], const bool (&there)[kMine], float shift, float inverse,
                                                float (&score)[kMine]) {
-    if (!p.sigmoid && p.renormalise) {  // softmax over the chosen
-        shift = -INFINITY;
+    float scale = 1.f;  // e^m
+    if (p.sigmoid) shift = 0.f;
+    if (p.renormalise) {
+        float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
-            if (there[i]) shift = fmaxf(shift, l[i]);
-        shift = most<kLanes>(shift);
-        if (shift == -INFINITY) shift = 0.f;
+            if (there[i]) top = fmaxf(top, l[i]);
+        top = most<kLanes>(top);
+        shift = top == -INFINITY ? 0.f : p.sigmoid ? fminf(top, 0.f) : top;
         inverse = 1.f;
+        if (p.sigmoid) scale = expf(shift);
     }
     float sum = 0.f;
 #pragma unroll
@@ -263,8 +269,13 @@ __device__ __forceinline__ float chosen_scores(const RouteArgs &p, const float (
         score[i] = 0.f;
         if (i * kLanes >= p.top_k) continue;
         if (there[i]) {
-            if (p.sigmoid) score[i] = 1.f / (1.f + expf(-l[i]));
-            else if (inverse != 0.f) score[i] = expf(l[i] - shift) * inverse;
+            if (p.sigmoid) {
+                const bool low = l[i] < 0.f;
+                const float e = expf(low ? l[i] - shift : -l[i]);
+                score[i] = (low ? e : 1.f) / (1.f + (low ? e * scale : e));
+            } else if (inverse != 0.f) {
+                score[i] = expf(l[i] - shift) * inverse;
+            }
         }
         sum += score[i];
     }
