@@ -13,6 +13,7 @@
 // a row's first and last vector are masked out.
 #pragma once
 
+#include "fda_norm_copy.h"
 #include "fda_rows.cuh"
 
 #include <algorithm>
@@ -84,13 +85,13 @@ __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_
 template <int kLeft>
 __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
-// at: where the row's first vector of the lane starts in the tensor; left: rows from this one on, of which only the last may end inside a
-// vector at the tensor's end.  kLanes: neighbouring lanes that share the row.
+// at: where the row's first vector of the lane starts in the tensor; left: rows from this one on.  kLanes: neighbouring lanes that share
+// the row.
 template <typename E, int kLanes, int kWidth, int kVectors, bool kRagged>
 __device__ __forceinline__ void copy_row(unsigned slot, unsigned pitch, const void *tensor, const Columns<kWidth, kVectors, kRagged> &c,
                                          long long at, long long left) {
     constexpr int kUnits = kWidth * (int)sizeof(E) / 16, kEach = 16 / (int)sizeof(E);
-    const int lane = threadIdx.x % kLanes;
+    const int lane = threadIdx.x % kLanes, room = kRagged ? room_of(left, c.width, kEach) : 0;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
 #pragma unroll
@@ -98,8 +99,7 @@ __device__ __forceinline__ void copy_row(unsigned slot, unsigned pitch, const vo
             // elements from the lane's own vector to what it copies
             const int ahead = kUnits == 1 ? 0 : (u * kLanes + lane) * kEach - lane * kWidth;
             const int rest = kUnits == 1 ? c.count[i] : c.width - (c.first[i] + ahead);
-            const int last = kRagged ? max(0, min(kEach, rest)) * (int)sizeof(E) : 16;
-            const int bytes = rest <= 0 || left <= 0 ? 0 : kRagged && left == 1 ? last : 16;
+            const int bytes = kRagged ? copied_elements(c.first[i] + ahead, c.width, kEach, room) * (int)sizeof(E) : rest <= 0 || left <= 0 ? 0 : 16;
             const E *from = static_cast<const E *>(tensor) + at + (c.first[i] - c.first[0]) + ahead;
             copy16(slot + (i * kUnits + u) * pitch, bytes ? from : tensor, bytes);
         }
