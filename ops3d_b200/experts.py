@@ -169,7 +169,8 @@ class ExpertFeedForward(nn.Module):
 
     ``router`` ``[n_experts, d_model]`` makes the logits; the options are those of ``route_experts``.  With ``balanced`` a buffer
     ``balance`` is its bias: raise an expert's entry to send it more tokens.  ``forward`` takes a mask of tokens that are padding (True: no
-    expert) and with ``return_order`` returns the rows' order too, whose ``group_start_index.diff()`` is how many tokens each expert had."""
+    expert; it may hold anything) and with ``return_order`` returns the rows' order too, whose
+    ``group_start_index.diff()`` is how many tokens each expert had."""
 
     def __init__(self, d_model: int = 256, d_hidden: int = 1024, n_experts: int = 8, top_k: int = 2, activation: str = "gelu",
                  score: str = "softmax", n_groups: int = 1, top_groups: int = 1, group_score: str = "max", renormalise: bool = True,
@@ -191,9 +192,12 @@ class ExpertFeedForward(nn.Module):
         self.experts = FeedForward(d_model, d_hidden, activation, n_groups=n_experts, residual=False)
 
     def forward(self, x, padding_mask=None, return_order=False):
-        h = x if self.norm is None else self.norm(x)
+        # nothing that padding holds, a NaN either, gets into the gradients of norm and router; no row of it is moved
+        kept = x if padding_mask is None else x.masked_fill(padding_mask[..., None], 0.0)
+        h = x if self.norm is None else self.norm(kept)
         balance = None if self.balance is None else self.balance.float()
-        weights, experts = route_experts(fused_linear(h, like(h, self.router)), self.top_k, balance, **self.routing)
+        logits = fused_linear(kept if self.norm is None else h, like(h, self.router))
+        weights, experts = route_experts(logits, self.top_k, balance, **self.routing)
         if padding_mask is not None:
             experts = experts.masked_fill(padding_mask[..., None], -1)
         rows, order = dispatch_rows(h, experts, self.n_experts)
