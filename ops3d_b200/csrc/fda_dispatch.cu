@@ -432,12 +432,14 @@ __global__ void __launch_bounds__(1024) sort_scan_kernel(const SortArgs p) {
 // How a block of the moving kernel learns how many entries of each expert there are, and how many before its own.
 enum Counted {
     kByItself,  // it counts all entries
-    kPerBlock,  // counts of each block: it adds them up
+    kPerBlock,  // counts of each block: it adds them up, of up to kFewExperts
     kScanned    // added up by sort_scan_kernel
 };
 
 constexpr int kPart = 2048;  // entries of a block that are placed at a time
 constexpr int kMoveThreads = 512, kMoveWarps = kMoveThreads / 32;
+constexpr int kFewExperts = 32;
+static_assert(kFewExperts <= kMoveThreads, "a thread takes one expert");
 
 constexpr int kAheadBytes = 256 * 1024;  // of a block: together they fit L2
 
@@ -474,21 +476,18 @@ __global__ void __launch_bounds__(kMoveThreads, 2) dispatch_kernel(const SortArg
         __syncthreads();
         for (int e = threadIdx.x; e < E; e += kMoveThreads) total[e] += next[e];
     } else if (kCounted == kPerBlock) {
-        // threads side by side take neighbouring experts of one block
-        const int rows = max(1, kMoveThreads / E);
-        for (int base = 0; base < E; base += kMoveThreads) {
-            const int e = E >= kMoveThreads ? base + threadIdx.x : threadIdx.x % E, row = E >= kMoveThreads ? 0 : threadIdx.x / E;
-            int all = 0, before = 0;
-            if (e < E && row < rows) {
+        // threads side by side take neighbouring experts of one block; there are few experts
+        const int e = threadIdx.x % E, row = threadIdx.x / E, rows = kMoveThreads / E;
+        int all = 0, before = 0;
+        if (row < rows) {
 #pragma unroll 8
-                for (int c = row; c < p.chunks; c += rows) {
-                    const int n = p.counts[(size_t)c * E + e];
-                    all += n;
-                    if (c < (int)blockIdx.x) before += n;
-                }
-                atomicAdd(&total[e], all);
-                atomicAdd(&next[e], before);
+            for (int c = row; c < p.chunks; c += rows) {
+                const int n = p.counts[(size_t)c * E + e];
+                all += n;
+                if (c < (int)blockIdx.x) before += n;
             }
+            atomicAdd(&total[e], all);
+            atomicAdd(&next[e], before);
         }
     } else {
         for (int e = threadIdx.x; e < E; e += kMoveThreads) {
@@ -697,7 +696,7 @@ Counted counted(const SortArgs &s) {
     if (s.entries <= kFewEntries) return kByItself;
     // blocks add up a few experts' counts while a third launch would start: 147456 entries by 16 experts 25.6 us so and 27.4 with a scan, 80000
     // by 64 experts 19.5 and 18.7
-    return s.n_experts <= 32 ? kPerBlock : kScanned;
+    return s.n_experts <= kFewExperts ? kPerBlock : kScanned;
 }
 
 template <typename T, int kLanes, bool kRagged>

@@ -10,12 +10,16 @@
 // a token for which it is not is decided by scores in 64 bits, so that no choice depends on how an exponential rounds.  A NaN
 // counts as minus infinity in comparisons, and stays one in the weights.
 //
-// kLanes (8, or 16 beyond 512 experts) lanes take a token, so that a warp's instructions serve four.  A lane holds octets of
-// neighbouring experts, octet o of the token belonging to lane o mod kLanes.  Their values lie in shared memory, their largest in a
-// register: a step of the choice takes the largest of these over the lanes, then a lane looks at each value of the octet that has it.
-// Bound by instructions, no pipe of which is full (comparisons and selections 50 %, shuffles and shared memory 56 %, issue slots 61 %):
-// 149504 tokens x 256 experts, 8 chosen, bf16: 60 us by logits, 84 by biased softmax scores, of which the bytes would take 14; 37376 x 64 in 8 groups
-// 17 us.
+// kLanes lanes take a token: 4 up to 64 experts, 8 up to 512, 16 beyond, so that a warp's instructions serve eight, four or two.  A lane
+// holds octets of neighbouring experts, octet o of the token belonging to lane o mod kLanes.  Their values lie in shared memory, their
+// largest in a register: a step of the choice takes the largest of these over the lanes, then eight lanes (four that look at two each) look at
+// the octet that has it.  Bound by instructions, no pipe of which is full (comparisons and selections 50 %, shuffles and shared memory 56 %,
+// issue slots 61 %); beyond 128 experts 64 registers (128 beyond 256) spill some 350 bytes a thread.  149504 tokens x 256 experts, 8 chosen, bf16:
+// 60 us by logits, 83 by biased softmax scores, of which the bytes would take 14; 37376 x 64 in 8 groups 17 us.
+//
+// How many tokens are decided in 64 bits depends on the logits: an error is taken relative to the token's largest score, so that low scores of a
+// peaked softmax, or scores of saturated sigmoids, count as equal.  149504 x 256 f32 with a bias of zeros, by the logits' standard deviation
+// (1.5, 4, 6, 8): softmax 90, 109, 189, 296 us, sigmoid 89, 239, 609, 628 us; every token so 660 us.
 #include "fda_rows.cuh"
 
 #include <algorithm>

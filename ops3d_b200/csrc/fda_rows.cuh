@@ -83,10 +83,6 @@ struct Raw {
     static constexpr int kUnits = kWidth * (int)sizeof(T) / 16;
     uint4 u[kUnits];
 
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) u[i] = make_uint4(0, 0, 0, 0);
-    }
     __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) u[i] = reinterpret_cast<const uint4 *>(p)[i];
