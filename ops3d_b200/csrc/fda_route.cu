@@ -247,6 +247,17 @@ __device__ __forceinline__ void softmax_of(float (&v)[kOctets][8], bool quick, f
     inverse = sum == 0.f ? 0.f : 1.f / sum;
 }
 
+// The largest of a token's chosen logits, 0 where there is none above minus infinity.
+template <int kLanes, int kMine>
+__device__ __forceinline__ float largest_chosen(const float (&l)[kMine], const bool (&there)[kMine]) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+        if (there[i]) top = fmaxf(top, l[i]);
+    top = most<kLanes>(top);
+    return top == -INFINITY ? 0.f : top;
+}
+
 // Scores of the chosen experts with the logits l (kMine of them in a lane; those that are not there have there[i] false), before
 // scaling, and what the weights are divided by.  Renormalised scores are ratios, which stay what they are where the scores themselves leave fp32's
 // range: a softmax is taken over the chosen alone, and with m = min(0, largest chosen logit) a sigmoid's share of them is
@@ -255,33 +266,32 @@ __device__ __forceinline__ void softmax_of(float (&v)[kOctets][8], bool quick, f
 template <int kLanes, int kMine>
 __device__ __forceinline__ float chosen_scores(const RouteArgs &p, const float (&l)[kMine], const bool (&there)[kMine], float shift, float inverse,
                                                float (&score)[kMine]) {
-    float scale = 1.f;  // e^m
-    if (p.sigmoid) shift = 0.f;
-    if (p.renormalise) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kMine; ++i)
-            if (there[i]) top = fmaxf(top, l[i]);
-        top = most<kLanes>(top);
-        shift = top == -INFINITY ? 0.f : p.sigmoid ? fminf(top, 0.f) : top;
-        inverse = 1.f;
-        if (p.sigmoid) scale = expf(shift);
-    }
     float sum = 0.f;
+    if (p.sigmoid) {
+        const float m = p.renormalise ? fminf(largest_chosen<kLanes>(l, there), 0.f) : 0.f, scale = expf(m);
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-        score[i] = 0.f;
-        if (i * kLanes >= p.top_k) continue;
-        if (there[i]) {
-            if (p.sigmoid) {
+        for (int i = 0; i < kMine; ++i) {
+            score[i] = 0.f;
+            if (i * kLanes >= p.top_k) continue;
+            if (there[i]) {
                 const bool low = l[i] < 0.f;
-                const float e = expf(low ? l[i] - shift : -l[i]);
+                const float e = expf(low ? l[i] - m : -l[i]);
                 score[i] = (low ? e : 1.f) / (1.f + (low ? e * scale : e));
-            } else if (inverse != 0.f) {
-                score[i] = expf(l[i] - shift) * inverse;
             }
+            sum += score[i];
         }
-        sum += score[i];
+    } else {
+        if (p.renormalise) {
+            shift = largest_chosen<kLanes>(l, there);
+            inverse = 1.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            score[i] = 0.f;
+            if (i * kLanes >= p.top_k) continue;
+            if (there[i] && inverse != 0.f) score[i] = expf(l[i] - shift) * inverse;
+            sum += score[i];
+        }
     }
     return p.renormalise ? total<kLanes>(sum) : 1.f;
 }
