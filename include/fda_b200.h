@@ -506,9 +506,9 @@ int fda_layer_norm_backward(const void *x, const void *weight, const void *resid
  *   experts [top_k] int64: the candidates with the largest select, in descending order
  *   weights [top_k] fp32: scale * score / (sum of the chosen scores) with renormalise, else scale * score
  * Ties go to the lower index.  Choices are those of exact scores: where fp32 cannot tell two apart they are computed in 64 bits.  NaN
- * compares as minus infinity and stays NaN in the weights; renormalised softmax weights are the softmax over the chosen logits; scores
- * that are all 0 (every logit minus infinity) give weights of 0.  n_experts <= 1024, top_k <= 32, n_groups <= 32
- * (FDA_ERR_TOO_LARGE_STATIC); top_k <= candidates.
+ * compares as minus infinity and stays NaN in the weights; renormalised softmax weights are the softmax over the chosen logits, renormalised
+ * sigmoid weights are ratios that do not vanish where the scores do; scores that are all 0 (every logit minus infinity) give weights of
+ * 0.  n_experts <= 1024, top_k <= 32, n_groups <= 32 (FDA_ERR_TOO_LARGE_STATIC); top_k <= candidates.
  * Backward: grad_logits [tokens][n_experts] of `dtype` from the gradient of the weights; `experts` is the forward's (an index outside
  * 0 .. n_experts - 1 gets no gradient).  The choice itself has none.  No counterpart in the reference.
  */

@@ -14,7 +14,7 @@
 // holds octets of neighbouring experts, octet o of the token belonging to lane o mod kLanes.  Their values lie in shared memory, their
 // largest in a register: a step of the choice takes the largest of these over the lanes, then eight lanes (four that look at two each) look at
 // the octet that has it.  Bound by instructions, no pipe of which is full (comparisons and selections 50 %, shuffles and shared memory 56 %,
-// issue slots 61 %); beyond 128 experts 64 registers (128 beyond 256) spill some 350 bytes a thread.  149504 tokens x 256 experts, 8 chosen, bf16:
+// issue slots 61 %); beyond 128 experts 64 registers (128 beyond 256) spill some 300 bytes a thread.  149504 tokens x 256 experts, 8 chosen, bf16:
 // 60 us by logits, 83 by biased softmax scores, of which the bytes would take 14; 37376 x 64 in 8 groups 17 us.
 //
 // How many tokens are decided in 64 bits depends on the logits: an error is taken relative to the token's largest score, so that low scores of a

@@ -18,9 +18,11 @@
         the sum of ``weight * row`` over each token's entries, + residual; an entry of no expert adds nothing
         weights ``[..., top_k]`` (None: 1), residual and y ``[..., features]``
 
-Ties go to the lower index.  Which experts are chosen does not depend on how an exponential rounds: scores that fp32 cannot tell apart
-are computed in 64 bits.  NaN compares as minus infinity and stays NaN in the weights; renormalised softmax weights are the softmax over the
-chosen logits; a token whose scores are all 0 (every logit minus infinity) has weights of 0.  The choice has no gradient: ``bias`` (kept
+Ties go to the lower index.  Which experts are chosen does not depend on how an exponential rounds in fp32: scores that it cannot tell apart
+are computed in 64 bits (which leaves sums of scores and biases that only differ beyond them).  Such tokens take longer: a peaked softmax or
+saturated sigmoids beside a bias several times as long.  NaN compares as minus infinity and stays NaN in the weights; renormalised softmax weights
+are the softmax over the chosen logits, and renormalised sigmoid weights are ratios that do not vanish where the scores do; a token whose scores
+are all 0 (every logit minus infinity) has weights of 0.  The choice has no gradient: ``bias`` (kept
 outside of training to balance the experts) gets none, logits get that of the weights.
 
 CUDA tensors in float32, float16 or bfloat16 of any sizes and strides (one that is not contiguous is copied); index tensors int64.  Nothing is
@@ -167,7 +169,7 @@ class ExpertFeedForward(nn.Module):
     """``x + sum over a token's experts of weight * (W2 act(W1 h + b1) + b2)``, ``h = norm(x)`` (without the outer ``x`` where
     ``residual=False``, ``h = x`` where ``norm=False``).
 
-    ``router`` ``[n_experts, d_model]`` makes the logits; the options are those of ``route_experts``.  With ``balanced`` a buffer
+    ``router`` ``[n_experts, d_model]`` makes the logits, in the rows' type (autocast's under autocast); the options are those of ``route_experts``.  With ``balanced`` a buffer
     ``balance`` is its bias: raise an expert's entry to send it more tokens.  ``forward`` takes a mask of tokens that are padding (True: no
     expert; it may hold anything) and with ``return_order`` returns the rows' order too, whose
     ``group_start_index.diff()`` is how many tokens each expert had."""
